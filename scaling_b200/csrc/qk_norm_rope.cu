@@ -1,0 +1,712 @@
+// Per-head norm and rotary embedding of queries and keys in one pass over the projections, forward and backward, and
+// the same forward pass writing keys and values into a paged cache.
+//
+// A row is one head of one token, x[0 .. D).  With r = 1 / sqrt(mean((x - mu)^2) + eps) (mu = 0 for RMS) and
+// xhat = (x - mu) r:
+//   y = xhat * w + b,  out = R(pos) y        R rotates the pairs of the first `rot` elements by pos * base^(-2 i / rot)
+//   dy = R(pos)^T dout,  db = sum_rows dy,  dw = sum_rows dy * xhat,  g = dy * w,
+//   dx = r (g - [mean(g)] - xhat mean(g xhat))                          (mean(g) for LayerNorm only)
+// (src/scaling/core/nn/attention/attention.py:812-850 norms, transposes and rotates in separate passes.)
+//
+// The work is a stream: every element is read and written once (x twice over a training step, because the backward
+// pass recomputes mu and r from x instead of reading stored ones).  A row is held by G lanes in registers, each with two
+// 16-byte chunks A and B that are chosen so that every rotary pair lies inside one lane: for the rotate-half convention
+// A = [l V, l V + V) and B = A + rot / 2, for interleaved pairs and the unrotated rest A and B are neighbours.  So the
+// rotation needs no exchange; only the row sums go through shuffles.  Statistics, weights, sines and products stay in
+// fp32 and are rounded once, at the store.
+//
+// Angles: a position of 10^5 times a frequency near 1 in fp32 is off by 10^-2 rad.  The host computes turns per position
+// base^(-2 i / rot) / (2 pi) in fp64; a thread multiplies by the position, drops the whole turns in fp64 and takes
+// sincospi of what is left in fp32.  One thread per (token, pair) fills a table in shared memory that all heads of the
+// token read.
+#include <cmath>
+
+#include "common.cuh"
+
+namespace {
+
+constexpr int QN_THREADS = 256;
+constexpr int QN_MAX_D = 256;
+constexpr int QN_MAX_SLOTS = 64;          // tokens per tile
+constexpr int QN_TABLE_BYTES = 24 * 1024; // sine table of a tile
+
+struct QnRows {  // one of q, k, v: the heads of every token
+  const void* x;
+  void* y;       // forward: out, backward: dx
+  const void* dy;
+  const void* w; // null: no norm
+  const void* b;
+  long x_tok, x_head, y_tok, y_head, dy_tok, dy_head;
+  int heads;
+};
+
+struct QnParams {
+  QnRows q, k, v;
+  const int* pos;   // [T], or null in the paged form: the token's place in its sequence
+  int T, D, rot, interleaved, rms, w_dtype;
+  float eps;
+  int tile;         // tokens per tile
+  int log_g;        // lanes per row, as a power of two
+  // paged form: k.y / v.y are the caches, y_head the stride between heads of a slot
+  const int* table;
+  const int* cu;
+  const int* lens;
+  long table_ld, k_page, k_slot, v_page, v_slot;
+  int batch, cols, num_pages, page_shift;
+  int* status;
+  // backward
+  float* partial;   // [blocks][2 * D]: sums of dw and db of each block
+  int q_blocks;     // blocks 0 .. q_blocks - 1 take q, the others k
+  double turns[QN_MAX_D / 2];
+};
+
+__device__ __forceinline__ float qn_load_any(const void* p, int i, int dtype) {
+  if (dtype == SB_DT_F32) return reinterpret_cast<const float*>(p)[i];
+  if (dtype == SB_DT_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+
+// N consecutive elements as one access
+template <typename T, int N> struct alignas(sizeof(T) * N) QnVec { T e[N]; };
+
+// What a lane holds of a row: NP pairs of chunks of V elements.  Pair p of lane l is number c = l + p G:
+//   rotate-half and c < rot / (2 V): A = c, B = c + rot / (2 V); otherwise A = 2 c, B = 2 c + 1.
+template <int V> struct QnChunks {
+  int a, b;
+  __device__ __forceinline__ QnChunks(int c, int rot, int interleaved) {
+    const int half = rot / (2 * V);
+    const bool split = !interleaved && c < half;
+    a = split ? c : 2 * c;
+    b = split ? c + half : 2 * c + 1;
+  }
+};
+
+// Place of element i (< V) of pair c in the sine table of one token, in float2 units.  Consecutive lanes touch
+// consecutive 16-byte words (no bank conflicts); np = pairs per row that the table covers.
+template <int V> __device__ __forceinline__ int qn_table_slot(int c, int i, int np) {
+  return V == 1 ? c : (((i >> 1) * np + c) << 1) + (i & 1);
+}
+// Place of element e of a weight vector in shared memory: four consecutive elements stay together, chunks interleave.
+template <int V> __device__ __forceinline__ int qn_weight_slot(int e, int chunks) {
+  if (V < 4) return e;
+  const int c = e / V, j = e % V;
+  return ((j >> 2) * chunks + c) * 4 + (j & 3);
+}
+
+template <int V> __device__ __forceinline__ void qn_read_weights(const float* s, int chunk, int chunks, float (&w)[V]) {
+  if constexpr (V < 4) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] = s[chunk * V + i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 t = *reinterpret_cast<const float4*>(s + ((i >> 2) * chunks + chunk) * 4);
+      w[i] = t.x; w[i + 1] = t.y; w[i + 2] = t.z; w[i + 3] = t.w;
+    }
+  }
+}
+
+// Rotation of a chunk pair by the table's angles (sign +1: forward, -1: transposed).
+template <int V>
+__device__ __forceinline__ void qn_rotate(float (&a)[V], float (&b)[V], const float2* tbl, int c, int np, int rot,
+                                          int interleaved, float sign) {
+  if constexpr (V == 1) {  // both conventions: the pair is (a, b)
+    const int angles = rot >> 1;
+    if (c < angles) {
+      const float2 t = tbl[c];
+      const float s = t.y * sign, x = a[0], y = b[0];
+      a[0] = x * t.x - y * s;
+      b[0] = y * t.x + x * s;
+    }
+  } else {
+    if (c * 2 * V >= rot) return;  // neither chunk is rotated (rotate-half: c >= rot / (2 V) is the same test)
+    float2 t[V];
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float4 u = *reinterpret_cast<const float4*>(tbl + ((i >> 1) * np + c) * 2);
+      t[i] = make_float2(u.x, u.y * sign);
+      t[i + 1] = make_float2(u.z, u.w * sign);
+    }
+    if (!interleaved) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float x = a[i], y = b[i];
+        a[i] = x * t[i].x - y * t[i].y;
+        b[i] = y * t[i].x + x * t[i].y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        if (2 * c * V + 2 * i < rot) {
+          const float x = a[2 * i], y = a[2 * i + 1];
+          a[2 * i] = x * t[i].x - y * t[i].y;
+          a[2 * i + 1] = y * t[i].x + x * t[i].y;
+        }
+        if ((2 * c + 1) * V + 2 * i < rot) {
+          const float x = b[2 * i], y = b[2 * i + 1];
+          b[2 * i] = x * t[V / 2 + i].x - y * t[V / 2 + i].y;
+          b[2 * i + 1] = y * t[V / 2 + i].x + x * t[V / 2 + i].y;
+        }
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ float qn_group_sum(float v, int g) {
+  for (int o = g >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Sines and cosines of a tile's tokens; positions come from `spos`.
+template <int V>
+__device__ __forceinline__ void qn_fill_table(const QnParams& p, float2* tbl, const int* spos, int n_tok, int np) {
+  const int angles = p.rot >> 1;
+  for (int i = threadIdx.x; i < n_tok * angles; i += QN_THREADS) {
+    const int t = i / angles, a = i - t * angles;
+    const double turns = (double)spos[t] * p.turns[a];
+    const float rest = (float)(turns - rint(turns));
+    float s, c;
+    sincospif(2.f * rest, &s, &c);
+    tbl[t * np * V + qn_table_slot<V>(a / V, a % V, np)] = make_float2(c, s);
+  }
+}
+
+// Row statistics of x held as NP pairs; chunks beyond the row (ha / hb false) hold zeros.
+template <int V, int NP>
+__device__ __forceinline__ void qn_stats(const float (&a)[NP][V], const float (&b)[NP][V], const bool (&ha)[NP],
+                                         const bool (&hb)[NP], int D, int rms, float eps, int g, float& mu, float& r) {
+  mu = 0.f;
+  if (!rms) {
+    float s = 0.f;
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+      for (int i = 0; i < V; ++i) s += a[p][i] + b[p][i];
+    mu = qn_group_sum(s, g) / D;
+  }
+  float ss = 0.f;  // around the mean, from registers: no cancellation
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float da = ha[p] ? a[p][i] - mu : 0.f, db = hb[p] ? b[p][i] - mu : 0.f;
+      ss = fmaf(da, da, ss);
+      ss = fmaf(db, db, ss);
+    }
+  r = rsqrtf(qn_group_sum(ss, g) / D + eps);
+}
+
+// ============================================================================ forward
+// One CTA per tile of tokens.  PAGED: k and v go to their slots of the cache, positions come from the sequence lengths.
+template <typename T, int V, int NP, bool PAGED>
+__global__ void __launch_bounds__(QN_THREADS, 4) qn_fwd_kernel(const __grid_constant__ QnParams p) {
+  extern __shared__ __align__(16) float smem[];
+  using Vec = QnVec<T, V>;
+  const int D = p.D, chunks = (D + V - 1) / V, np = (p.rot + 2 * V - 1) / (2 * V);
+  float* sw = smem;                                     // q weight, q bias, k weight, k bias
+  float2* tbl = reinterpret_cast<float2*>(smem + 4 * QN_MAX_D);
+  __shared__ int spos[QN_MAX_SLOTS];
+  __shared__ int spage[QN_MAX_SLOTS], sslot[QN_MAX_SLOTS];  // spage -1: nothing to write, -2: behind the last sequence
+  const int t0 = blockIdx.x * p.tile, n_tok = min(p.tile, p.T - t0);
+  const int g = 1 << p.log_g, lane = threadIdx.x & (g - 1), grp = threadIdx.x >> p.log_g;
+  const int n_grp = QN_THREADS >> p.log_g;
+
+  for (int i = threadIdx.x; i < D; i += QN_THREADS) {
+    const int s = qn_weight_slot<V>(i, chunks);
+    if (p.q.w) sw[s] = qn_load_any(p.q.w, i, p.w_dtype);
+    if (p.q.b) sw[QN_MAX_D + s] = qn_load_any(p.q.b, i, p.w_dtype);
+    if (p.k.w) sw[2 * QN_MAX_D + s] = qn_load_any(p.k.w, i, p.w_dtype);
+    if (p.k.b) sw[3 * QN_MAX_D + s] = qn_load_any(p.k.b, i, p.w_dtype);
+  }
+  if (threadIdx.x < n_tok) {
+    const int t = t0 + threadIdx.x;
+    if constexpr (PAGED) {
+      int lo = 0, hi = p.batch;  // first b with cu[b + 1] > t
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (p.cu[mid + 1] > t) hi = mid; else lo = mid + 1;
+      }
+      int page = -2, slot = 0, at = 0;
+      if (lo < p.batch && p.cu[lo] <= t) {
+        const long long pos = (long long)p.lens[lo] - p.cu[lo + 1] + t;  // the new tokens are the sequence's last
+        page = -1;
+        if (pos >= 0 && (pos >> p.page_shift) < p.cols) {
+          const int id = p.table[lo * p.table_ld + (pos >> p.page_shift)];
+          if (id >= 0 && id < p.num_pages) page = id;
+          slot = (int)(pos & ((1 << p.page_shift) - 1));
+          at = (int)pos;
+        }
+        if (page < 0) *p.status = SB_ERR_BAD_ARG;  // the token has no place in the cache: reported, nothing written
+      }
+      spage[threadIdx.x] = page;
+      sslot[threadIdx.x] = slot;
+      spos[threadIdx.x] = p.pos ? p.pos[t] : at;
+    } else {
+      spos[threadIdx.x] = p.pos ? p.pos[t] : 0;
+    }
+  }
+  __syncthreads();
+  if (p.rot) {
+    qn_fill_table<V>(p, tbl, spos, n_tok, np);
+    __syncthreads();
+  }
+
+  int ca[NP], cb[NP];
+  bool ha[NP], hb[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const QnChunks<V> c(lane + i * g, p.rot, p.interleaved);
+    ca[i] = c.a; cb[i] = c.b;
+    ha[i] = c.a < chunks; hb[i] = c.b < chunks;
+  }
+#pragma unroll 1
+  for (int kind = 0; kind < (PAGED ? 3 : 2); ++kind) {
+    const QnRows& R = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
+    const int rows = n_tok * R.heads, iters = (rows + n_grp - 1) / n_grp;
+    const float* w = sw + kind * 2 * QN_MAX_D;
+    const float* bias = w + QN_MAX_D;
+    const bool plain = kind == 2 || (!R.w && !p.rot);  // a copy, bit by bit
+#pragma unroll 1
+    for (int it = 0; it < iters; ++it) {  // the same trip count for every lane: the shuffles name all of them
+      const int row = grp + it * n_grp;
+      const bool live = row < rows;
+      const int tl = live ? row / R.heads : 0, h = row - tl * R.heads;
+      const T* x = reinterpret_cast<const T*>(R.x) + (long)(t0 + tl) * R.x_tok + (long)h * R.x_head;
+      Vec va[NP], vb[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        if (live && ha[i]) va[i] = *reinterpret_cast<const Vec*>(x + ca[i] * V);
+        if (live && hb[i]) vb[i] = *reinterpret_cast<const Vec*>(x + cb[i] * V);
+      }
+      if (!plain) {
+        float a[NP][V], b[NP][V];
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            a[i][j] = live && ha[i] ? sb::to_f(va[i].e[j]) : 0.f;
+            b[i][j] = live && hb[i] ? sb::to_f(vb[i].e[j]) : 0.f;
+          }
+        if (R.w) {
+          float mu, r;
+          qn_stats<V, NP>(a, b, ha, hb, D, p.rms, p.eps, g, mu, r);
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            float wa[V], wb[V];
+            if (ha[i]) {
+              qn_read_weights<V>(w, ca[i], chunks, wa);
+#pragma unroll
+              for (int j = 0; j < V; ++j) a[i][j] = (a[i][j] - mu) * r * wa[j];
+            }
+            if (hb[i]) {
+              qn_read_weights<V>(w, cb[i], chunks, wb);
+#pragma unroll
+              for (int j = 0; j < V; ++j) b[i][j] = (b[i][j] - mu) * r * wb[j];
+            }
+            if (R.b) {
+              if (ha[i]) {
+                qn_read_weights<V>(bias, ca[i], chunks, wa);
+#pragma unroll
+                for (int j = 0; j < V; ++j) a[i][j] += wa[j];
+              }
+              if (hb[i]) {
+                qn_read_weights<V>(bias, cb[i], chunks, wb);
+#pragma unroll
+                for (int j = 0; j < V; ++j) b[i][j] += wb[j];
+              }
+            }
+          }
+        }
+        if (p.rot) {
+#pragma unroll
+          for (int i = 0; i < NP; ++i)
+            qn_rotate<V>(a[i], b[i], tbl + tl * np * V, lane + i * g, np, p.rot, p.interleaved, 1.f);
+        }
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            va[i].e[j] = sb::from_f<T>(a[i][j]);
+            vb[i].e[j] = sb::from_f<T>(b[i][j]);
+          }
+      }
+      T* y = reinterpret_cast<T*>(R.y);
+      bool store = live;
+      if (PAGED && live) {
+        const int page = spage[tl];
+        if (kind == 0) {
+          y += (long)(t0 + tl) * R.y_tok + (long)h * R.y_head;
+          if (page == -2) {  // behind the last sequence: zeros
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+#pragma unroll
+              for (int j = 0; j < V; ++j) va[i].e[j] = vb[i].e[j] = sb::from_f<T>(0.f);
+          }
+        } else {
+          store = page >= 0;
+          y += (long)page * (kind == 1 ? p.k_page : p.v_page) + (long)sslot[tl] * (kind == 1 ? p.k_slot : p.v_slot) +
+               (long)h * R.y_head;
+        }
+      } else if (live) {
+        y += (long)(t0 + tl) * R.y_tok + (long)h * R.y_head;
+      }
+      if (store) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          if (ha[i]) *reinterpret_cast<Vec*>(y + ca[i] * V) = va[i];
+          if (hb[i]) *reinterpret_cast<Vec*>(y + cb[i] * V) = vb[i];
+        }
+      }
+    }
+  }
+}
+
+// ============================================================================ backward
+// A block takes either q or k, walks over tiles of tokens and keeps its share of dw and db in registers (each lane owns
+// the same chunks in every row); the block's sums go to one row of `partial`, added up in a fixed order afterwards.
+template <typename T, int V, int NP>
+__global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_constant__ QnParams p) {
+  extern __shared__ __align__(16) float smem[];
+  using Vec = QnVec<T, V>;
+  const int D = p.D, chunks = (D + V - 1) / V, np = (p.rot + 2 * V - 1) / (2 * V);
+  const bool is_q = (int)blockIdx.x < p.q_blocks;
+  const QnRows& R = is_q ? p.q : p.k;
+  const int blk = is_q ? blockIdx.x : blockIdx.x - p.q_blocks;
+  const int n_blk = is_q ? p.q_blocks : (int)gridDim.x - p.q_blocks;
+  float* sw = smem;
+  float2* tbl = reinterpret_cast<float2*>(smem + QN_MAX_D);
+  __shared__ int spos[QN_MAX_SLOTS];
+  const int g = 1 << p.log_g, lane = threadIdx.x & (g - 1), grp = threadIdx.x >> p.log_g;
+  const int n_grp = QN_THREADS >> p.log_g;
+  for (int i = threadIdx.x; i < D; i += QN_THREADS) sw[qn_weight_slot<V>(i, chunks)] = qn_load_any(R.w, i, p.w_dtype);
+  int ca[NP], cb[NP];
+  bool ha[NP], hb[NP];
+  float dwa[NP][V], dwb[NP][V], dba[NP][V], dbb[NP][V];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const QnChunks<V> c(lane + i * g, p.rot, p.interleaved);
+    ca[i] = c.a; cb[i] = c.b;
+    ha[i] = c.a < chunks; hb[i] = c.b < chunks;
+#pragma unroll
+    for (int j = 0; j < V; ++j) dwa[i][j] = dwb[i][j] = dba[i][j] = dbb[i][j] = 0.f;
+  }
+  const int tiles = (p.T + p.tile - 1) / p.tile;
+#pragma unroll 1
+  for (int tile = blk; tile < tiles; tile += n_blk) {
+    const int t0 = tile * p.tile, n_tok = min(p.tile, p.T - t0);
+    __syncthreads();  // the table of the tile before is no longer read
+    if (p.rot) {
+      if (threadIdx.x < n_tok) spos[threadIdx.x] = p.pos[t0 + threadIdx.x];
+      __syncthreads();
+      qn_fill_table<V>(p, tbl, spos, n_tok, np);
+    }
+    __syncthreads();
+    const int rows = n_tok * R.heads, iters = (rows + n_grp - 1) / n_grp;
+#pragma unroll 1
+    for (int it = 0; it < iters; ++it) {
+      const int row = grp + it * n_grp;
+      const bool live = row < rows;
+      const int tl = live ? row / R.heads : 0, h = row - tl * R.heads;
+      const T* x = reinterpret_cast<const T*>(R.x) + (long)(t0 + tl) * R.x_tok + (long)h * R.x_head;
+      const T* dy = reinterpret_cast<const T*>(R.dy) + (long)(t0 + tl) * R.dy_tok + (long)h * R.dy_head;
+      Vec va[NP], vb[NP], ya[NP], yb[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        if (live && ha[i]) {
+          va[i] = *reinterpret_cast<const Vec*>(x + ca[i] * V);
+          ya[i] = *reinterpret_cast<const Vec*>(dy + ca[i] * V);
+        }
+        if (live && hb[i]) {
+          vb[i] = *reinterpret_cast<const Vec*>(x + cb[i] * V);
+          yb[i] = *reinterpret_cast<const Vec*>(dy + cb[i] * V);
+        }
+      }
+      float a[NP][V], b[NP][V], da[NP][V], db[NP][V];
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          a[i][j] = live && ha[i] ? sb::to_f(va[i].e[j]) : 0.f;
+          b[i][j] = live && hb[i] ? sb::to_f(vb[i].e[j]) : 0.f;
+          da[i][j] = live && ha[i] ? sb::to_f(ya[i].e[j]) : 0.f;
+          db[i][j] = live && hb[i] ? sb::to_f(yb[i].e[j]) : 0.f;
+        }
+      if (p.rot) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+          qn_rotate<V>(da[i], db[i], tbl + tl * np * V, lane + i * g, np, p.rot, p.interleaved, -1.f);
+      }
+      float mu, r;
+      qn_stats<V, NP>(a, b, ha, hb, D, p.rms, p.eps, g, mu, r);
+      float s1 = 0.f, s2 = 0.f;  // sums of g and of g * xhat
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        float w[V];
+        if (ha[i]) {
+          qn_read_weights<V>(sw, ca[i], chunks, w);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            a[i][j] = (a[i][j] - mu) * r;
+            if (live) dwa[i][j] = fmaf(da[i][j], a[i][j], dwa[i][j]);
+            dba[i][j] += da[i][j];
+            da[i][j] *= w[j];
+            s1 += da[i][j];
+            s2 = fmaf(da[i][j], a[i][j], s2);
+          }
+        }
+        if (hb[i]) {
+          qn_read_weights<V>(sw, cb[i], chunks, w);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            b[i][j] = (b[i][j] - mu) * r;
+            if (live) dwb[i][j] = fmaf(db[i][j], b[i][j], dwb[i][j]);
+            dbb[i][j] += db[i][j];
+            db[i][j] *= w[j];
+            s1 += db[i][j];
+            s2 = fmaf(db[i][j], b[i][j], s2);
+          }
+        }
+      }
+      s2 = qn_group_sum(s2, g) / D;
+      s1 = p.rms ? 0.f : qn_group_sum(s1, g) / D;
+      T* y = reinterpret_cast<T*>(R.y) + (long)(t0 + tl) * R.y_tok + (long)h * R.y_head;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          va[i].e[j] = sb::from_f<T>(r * (da[i][j] - s1 - a[i][j] * s2));
+          vb[i].e[j] = sb::from_f<T>(r * (db[i][j] - s1 - b[i][j] * s2));
+        }
+        if (live && ha[i]) *reinterpret_cast<Vec*>(y + ca[i] * V) = va[i];
+        if (live && hb[i]) *reinterpret_cast<Vec*>(y + cb[i] * V) = vb[i];
+      }
+    }
+  }
+  if (!p.partial) return;
+  // sums over the row groups of a warp, then over the warps, in a fixed order
+  float* red = smem;  // [warps][2][QN_MAX_D], after the last use of weights and table
+  __syncthreads();
+  const int warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      for (int o = g; o < 32; o <<= 1) {
+        dwa[i][j] += __shfl_xor_sync(0xffffffffu, dwa[i][j], o);
+        dwb[i][j] += __shfl_xor_sync(0xffffffffu, dwb[i][j], o);
+        dba[i][j] += __shfl_xor_sync(0xffffffffu, dba[i][j], o);
+        dbb[i][j] += __shfl_xor_sync(0xffffffffu, dbb[i][j], o);
+      }
+      if ((threadIdx.x & 31) < g) {
+        float* dst = red + warp * 2 * QN_MAX_D;
+        if (ha[i]) { dst[ca[i] * V + j] = dwa[i][j]; dst[QN_MAX_D + ca[i] * V + j] = dba[i][j]; }
+        if (hb[i]) { dst[cb[i] * V + j] = dwb[i][j]; dst[QN_MAX_D + cb[i] * V + j] = dbb[i][j]; }
+      }
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * D; i += QN_THREADS) {
+    const int which = i >= D, e = which ? i - D : i;
+    float s = 0.f;
+    for (int wp = 0; wp < QN_THREADS / 32; ++wp) s += red[wp * 2 * QN_MAX_D + which * QN_MAX_D + e];
+    p.partial[(size_t)blockIdx.x * 2 * D + i] = s;
+  }
+}
+
+// Sums of the blocks' partial rows: blockIdx.y = 0 q, 1 k; 32 columns per block (of 2 D: dw then db), 32 row lanes.
+template <typename W>
+__global__ void __launch_bounds__(1024) qn_bwd_sum_kernel(const float* __restrict__ partial, int D, int q_blocks,
+                                                          int blocks, W* dwq, W* dbq, W* dwk, W* dbk, int accumulate) {
+  __shared__ float red[32][33];
+  const int col = blockIdx.x * 32 + threadIdx.x;
+  const int b0 = blockIdx.y ? q_blocks : 0, b1 = blockIdx.y ? blocks : q_blocks;
+  float s = 0.f;
+  if (col < 2 * D)
+    for (int b = b0 + threadIdx.y; b < b1; b += 32) s += partial[(size_t)b * 2 * D + col];
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  s = sb::warp_sum(red[threadIdx.x][threadIdx.y]);  // warp y sums column y of this block
+  const int c = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && c < 2 * D) {
+    W* dst = blockIdx.y ? (c < D ? dwk : dbk) : (c < D ? dwq : dbq);
+    const int e = c < D ? c : c - D;
+    if (dst) dst[e] = sb::from_f<W>(accumulate ? sb::to_f(dst[e]) + s : s);
+  }
+}
+
+int qn_log_lanes(int pairs, int cap) {
+  int l = 0;
+  while ((1 << l) < pairs && (1 << l) < cap) ++l;
+  return l;
+}
+bool qn_vec_ok(const QnRows& r, int esize, bool with_dy) {
+  if (r.heads == 0) return true;
+  const long v = 16 / esize;
+  if ((reinterpret_cast<uintptr_t>(r.x) | reinterpret_cast<uintptr_t>(r.y)) & 15) return false;
+  if (r.x_tok % v || r.x_head % v || r.y_tok % v || r.y_head % v) return false;
+  return !with_dy || (!(reinterpret_cast<uintptr_t>(r.dy) & 15) && r.dy_tok % v == 0 && r.dy_head % v == 0);
+}
+
+// Fills in what follows from the sizes; returns true when rows move as 16-byte chunks (V elements, one pair per lane):
+// aligned rows whose rotated part, for rotate-half, splits into whole chunks.  Everything else moves element by element.
+bool qn_plan(QnParams* p, int esize, bool vec_ok, double base) {
+  const int v = 16 / esize;
+  const bool fast = vec_ok && p->D % v == 0 && (p->rot == 0 || p->interleaved || (p->rot / 2) % v == 0) && p->D / v <= 64;
+  const int V = fast ? v : 1;
+  const int chunks = (p->D + V - 1) / V, pairs = (chunks + 1) / 2;
+  p->log_g = fast ? qn_log_lanes(pairs, 32) : 5;
+  for (int i = 0; i < p->rot / 2; ++i)
+    p->turns[i] = pow(base, -2.0 * i / p->rot) / 6.283185307179586476925;
+  return fast;
+}
+int qn_table_bytes_per_token(const QnParams& p, int V) { return p.rot ? ((p.rot + 2 * V - 1) / (2 * V)) * V * 8 : 0; }
+
+}  // namespace
+
+static int qn_check(const QnParams& p, int dtype) {
+  if (dtype != SB_DT_F32 && dtype != SB_DT_BF16 && dtype != SB_DT_F16) return SB_ERR_BAD_ARG;
+  if (p.w_dtype != SB_DT_F32 && p.w_dtype != SB_DT_BF16 && p.w_dtype != SB_DT_F16) return SB_ERR_BAD_ARG;
+  if (p.D < 1 || p.T < 0 || p.q.heads < 0 || p.k.heads < 0) return SB_ERR_BAD_ARG;
+  if (p.D > QN_MAX_D) return SB_ERR_TOO_LARGE;
+  if (p.rot < 0 || p.rot % 2 || p.rot > p.D) return SB_ERR_BAD_ARG;
+  return SB_OK;
+}
+
+template <typename T>
+static int qn_launch_fwd(QnParams& p, bool paged, bool vec_ok, double base, int sms, cudaStream_t stream) {
+  const bool fast = qn_plan(&p, sizeof(T), vec_ok, base);
+  constexpr int VF = 16 / sizeof(T);
+  const int per_tok = qn_table_bytes_per_token(p, fast ? VF : 1);
+  // Tokens per CTA: enough rows for four rounds of the CTA's row groups, so that the table and the weights are worth
+  // their barrier, but not so many that SMs go without a CTA.
+  const int heads = p.q.heads + p.k.heads + (paged ? p.v.heads : 0);
+  const int groups = QN_THREADS >> p.log_g;
+  int tile = (4 * groups + heads - 1) / heads;
+  if (tile > QN_MAX_SLOTS) tile = QN_MAX_SLOTS;
+  if (per_tok && tile > QN_TABLE_BYTES / per_tok) tile = QN_TABLE_BYTES / per_tok;
+  while (tile > 1 && (p.T + tile - 1) / tile < 2 * sms) tile = (tile + 1) / 2;
+  p.tile = tile;
+  const int smem = 4 * QN_MAX_D * 4 + tile * per_tok;
+  const int grid = (p.T + tile - 1) / tile;
+  if (paged) {
+    if (fast) qn_fwd_kernel<T, VF, 1, true><<<grid, QN_THREADS, smem, stream>>>(p);
+    else qn_fwd_kernel<T, 1, 4, true><<<grid, QN_THREADS, smem, stream>>>(p);
+  } else {
+    if (fast) qn_fwd_kernel<T, VF, 1, false><<<grid, QN_THREADS, smem, stream>>>(p);
+    else qn_fwd_kernel<T, 1, 4, false><<<grid, QN_THREADS, smem, stream>>>(p);
+  }
+  SB_CHECK_LAUNCH();
+  return SB_OK;
+}
+
+// q_out / k_out [T, heads, D] = rotated norms of q and k (token and head strides in elements, innermost stride 1).
+// Null weights: no norm.  pos: int32 [T], needed when rot > 0.  base: of the rotary frequencies.
+SB_API int sb200_qk_norm_rope_fwd(const void* q, const void* k, void* q_out, void* k_out, const void* q_w,
+                                  const void* k_w, const void* q_b, const void* k_b, const int* pos, int T, int Hq,
+                                  int Hk, int D, long q_tok, long q_head, long k_tok, long k_head, float eps, int rms,
+                                  int rot, double base, int interleaved, int dtype, int w_dtype, int sms,
+                                  cudaStream_t stream) {
+  QnParams p = {};
+  p.q = {q, q_out, nullptr, q_w, q_b, q_tok, q_head, (long)Hq * D, D, 0, 0, Hq};
+  p.k = {k, k_out, nullptr, k_w, k_b, k_tok, k_head, (long)Hk * D, D, 0, 0, Hk};
+  p.pos = pos; p.T = T; p.D = D; p.rot = rot; p.interleaved = interleaved; p.rms = rms; p.w_dtype = w_dtype; p.eps = eps;
+  if (int rc = qn_check(p, dtype)) return rc;
+  if (rot && (!pos || !(base > 0.0))) return SB_ERR_BAD_ARG;
+  if (T == 0 || Hq + Hk == 0) return SB_OK;
+  const int es = dtype == SB_DT_F32 ? 4 : 2;
+  const bool vec = qn_vec_ok(p.q, es, false) && qn_vec_ok(p.k, es, false);
+  SB_DISPATCH_DTYPE(dtype, E, { return qn_launch_fwd<E>(p, false, vec, base, sms, stream); });
+  return SB_OK;
+}
+
+// The paged form.  Row t belongs to the sequence b with cu[b] <= t < cu[b + 1]; its position is
+// lens[b] - cu[b + 1] + t, and k / v go to row pos % page_size of page table[b][pos / page_size] of the caches
+// [num_pages, page_size, Hk, D] (page, row and head strides in elements, page_size a power of two).  A position outside
+// the table or a page outside the cache writes nothing and sets *status.  Rows behind the last sequence give zeros in
+// q_out and touch no page.  pos may override the rotation angles; q may be null (Hq = 0).
+SB_API int sb200_paged_append(const void* q, const void* k, const void* v, void* q_out, void* k_cache, void* v_cache,
+                              const void* q_w, const void* k_w, const void* q_b, const void* k_b, const int* pos,
+                              const int* table, const int* cu, const int* lens, int T, int batch, int Hq, int Hk, int D,
+                              long q_tok, long q_head, long k_tok, long k_head, long v_tok, long v_head, long k_page,
+                              long k_slot, long kc_head, long v_page, long v_slot, long vc_head, long table_ld,
+                              int cols, int num_pages, int page_size, float eps, int rms, int rot, double base,
+                              int interleaved, int dtype, int w_dtype, int sms, int* status, cudaStream_t stream) {
+  QnParams p = {};
+  p.q = {q, q_out, nullptr, q_w, q_b, q_tok, q_head, (long)Hq * D, D, 0, 0, Hq};
+  p.k = {k, k_cache, nullptr, k_w, k_b, k_tok, k_head, 0, kc_head, 0, 0, Hk};
+  p.v = {v, v_cache, nullptr, nullptr, nullptr, v_tok, v_head, 0, vc_head, 0, 0, Hk};
+  p.pos = pos; p.T = T; p.D = D; p.rot = rot; p.interleaved = interleaved; p.rms = rms; p.w_dtype = w_dtype; p.eps = eps;
+  if (int rc = qn_check(p, dtype)) return rc;
+  if (batch < 0 || cols < 0 || num_pages < 0 || page_size < 1 || (page_size & (page_size - 1)) || !status || Hk < 1)
+    return SB_ERR_BAD_ARG;
+  if (rot && !(base > 0.0)) return SB_ERR_BAD_ARG;
+  if (T == 0) return SB_OK;
+  p.table = table; p.cu = cu; p.lens = lens; p.table_ld = table_ld; p.batch = batch; p.cols = cols;
+  p.num_pages = num_pages; p.status = status;
+  p.k_page = k_page; p.k_slot = k_slot; p.v_page = v_page; p.v_slot = v_slot;
+  while ((1 << p.page_shift) < page_size) ++p.page_shift;
+  const int es = dtype == SB_DT_F32 ? 4 : 2;
+  const long v16 = 16 / es;
+  const bool vec = qn_vec_ok(p.q, es, false) && qn_vec_ok(p.k, es, false) && qn_vec_ok(p.v, es, false) &&
+                   k_page % v16 == 0 && k_slot % v16 == 0 && v_page % v16 == 0 && v_slot % v16 == 0;
+  SB_DISPATCH_DTYPE(dtype, E, { return qn_launch_fwd<E>(p, true, vec, base, sms, stream); });
+  return SB_OK;
+}
+
+// Blocks of the backward launch = rows of its workspace (2 D floats each).
+SB_API int sb200_qk_norm_rope_bwd_blocks(int T, int sms) {
+  const long want = 2L * sms;
+  return (int)(want < T ? (want < 2 ? 2 : want) : (T < 2 ? 2 : T));
+}
+
+template <typename T>
+static int qn_launch_bwd(QnParams& p, bool vec_ok, double base, int blocks, cudaStream_t stream) {
+  const bool fast = qn_plan(&p, sizeof(T), vec_ok, base);
+  constexpr int VF = 16 / sizeof(T);
+  const int per_tok = qn_table_bytes_per_token(p, fast ? VF : 1);
+  const int heads = p.q.heads > p.k.heads ? p.q.heads : p.k.heads;
+  const int groups = QN_THREADS >> p.log_g;
+  // blocks shared out by rows, at least one each
+  int qb = (int)(((long)blocks * p.q.heads + (p.q.heads + p.k.heads) / 2) / (p.q.heads + p.k.heads));
+  p.q_blocks = qb < 1 ? 1 : qb > blocks - 1 ? blocks - 1 : qb;
+  int tile = (4 * groups + heads - 1) / heads;
+  if (tile > QN_MAX_SLOTS) tile = QN_MAX_SLOTS;
+  if (per_tok && tile > QN_TABLE_BYTES / per_tok) tile = QN_TABLE_BYTES / per_tok;
+  while (tile > 1 && (p.T + tile - 1) / tile < 4 * p.q_blocks) tile = (tile + 1) / 2;
+  p.tile = tile;
+  int smem = QN_MAX_D * 4 + tile * per_tok;
+  const int red = (QN_THREADS / 32) * 2 * QN_MAX_D * 4;
+  if (smem < red) smem = red;
+  if (fast) qn_bwd_kernel<T, VF, 1><<<blocks, QN_THREADS, smem, stream>>>(p);
+  else qn_bwd_kernel<T, 1, 4><<<blocks, QN_THREADS, smem, stream>>>(p);
+  SB_CHECK_LAUNCH();
+  return SB_OK;
+}
+
+// dq / dk [T, heads, D] (contiguous) from d_q_out / d_k_out and the inputs; dwq .. dbk (any may be null) in w_dtype,
+// written, or added to with accumulate.  partial: [blocks, 2 D] floats, or null when no weight gradient is wanted;
+// blocks as sb200_qk_norm_rope_bwd_blocks says.
+SB_API int sb200_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, const void* q, const void* k, const void* q_w,
+                                  const void* k_w, const int* pos, void* dq, void* dk, void* dwq, void* dwk, void* dbq,
+                                  void* dbk, float* partial, int blocks, int T, int Hq, int Hk, int D, long dqo_tok,
+                                  long dqo_head, long dko_tok, long dko_head, long q_tok, long q_head, long k_tok,
+                                  long k_head, float eps, int rms, int rot, double base, int interleaved,
+                                  int accumulate, int dtype, int w_dtype, cudaStream_t stream) {
+  QnParams p = {};
+  p.q = {q, dq, dq_out, q_w, nullptr, q_tok, q_head, (long)Hq * D, D, dqo_tok, dqo_head, Hq};
+  p.k = {k, dk, dk_out, k_w, nullptr, k_tok, k_head, (long)Hk * D, D, dko_tok, dko_head, Hk};
+  p.pos = pos; p.T = T; p.D = D; p.rot = rot; p.interleaved = interleaved; p.rms = rms; p.w_dtype = w_dtype; p.eps = eps;
+  p.partial = partial;
+  if (int rc = qn_check(p, dtype)) return rc;
+  if ((rot && (!pos || !(base > 0.0))) || !q_w || !k_w || T < 1 || Hq < 1 || Hk < 1 || blocks < 2) return SB_ERR_BAD_ARG;
+  const int es = dtype == SB_DT_F32 ? 4 : 2;
+  const bool vec = qn_vec_ok(p.q, es, true) && qn_vec_ok(p.k, es, true);
+  int rc = SB_ERR_BAD_ARG;
+  SB_DISPATCH_DTYPE(dtype, E, { rc = qn_launch_bwd<E>(p, vec, base, blocks, stream); });
+  if (rc || !partial) return rc;
+  SB_DISPATCH_DTYPE(w_dtype, W, {
+    qn_bwd_sum_kernel<W><<<dim3((2 * D + 31) / 32, 2), dim3(32, 32), 0, stream>>>(
+        partial, D, p.q_blocks, blocks, (W*)dwq, (W*)dbq, (W*)dwk, (W*)dbk, accumulate);
+  });
+  SB_CHECK_LAUNCH();
+  return SB_OK;
+}

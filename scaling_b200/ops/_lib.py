@@ -7,10 +7,11 @@ product, the torch expressions in ``scaling_b200.ops`` exist for CPU ranks and a
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
-from ctypes import c_float, c_int, c_long, c_void_p
+from ctypes import c_double, c_float, c_int, c_long, c_void_p
 from typing import Optional
 
 import torch
@@ -65,6 +66,10 @@ _SIGS = {
     "sb200_gelu_bwd": [c_void_p, c_void_p, c_void_p, c_long, c_int, c_void_p],
     "sb200_dropout_add": [c_void_p, c_void_p, c_void_p, c_long, c_float, c_float, c_float, c_void_p, ctypes.c_uint, c_long, c_int, c_int, c_void_p],
     "sb200_rope": [c_void_p, c_void_p, c_int, c_int, c_int, c_long, c_long, c_float, c_int, c_int, c_int, c_void_p],
+    "sb200_qk_norm_rope_fwd": [c_void_p] * 9 + [c_int] * 4 + [c_long] * 4 + [c_float, c_int, c_int, c_double, c_int, c_int, c_int, c_int, c_void_p],
+    "sb200_qk_norm_rope_bwd_blocks": [c_int, c_int],
+    "sb200_qk_norm_rope_bwd": [c_void_p] * 14 + [c_int] * 5 + [c_long] * 8 + [c_float, c_int, c_int, c_double, c_int, c_int, c_int, c_int, c_void_p],
+    "sb200_paged_append": [c_void_p] * 14 + [c_int] * 5 + [c_long] * 13 + [c_int] * 3 + [c_float, c_int, c_int, c_double, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "sb200_masked_softmax_fwd": [c_void_p, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_float, c_int, c_void_p],
     "sb200_masked_softmax_bwd": [c_void_p, c_void_p, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_float, c_int, c_void_p],
     "sb200_colsum_splits": [c_long, c_int, c_int, c_int],
@@ -131,7 +136,7 @@ class _Counting:
 
 
 _NO_LAUNCH = {"sb200_p2p_max_ranks", "sb200_colsum_splits", "sb200_norm_bwd_partial_rows", "sb200_norm_bwd_partial_rows_h", "sb200_sumsq_max_partials",
-              "sb200_bind_device", "sb200_fa_last_driver_error"}
+              "sb200_bind_device", "sb200_fa_last_driver_error", "sb200_qk_norm_rope_bwd_blocks"}
 
 
 def kernel_calls() -> int:
@@ -207,6 +212,13 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def stream() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+def on_device_of(t: torch.Tensor):
+    """Context in which the device of ``t`` is current (launches, streams and workspaces follow the current device)."""
+    if t.device.index is None or t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 _SM_COUNT: dict[int, int] = {}

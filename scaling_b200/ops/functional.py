@@ -537,6 +537,157 @@ def rope(x: torch.Tensor, pos: torch.Tensor, rot_dim: Optional[int] = None, base
     return rope_reference(x, pos, rot_dim, base, interleaved)
 
 
+# --------------------------------------------------------------------------- per-head norm + RoPE
+def rotate_reference(x: torch.Tensor, pos: torch.Tensor, rotary: tuple[int, float, bool]) -> torch.Tensor:
+    """Rotation of ``x[tokens, heads, d]`` (fp32 or fp64, result in the same type) with angles formed in fp64, which
+    keeps them exact to fp32 at positions where an fp32 product is off by whole digits."""
+    rot_dim, base, interleaved = rotary
+    half = rot_dim // 2
+    inv = float(base) ** (-2.0 * torch.arange(half, device=x.device, dtype=torch.float64) / rot_dim)
+    ang = pos.to(torch.float64)[:, None] * inv[None, :]
+    cos, sin = ang.cos().to(x.dtype)[:, None, :], ang.sin().to(x.dtype)[:, None, :]
+    rot, rest = x[..., :rot_dim], x[..., rot_dim:]
+    if interleaved:
+        a, b = rot[..., 0::2], rot[..., 1::2]
+        out = torch.stack((a * cos - b * sin, b * cos + a * sin), dim=-1).flatten(-2)
+    else:
+        a, b = rot[..., :half], rot[..., half:]
+        out = torch.cat((a * cos - b * sin, b * cos + a * sin), dim=-1)
+    return torch.cat((out, rest), dim=-1)
+
+
+def head_norm_rope_reference(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+                             pos: Optional[torch.Tensor], rotary: Optional[tuple[int, float, bool]], eps: float,
+                             rms: bool) -> torch.Tensor:
+    """Torch expression of ``qk_norm_rope`` for one of q and k, in fp32 (fp64 for fp64 inputs), rounded once."""
+    y = x if x.dtype == torch.float64 else x.float()
+    if weight is not None:
+        if not rms:
+            y = y - y.mean(-1, keepdim=True)
+        y = y * torch.rsqrt(y.pow(2).mean(-1, keepdim=True) + eps) * weight.to(y.dtype)
+        if bias is not None:
+            y = y + bias.to(y.dtype)
+    if rotary is not None:
+        assert pos is not None
+        y = rotate_reference(y, pos, rotary)
+    return y.to(x.dtype)
+
+
+def rotary_args(rotary: Optional[tuple[int, float, bool]], head_dim: int) -> tuple[int, float, bool]:
+    """``(rotary dimensions, base, interleaved)`` checked against the head size; ``(0, 1.0, False)`` for None."""
+    if rotary is None:
+        return 0, 1.0, False
+    rot, base, interleaved = rotary
+    if rot <= 0 or rot % 2 or rot > head_dim or not base > 0:
+        raise ValueError(f"rotary dimensions must be even, positive and at most the head size {head_dim} and the base "
+                         f"positive, got {rotary}")
+    return int(rot), float(base), bool(interleaved)
+
+
+def check_head_norm(name: str, x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+                    rms: bool) -> None:
+    if x.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {tuple(x.shape)}")
+    for what, p in (("weight", weight), ("bias", bias)):
+        if p is not None and (p.dim() != 1 or p.shape[0] != x.shape[2] or p.device != x.device):
+            raise ValueError(f"{name} {what} must have one element per head dimension ({x.shape[2]}) on {x.device}, got "
+                             f"{tuple(p.shape)} on {p.device}")
+    if bias is not None and (rms or weight is None):
+        raise ValueError(f"{name} bias: only a layer norm with a weight has one")
+
+
+def _common_dtype(*params: Optional[torch.Tensor]) -> tuple[Optional[torch.Tensor], ...]:
+    """Norm parameters of one kernel call in one type (fp32 where they differ or the kernels do not know the type)."""
+    kinds = {p.dtype for p in params if p is not None}
+    same = len(kinds) <= 1 and kinds <= set(_KERNEL_DTYPES)
+    return tuple(None if p is None else (p if same else p.float()).contiguous() for p in params)
+
+
+def _unit_inner(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+class _QKNormRopeFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, bq, bk, pos, rot, base, interleaved, eps, rms):  # type: ignore[override]
+        q, k = _unit_inner(q), _unit_inner(k)
+        T, Hq, D = q.shape
+        Hk = k.shape[1]
+        qo = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+        ko = torch.empty((T, Hk, D), dtype=q.dtype, device=q.device)
+        with _lib.on_device_of(q):
+            check(lib().sb200_qk_norm_rope_fwd(
+                q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), wq.data_ptr(), wk.data_ptr(), ptr(bq), ptr(bk),
+                ptr(pos), T, Hq, Hk, D, q.stride(0), q.stride(1), k.stride(0), k.stride(1), eps, int(rms), rot, base,
+                int(interleaved), dt(q.dtype), dt(wq.dtype), sm_count(), stream()), "sb200_qk_norm_rope_fwd")
+        ctx.save_for_backward(q, k, wq, wk, pos)
+        ctx.params = (wq, wk, bq, bk)  # the parameter objects themselves (for their persistent .grad buffers)
+        ctx.cfg = (rot, base, interleaved, eps, rms)
+        return qo, ko
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dqo, dko):  # type: ignore[override]
+        q, k, wq, wk, pos = ctx.saved_tensors
+        rot, base, interleaved, eps, rms = ctx.cfg
+        dqo, dko = _unit_inner(dqo), _unit_inner(dko)
+        T, Hq, D = q.shape
+        Hk = k.shape[1]
+        dq = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+        dk = torch.empty((T, Hk, D), dtype=q.dtype, device=q.device)
+        params = ctx.params
+        wanted = [p is not None and ctx.needs_input_grad[2 + i] for i, p in enumerate(params)]
+        with _lib.on_device_of(q):
+            blocks = lib().sb200_qk_norm_rope_bwd_blocks(T, sm_count())
+            partial = torch.empty((blocks, 2 * D), dtype=torch.float32, device=q.device) if any(wanted) else None
+            # parameters with persistent gradient buffers get their gradients added in place, unless two of them share one
+            mains = [fused_grad_target(p) if w else None for p, w in zip(params, wanted)]
+            fused = (any(wanted) and all(m is not None and m.dtype == wq.dtype for m, w in zip(mains, wanted) if w)
+                     and len({m.data_ptr() for m in mains if m is not None}) == sum(wanted))
+            grads = mains if fused else [torch.empty_like(p) if w else None for p, w in zip(params, wanted)]
+            check(lib().sb200_qk_norm_rope_bwd(
+                dqo.data_ptr(), dko.data_ptr(), q.data_ptr(), k.data_ptr(), wq.data_ptr(), wk.data_ptr(), ptr(pos),
+                dq.data_ptr(), dk.data_ptr(), ptr(grads[0]), ptr(grads[1]), ptr(grads[2]), ptr(grads[3]), ptr(partial),
+                blocks, T, Hq, Hk, D, dqo.stride(0), dqo.stride(1), dko.stride(0), dko.stride(1), q.stride(0),
+                q.stride(1), k.stride(0), k.stride(1), eps, int(rms), rot, base, int(interleaved), int(fused),
+                dt(q.dtype), dt(wq.dtype), stream()), "sb200_qk_norm_rope_bwd")
+        if fused:
+            grads = [None] * 4
+        return (dq, dk, *grads, None, None, None, None, None, None)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                 q_bias: Optional[torch.Tensor] = None, k_bias: Optional[torch.Tensor] = None,
+                 positions: Optional[torch.Tensor] = None, rotary: Optional[tuple[int, float, bool]] = None,
+                 eps: float = 1e-5, rms: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """Per-head norm of queries and keys with the rotary embedding in the same pass: ``q [tokens, heads, d]`` and
+    ``k [tokens, kv_heads, d]`` (any strides) give new contiguous tensors; differentiable in q, k, weights and biases.
+
+    Every head of every token is normalised over its ``d`` elements (``rms``: RMSNorm, else LayerNorm with optional
+    biases), scaled by the weight ``[d]``, and its first ``rotary[0]`` elements are rotated by ``positions[token]``;
+    ``rotary = (rotary dimensions, base, interleaved)`` or None.  Equals ``rope(rms_norm(q, ...), ...)`` up to
+    rounding: the result is rounded once, angles are exact at far positions.  Head sizes up to 256."""
+    for name, x, w, b in (("q", q, q_weight, q_bias), ("k", k, k_weight, k_bias)):
+        if w is None:
+            raise ValueError("qk_norm_rope needs a weight for queries and for keys")
+        check_head_norm(name, x, w, b, rms)
+    if q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.dtype != k.dtype or q.device != k.device:
+        raise ValueError(f"q {tuple(q.shape)} {q.dtype} {q.device} and k {tuple(k.shape)} {k.dtype} {k.device} do not match")
+    rot, base, interleaved = rotary_args(rotary, q.shape[2])
+    if rot and (positions is None or positions.dim() != 1 or positions.shape[0] != q.shape[0]
+                or positions.device != q.device or positions.dtype.is_floating_point):
+        raise ValueError(f"the rotation needs one integer position per token ({q.shape[0]}) on {q.device}")
+    if not q.is_cuda or q.numel() == 0 or k.numel() == 0:
+        return (head_norm_rope_reference(q, q_weight, q_bias, positions, rotary, eps, rms),
+                head_norm_rope_reference(k, k_weight, k_bias, positions, rotary, eps, rms))
+    if q.dtype not in _KERNEL_DTYPES or q.shape[2] > 256:
+        raise _lib.KernelError(f"qk_norm_rope: {q.dtype} with head size {q.shape[2]} is not supported (fp32, bf16, fp16 "
+                               "up to 256)")
+    pos = positions.to(torch.int32).contiguous() if rot else None
+    wq, wk, bq, bk = _common_dtype(q_weight, k_weight, q_bias, k_bias)
+    return _QKNormRopeFn.apply(q, k, wq, wk, bq, bk, pos, rot, base, interleaved, float(eps), bool(rms))
+
+
 # --------------------------------------------------------------------------- masked softmax
 class _MaskedSoftmaxFn(torch.autograd.Function):
     @staticmethod
