@@ -70,6 +70,8 @@ _SIGS = {
     "sb200_qk_norm_rope_bwd_blocks": [c_int, c_int],
     "sb200_qk_norm_rope_bwd": [c_void_p] * 14 + [c_int] * 5 + [c_long] * 8 + [c_float, c_int, c_int, c_double, c_int, c_int, c_int, c_int, c_void_p],
     "sb200_paged_append": [c_void_p] * 14 + [c_int] * 5 + [c_long] * 13 + [c_int] * 3 + [c_float, c_int, c_int, c_double, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
+    "sb200_paged_attention_workspace": [c_int] * 5 + [c_long, c_int],
+    "sb200_paged_attention": [c_void_p] * 8 + [c_long] + [c_int] * 8 + [c_long] * 11 + [c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p],
     "sb200_masked_softmax_fwd": [c_void_p, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_float, c_int, c_void_p],
     "sb200_masked_softmax_bwd": [c_void_p, c_void_p, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_float, c_int, c_void_p],
     "sb200_colsum_splits": [c_long, c_int, c_int, c_int],
@@ -92,6 +94,9 @@ _SIGS = {
     "sb200_gemm_fp8": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_long, c_long, c_long, c_int, c_int, c_int, c_int, c_int, c_void_p, c_long, c_void_p, c_void_p],
     "sb200_gemm": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_long, c_long, c_long, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
 }
+
+
+_RESTYPES = {"sb200_paged_attention_workspace": c_long}
 
 
 def available() -> bool:
@@ -136,7 +141,7 @@ class _Counting:
 
 
 _NO_LAUNCH = {"sb200_p2p_max_ranks", "sb200_colsum_splits", "sb200_norm_bwd_partial_rows", "sb200_norm_bwd_partial_rows_h", "sb200_sumsq_max_partials",
-              "sb200_bind_device", "sb200_fa_last_driver_error", "sb200_qk_norm_rope_bwd_blocks"}
+              "sb200_bind_device", "sb200_fa_last_driver_error", "sb200_qk_norm_rope_bwd_blocks", "sb200_paged_attention_workspace"}
 
 
 def kernel_calls() -> int:
@@ -170,7 +175,7 @@ def lib() -> "_Counting":
             if hasattr(handle, name):
                 fn = getattr(handle, name)
                 fn.argtypes = argtypes
-                fn.restype = c_int
+                fn.restype = _RESTYPES.get(name, c_int)
         _LIB = _Counting(handle)
         return _LIB
 

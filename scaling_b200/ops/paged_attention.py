@@ -14,6 +14,7 @@ The torch expressions, which run on CPU tensors, raise ``ValueError`` at once.
 
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
@@ -142,4 +143,100 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
             k_cache.stride(1), k_cache.stride(2), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2),
             page_table.stride(0), page_table.shape[1], num_pages, page_size, float(eps), int(rms), rot, base,
             int(interleaved), code, w_code, sm_count(), status_word().data_ptr(), stream()), "sb200_paged_append")
+    return out
+
+
+def paged_attention_reference(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                              cu_seqlens: torch.Tensor, seq_lens: torch.Tensor, causal: bool, scale: float,
+                              window: Optional[int], out: torch.Tensor) -> torch.Tensor:
+    """Sequence by sequence in fp32 (fp64 for fp64 inputs); raises on visible pages outside the cache."""
+    size, kv_heads = k_cache.shape[1], k_cache.shape[2]
+    acc = torch.float64 if q.dtype == torch.float64 else torch.float32
+    group = q.shape[1] // kv_heads
+    cu = cu_seqlens.tolist()
+    for b, length in enumerate(seq_lens.tolist()):
+        start, end = min(max(cu[b], 0), q.shape[0]), min(cu[b + 1], q.shape[0])
+        n = end - start
+        if n <= 0:
+            continue
+        if not 0 <= length <= page_table.shape[1] * size:
+            raise ValueError(f"sequence {b} has length {length}, its page table {page_table.shape[1] * size} places")
+        pos = torch.arange(length - n, length, device=q.device)
+        lo = torch.zeros_like(pos) if window is None else (pos - window).clamp_(min=0)
+        hi = pos + 1 if causal else torch.full_like(pos, length)
+        if window is not None and not causal:
+            hi = torch.minimum(hi, pos + window + 1)
+        first, last = int(lo.min()) // size, -(-max(int(hi.max()), 0) // size)
+        pages = page_table[b, first:last].to(torch.int64)
+        if pages.numel() and (int(pages.min()) < 0 or int(pages.max()) >= k_cache.shape[0]):
+            raise ValueError(f"sequence {b} sees a page outside the cache")
+        j = torch.arange(first * size, max(min(last * size, length), first * size), device=q.device)
+        seen = (j[None] >= lo[:, None]) & (j[None] < hi[:, None])  # [n, keys]
+        k, v = (c[pages].reshape(-1, kv_heads, c.shape[3])[:j.numel()].to(acc) for c in (k_cache, v_cache))
+        v = v.masked_fill(~seen.any(0)[:, None, None], 0.0)
+        qs = q[start:end].reshape(n, kv_heads, group, -1).to(acc)
+        s = torch.einsum("nhgd,jhd->hgnj", qs, k).mul_(scale).masked_fill_(~seen, float("-inf"))
+        p = torch.nan_to_num(torch.softmax(s, -1), nan=0.0) if not seen.any(1).all() else torch.softmax(s, -1)
+        out[start:end] = torch.einsum("hgnj,jhd->nhgd", p, v).reshape(n, q.shape[1], -1).to(q.dtype)
+    return out
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    cu_seqlens: torch.Tensor, seq_lens: torch.Tensor, causal: bool = True,
+                    scale: Optional[float] = None, window: Optional[int] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the new tokens ``q [tokens, heads, d]`` of many sequences over their cached keys and values, one token
+    or a long chunk each; returns ``[tokens, heads, d]`` (``out``, if given).
+
+    Heads are a multiple of the cache's KV heads.  A query at position ``i`` of its sequence sees the cached positions
+    ``j <= i`` (all of them without ``causal``) with ``|i - j| <= window``; keys of the new tokens are read from the
+    cache, so they are written first (``paged_append``).  A query that sees nothing gives zeros.  Pages that no query of
+    the call sees may be missing from the table.  Rows behind the last sequence are left as they were in ``out`` and are
+    zero without it.  Whatever the cache holds behind a sequence's last token has no effect; keys and values of its
+    tokens are finite.  On GPUs: bf16 and fp16, head sizes that are multiples of 8 up to 128, pages of 8 tokens and more.
+    In inference only: no backward pass."""
+    _check_cache(k_cache, v_cache, page_table, cu_seqlens, seq_lens)
+    _no_grad_inputs("paged_attention", q, k_cache, v_cache)
+    _check_rows("q", q, k_cache)
+    tokens, heads, d = q.shape
+    num_pages, page_size, kv_heads = k_cache.shape[:3]
+    if kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads are not a multiple of {kv_heads} kv heads")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"the softmax scale must be positive and finite, got {scale}")
+    if window is not None and window < 0:
+        raise ValueError(f"window must not be negative, got {window}")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device):
+        raise ValueError(f"out {tuple(out.shape)} {out.dtype} {out.device} does not match q {tuple(q.shape)} {q.dtype}")
+    if not q.is_cuda:
+        return paged_attention_reference(q, k_cache, v_cache, page_table, cu_seqlens, seq_lens, causal, scale, window,
+                                         torch.zeros_like(q) if out is None else out)
+    if q.dtype not in (torch.bfloat16, torch.float16) or d % 8 or not 8 <= d <= 128 or page_size < 8:
+        raise _lib.KernelError(f"paged_attention: {q.dtype} with head size {d} and pages of {page_size} is not supported "
+                               "(bf16 / fp16, multiples of 8 up to 128, pages of 8 and more)")
+    zero_tail = out is None
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if q.numel() == 0:
+        return out
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("out", out)):
+        if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1]) or t.data_ptr() % 16:
+            raise _lib.KernelError(f"paged_attention: {name} must start and have its rows on 16-byte boundaries, strides "
+                                   f"{t.stride()}")
+    if num_pages == 0:
+        raise ValueError("the cache has no pages")
+    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+    with _lib.on_device_of(q):
+        batch, cols, sms = seq_lens.shape[0], page_table.shape[1], sm_count()
+        size = lib().sb200_paged_attention_workspace(tokens, batch, heads, kv_heads, d, cols * page_size, sms)
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+        check(lib().sb200_paged_attention(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), page_table.data_ptr(),
+            cu_seqlens.data_ptr(), seq_lens.data_ptr(), workspace.data_ptr(), size, tokens, batch, heads, kv_heads, d,
+            num_pages, page_size, cols, page_table.stride(0), q.stride(0), q.stride(1), out.stride(0), out.stride(1),
+            k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), v_cache.stride(0), v_cache.stride(1),
+            v_cache.stride(2), int(causal), -1 if window is None else min(int(window), 2 ** 30), scale, int(zero_tail),
+            dt(q.dtype), sms, status_word().data_ptr(), stream()), "sb200_paged_attention")
     return out

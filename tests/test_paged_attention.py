@@ -1,0 +1,535 @@
+"""Writes into a paged key/value cache and attention over it, against plain evaluations in 64 bits."""
+
+import math
+import random
+
+import pytest
+import torch
+
+from scaling_b200.ops import functional as K
+from scaling_b200.ops._lib import KernelError
+from scaling_b200.ops.paged_attention import paged_append, paged_attention
+from tests.test_qk_norm_rope import FWD_STEPS, _close, _turn, definition
+
+DEV = "cuda"
+
+
+class Batch:
+    """Packed new tokens of several sequences and their pages in a cache (pages in random order, every unused entry of
+    the table -1, every unused element of the caches NaN)."""
+
+    def __init__(self, lens, new, page, kv_heads, dim, dtype, device, heads=None, spare_rows=0, seed=0, fill=float("nan"),
+                 joint=False):
+        rng = random.Random(seed)
+        g = torch.Generator().manual_seed(seed)
+        self.lens, self.new, self.page = list(lens), list(new), page
+        counts = [-(-n // page) for n in self.lens]
+        ids = list(range(sum(counts) + 3))
+        rng.shuffle(ids)
+        cols = max(counts + [1]) + 1
+        table = torch.full((len(self.lens), cols), -1, dtype=torch.int32)
+        at = 0
+        for b, c in enumerate(counts):
+            table[b, :c] = torch.tensor(ids[at:at + c], dtype=torch.int32)
+            at += c
+        self.table_cpu = table
+        self.table = table.to(device)
+        cu = [0]
+        for n in self.new:
+            cu.append(cu[-1] + n)
+        self.cu = torch.tensor(cu, dtype=torch.int32, device=device)
+        self.seq_lens = torch.tensor(self.lens, dtype=torch.int32, device=device)
+        self.tokens = cu[-1]
+        rows = self.tokens + spare_rows
+        shape = (len(ids), page, kv_heads, dim)
+        if joint:  # keys and values of a page side by side in one tensor
+            both = torch.full((len(ids), 2, page, kv_heads, dim), fill, dtype=dtype, device=device)
+            self.k_cache, self.v_cache = both[:, 0], both[:, 1]
+        else:
+            self.k_cache = torch.full(shape, fill, dtype=dtype, device=device)
+            self.v_cache = torch.full(shape, fill, dtype=dtype, device=device)
+        mk = lambda h: torch.randn(rows, h, dim, generator=g).to(dtype).to(device)  # noqa: E731
+        self.q, self.k, self.v = mk(heads or kv_heads), mk(kv_heads), mk(kv_heads)
+
+    def place(self, b, p):
+        return int(self.table_cpu[b, p // self.page]), p % self.page
+
+    def positions(self):
+        return [(b, length - n + i) for b, (n, length) in enumerate(zip(self.new, self.lens)) for i in range(n)]
+
+    def fill_history(self, seed=1, scale=1.0):
+        """Random keys and values at every position of every sequence (the new ones included)."""
+        g = torch.Generator().manual_seed(seed)
+        kc, vc = self.k_cache.cpu(), self.v_cache.cpu()
+        for b, length in enumerate(self.lens):
+            for i in range(-(-length // self.page)):
+                n = min(self.page, length - i * self.page)
+                page = int(self.table_cpu[b, i])
+                kc[page, :n] = (scale * torch.randn(n, *kc.shape[2:], generator=g)).to(kc.dtype)
+                vc[page, :n] = torch.randn(n, *vc.shape[2:], generator=g).to(vc.dtype)
+        self.k_cache.copy_(kc)
+        self.v_cache.copy_(vc)
+
+    def args(self):
+        return self.k_cache, self.v_cache, self.table, self.cu, self.seq_lens
+
+
+APPENDS = [
+    # lens, new, page, heads, kv_heads, dim, rotary, norm
+    ([5], [1], 16, 4, 4, 64, (64, 10000.0, False), "rms"),
+    ([17, 3, 40], [1, 1, 1], 16, 8, 2, 128, (128, 10000.0, True), "rms"),
+    ([30, 16, 0, 9], [30, 7, 0, 2], 8, 3, 1, 80, (20, 10000.0, False), "layer"),
+    ([300, 1], [123, 1], 64, 4, 2, 64, (32, 500000.0, False), "none"),
+    ([64, 65], [64, 65], 32, 2, 2, 50, None, "layer"),
+    ([70, 80], [9, 80], 128, 5, 5, 32, None, "none"),
+]
+
+
+def _append_case(lens, new, page, heads, kv_heads, dim, rotary, norm, dtype, device, joint=False, spare=0):
+    b = Batch(lens, new, page, kv_heads, dim, dtype, device, heads=heads, spare_rows=spare, joint=joint)
+    g = torch.Generator().manual_seed(7)
+    w = lambda base: (base + 0.2 * torch.randn(dim, generator=g)).to(dtype).to(device)  # noqa: E731
+    kw = {}
+    if norm != "none":
+        kw.update(q_weight=w(1.0), k_weight=w(1.0))
+    if norm == "layer":
+        kw.update(q_bias=w(0.0), k_bias=w(0.0))
+    q = paged_append(b.k, b.v, *b.args(), q=b.q, rotary=rotary, rms=norm == "rms", **kw)
+    return b, q, kw
+
+
+def _check_append(b, q, kw, rotary, norm):
+    pos = torch.tensor([p for _, p in b.positions()], dtype=torch.int64, device=q.device)
+
+    def want(x, w, bias):
+        x = x[:b.tokens]
+        if norm == "none":
+            return _turn(x.double(), pos, rotary, 1.0), x.double().abs().amax(-1, keepdim=True)
+        return definition(x, w, bias, pos, rotary, 1e-5, norm == "rms")
+
+    wq, size = want(b.q, kw.get("q_weight"), kw.get("q_bias"))
+    _close(q[:b.tokens], wq, size, FWD_STEPS, "q")
+    assert torch.count_nonzero(q[b.tokens:]) == 0
+    wk, size = want(b.k, kw.get("k_weight"), kw.get("k_bias"))
+    touched = torch.zeros(b.k_cache.shape[:2], dtype=torch.bool, device=q.device)
+    places = [b.place(*p) for p in b.positions()]
+    page = torch.tensor([x for x, _ in places], dtype=torch.int64, device=q.device)
+    slot = torch.tensor([y for _, y in places], dtype=torch.int64, device=q.device)
+    touched[page, slot] = True
+    _close(b.k_cache[page, slot], wk, size, FWD_STEPS, "k")
+    if rotary is None and norm == "none":
+        assert torch.equal(b.k_cache[page, slot], b.k[:b.tokens]) and torch.equal(q[:b.tokens], b.q[:b.tokens])
+    assert torch.equal(b.v_cache[page, slot], b.v[:b.tokens])
+    for c in (b.k_cache, b.v_cache):  # everything else keeps what it held
+        assert torch.isnan(c[~touched]).all()
+
+
+@pytest.mark.parametrize("lens,new,page,heads,kv_heads,dim,rotary,norm", APPENDS)
+def test_append_torch_expression(lens, new, page, heads, kv_heads, dim, rotary, norm):
+    b, q, kw = _append_case(lens, new, page, heads, kv_heads, dim, rotary, norm, torch.float32, "cpu", spare=3)
+    _check_append(b, q, kw, rotary, norm)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("joint", [False, True])
+@pytest.mark.parametrize("lens,new,page,heads,kv_heads,dim,rotary,norm", APPENDS)
+def test_append_kernel(lens, new, page, heads, kv_heads, dim, rotary, norm, joint, dtype):
+    b, q, kw = _append_case(lens, new, page, heads, kv_heads, dim, rotary, norm, dtype, DEV, joint=joint, spare=3)
+    _check_append(b, q, kw, rotary, norm)
+    K.check_status()
+
+
+def _append_refused(device):
+    b = Batch([20, 5], [4, 1], 16, 2, 64, torch.float32, device, heads=4)
+    ok = lambda **kw: {**dict(q=b.q, rotary=(64, 10000.0, False)), **kw}  # noqa: E731
+    w = torch.ones(64, device=device)
+    paged_append(b.k, b.v, *b.args(), **ok())
+    kc, vc, table, cu, sl = b.args()
+    bad = [
+        lambda: paged_append(b.k, b.v[:4], *b.args(), **ok()),
+        lambda: paged_append(b.k[:, :1], b.v[:, :1], *b.args(), **ok()),
+        lambda: paged_append(b.k.bfloat16(), b.v, *b.args(), **ok()),
+        lambda: paged_append(b.k[..., :32], b.v, *b.args(), **ok()),
+        lambda: paged_append(b.k, b.v, kc, vc[:, :8], table, cu, sl, **ok()),
+        lambda: paged_append(b.k, b.v, kc[:, :12], vc[:, :12], table, cu, sl, **ok()),      # page size 12
+        lambda: paged_append(b.k, b.v, kc, vc, table.long(), cu, sl, **ok()),
+        lambda: paged_append(b.k, b.v, kc, vc, table, cu[:2], sl, **ok()),
+        lambda: paged_append(b.k, b.v, kc, vc, table[:1], cu, sl, **ok()),
+        lambda: paged_append(b.k, b.v, kc, vc, table.t(), cu, sl, **ok()),
+        lambda: paged_append(b.k, b.v, *b.args(), **ok(q=b.q[:3])),
+        lambda: paged_append(b.k, b.v, *b.args(), q=None, q_weight=w),
+        lambda: paged_append(b.k, b.v, *b.args(), **ok(k_bias=w)),
+        lambda: paged_append(b.k, b.v, *b.args(), **ok(rotary=(66, 10000.0, False))),
+        lambda: paged_append(b.k, b.v, *b.args(), **ok(positions=torch.zeros(4, dtype=torch.int32, device=device))),
+        lambda: paged_append(b.k, b.v, *b.args(), **ok(positions=torch.zeros(5, device=device))),
+    ]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(KernelError):
+        paged_append(b.k.requires_grad_(), b.v, *b.args(), **ok())
+    with torch.no_grad():
+        paged_append(b.k, b.v, *b.args(), **ok())
+
+
+def test_append_refusals():
+    _append_refused("cpu")
+
+
+def _bad_places(b):
+    """(what is wrong, table, cu, seq_lens) of calls that name a place outside the cache or the table."""
+    kc, _, table, cu, sl = b.args()
+    for bad_id in (-1, kc.shape[0], 2 ** 31 - 1, -2 ** 31):
+        t = table.clone()
+        t[0, 1] = bad_id
+        yield f"page {bad_id}", t, cu, sl
+    for length in (2, 10 ** 6, -3):  # fewer than the new tokens, beyond the table, negative
+        s = sl.clone()
+        s[0] = length
+        yield f"length {length}", table, cu, s
+
+
+def test_append_bad_places_on_the_cpu():
+    b = Batch([20, 5], [6, 1], 16, 2, 64, torch.float32, "cpu")
+    for what, table, cu, sl in _bad_places(b):
+        with pytest.raises(ValueError):
+            paged_append(b.k, b.v, b.k_cache, b.v_cache, table, cu, sl)
+
+
+@pytest.mark.gpu
+def test_append_bad_places_are_reported_and_touch_nothing_else():
+    for i in range(7):
+        b = Batch([20, 5], [6, 1], 16, 2, 64, torch.float32, DEV)
+        what, table, cu, sl = list(_bad_places(b))[i]
+        paged_append(b.k, b.v, b.k_cache, b.v_cache, table, cu, sl)
+        with pytest.raises(KernelError):
+            K.check_status()
+        K.check_status()  # the error is reported once
+        page, slot = b.place(1, 4)
+        assert torch.equal(b.k_cache[page, slot], b.k[6]) and torch.equal(b.v_cache[page, slot], b.v[6]), what
+        written = (~torch.isnan(b.k_cache[..., 0, 0])).sum().item()
+        # the rows of the first sequence that have a place: positions 14, 15 lie in the good page, 16 .. 19 in the bad one;
+        # with a length of 2 only the last two of its six new tokens have a position
+        assert written == (1 + 2 if what.startswith("page") or what == "length 2" else 1), what
+
+
+@pytest.mark.gpu
+def test_append_captured_into_a_graph_follows_new_lengths():
+    b = Batch([100, 50], [1, 1], 16, 2, 64, torch.bfloat16, DEV, heads=4)
+    w = torch.ones(64, dtype=torch.bfloat16, device=DEV)
+    b.seq_lens.copy_(torch.tensor([98, 48]))
+    K.check_status()
+    paged_append(b.k, b.v, *b.args(), q=b.q, q_weight=w, k_weight=w, rotary=(64, 10000.0, False))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q = paged_append(b.k, b.v, *b.args(), q=b.q, q_weight=w, k_weight=w, rotary=(64, 10000.0, False))
+    for step in (99, 100):
+        b.seq_lens.copy_(torch.tensor([step, step - 50]))
+        graph.replay()
+        eager = paged_append(b.k, b.v, *b.args(), q=b.q, q_weight=w, k_weight=w, rotary=(64, 10000.0, False))
+        assert torch.equal(q, eager)
+    for pos in (97, 98, 99):
+        page, slot = b.place(0, pos)
+        assert torch.equal(b.v_cache[page, slot], b.v[0])
+
+
+# ------------------------------------------------------------------------------------------------ attention
+def attention_in_64_bits(b, causal, scale, window, q=None):
+    """(out, bound): the definition key by key, and the error that the kernel's roundings may leave.
+
+    Per probability: half a step of the 16-bit type (relative), the score's fp32 error - a chain of D products and sums,
+    taken with full steps for a tensor core that truncates, times the scale - and 2^-21 for the argument and the
+    exponential, twice because it enters sum and quotient; a chain of as many fp32 additions as there are keys; the output
+    is rounded once."""
+    q = b.q if q is None else q
+    kv, d = b.k_cache.shape[2], b.k_cache.shape[3]
+    group = q.shape[1] // kv
+    half = torch.finfo(q.dtype).eps / 2
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    bound = torch.zeros_like(out)
+    at = 0
+    for s, (n, length) in enumerate(zip(b.new, b.lens)):
+        places = [b.place(s, j) for j in range(length)]
+        page = torch.tensor([x for x, _ in places], dtype=torch.int64, device=q.device)
+        slot = torch.tensor([y for _, y in places], dtype=torch.int64, device=q.device)
+        for i in range(n):
+            pos = length - n + i
+            lo = 0 if window is None else max(0, pos - window)
+            hi = pos + 1 if causal else (length if window is None else min(length, pos + window + 1))
+            if hi <= lo:
+                continue
+            k = b.k_cache[page[lo:hi], slot[lo:hi]].double()
+            v = b.v_cache[page[lo:hi], slot[lo:hi]].double()
+            qi = q[at + i].double().view(kv, group, d)
+            z = torch.einsum("hgd,jhd->hgj", qi, k) * scale
+            size = torch.einsum("hgd,jhd->hgj", qi.abs(), k.abs()).amax(-1, keepdim=True) * scale
+            prob = torch.softmax(z, -1)
+            out[at + i] = torch.einsum("hgj,jhd->hgd", prob, v).reshape(-1, d)
+            w = torch.einsum("hgj,jhd->hgd", prob, v.abs())
+            rel = half + 2 * (size * (d + 8) * 2.0 ** -23 + 2.0 ** -21) + (hi - lo) * 2.0 ** -23
+            bound[at + i] = (rel * w).reshape(-1, d)
+        at += n
+    return out, bound + half * (out.abs() + bound) + half * torch.finfo(q.dtype).tiny
+
+
+ATTENDS = [
+    # lens, new, page, heads, kv_heads, dim, window, causal
+    ([1], [1], 16, 1, 1, 64, None, True),
+    ([5], [1], 16, 4, 4, 64, None, True),
+    ([300], [1], 16, 12, 12, 64, None, True),
+    ([127, 128, 129, 255, 257], [1] * 5, 16, 8, 2, 128, None, True),
+    ([700, 3, 1500], [1, 1, 1], 64, 40, 1, 128, None, True),
+    ([3000], [1], 8, 71, 1, 64, None, True),
+    ([4100, 17], [2, 1], 128, 4, 2, 128, None, True),
+    ([130, 64], [130, 64], 32, 6, 2, 64, None, True),          # whole prompts, group 3
+    ([300, 333], [260, 129], 16, 4, 4, 128, None, True),       # chunks that end inside a 128-row tile
+    ([600], [300], 256, 8, 8, 32, None, True),
+    ([90, 0, 200, 40], [1, 0, 100, 0], 16, 9, 3, 96, None, True),   # sequences without new tokens, one without any
+    ([250, 100], [70, 100], 16, 4, 2, 80, None, False),
+    ([400, 1000], [200, 1], 32, 4, 2, 64, 100, True),
+    ([400, 1000], [200, 3], 32, 2, 2, 128, 0, True),           # a window of the token itself
+    ([500], [130], 16, 4, 1, 8, 37, False),
+    ([2, 300], [5, 9], 16, 4, 2, 64, None, True),              # more new tokens than the length: rows that see nothing
+    ([257] * 40, [1] * 40, 16, 4, 4, 64, None, True),          # more sequences than a warp has lanes
+]
+
+
+def _attend_batch(lens, new, page, heads, kv_heads, dim, dtype, device, **kw):
+    b = Batch(lens, new, page, kv_heads, dim, dtype, device, heads=heads, **kw)
+    b.fill_history()
+    b.q = (1.5 * b.q.float()).to(dtype)
+    return b
+
+
+def _check_attention(b, out, causal, window, scale=None):
+    scale = 1.0 / math.sqrt(b.q.shape[2]) if scale is None else scale
+    want, bound = attention_in_64_bits(b, causal, scale, window)
+    assert torch.isfinite(out).all()
+    err = (out.double() - want).abs()
+    assert (err <= bound).all(), f"{(err / bound.clamp(min=1e-300)).max().item():.3g} of the bound"
+
+
+@pytest.mark.parametrize("lens,new,page,heads,kv_heads,dim,window,causal", ATTENDS)
+def test_attention_torch_expression(lens, new, page, heads, kv_heads, dim, window, causal):
+    b = _attend_batch(lens, new, page, heads, kv_heads, dim, torch.float64, "cpu", spare_rows=2)
+    out = paged_attention(b.q, *b.args(), causal=causal, window=window)
+    want, _ = attention_in_64_bits(b, causal, 1.0 / math.sqrt(dim), window)
+    assert torch.allclose(out, want, rtol=1e-9, atol=1e-9)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,new,page,heads,kv_heads,dim,window,causal", ATTENDS)
+def test_attention_kernel(lens, new, page, heads, kv_heads, dim, window, causal, dtype):
+    b = _attend_batch(lens, new, page, heads, kv_heads, dim, dtype, DEV, spare_rows=2)
+    out = paged_attention(b.q, *b.args(), causal=causal, window=window)
+    K.check_status()
+    _check_attention(b, out, causal, window)
+    again = paged_attention(b.q, *b.args(), causal=causal, window=window)
+    assert torch.equal(out, again)
+
+
+def _attention_refused(device, dtype):
+    b = _attend_batch([20, 5], [4, 1], 16, 4, 2, 64, dtype, device)
+    paged_attention(b.q, *b.args())
+    kc, vc, table, cu, sl = b.args()
+    bad = [
+        lambda: paged_attention(b.q[:, :3], *b.args()),
+        lambda: paged_attention(b.q[..., :32], *b.args()),
+        lambda: paged_attention(b.q.double().float(), kc.double(), vc.double(), table, cu, sl),
+        lambda: paged_attention(b.q, kc, vc[:, :8], table, cu, sl),
+        lambda: paged_attention(b.q, kc[:, :12], vc[:, :12], table, cu, sl),
+        lambda: paged_attention(b.q, kc, vc, table.long(), cu, sl),
+        lambda: paged_attention(b.q, kc, vc, table, cu[:2], sl),
+        lambda: paged_attention(b.q, *b.args(), scale=0.0),
+        lambda: paged_attention(b.q, *b.args(), scale=float("nan")),
+        lambda: paged_attention(b.q, *b.args(), scale=-1.0),
+        lambda: paged_attention(b.q, *b.args(), window=-2),
+        lambda: paged_attention(b.q, *b.args(), out=b.q[:3]),
+        lambda: paged_attention(b.q, *b.args(), out=b.q.double()),
+    ]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(KernelError):
+        paged_attention(b.q.requires_grad_(), *b.args())
+    with torch.no_grad():
+        paged_attention(b.q, *b.args())
+
+
+def test_attention_refusals():
+    _attention_refused("cpu", torch.float32)
+
+
+@pytest.mark.gpu
+def test_attention_gpu_refusals():
+    _attention_refused(DEV, torch.bfloat16)
+    for dtype, page, dim in ((torch.float32, 16, 64), (torch.bfloat16, 4, 64), (torch.bfloat16, 16, 68), (torch.bfloat16, 16, 136)):
+        b = Batch([20], [1], page, 1, dim, dtype, DEV)
+        with pytest.raises(KernelError):
+            paged_attention(b.q, *b.args())
+    b = Batch([20], [1], 16, 1, 64, torch.bfloat16, DEV)
+    wide = torch.zeros(*b.k_cache.shape[:3], 65, dtype=torch.bfloat16, device=DEV)[..., :64]
+    with pytest.raises(KernelError):
+        paged_attention(b.q, wide, b.v_cache, b.table, b.cu, b.seq_lens)
+
+
+def test_attention_bad_pages_on_the_cpu():
+    b = _attend_batch([20, 5], [6, 1], 16, 2, 2, 64, torch.float32, "cpu")
+    kc, vc, table, cu, sl = b.args()
+    for bad in (-1, kc.shape[0]):
+        t = table.clone()
+        t[0, 0] = bad
+        with pytest.raises(ValueError):
+            paged_attention(b.q, kc, vc, t, cu, sl)
+    s = sl.clone()
+    s[1] = 10 ** 6
+    with pytest.raises(ValueError):
+        paged_attention(b.q, kc, vc, table, cu, s)
+
+
+@pytest.mark.gpu
+def test_attention_bad_pages_are_reported_and_leave_other_sequences_alone():
+    b = _attend_batch([200, 150], [6, 3], 16, 4, 2, 64, torch.bfloat16, DEV)
+    good = paged_attention(b.q, *b.args())
+    K.check_status()
+    kc, vc, table, cu, sl = b.args()
+    for bad in (-1, kc.shape[0], 2 ** 31 - 1, -2 ** 31):
+        t = table.clone()
+        t[0, 3] = bad
+        out = paged_attention(b.q, kc, vc, t, cu, sl)
+        with pytest.raises(KernelError):
+            K.check_status()
+        assert torch.equal(out[6:], good[6:])
+        # the same entry outside every query's window is not looked at
+        near = paged_attention(b.q, kc, vc, t, cu, sl, window=90)
+        K.check_status()
+        assert torch.equal(near, paged_attention(b.q, kc, vc, table, cu, sl, window=90))
+    for length in (10 ** 6, -4):
+        s = sl.clone()
+        s[0] = length
+        out = paged_attention(b.q, kc, vc, table, cu, s)
+        with pytest.raises(KernelError):
+            K.check_status()
+        want, bound = attention_in_64_bits(b, True, 0.125, None)  # another length: the work is cut at other places
+        assert ((out.double() - want).abs() <= bound)[6:9].all()
+
+
+@pytest.mark.gpu
+def test_rows_behind_the_last_sequence_and_given_outputs():
+    b = _attend_batch([50, 300], [3, 140], 16, 4, 2, 64, torch.float16, DEV, spare_rows=5)
+    plain = paged_attention(b.q, *b.args())
+    assert torch.count_nonzero(plain[b.tokens:]) == 0
+    wide = torch.full((b.q.shape[0], 6, 72), 7.0, dtype=torch.float16, device=DEV)
+    out = paged_attention(b.q, *b.args(), out=wide[:, 1:5, :64])
+    assert out.data_ptr() == wide[:, 1:5].data_ptr()
+    assert torch.equal(out[:b.tokens], plain[:b.tokens])
+    assert (wide[b.tokens:] == 7).all() and (wide[:, 0] == 7).all() and (wide[:, 5] == 7).all() and (wide[..., 64:] == 7).all()
+    # no sequence at all
+    none = paged_attention(b.q, b.k_cache, b.v_cache, b.table[:0], b.cu[:1], b.seq_lens[:0])
+    assert torch.count_nonzero(none) == 0
+    K.check_status()
+
+
+@pytest.mark.gpu
+def test_views_joint_caches_and_odd_query_strides():
+    b = _attend_batch([90, 700], [1, 33], 32, 8, 2, 64, torch.bfloat16, DEV, joint=True)
+    _check_attention(b, paged_attention(b.q, *b.args()), True, None)
+    want = paged_attention(b.q, *b.args())
+    odd = torch.zeros(b.q.shape[0], 8, 67, dtype=torch.bfloat16, device=DEV)
+    odd[..., 3:] = b.q
+    assert torch.equal(paged_attention(odd[..., 3:], *b.args()), want)
+    turned = b.q.permute(1, 0, 2).contiguous().permute(1, 0, 2)
+    assert torch.equal(paged_attention(turned, *b.args()), want)
+
+
+@pytest.mark.gpu
+def test_scores_far_apart_and_growing():
+    """Scores of hundreds, growing along the sequence, so that the running reference moves at every tile."""
+    for sign in (1.0, -1.0):
+        b = _attend_batch([1500, 900], [200, 1], 16, 4, 2, 128, torch.bfloat16, DEV)
+        for s, length in enumerate(b.lens):
+            for j in range(length):
+                page, slot = b.place(s, j)
+                b.k_cache[page, slot] = sign * (j / 40.0) / 16.0
+        b.q.fill_(1.0)
+        out = paged_attention(b.q, *b.args(), scale=1.0)
+        _check_attention(b, out, True, None, scale=1.0)
+
+
+@pytest.mark.gpu
+def test_attention_captured_into_a_graph_follows_lengths_tables_and_queries():
+    b = _attend_batch([2000, 333, 80], [1, 1, 1], 16, 8, 2, 128, torch.bfloat16, DEV)
+    args = b.args()
+    paged_attention(b.q, *args)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(paged_attention(b.q, *args))
+        graphs.append(g)
+    side = torch.cuda.Stream()
+    for lens in ([2000, 333, 80], [17, 1, 64], [1999, 332, 79]):
+        b.seq_lens.copy_(torch.tensor(lens))
+        b.q.mul_(0.9)
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        with torch.cuda.stream(side):  # two calls at once: each graph has a workspace of its own
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        eager = paged_attention(b.q, *args)
+        assert torch.equal(outs[0], eager) and torch.equal(outs[1], eager)
+
+
+@pytest.mark.gpu
+def test_cache_offsets_beyond_32_bits():
+    pages = 2 ** 31 // (64 * 2 * 128) + 40  # the last pages start past 2^31 elements
+    kc = torch.zeros(pages, 64, 2, 128, dtype=torch.bfloat16, device=DEV)
+    vc = torch.zeros_like(kc)
+    b = Batch([150], [3], 64, 2, 128, torch.bfloat16, DEV, heads=4)
+    last = torch.tensor([[pages - 1, pages - 5, pages - 2]], dtype=torch.int32, device=DEV)
+    b.table, b.table_cpu, b.k_cache, b.v_cache = last, last.cpu(), kc, vc
+    g = torch.Generator().manual_seed(3)
+    for j in last[0].tolist():
+        kc[j] = torch.randn(64, 2, 128, generator=g)
+        vc[j] = torch.randn(64, 2, 128, generator=g)
+    w = torch.ones(128, dtype=torch.bfloat16, device=DEV)
+    q = paged_append(b.k, b.v, *b.args(), q=b.q, q_weight=w, k_weight=w, rotary=(128, 10000.0, False))
+    page, slot = b.place(0, 149)
+    assert torch.equal(vc[page, slot], b.v[2])
+    b.q = q
+    _check_attention(b, paged_attention(q, *b.args()), True, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,heads,kv_heads,window", [(64, 12, 12, None), (128, 8, 2, None), (64, 8, 1, 60)])
+def test_prompt_in_chunks_then_tokens_equals_one_pass(dim, heads, kv_heads, window):
+    """Append and attend chunk by chunk and token by token, against the whole sequence at once in 64 bits."""
+    dtype, page, total = torch.bfloat16, 16, 400
+    g = torch.Generator().manual_seed(5)
+    lens = [total, 290]
+    x = [[torch.randn(n, h, dim, generator=g).to(dtype).to(DEV) for h in (heads, kv_heads, kv_heads)] for n in lens]
+    wq, wk = ((1 + 0.2 * torch.randn(dim, generator=g)).to(dtype).to(DEV) for _ in range(2))
+    whole = Batch(lens, lens, page, kv_heads, dim, dtype, DEV, heads=heads)
+    rotary = (dim, 10000.0, False)
+    outs = [[], []]
+    done = [0, 0]
+    for chunk in (250, 39, 1, 1, 109):
+        new = [min(chunk, n - d) for n, d in zip(lens, done)]
+        starts = list(done)
+        done = [d + n for d, n in zip(done, new)]
+        cu = torch.tensor([0, new[0], sum(new)], dtype=torch.int32, device=DEV)
+        sl = torch.tensor(done, dtype=torch.int32, device=DEV)
+        q, k, v = (torch.cat([x[s][c][starts[s]:done[s]] for s in range(2)]) for c in range(3))
+        q = paged_append(k, v, whole.k_cache, whole.v_cache, whole.table, cu, sl, q=q, q_weight=wq, k_weight=wk, rotary=rotary)
+        o = paged_attention(q, whole.k_cache, whole.v_cache, whole.table, cu, sl, window=window)
+        outs[0].append(o[:new[0]])
+        outs[1].append(o[new[0]:])
+    K.check_status()
+    pos = torch.cat([torch.arange(n, device=DEV) for n in lens])
+    qn, _ = K.qk_norm_rope(torch.cat([x[0][0], x[1][0]]), torch.cat([x[0][1], x[1][1]]), wq, wk, positions=pos, rotary=rotary)
+    whole.q = qn
+    _check_attention(whole, torch.cat(outs[0] + outs[1]), True, window)
