@@ -20,7 +20,8 @@
 //  * S of a group takes 128 TMEM columns; its probabilities overwrite the first 64 as packed 16-bit values and are
 //    the TMEM operand of O += P V.  O stays in TMEM over the whole item.
 //  * K and V tiles come by TMA through a ring that does not know items: the loader runs ahead into the next ones.
-// Warp roles: 0-3 and 4-7 softmax groups, 8 TMA loader, 9 MMA issuer, 10 scheduler, which also copies the queries.
+// Warp roles: 0-3 and 4-7 softmax groups, 8 and 11 TMA loaders of K and of V (a page of 16 tokens is a copy of its own, and
+// one warp alone issues them no faster than the memory delivers), 9 MMA issuer, 10 scheduler, which also copies the queries.
 //
 // Rounding: scores, sums and outputs are fp32; P is rounded to the 16-bit element type for the second product (half a
 // step per probability, averaged over the row), the output once.
@@ -32,8 +33,10 @@ namespace {
 
 constexpr int PA_TILE = 128;
 constexpr int PA_ITEM_ROWS = 256;
-constexpr int PA_WARPS = 11;
+constexpr int PA_WARPS = 12;
 constexpr int PA_THREADS = PA_WARPS * 32;
+// registers per thread after the roles part: 128 x 80 + 256 x 208 = 63488 of the 384 x 168 that the launch holds
+constexpr int PA_REGS_FEW = 80, PA_REGS_MANY = 208;
 constexpr int PA_PANEL = 16384;   // 128 rows x 128 bytes
 constexpr int PA_ITEMS = 4;       // descriptors in flight
 constexpr int PA_COMBINE_THREADS = 256;
@@ -46,6 +49,12 @@ struct PaParams {
   const int* lens;
   long table_ld, q_tok, q_head, o_tok, o_head;
   int T, batch, Hkv, group, D, cols, num_pages, page_shift;
+  uint32_t group_inv;  // floor(2^32 / group) + 1 (group > 1): (n * group_inv) >> 32 = n / group for n < 2^32 / group
+  // layout of a K or V tile in shared memory: 8-row groups of 128-byte rows, `group_step` bytes apart, the second 64
+  // columns `panel_step` bytes behind the first.  boxes: copies per page (1: both panels at once); page_groups8: 8-row
+  // groups of the tensor maps from one page to the next, and outside: a group beyond the cache
+  uint32_t group_step, panel_step;
+  int boxes, k_page8, v_page8, k_outside, v_outside;
   int causal, window;  // window < 0: unlimited
   float sl2;
   float* part_o;       // [2 slots per CTA][part_rows][DP]
@@ -57,12 +66,12 @@ struct PaParams {
 
 // One descriptor of the scheduler's ring.
 struct PaItem {
-  int row0, n, L;    // first packed row, new tokens, total tokens of the sequence
-  int seq, hk, m;    // sequence, KV head, item of 256 rows inside the sequence
+  int row0, pos0;    // packed row and position of the item's first token
+  int L, seq, hk;    // total tokens, sequence, KV head
+  int rows, rem;     // query rows; the first one is head `rem` of the group
   int tile0, count;  // first key tile and number of key tiles (0: the end)
   int lo, hi;        // keys that some row of the item sees
   int slot;          // partial slot, or -1: the item is complete
-  int pad;
 };
 
 template <int PANELS> struct PaCfg {
@@ -87,10 +96,11 @@ template <bool F16> __device__ __forceinline__ uint32_t pa_pack(float a, float b
     return *reinterpret_cast<uint32_t*>(&t);
   }
 }
-__device__ __forceinline__ void pa_tma_4d(void* dst, const void* tmap, uint64_t* bar, int x, int y, int z, int w) {
+__device__ __forceinline__ void pa_tma_5d(uint32_t dst, const void* tmap, uint64_t* bar, int x, int group8, int head) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-      ::"r"(sb::smem_u32(dst)), "l"(tmap), "r"(sb::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(tmap), "r"(sb::smem_u32(bar)), "r"(x), "r"(0), "r"(group8), "r"(head)
       : "memory");
 }
 // Bounded wait of a whole warp: every lane gets the same answer, also when the wait gives up, so that no lane is missing
@@ -98,16 +108,44 @@ __device__ __forceinline__ void pa_tma_4d(void* dst, const void* tmap, uint64_t*
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   return __all_sync(0xffffffffu, sb::mbar_wait(bar, parity, abort_flag));
 }
-// D[tmem] (+)= A[tmem] * B[smem]: A holds two 16-bit values of a row per 32-bit column
-__device__ __forceinline__ void pa_umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// tcgen05 instructions of one elected lane, predicated instead of branched around: the warp stays converged, so that
+// descriptors and addresses, which are the same in all lanes, live in uniform registers.
+// D[tmem] (+)= A[smem] * B[smem]
+__device__ __forceinline__ void pa_umma_ss(uint32_t leader, uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accumulate) {
   asm volatile(
       "{\n"
-      ".reg .pred p;\n"
+      ".reg .pred p, q;\n"
       "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
-      "}\n" ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
 }
+// D[tmem] (+)= A[tmem] * B[smem]: A holds two 16-bit values of a row per 32-bit column
+__device__ __forceinline__ void pa_umma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "setp.ne.b32 q, %5, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n" ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+// the barrier is reached once all MMAs issued so far by the leader are complete
+__device__ __forceinline__ void pa_commit(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n"
+      ".reg .pred q;\n"
+      "setp.ne.b32 q, %1, 0;\n"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+      "}\n" ::"r"(sb::smem_u32(bar)), "r"(leader)
+      : "memory");
+}
+template <int N> __device__ __forceinline__ void pa_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void pa_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void pa_tmem_st32(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -140,6 +178,8 @@ __device__ __forceinline__ PaSeq pa_seq(const PaParams& p, int b) {
   s.L = L;
   return s;
 }
+// n / group for n < group + 256
+__device__ __forceinline__ int pa_div(const PaParams& p, int n) { return p.group == 1 ? n : (int)__umulhi(n, p.group_inv); }
 // keys that some row of item m sees
 __device__ __forceinline__ void pa_item_keys(const PaParams& p, int n, int L, int m, int& lo, int& hi) {
   const int rows = n * p.group;
@@ -158,89 +198,108 @@ __device__ __forceinline__ int pa_item_tiles(const PaParams& p, int n, int L, in
 __device__ __forceinline__ int pa_items(const PaParams& p, int n) {
   return (n * p.group + PA_ITEM_ROWS - 1) / PA_ITEM_ROWS;
 }
-__device__ __forceinline__ long long pa_scan(long long v, int lane) {
+__device__ __forceinline__ int pa_scan(int v, int lane) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long t = __shfl_up_sync(0xffffffffu, v, o);
+    const int t = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += t;
   }
   return v;
 }
+__device__ __forceinline__ int pa_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
 // Tiles of all items of one KV head of sequence 32 * chunk + lane (0 beyond the last sequence); the whole warp calls.
-__device__ __forceinline__ long long pa_chunk_tiles(const PaParams& p, int chunk, int lane, PaSeq& s) {
+__device__ __forceinline__ int pa_chunk_tiles(const PaParams& p, int chunk, int lane, PaSeq& s) {
   const int b = chunk * 32 + lane;
   s = PaSeq{0, 0, 0};
   if (b < p.batch) s = pa_seq(p, b);
   const int items = pa_items(p, s.n);
-  long long tiles = items == 1 ? pa_item_tiles(p, s.n, s.L, 0) : 0;
+  int tiles = items == 1 ? pa_item_tiles(p, s.n, s.L, 0) : 0;
   unsigned many = __ballot_sync(0xffffffffu, items > 1);
   while (many) {  // long chunks: the warp shares the items of one sequence
     const int src = __ffs(many) - 1;
     many &= many - 1;
     const int n = __shfl_sync(0xffffffffu, s.n, src), L = __shfl_sync(0xffffffffu, s.L, src);
     const int cnt = pa_items(p, n);
-    long long sum = 0;
+    int sum = 0;
     for (int m = lane; m < cnt; m += 32) sum += pa_item_tiles(p, n, L, m);
-    sum = __shfl_sync(0xffffffffu, pa_scan(sum, lane), 31);
+    sum = pa_sum(sum);
     if (lane == src) tiles = sum;
   }
   return tiles;
 }
 
-struct PaCursor {      // where a CTA's piece of the line starts, and how long it is
-  int seq, hk, m, tile;
-  long long left, u0, total;
-  int ctas;
+// The line of `total` tiles is cut into `ctas` pieces of `per` tiles, the first `rest` of them one longer.
+struct PaCut {
+  int total, ctas, per, rest;
+  __device__ __forceinline__ int start(int c) const { return c * per + min(c, rest); }
+  __device__ __forceinline__ int owner(int tile) const {
+    const int longer = rest * (per + 1);
+    return tile < longer ? tile / (per + 1) : rest + (tile - longer) / per;
+  }
+};
+struct PaCursor {  // where a CTA's piece of the line starts, and how long it is
+  PaSeq s;
+  int seq, hk, m, tile, left, unit;
+  PaCut cut;
 };
 
 // The whole warp; sums[c] = tiles per KV head of sequences 32 c .. 32 c + 31.
-__device__ __forceinline__ void pa_find(const PaParams& p, const long long* sums, int chunks, int lane, PaCursor& c) {
-  long long total = 0;
-  for (int i = lane; i < chunks; i += 32) total += sums[i];
-  total = __shfl_sync(0xffffffffu, pa_scan(total, lane), 31) * p.Hkv;
-  c.total = total;
-  c.ctas = (int)min((long long)gridDim.x, (total + 1) / 2);  // two tiles per CTA at least: one for each softmax group
-  c.left = 0;
-  c.u0 = 0;
-  c.seq = c.hk = c.m = c.tile = 0;
-  if ((int)blockIdx.x >= c.ctas) return;
-  c.u0 = total * blockIdx.x / c.ctas;
-  c.left = total * (blockIdx.x + 1) / c.ctas - c.u0;
-  long long off = c.u0;
-  int chunk = 0;
-  for (int base = 0; base < chunks; base += 32) {
-    const long long v = base + lane < chunks ? sums[base + lane] * p.Hkv : 0;
-    const long long inc = pa_scan(v, lane);
-    const unsigned hit = __ballot_sync(0xffffffffu, inc > off);
-    if (hit) {
-      const int k = __ffs(hit) - 1;
-      chunk = base + k;
-      off -= __shfl_sync(0xffffffffu, inc - v, k);
-      break;
+__device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int chunks, int lane, PaCursor& c) {
+  long long all = 0;
+  for (int i = lane; i < chunks; i += 32) all += sums[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  all *= p.Hkv;
+  c = PaCursor{};
+  if (all > 0x7fffffff) {  // months of work
+    if (lane == 0) *p.status = SB_ERR_TOO_LARGE;
+    return;
+  }
+  PaCut& cut = c.cut;
+  cut.total = (int)all;
+  cut.ctas = min((int)gridDim.x, (cut.total + 1) / 2);  // two tiles per CTA at least: one for each softmax group
+  if ((int)blockIdx.x >= cut.ctas) return;
+  cut.per = cut.total / cut.ctas;
+  cut.rest = cut.total - cut.per * cut.ctas;
+  c.unit = cut.start(blockIdx.x);
+  c.left = cut.per + ((int)blockIdx.x < cut.rest);
+  int off = c.unit, chunk = 0;
+  if (chunks > 1) {
+    for (int base = 0; base < chunks; base += 32) {
+      const int v = base + lane < chunks ? sums[base + lane] * p.Hkv : 0, inc = pa_scan(v, lane);
+      const unsigned hit = __ballot_sync(0xffffffffu, inc > off);
+      if (hit) {
+        const int k = __ffs(hit) - 1;
+        chunk = base + k;
+        off -= __shfl_sync(0xffffffffu, inc - v, k);
+        break;
+      }
+      off -= __shfl_sync(0xffffffffu, inc, 31);
     }
-    off -= __shfl_sync(0xffffffffu, inc, 31);
   }
   PaSeq s;
-  const long long tiles = pa_chunk_tiles(p, chunk, lane, s), v = tiles * p.Hkv, inc = pa_scan(v, lane);
+  const int tiles = pa_chunk_tiles(p, chunk, lane, s), v = tiles * p.Hkv, inc = pa_scan(v, lane);
   const int k = __ffs(__ballot_sync(0xffffffffu, inc > off)) - 1;
   off -= __shfl_sync(0xffffffffu, inc - v, k);
-  const long long per_head = __shfl_sync(0xffffffffu, tiles, k);
-  const int n = __shfl_sync(0xffffffffu, s.n, k), L = __shfl_sync(0xffffffffu, s.L, k);
+  const int per_head = __shfl_sync(0xffffffffu, tiles, k);
+  c.s = PaSeq{__shfl_sync(0xffffffffu, s.row0, k), __shfl_sync(0xffffffffu, s.n, k), __shfl_sync(0xffffffffu, s.L, k)};
   c.seq = chunk * 32 + k;
-  c.hk = (int)(off / per_head);
+  c.hk = off / per_head;
   off -= c.hk * per_head;
-  const int items = pa_items(p, n);
-  for (int base = 0; base < items; base += 32) {
-    const long long t = base + lane < items ? pa_item_tiles(p, n, L, base + lane) : 0;
-    const long long ti = pa_scan(t, lane);
-    const unsigned hit = __ballot_sync(0xffffffffu, ti > off);
-    if (hit) {
-      const int j = __ffs(hit) - 1;
-      c.m = base + j;
-      c.tile = (int)(off - __shfl_sync(0xffffffffu, ti - t, j));
-      break;
+  const int items = pa_items(p, c.s.n);
+  c.tile = off;
+  if (items > 1) {
+    for (int base = 0; base < items; base += 32) {
+      const int t = base + lane < items ? pa_item_tiles(p, c.s.n, c.s.L, base + lane) : 0, ti = pa_scan(t, lane);
+      const unsigned hit = __ballot_sync(0xffffffffu, ti > off);
+      if (hit) {
+        const int j = __ffs(hit) - 1;
+        c.m = base + j;
+        c.tile = off - __shfl_sync(0xffffffffu, ti - t, j);
+        break;
+      }
+      off -= __shfl_sync(0xffffffffu, ti, 31);
     }
-    off -= __shfl_sync(0xffffffffu, ti, 31);
   }
 }
 
@@ -308,79 +367,78 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     sb::tmem_relinquish();
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // tiles of 32 sequences at a time, in memory that the ring takes over afterwards
-  long long* sums = reinterpret_cast<long long*>(sRing);
+  // tiles of 32 sequences at a time, where the scheduler puts the queries afterwards
+  int* sums = reinterpret_cast<int*>(sQ);
   const int chunks = (p.batch + 31) / 32;
   for (int c = warp; c < chunks; c += PA_WARPS) {
     PaSeq s;
-    const long long t = pa_scan(pa_chunk_tiles(p, c, lane, s), lane);
-    if (lane == 31) sums[c] = t;
+    const int t = pa_sum(pa_chunk_tiles(p, c, lane, s));
+    if (lane == 0) sums[c] = t;
   }
   sb::tc_fence_before();
   __syncthreads();
   sb::tc_fence_after();
-  PaCursor cur;
-  if (warp == 10) pa_find(p, sums, chunks, lane, cur);
-  sb::fence_proxy_async_smem();
-  __syncthreads();
   const uint32_t tmem_base = *tmem_slot;
 
+  if (warp >= 8) {
+  pa_regs_dec<PA_REGS_FEW>();  // one instruction for the whole warpgroup
   if (warp == 10) {
     // ------------------------------------------------------------------ scheduler and query loads
+    PaCursor cur;
+    pa_find(p, sums, chunks, lane, cur);
+    __syncwarp();
     int* desc = p.part_desc + 8 * blockIdx.x;
-    bool starts = false;
-    int i = 0, q_cnt = 0;
-    PaSeq s = {0, 0, 0};
-    if (cur.left > 0) s = pa_seq(p, cur.seq);
-    bool ok = true;
-    long long unit = cur.u0;  // line position of the item's first tile in this piece
-    while (ok) {
+    bool starts = false, ok = true;
+    int q_cnt = 0;
+    for (int i = 0; ok; ++i) {
       const int slot = i % PA_ITEMS;
       if (!pa_wait(&item_empty[slot], ((i / PA_ITEMS) & 1) ^ 1, abort_flag)) break;
       PaItem it = {};
+      int tiles = 0;
       if (cur.left > 0) {
         int lo, hi;
-        pa_item_keys(p, s.n, s.L, cur.m, lo, hi);
-        const int tiles = max((hi + PA_TILE - 1) / PA_TILE - lo / PA_TILE, 1);
-        const int take = (int)min((long long)(tiles - cur.tile), cur.left);
+        pa_item_keys(p, cur.s.n, cur.s.L, cur.m, lo, hi);
+        tiles = max((hi + PA_TILE - 1) / PA_TILE - lo / PA_TILE, 1);
+        const int take = min(tiles - cur.tile, cur.left);
         const bool first = cur.tile == 0, last = cur.tile + take == tiles;
-        it = PaItem{s.row0, s.n, s.L, cur.seq, cur.hk, cur.m, lo / PA_TILE + cur.tile, take, lo, hi,
-                    first && last ? -1 : 2 * (int)blockIdx.x + (first ? 1 : 0), 0};
+        const int tok0 = cur.m * PA_ITEM_ROWS / p.group;
+        it = PaItem{cur.s.row0 + tok0, cur.s.L - cur.s.n + tok0, cur.s.L, cur.seq, cur.hk,
+                    min(cur.s.n * p.group - cur.m * PA_ITEM_ROWS, PA_ITEM_ROWS), cur.m * PA_ITEM_ROWS - tok0 * p.group,
+                    lo / PA_TILE + cur.tile, take, lo, hi,
+                    first && last ? -1 : 2 * (int)blockIdx.x + (first ? 1 : 0)};
         if (first && !last) {  // the CTA that starts an item names the one that ends it
           starts = true;
-          const long long end = unit + tiles - 1;
           if (lane == 0) {
-            desc[1] = s.row0; desc[2] = s.n; desc[3] = cur.hk; desc[4] = cur.m;
-            desc[5] = (int)(((end + 1) * cur.ctas - 1) / cur.total);
+            desc[1] = it.row0; desc[2] = it.rem; desc[3] = it.hk; desc[4] = it.rows;
+            desc[5] = cur.cut.owner(cur.unit + tiles - 1);
           }
         }
         cur.left -= take;
-        unit += take;
+        cur.unit += take;
       }
       if (lane == 0) {
         items[slot] = it;
         sb::mbar_arrive(&item_full[slot]);
       }
-      ++i;
       if (it.count == 0) break;
       // queries of the item: one slot, or two of them, as 16-byte chunks in the swizzled K-major layout
-      const int rows = min(s.n * p.group - cur.m * PA_ITEM_ROWS, PA_ITEM_ROWS);
-      const int slots = rows > PA_TILE ? 2 : 1;
-      for (int x = 0; x < slots && ok; ++x) {
+      const int slots = it.rows > PA_TILE ? 2 : 1;
+      for (int x = 0; x < slots; ++x) {
         const int qs = (q_cnt + x) & 1;
         ok = pa_wait(&q_empty[qs], (((q_cnt + x) >> 1) & 1) ^ 1, abort_flag);
         if (!ok) break;
-        const uint32_t dst = sb::smem_u32(sQ + qs * TILE_BYTES);
-        const int base = cur.m * PA_ITEM_ROWS + x * PA_TILE, live = min(rows - x * PA_TILE, PA_TILE);
         constexpr int CH = DP / 8;  // chunks per row
-        const int ch = lane % CH, rr = lane / CH;
-        const int end = (live + 31) & ~31;  // whole warps of rows: lanes without a row read zeros
-        for (int r = rr; r < end; r += 32 / CH) {
-          const int row = base + r, t = row / p.group, h = row - t * p.group;
+        const int ch = lane % CH, live = min(it.rows - x * PA_TILE, PA_TILE), end = (live + 31) & ~31;
+        const uint32_t dst = sb::smem_u32(sQ + qs * TILE_BYTES) + (ch >> 3) * PA_PANEL;
+        const uint16_t* base = reinterpret_cast<const uint16_t*>(p.q) + (long)it.row0 * p.q_tok +
+                               (long)it.hk * p.group * p.q_head + ch * 8;
+        // whole warps of rows: lanes without a row read zeros
+#pragma unroll 4
+        for (int r = lane / CH; r < end; r += 32 / CH) {
+          const int row = it.rem + x * PA_TILE + r, t = pa_div(p, row), h = row - t * p.group;
           const bool take = r < live && ch * 8 < p.D;
-          const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) +
-                                (take ? (long)(s.row0 + t) * p.q_tok + (long)(cur.hk * p.group + h) * p.q_head + ch * 8 : 0);
-          pa_cp16(dst + (ch >> 3) * PA_PANEL + r * 128 + (((ch & 7) ^ (r & 7)) << 4), src, take);
+          pa_cp16(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4),
+                  take ? base + (long)t * p.q_tok + (long)h * p.q_head : reinterpret_cast<const uint16_t*>(p.q), take);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         sb::fence_proxy_async_smem();
@@ -388,27 +446,26 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         if (lane == 0) sb::mbar_arrive(&q_full[qs]);
       }
       q_cnt += slots;
-      if (cur.left > 0) {
-        cur.tile = 0;
-        if (++cur.m == pa_items(p, s.n)) {
-          cur.m = 0;
-          if (++cur.hk == p.Hkv) {
-            cur.hk = 0;
-            do { s = pa_seq(p, ++cur.seq); } while (s.n == 0 && cur.seq + 1 < p.batch);
-          }
+      cur.tile = 0;
+      if (cur.left > 0 && ++cur.m == pa_items(p, cur.s.n)) {
+        cur.m = 0;
+        if (++cur.hk == p.Hkv) {
+          cur.hk = 0;
+          do { cur.s = pa_seq(p, ++cur.seq); } while (cur.s.n == 0 && cur.seq + 1 < p.batch);
         }
       }
     }
     if (lane == 0) desc[0] = starts && ok;
-  } else if (warp == 8) {
-    // ------------------------------------------------------------------ K and V tiles
-    if (lane == 0) {
-      sb::tma_prefetch_desc(&tmK);
-      sb::tma_prefetch_desc(&tmV);
-    }
+  } else if (warp != 9) {
+    // ------------------------------------------------------------------ K tiles (warp 8), V tiles (warp 11)
+    const bool is_v = warp == 11;
+    const CUtensorMap* tm = is_v ? &tmV : &tmK;
+    if (lane == 0) sb::tma_prefetch_desc(tm);
     const int page = 1 << p.page_shift;
-    const int box = min(page, PA_TILE), per_tile = PA_TILE / box;  // rows per box, boxes per tile and panel
-    const int bi = lane % per_tile, pn = lane / per_tile;          // this lane's box and panel
+    const int box = min(page, PA_TILE), per_tile = PA_TILE / box;  // rows per copy, pages per tile
+    const int bi = lane % per_tile, pn = lane / per_tile;          // this lane's page of the tile, and its panel
+    const int page8 = is_v ? p.v_page8 : p.k_page8, outside = is_v ? p.v_outside : p.k_outside;
+    const uint32_t dst = sb::smem_u32(sRing) + bi * (box >> 3) * p.group_step + pn * p.panel_step;
     uint32_t ring = 0;
     bool ok = true;
     for (int i = 0; ok; ++i) {
@@ -418,102 +475,98 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       __syncwarp();
       if (lane == 0) sb::mbar_arrive(&item_empty[slot]);
       if (it.count == 0) break;
-      const int lead = it.n * p.group - it.m * PA_ITEM_ROWS > PA_TILE ? 1 : 2;
+      const int lead = it.rows > PA_TILE ? 1 : 2;
       const int* trow = p.table + (long)it.seq * p.table_ld;
-      int win[2] = {-64, -64}, ids[2] = {0, 0};  // 32 page numbers at a time, for K and for V
-      auto load = [&](int t, int kv) -> bool {
-        const int stage = ring % STAGES;
+      int win = -64, where = 0;  // 32 pages at a time: their first 8-row group in the tensor map
+      for (int t = 0; t < it.count; ++t) {
         const int key0 = (it.tile0 + t) * PA_TILE, page0 = key0 >> p.page_shift;
-        if (page0 < win[kv] || page0 + per_tile > win[kv] + 32) {
-          win[kv] = page0;
+        if (page0 + per_tile > win + 32) {
+          win = page0;
           const int idx = page0 + lane;
-          int id = p.num_pages;  // a box outside the cache reads zeros
+          where = outside;  // a copy from outside the cache reads zeros
           if (idx < p.cols && ((idx + 1) << p.page_shift) > it.lo && (idx << p.page_shift) < it.hi) {
             const int got = trow[idx];
-            if (got >= 0 && got < p.num_pages) id = got;
+            if (got >= 0 && got < p.num_pages) where = got * page8;
             else *p.status = SB_ERR_BAD_ARG;  // a visible page outside the cache: reported, its keys read as zeros
           }
-          ids[kv] = id;
         }
-        const int id = __shfl_sync(0xffffffffu, ids[kv], page0 - win[kv] + bi);
-        if (!pa_wait(&empty[stage], ((ring / STAGES) & 1) ^ 1, abort_flag)) return false;
-        uint8_t* dst = sRing + stage * TILE_BYTES;
-        if (lane == 0) sb::mbar_expect_tx(&full[stage], TILE_BYTES);
-        __syncwarp();
-        if (pn < PANELS)
-          pa_tma_4d(dst + pn * PA_PANEL + bi * box * 128, kv ? &tmV : &tmK, &full[stage], pn * 64, it.hk,
-                    key0 & (page - 1), id);
-        ++ring;
-        return true;
-      };
-      for (int t = 0; t < lead && t < it.count && ok; ++t) ok = load(t, 0);
-      for (int t = 0; t < it.count && ok; ++t) {
-        ok = load(t, 1);
-        if (ok && t + lead < it.count) ok = load(t + lead, 0);
-      }
-    }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------------ MMA issue
-    if (lane == 0) {
-      const uint32_t idesc_s = sb::umma_idesc_f16(PA_TILE, PA_TILE, F16 ? 0 : 1, 0, 0);
-      const uint32_t idesc_o = sb::umma_idesc_f16(PA_TILE, DP, F16 ? 0 : 1, 0, 1);
-      const uint32_t ring_addr = sb::smem_u32(sRing), q_addr = sb::smem_u32(sQ);
-      uint32_t ring = 0, p_cnt[2] = {0, 0};
-      int q_cnt = 0;
-      bool ok = true;
-      for (int i = 0; ok; ++i) {
-        const int slot = i % PA_ITEMS;
-        if (!sb::mbar_wait(&item_full[slot], (i / PA_ITEMS) & 1, abort_flag)) break;
-        const int count = items[slot].count, rows = items[slot].n * p.group - items[slot].m * PA_ITEM_ROWS;
-        sb::mbar_arrive(&item_empty[slot]);
-        if (count == 0) break;
-        const int two_q = rows > PA_TILE, lead = two_q ? 1 : 2, n = two_q ? 2 * count : count;
-        for (int x = 0; x <= two_q && ok; ++x)
-          ok = sb::mbar_wait(&q_full[(q_cnt + x) & 1], ((q_cnt + x) >> 1) & 1, abort_flag);
+        const int first8 = __shfl_sync(0xffffffffu, where, page0 - win + bi);
+        const uint32_t e = ring + (is_v ? pa_v_place(t, lead, it.count) : pa_k_place(t, lead)), st = e % STAGES;
+        ok = pa_wait(&empty[st], ((e / STAGES) & 1) ^ 1, abort_flag);
         if (!ok) break;
-        // virtual tile v: group v & 1; key tile v (one query slot) or v / 2 (two)
-        auto issue_s = [&](int v) -> bool {
-          const uint32_t e = ring + pa_k_place(two_q ? v >> 1 : v, lead), st = e % STAGES;
-          if (!sb::mbar_wait(&full[st], (e / STAGES) & 1, abort_flag)) return false;
-          sb::tc_fence_after();
-          const int qs = (q_cnt + (two_q ? v & 1 : 0)) & 1;
-          const uint32_t qa = q_addr + qs * TILE_BYTES, ka = ring_addr + st * TILE_BYTES;
-#pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * PA_PANEL + (kk & 3) * 32;
-            sb::umma_f16_ss(tmem_base + S_COL + (v & 1) * PA_TILE, sb::umma_smem_desc(qa + off, 16, 1024),
-                            sb::umma_smem_desc(ka + off, 16, 1024), idesc_s, kk != 0);
-          }
-          sb::umma_commit(&s_full[v & 1]);
-          if (!two_q || (v & 1)) sb::umma_commit(&empty[st]);
-          if (two_q ? v >= n - 2 : v == n - 1) sb::umma_commit(&q_empty[qs]);
-          return true;
-        };
-        ok = issue_s(0);
-        if (ok && n > 1) ok = issue_s(1);
-        for (int v = 0; v < n && ok; ++v) {
-          const int x = v & 1;
-          const uint32_t e = ring + pa_v_place(two_q ? v >> 1 : v, lead, count), st = e % STAGES;
-          ok = sb::mbar_wait(&p_full[x], p_cnt[x] & 1, abort_flag) && sb::mbar_wait(&full[st], (e / STAGES) & 1, abort_flag);
-          if (ok && v == 0 && i > 0) ok = sb::mbar_wait(epi_done, (i - 1) & 1, abort_flag);  // O of the item before is read
-          if (!ok) break;
-          ++p_cnt[x];
-          sb::tc_fence_after();
-          const uint32_t va = ring_addr + st * TILE_BYTES, pa = tmem_base + S_COL + x * PA_TILE;
-#pragma unroll
-          for (int kk = 0; kk < PA_TILE / 16; ++kk)
-            pa_umma_ts(tmem_base + O_COL + x * DP, pa + kk * 8, sb::umma_smem_desc(va + kk * 2048, PA_PANEL, 1024), idesc_o,
-                       v > 1 || kk != 0);
-          if (!two_q || x) sb::umma_commit(&empty[st]);
-          if (v + 2 >= n) sb::umma_commit(&o_full[x]);
-          if (v + 2 < n) ok = issue_s(v + 2);
-        }
-        ring += 2 * count;
-        q_cnt += 1 + two_q;
+        if (lane == 0) sb::mbar_expect_tx(&full[st], TILE_BYTES);
+        __syncwarp();
+        if (pn < p.boxes)
+          pa_tma_5d(dst + st * TILE_BYTES, tm, &full[st], pn * 64, first8 + ((key0 & (page - 1)) >> 3), it.hk);
       }
+      ring += 2 * it.count;
     }
   } else {
+    // ------------------------------------------------------------------ MMA issue
+    const uint32_t leader = lane == 0;
+    const uint32_t idesc_s = sb::umma_idesc_f16(PA_TILE, PA_TILE, F16 ? 0 : 1, 0, 0);  // K-major both
+    const uint32_t idesc_o = sb::umma_idesc_f16(PA_TILE, DP, F16 ? 0 : 1, 0, 1);       // V is MN-major
+    const uint64_t q_desc = sb::umma_smem_desc(sb::smem_u32(sQ), 16, 1024);
+    const uint64_t k_desc = sb::umma_smem_desc(sb::smem_u32(sRing), 16, p.group_step);
+    const uint64_t v_desc = sb::umma_smem_desc(sb::smem_u32(sRing), p.panel_step, p.group_step);
+    const uint32_t k_panel = p.panel_step >> 4, v_step = (2 * p.group_step) >> 4;  // descriptors count 16-byte units
+    uint32_t ring = 0, p_cnt0 = 0, p_cnt1 = 0;
+    int q_cnt = 0;
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      const int slot = i % PA_ITEMS;
+      if (!pa_wait(&item_full[slot], (i / PA_ITEMS) & 1, abort_flag)) break;
+      const int count = __shfl_sync(0xffffffffu, items[slot].count, 0);
+      const int two_q = __shfl_sync(0xffffffffu, items[slot].rows > PA_TILE, 0);
+      if (lane == 0) sb::mbar_arrive(&item_empty[slot]);
+      if (count == 0) break;
+      const int lead = two_q ? 1 : 2, n = two_q ? 2 * count : count;
+      ok = pa_wait(&q_full[q_cnt & 1], (q_cnt >> 1) & 1, abort_flag);
+      if (ok && two_q) ok = pa_wait(&q_full[(q_cnt + 1) & 1], ((q_cnt + 1) >> 1) & 1, abort_flag);
+      if (!ok) break;
+      // virtual tile v: group v & 1; key tile v (one query slot) or v / 2 (two)
+      auto issue_s = [&](int v) -> bool {
+        const uint32_t e = ring + pa_k_place(two_q ? v >> 1 : v, lead), st = e % STAGES;
+        if (!pa_wait(&full[st], (e / STAGES) & 1, abort_flag)) return false;
+        sb::tc_fence_after();
+        const int qs = (q_cnt + (two_q ? v & 1 : 0)) & 1;
+        const uint64_t qd = q_desc + qs * (TILE_BYTES >> 4), kd = k_desc + st * (TILE_BYTES >> 4);
+        const uint32_t d = tmem_base + S_COL + (v & 1) * PA_TILE;
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk)
+          pa_umma_ss(leader, d, qd + (kk >> 2) * (PA_PANEL >> 4) + (kk & 3) * 2, kd + (kk >> 2) * k_panel + (kk & 3) * 2,
+                     idesc_s, kk != 0);
+        pa_commit(leader, &s_full[v & 1]);
+        if (!two_q || (v & 1)) pa_commit(leader, &empty[st]);
+        if (two_q ? v >= n - 2 : v == n - 1) pa_commit(leader, &q_empty[qs]);
+        return true;
+      };
+      ok = issue_s(0);
+      if (ok && n > 1) ok = issue_s(1);
+      for (int v = 0; v < n && ok; ++v) {
+        const int x = v & 1;
+        const uint32_t e = ring + pa_v_place(two_q ? v >> 1 : v, lead, count), st = e % STAGES;
+        ok = pa_wait(&p_full[x], (x ? p_cnt1 : p_cnt0) & 1, abort_flag) && pa_wait(&full[st], (e / STAGES) & 1, abort_flag);
+        if (ok && v == 0 && i > 0) ok = pa_wait(epi_done, (i - 1) & 1, abort_flag);  // O of the item before is read
+        if (!ok) break;
+        if (x) ++p_cnt1; else ++p_cnt0;
+        sb::tc_fence_after();
+        const uint64_t vd = v_desc + st * (TILE_BYTES >> 4);
+        const uint32_t pa = tmem_base + S_COL + x * PA_TILE, d = tmem_base + O_COL + x * DP;
+#pragma unroll
+        for (int kk = 0; kk < PA_TILE / 16; ++kk)
+          pa_umma_ts(leader, d, pa + kk * 8, vd + kk * v_step, idesc_o, v > 1 || kk != 0);
+        if (!two_q || x) pa_commit(leader, &empty[st]);
+        if (v + 2 >= n) pa_commit(leader, &o_full[x]);
+        if (v + 2 < n) ok = issue_s(v + 2);
+      }
+      ring += 2 * count;
+      q_cnt += 1 + two_q;
+    }
+  }
+  } else {
     // ------------------------------------------------------------------ softmax and output
+    pa_regs_inc<PA_REGS_MANY>();
     const int x = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16);
     const uint32_t s_addr = t_lane + S_COL + x * PA_TILE, o_addr = t_lane + O_COL + x * DP;
@@ -527,17 +580,17 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       __syncwarp();
       if (lane == 0) sb::mbar_arrive(&item_empty[islot]);
       if (it.count == 0) break;
-      const int rows = min(it.n * p.group - it.m * PA_ITEM_ROWS, PA_ITEM_ROWS);
+      const int rows = it.rows;
       const bool two_q = rows > PA_TILE;
       const int lead = two_q ? 1 : 2;
       const int row = two_q ? x * PA_TILE + r : r;          // row of the item
       const int warp_rows = rows - (row - lane);             // <= 0: no row of this warp exists
-      const int grow = it.m * PA_ITEM_ROWS + row, tok = grow / p.group, head = it.hk * p.group + (grow - tok * p.group);
+      const int tok = pa_div(p, it.rem + row), head = it.hk * p.group + (it.rem + row - tok * p.group);
       // visible keys of the row; lanes without a row see everything (their queries are zeros), so that they do not
       // send the warp through the masked path
       int lo = 0, hi = 0x7fffffff;
       if (row < rows) {
-        const int pos = it.L - it.n + tok;
+        const int pos = it.pos0 + tok;
         if (p.window >= 0) lo = max(0, pos - p.window);
         hi = p.causal ? min(pos + 1, it.L) : (p.window >= 0 ? (int)min((long)it.L, (long)pos + p.window + 1) : it.L);
       }
@@ -605,10 +658,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           const uint32_t e = ring + pa_v_place(t, lead, it.count), st = e % STAGES;
           if (!pa_wait(&full[st], (e / STAGES) & 1, abort_flag)) { ok = false; break; }
           if (key0 + r >= it.hi) {
-            uint8_t* dst = sRing + st * TILE_BYTES + r * 128;
+            uint8_t* dst = sRing + st * TILE_BYTES + (r >> 3) * p.group_step + (r & 7) * 128;
 #pragma unroll
             for (int c = 0; c < PANELS * 8; ++c)
-              *reinterpret_cast<uint4*>(dst + (c >> 3) * PA_PANEL + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(dst + (c >> 3) * p.panel_step + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           sb::fence_proxy_async_smem();
         }
@@ -730,8 +783,7 @@ __global__ void __launch_bounds__(PA_COMBINE_THREADS) pa_combine_kernel(const Pa
   }
   const int* desc = p.part_desc + 8 * blockIdx.x;
   if (!desc[0]) return;
-  const int row0 = desc[1], n = desc[2], hk = desc[3], m = desc[4], last = desc[5];
-  const int rows = min(n * p.group - m * PA_ITEM_ROWS, PA_ITEM_ROWS);
+  const int row0 = desc[1], rem = desc[2], hk = desc[3], rows = desc[4], last = desc[5];
   const int quad = threadIdx.x % QUADS, pg = threadIdx.x / QUADS;
   for (int row = blockIdx.y; row < rows; row += gridDim.y) {
     float ref = -INFINITY, l = 0.f;
@@ -767,7 +819,7 @@ __global__ void __launch_bounds__(PA_COMBINE_THREADS) pa_combine_kernel(const Pa
         acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
       }
       const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-      const int grow = m * PA_ITEM_ROWS + row, tok = grow / p.group, head = hk * p.group + (grow - tok * p.group);
+      const int tok = pa_div(p, rem + row), head = hk * p.group + (rem + row - tok * p.group);
       if (quad * 4 < p.D) {
         uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (long)(row0 + tok) * p.o_tok + (long)head * p.o_head + quad * 4;
         *reinterpret_cast<uint2*>(dst) = make_uint2(pa_pack<F16>(acc.x * inv, acc.y * inv), pa_pack<F16>(acc.z * inv, acc.w * inv));
@@ -788,16 +840,23 @@ PaEncodeFn pa_encode() {
   }();
   return fn;
 }
-// a cache as [page][row][head][D], 64 columns x min(page_size, 128) rows per box
+// A cache seen as [head][8-row group][64-column panel][row of the group][column]: one copy brings the panels of up to 128
+// rows of a page as the 1024-byte blocks that the matrix descriptors step over.  With a head size that is no multiple of
+// 64 there is one panel dimension of true width, so that columns beyond the head read zeros.
 int pa_tmap(CUtensorMap* m, const void* base, int D, int heads, int page_size, int pages, long page, long row, long head,
-            bool f16) {
+            bool f16, bool joined, int* page8, int* outside) {
   if (!pa_encode()) return SB_ERR_DRIVER;
-  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)page_size, (cuuint64_t)pages};
-  cuuint64_t strides[3] = {(cuuint64_t)head * 2, (cuuint64_t)row * 2, (cuuint64_t)page * 2};
-  cuuint32_t box[4] = {64, 1, (cuuint32_t)(page_size < PA_TILE ? page_size : PA_TILE), 1};
-  cuuint32_t es[4] = {1, 1, 1, 1};
+  if (row <= 0 || (pages > 1 && page % (8 * row))) return SB_ERR_BAD_ARG;
+  const long step = pages == 1 ? page_size / 8 : page / (8 * row), groups = (pages - 1) * step + page_size / 8;
+  if (step < 0 || groups > (1L << 30)) return SB_ERR_TOO_LARGE;
+  *page8 = (int)step;
+  *outside = (int)groups;
+  cuuint64_t dims[5] = {(cuuint64_t)(joined ? 64 : D), 8, (cuuint64_t)(joined ? 2 : 1), (cuuint64_t)groups, (cuuint64_t)heads};
+  cuuint64_t strides[4] = {(cuuint64_t)row * 2, 128, (cuuint64_t)row * 16, (cuuint64_t)head * 2};
+  cuuint32_t box[5] = {64, 8, (cuuint32_t)(joined ? 2 : 1), (cuuint32_t)((page_size < PA_TILE ? page_size : PA_TILE) / 8), 1};
+  cuuint32_t es[5] = {1, 1, 1, 1, 1};
   const CUresult r =
-      pa_encode()(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base),
+      pa_encode()(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base),
                   dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? SB_OK : SB_ERR_DRIVER;
@@ -850,7 +909,7 @@ SB_API long sb200_paged_attention_workspace(int T, int batch, int Hq, int Hkv, i
 }
 
 // out[t, h] for the new tokens of `batch` sequences, q / out [T, Hq, D] (token and head strides in elements), caches
-// [num_pages, page_size, Hkv, D] (page, row and head strides), bf16 or fp16.  Sequence b: rows cu[b] .. cu[b + 1] of q, its
+// [num_pages, page_size, Hkv, D] (page, row and head strides; a page stride is a multiple of 8 row strides), bf16 or fp16.  Sequence b: rows cu[b] .. cu[b + 1] of q, its
 // last new token at position lens[b] - 1; position j in row j % page_size of page table[b][j / page_size].  A query at
 // position i sees keys j <= i (causal), |i - j| <= window (window >= 0).  page_size is a power of two from 8, D a
 // multiple of 8 up to 128; pointers and strides are multiples of 16 bytes.  Rows behind the last sequence are left as
@@ -867,7 +926,7 @@ SB_API int sb200_paged_attention(const void* q, const void* k_cache, const void*
   if (page_size < 8 || (page_size & (page_size - 1)) || !(scale > 0.f && scale < 1e30f)) return SB_ERR_BAD_ARG;
   if (dtype != SB_DT_BF16 && dtype != SB_DT_F16) return SB_ERR_BAD_ARG;
   const long cap = (long)cols * page_size;
-  if ((long)T * Hq > (1L << 30) || cap > (1L << 30) || batch > (1 << 19)) return SB_ERR_TOO_LARGE;
+  if ((long)T * Hq > (1L << 30) || cap > (1L << 30) || batch > (1 << 17) || Hq / Hkv > (1 << 15)) return SB_ERR_TOO_LARGE;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
        reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return SB_ERR_BAD_ARG;
@@ -876,13 +935,21 @@ SB_API int sb200_paged_attention(const void* q, const void* k_cache, const void*
   const bool f16 = dtype == SB_DT_F16;
   CUtensorMap tmK, tmV;
   int rc;
-  if ((rc = pa_tmap(&tmK, k_cache, D, Hkv, page_size, num_pages, k_page, k_row, k_head, f16))) return rc;
-  if ((rc = pa_tmap(&tmV, v_cache, D, Hkv, page_size, num_pages, v_page, v_row, v_head, f16))) return rc;
-  const int ctas = (int)pa_ctas(T, batch, Hq, Hkv, cap, sms), dp = D <= 64 ? 64 : 128;
   PaParams p = {};
+  const bool joined = D == 128;
+  if ((rc = pa_tmap(&tmK, k_cache, D, Hkv, page_size, num_pages, k_page, k_row, k_head, f16, joined, &p.k_page8, &p.k_outside)))
+    return rc;
+  if ((rc = pa_tmap(&tmV, v_cache, D, Hkv, page_size, num_pages, v_page, v_row, v_head, f16, joined, &p.v_page8, &p.v_outside)))
+    return rc;
+  p.group_step = joined ? 2048 : 1024;
+  p.panel_step = joined ? 1024 : PA_PANEL;
+  p.boxes = joined || D <= 64 ? 1 : 2;
+  const int ctas = (int)pa_ctas(T, batch, Hq, Hkv, cap, sms), dp = D <= 64 ? 64 : 128;
   p.q = q; p.out = out; p.table = table; p.cu = cu; p.lens = lens;
   p.table_ld = table_ld; p.q_tok = q_tok; p.q_head = q_head; p.o_tok = o_tok; p.o_head = o_head;
-  p.T = T; p.batch = batch; p.Hkv = Hkv; p.group = Hq / Hkv; p.D = D; p.cols = cols; p.num_pages = num_pages;
+  p.T = T; p.batch = batch; p.Hkv = Hkv; p.group = Hq / Hkv;
+  p.group_inv = (uint32_t)((1UL << 32) / p.group + 1);
+  p.D = D; p.cols = cols; p.num_pages = num_pages;
   while ((1 << p.page_shift) < page_size) ++p.page_shift;
   p.causal = causal; p.window = window < (1 << 30) ? window : 1 << 30; p.sl2 = scale * 1.4426950408889634f;
   p.part_rows = pa_part_rows(T, p.group);

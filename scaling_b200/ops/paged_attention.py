@@ -224,6 +224,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1]) or t.data_ptr() % 16:
             raise _lib.KernelError(f"paged_attention: {name} must start and have its rows on 16-byte boundaries, strides "
                                    f"{t.stride()}")
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if num_pages > 1 and (t.stride(1) <= 0 or t.stride(0) % (8 * t.stride(1))):
+            raise _lib.KernelError(f"paged_attention: the page stride of {name} must be a multiple of eight row strides, "
+                                   f"got {t.stride()}")
     if num_pages == 0:
         raise ValueError("the cache has no pages")
     if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
