@@ -8,18 +8,24 @@
 // output is rescaled a few times per row instead of at every step; any reference gives the same quotient and
 // p_ij <= 2^8 stays far from overflow in both 16-bit types and in the fp32 sums.
 //
-// One kernel serves decoding, which is a stream over K and V, and chunks, which are matrix products:
-//  * An item is up to 256 query rows (tokens x heads that share a KV head, token-major) of one sequence and KV head.  All
-//    items together are a line of 128-key tiles that is cut into equal pieces, one per CTA (one CTA per SM): ragged lengths
-//    are balanced without the host knowing them.  A piece that starts or ends inside an item leaves an unnormalised
-//    partial result; a second kernel joins them in the order of the CTAs, so results do not depend on timing.
-//  * Two groups of four softmax warps (thread = query row = TMEM lane) work on different S = Q K^T at any time, so that
-//    the tensor core computes for one while the other takes exponentials.  Items of more than 128 rows give each group
-//    128 rows of its own ("two_q"); smaller items give both groups the same rows and every second key tile, and join the
-//    two states at the end of the item.
-//  * S of a group takes 128 TMEM columns; its probabilities overwrite the first 64 as packed 16-bit values and are
-//    the TMEM operand of O += P V.  O stays in TMEM over the whole item.
-//  * K and V tiles come by TMA through a ring that does not know items: the loader runs ahead into the next ones.
+// Two kernels share the frame.  An item is a block of query rows (tokens x heads that share a KV head, token-major) of one
+// sequence and KV head.  All items together are a line of 128-key tiles that is cut into equal pieces, one per CTA (one CTA
+// per SM): ragged lengths are balanced without the host knowing them.  A piece that starts or ends inside an item leaves an
+// unnormalised partial result; a last kernel joins them in the order of the CTAs, so results do not depend on timing.
+// K and V tiles come by TMA through a ring that does not know items: the loaders run ahead into the next ones.
+//
+// Wide (sequences with more than 64 rows): matrix products.  Items of 256 rows, S = Q K^T with query rows in the 128 TMEM
+//   lanes.  Two groups of four softmax warps (thread = query row = lane) work on different S at any time, so that the
+//   tensor core computes for one while the other takes exponentials.  Items of more than 128 rows give each group 128
+//   rows of its own ("two_q"); smaller items give both the same rows and every second key tile, and join the two states at
+//   the end.  The probabilities overwrite the first half of S as packed 16-bit values and are the TMEM operand of
+//   O += P V; O stays in TMEM over the whole item.
+// Narrow (at most 64 rows: decoding): a stream over K and V, so everything else has to be small against the tile's bytes.
+//   Rows in lanes would leave most lanes and three of four warps idle; here the keys are in the lanes: S^T = K Q^T
+//   [128 keys x rows], a thread takes the exponentials of one key for all rows, and O^T += V^T P [D x rows].  S^T of four
+//   tiles is in flight.  A thread keeps the row sums over its own keys; the rows' references are shared by the four warps
+//   of a group, which agree once per tile whether any score has outgrown them.
+//
 // Warp roles: 0-3 and 4-7 softmax groups, 8 and 11 TMA loaders of K and of V (a page of 16 tokens is a copy of its own, and
 // one warp alone issues them no faster than the memory delivers), 9 MMA issuer, 10 scheduler, which also copies the queries.
 //
@@ -32,7 +38,7 @@
 namespace {
 
 constexpr int PA_TILE = 128;
-constexpr int PA_ITEM_ROWS = 256;
+constexpr int PA_WIDE_ROWS = 256, PA_NARROW_ROWS = 64;  // rows per item
 constexpr int PA_WARPS = 12;
 constexpr int PA_THREADS = PA_WARPS * 32;
 // registers per thread after the roles part: 128 x 80 + 256 x 208 = 63488 of the 384 x 168 that the launch holds
@@ -40,6 +46,8 @@ constexpr int PA_REGS_FEW = 80, PA_REGS_MANY = 208;
 constexpr int PA_PANEL = 16384;   // 128 rows x 128 bytes
 constexpr int PA_ITEMS = 4;       // descriptors in flight
 constexpr int PA_COMBINE_THREADS = 256;
+// What the start and the end of an item cost, in tiles: added to its length on the work line.
+constexpr int PA_WIDE_COST = 2, PA_NARROW_COST = 1;
 
 struct PaParams {
   const void* q;
@@ -51,11 +59,12 @@ struct PaParams {
   int T, batch, Hkv, group, D, cols, num_pages, page_shift;
   uint32_t group_inv;  // floor(2^32 / group) + 1 (group > 1): (n * group_inv) >> 32 = n / group for n < 2^32 / group
   // layout of a K or V tile in shared memory: 8-row groups of 128-byte rows, `group_step` bytes apart, the second 64
-  // columns `panel_step` bytes behind the first.  boxes: copies per page (1: both panels at once); page_groups8: 8-row
-  // groups of the tensor maps from one page to the next, and outside: a group beyond the cache
+  // columns `panel_step` bytes behind the first.  boxes: copies per page (1: both panels at once); page8: 8-row groups of
+  // the tensor maps from one page to the next, outside: a group beyond the cache
   uint32_t group_step, panel_step;
   int boxes, k_page8, v_page8, k_outside, v_outside;
   int causal, window;  // window < 0: unlimited
+  int narrow_max;      // sequences with at most this many rows belong to the narrow kernel
   float sl2;
   float* part_o;       // [2 slots per CTA][part_rows][DP]
   float2* part_ml;     // [2 slots per CTA][part_rows]: reference (log2 domain) and sum
@@ -77,10 +86,24 @@ struct PaItem {
 template <int PANELS> struct PaCfg {
   static constexpr int DP = PANELS * 64;
   static constexpr int TILE_BYTES = PANELS * PA_PANEL;
-  static constexpr int STAGES = PANELS == 2 ? 5 : 12;
-  static constexpr int DATA = TILE_BYTES * (2 + STAGES);  // 224 KiB
-  static constexpr int SMEM = DATA + 2048 + 1024;         // (m, l) exchange and control words
+  static constexpr int STAGES = PANELS == 2 ? 5 : 10;
+  // wide: two slots of 128 query rows; narrow: two slots of 64 query rows and P of each group, [128 keys][64 rows]
+  static constexpr int FRONT = 65536;
+  static constexpr int DATA = FRONT + STAGES * TILE_BYTES;  // 224 KiB
+  static constexpr int SMEM = DATA + 2048 + 1024;           // exchange between the softmax warps, control words
 };
+
+template <int STAGES> struct PaCtrl {
+  uint64_t full[STAGES], empty[STAGES];  // ring
+  uint64_t q_full[2], q_empty[2];
+  uint64_t s_full[4], p_full[2], p_empty[2], o_full[2], merge[8], vote[2], fin, epi_done;
+  uint64_t item_full[PA_ITEMS], item_empty[PA_ITEMS];
+  PaItem items[PA_ITEMS];
+  alignas(16) int need[2][2][4];  // narrow: [group][round parity][warp]
+  uint32_t tmem_slot;
+  int abort;
+};
+static_assert(sizeof(PaCtrl<10>) <= 1024, "control words");
 
 __device__ __forceinline__ float pa_exp2(float x) {
   float y;
@@ -108,41 +131,23 @@ __device__ __forceinline__ void pa_tma_5d(uint32_t dst, const void* tmap, uint64
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   return __all_sync(0xffffffffu, sb::mbar_wait(bar, parity, abort_flag));
 }
-// tcgen05 instructions of one elected lane, predicated instead of branched around: the warp stays converged, so that
-// descriptors and addresses, which are the same in all lanes, live in uniform registers.
-// D[tmem] (+)= A[smem] * B[smem]
-__device__ __forceinline__ void pa_umma_ss(uint32_t leader, uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                           uint32_t accumulate) {
-  asm volatile(
-      "{\n"
-      ".reg .pred p, q;\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "setp.ne.b32 q, %5, 0;\n"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
-      "}\n" ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
-      : "memory");
-}
 // D[tmem] (+)= A[tmem] * B[smem]: A holds two 16-bit values of a row per 32-bit column
-__device__ __forceinline__ void pa_umma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
-                                           uint32_t accumulate) {
+__device__ __forceinline__ void pa_umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n"
-      ".reg .pred p, q;\n"
+      ".reg .pred p;\n"
       "setp.ne.b32 p, %4, 0;\n"
-      "setp.ne.b32 q, %5, 0;\n"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
-      "}\n" ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n" ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// the barrier is reached once all MMAs issued so far by the leader are complete
-__device__ __forceinline__ void pa_commit(uint32_t leader, uint64_t* bar) {
-  asm volatile(
-      "{\n"
-      ".reg .pred q;\n"
-      "setp.ne.b32 q, %1, 0;\n"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
-      "}\n" ::"r"(sb::smem_u32(bar)), "r"(leader)
-      : "memory");
+template <int N> __device__ __forceinline__ void pa_tmem_ld8(uint32_t taddr, uint32_t (&r)[N], int at) {
+  static_assert(N >= 8, "");
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[at]), "=r"(r[at + 1]), "=r"(r[at + 2]), "=r"(r[at + 3]), "=r"(r[at + 4]), "=r"(r[at + 5]),
+                 "=r"(r[at + 6]), "=r"(r[at + 7])
+               : "r"(taddr)
+               : "memory");
 }
 template <int N> __device__ __forceinline__ void pa_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void pa_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -160,6 +165,15 @@ __device__ __forceinline__ void pa_tmem_st32(uint32_t taddr, const uint32_t* r) 
 __device__ __forceinline__ void pa_cp16(uint32_t dst, const void* src, bool take) {  // zeros when !take
   const int bytes = take ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void pa_tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 
 // ------------------------------------------------------------------------------------------------ work line
@@ -181,22 +195,28 @@ __device__ __forceinline__ PaSeq pa_seq(const PaParams& p, int b) {
 // n / group for n < group + 256
 __device__ __forceinline__ int pa_div(const PaParams& p, int n) { return p.group == 1 ? n : (int)__umulhi(n, p.group_inv); }
 // keys that some row of item m sees
-__device__ __forceinline__ void pa_item_keys(const PaParams& p, int n, int L, int m, int& lo, int& hi) {
+template <bool NARROW> __device__ __forceinline__ void pa_item_keys(const PaParams& p, int n, int L, int m, int& lo, int& hi) {
+  constexpr int ROWS = NARROW ? PA_NARROW_ROWS : PA_WIDE_ROWS;
   const int rows = n * p.group;
-  const int first = m * PA_ITEM_ROWS / p.group, last = (min(rows, (m + 1) * PA_ITEM_ROWS) - 1) / p.group;
+  const int first = m * ROWS / p.group, last = (min(rows, (m + 1) * ROWS) - 1) / p.group;
   const int pos0 = L - n + first, pos1 = L - n + last;
   lo = p.window >= 0 ? max(0, pos0 - p.window) : 0;
   hi = p.causal ? pos1 + 1 : (p.window >= 0 ? (int)min((long)L, (long)pos1 + p.window + 1) : L);
   hi = max(min(hi, L), 0);
 }
-// key tiles of item m, at least one: a row without keys still has to be written
-__device__ __forceinline__ int pa_item_tiles(const PaParams& p, int n, int L, int m) {
+// key tiles between lo and hi, at least one: a row without keys still has to be written
+__device__ __forceinline__ int pa_tiles(int lo, int hi) { return max((hi + PA_TILE - 1) / PA_TILE - lo / PA_TILE, 1); }
+// length of item m on the line
+template <bool NARROW> __device__ __forceinline__ int pa_item_cost(const PaParams& p, int n, int L, int m) {
   int lo, hi;
-  pa_item_keys(p, n, L, m, lo, hi);
-  return max((hi + PA_TILE - 1) / PA_TILE - lo / PA_TILE, 1);
+  pa_item_keys<NARROW>(p, n, L, m, lo, hi);
+  return pa_tiles(lo, hi) + (NARROW ? PA_NARROW_COST : PA_WIDE_COST);
 }
-__device__ __forceinline__ int pa_items(const PaParams& p, int n) {
-  return (n * p.group + PA_ITEM_ROWS - 1) / PA_ITEM_ROWS;
+// items of a sequence of n new tokens in this kernel, per KV head
+template <bool NARROW> __device__ __forceinline__ int pa_items(const PaParams& p, int n) {
+  constexpr int ROWS = NARROW ? PA_NARROW_ROWS : PA_WIDE_ROWS;
+  const int rows = n * p.group;
+  return (rows <= p.narrow_max) == NARROW ? (rows + ROWS - 1) / ROWS : 0;
 }
 __device__ __forceinline__ int pa_scan(int v, int lane) {
 #pragma unroll
@@ -207,43 +227,44 @@ __device__ __forceinline__ int pa_scan(int v, int lane) {
   return v;
 }
 __device__ __forceinline__ int pa_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
-// Tiles of all items of one KV head of sequence 32 * chunk + lane (0 beyond the last sequence); the whole warp calls.
-__device__ __forceinline__ int pa_chunk_tiles(const PaParams& p, int chunk, int lane, PaSeq& s) {
+// Length of all items of one KV head of sequence 32 * chunk + lane (0 beyond the last sequence); the whole warp calls.
+template <bool NARROW> __device__ __forceinline__ int pa_chunk_cost(const PaParams& p, int chunk, int lane, PaSeq& s) {
   const int b = chunk * 32 + lane;
   s = PaSeq{0, 0, 0};
   if (b < p.batch) s = pa_seq(p, b);
-  const int items = pa_items(p, s.n);
-  int tiles = items == 1 ? pa_item_tiles(p, s.n, s.L, 0) : 0;
+  const int items = pa_items<NARROW>(p, s.n);
+  int cost = items == 1 ? pa_item_cost<NARROW>(p, s.n, s.L, 0) : 0;
   unsigned many = __ballot_sync(0xffffffffu, items > 1);
-  while (many) {  // long chunks: the warp shares the items of one sequence
+  while (many) {  // the warp shares the items of one sequence
     const int src = __ffs(many) - 1;
     many &= many - 1;
     const int n = __shfl_sync(0xffffffffu, s.n, src), L = __shfl_sync(0xffffffffu, s.L, src);
-    const int cnt = pa_items(p, n);
+    const int cnt = pa_items<NARROW>(p, n);
     int sum = 0;
-    for (int m = lane; m < cnt; m += 32) sum += pa_item_tiles(p, n, L, m);
+    for (int m = lane; m < cnt; m += 32) sum += pa_item_cost<NARROW>(p, n, L, m);
     sum = pa_sum(sum);
-    if (lane == src) tiles = sum;
+    if (lane == src) cost = sum;
   }
-  return tiles;
+  return cost;
 }
 
-// The line of `total` tiles is cut into `ctas` pieces of `per` tiles, the first `rest` of them one longer.
+// The line is cut into `ctas` pieces of `per`, the first `rest` of them one longer.
 struct PaCut {
-  int total, ctas, per, rest;
+  int ctas, per, rest;
   __device__ __forceinline__ int start(int c) const { return c * per + min(c, rest); }
-  __device__ __forceinline__ int owner(int tile) const {
+  __device__ __forceinline__ int owner(int place) const {
     const int longer = rest * (per + 1);
-    return tile < longer ? tile / (per + 1) : rest + (tile - longer) / per;
+    return place < longer ? place / (per + 1) : rest + (place - longer) / per;
   }
 };
 struct PaCursor {  // where a CTA's piece of the line starts, and how long it is
   PaSeq s;
-  int seq, hk, m, tile, left, unit;
+  int seq, hk, m, tile, left, place;
   PaCut cut;
 };
 
-// The whole warp; sums[c] = tiles per KV head of sequences 32 c .. 32 c + 31.
+// The whole warp; sums[c] = length per KV head of sequences 32 c .. 32 c + 31.
+template <bool NARROW>
 __device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int chunks, int lane, PaCursor& c) {
   long long all = 0;
   for (int i = lane; i < chunks; i += 32) all += sums[i];
@@ -256,14 +277,16 @@ __device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int 
     return;
   }
   PaCut& cut = c.cut;
-  cut.total = (int)all;
-  cut.ctas = min((int)gridDim.x, (cut.total + 1) / 2);  // two tiles per CTA at least: one for each softmax group
+  const int total = (int)all;
+  // two tiles per CTA at least, one for each softmax group
+  cut.ctas = min((int)gridDim.x, (total + 1) / (2 + (NARROW ? PA_NARROW_COST : PA_WIDE_COST)));
+  if (total > 0) cut.ctas = max(cut.ctas, 1);
   if ((int)blockIdx.x >= cut.ctas) return;
-  cut.per = cut.total / cut.ctas;
-  cut.rest = cut.total - cut.per * cut.ctas;
-  c.unit = cut.start(blockIdx.x);
+  cut.per = total / cut.ctas;
+  cut.rest = total - cut.per * cut.ctas;
+  c.place = cut.start(blockIdx.x);
   c.left = cut.per + ((int)blockIdx.x < cut.rest);
-  int off = c.unit, chunk = 0;
+  int off = c.place, chunk = 0;
   if (chunks > 1) {
     for (int base = 0; base < chunks; base += 32) {
       const int v = base + lane < chunks ? sums[base + lane] * p.Hkv : 0, inc = pa_scan(v, lane);
@@ -278,19 +301,19 @@ __device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int 
     }
   }
   PaSeq s;
-  const int tiles = pa_chunk_tiles(p, chunk, lane, s), v = tiles * p.Hkv, inc = pa_scan(v, lane);
+  const int cost = pa_chunk_cost<NARROW>(p, chunk, lane, s), v = cost * p.Hkv, inc = pa_scan(v, lane);
   const int k = __ffs(__ballot_sync(0xffffffffu, inc > off)) - 1;
   off -= __shfl_sync(0xffffffffu, inc - v, k);
-  const int per_head = __shfl_sync(0xffffffffu, tiles, k);
+  const int per_head = __shfl_sync(0xffffffffu, cost, k);
   c.s = PaSeq{__shfl_sync(0xffffffffu, s.row0, k), __shfl_sync(0xffffffffu, s.n, k), __shfl_sync(0xffffffffu, s.L, k)};
   c.seq = chunk * 32 + k;
   c.hk = off / per_head;
   off -= c.hk * per_head;
-  const int items = pa_items(p, c.s.n);
+  const int items = pa_items<NARROW>(p, c.s.n);
   c.tile = off;
   if (items > 1) {
     for (int base = 0; base < items; base += 32) {
-      const int t = base + lane < items ? pa_item_tiles(p, c.s.n, c.s.L, base + lane) : 0, ti = pa_scan(t, lane);
+      const int t = base + lane < items ? pa_item_cost<NARROW>(p, c.s.n, c.s.L, base + lane) : 0, ti = pa_scan(t, lane);
       const unsigned hit = __ballot_sync(0xffffffffu, ti > off);
       if (hit) {
         const int j = __ffs(hit) - 1;
@@ -303,269 +326,309 @@ __device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int 
   }
 }
 
-// Places of K and V tiles of an item in the ring: `lead` K tiles run ahead of V (1 with two_q, else 2: both groups need
-// their first S before the first V), then V and K alternate - the order in which the MMA warp takes them.
+// Places of K and V tiles of an item in the ring: `lead` K tiles run ahead of V, then V and K alternate - the order in which
+// the MMA warp takes them (narrow: 4; wide: 1 with two_q, else 2, the first S of both groups).
 __device__ __forceinline__ uint32_t pa_k_place(int t, int lead) { return t < lead ? t : 2 * t - lead + 1; }
 __device__ __forceinline__ uint32_t pa_v_place(int t, int lead, int count) { return t + min(t + lead, count); }
+template <bool NARROW> __device__ __forceinline__ int pa_lead(int rows) { return NARROW ? 4 : rows > PA_TILE ? 1 : 2; }
 
-// ============================================================================ main kernel
-template <int PANELS, bool F16>
-__global__ void __launch_bounds__(PA_THREADS, 1)
-    pa_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PaParams p) {
-  using Cfg = PaCfg<PANELS>;
-  constexpr int DP = Cfg::DP, TILE_BYTES = Cfg::TILE_BYTES, STAGES = Cfg::STAGES;
-  constexpr uint32_t S_COL = 0, O_COL = 256;  // two S buffers of 128 columns, two O of DP
-  extern __shared__ __align__(1024) uint8_t smem[];
-  uint8_t* sQ = smem;                          // two slots of 128 rows
-  uint8_t* sRing = smem + 2 * TILE_BYTES;
-  float2* xml = reinterpret_cast<float2*>(smem + Cfg::DATA);  // [group][row]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::DATA + 2048);
-  uint64_t* full = bars;                       // STAGES
-  uint64_t* empty = full + STAGES;             // STAGES
-  uint64_t* q_full = empty + STAGES;           // 2
-  uint64_t* q_empty = q_full + 2;              // 2
-  uint64_t* s_full = q_empty + 2;              // 2
-  uint64_t* p_full = s_full + 2;               // 2
-  uint64_t* o_full = p_full + 2;               // 2
-  uint64_t* epi_done = o_full + 2;             // 1
-  uint64_t* merge = epi_done + 1;              // [group][quadrant]
-  uint64_t* item_full = merge + 8;             // PA_ITEMS
-  uint64_t* item_empty = item_full + PA_ITEMS; // PA_ITEMS
-  PaItem* items = reinterpret_cast<PaItem*>(item_empty + PA_ITEMS);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + PA_ITEMS);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((2 * STAGES + 11 + 8 + 2 * PA_ITEMS) * 8 + PA_ITEMS * sizeof(PaItem) + 8 <= 1024, "control words");
-
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (sb::smem_u32(smem) & 1023) {  // the swizzled tiles need it; dynamic shared memory starts on such a boundary
-    if (threadIdx.x == 0) *p.status = SB_ERR_BAD_ARG;
-    return;
-  }
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < STAGES; ++i) {
-      sb::mbar_init(&full[i], 1);
-      sb::mbar_init(&empty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      sb::mbar_init(&q_full[i], 1);
-      sb::mbar_init(&q_empty[i], 1);
-      sb::mbar_init(&s_full[i], 1);
-      sb::mbar_init(&p_full[i], 4);
-      sb::mbar_init(&o_full[i], 1);
-    }
-    sb::mbar_init(epi_done, 8);
-    for (int i = 0; i < 8; ++i) sb::mbar_init(&merge[i], 1);
-    for (int i = 0; i < PA_ITEMS; ++i) {
-      sb::mbar_init(&item_full[i], 1);
-      sb::mbar_init(&item_empty[i], 10);
-    }
-    *abort_flag = 0;
-    sb::mbar_fence_init();
-  }
-  if (warp == 9) {
-    sb::tmem_alloc(tmem_slot, 512);
-    sb::tmem_relinquish();
-  }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // tiles of 32 sequences at a time, where the scheduler puts the queries afterwards
-  int* sums = reinterpret_cast<int*>(sQ);
-  const int chunks = (p.batch + 31) / 32;
-  for (int c = warp; c < chunks; c += PA_WARPS) {
-    PaSeq s;
-    const int t = pa_sum(pa_chunk_tiles(p, c, lane, s));
-    if (lane == 0) sums[c] = t;
-  }
-  sb::tc_fence_before();
-  __syncthreads();
-  sb::tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-
-  if (warp >= 8) {
-  pa_regs_dec<PA_REGS_FEW>();  // one instruction for the whole warpgroup
-  if (warp == 10) {
-    // ------------------------------------------------------------------ scheduler and query loads
-    PaCursor cur;
-    pa_find(p, sums, chunks, lane, cur);
-    __syncwarp();
-    int* desc = p.part_desc + 8 * blockIdx.x;
-    bool starts = false, ok = true;
-    int q_cnt = 0;
-    for (int i = 0; ok; ++i) {
-      const int slot = i % PA_ITEMS;
-      if (!pa_wait(&item_empty[slot], ((i / PA_ITEMS) & 1) ^ 1, abort_flag)) break;
-      PaItem it = {};
-      int tiles = 0;
-      if (cur.left > 0) {
-        int lo, hi;
-        pa_item_keys(p, cur.s.n, cur.s.L, cur.m, lo, hi);
-        tiles = max((hi + PA_TILE - 1) / PA_TILE - lo / PA_TILE, 1);
+// ============================================================================ roles that both kernels share
+// Warp 10: cuts the piece into items, publishes their descriptors and copies their queries.
+template <bool NARROW, int PANELS>
+__device__ __forceinline__ void pa_schedule(const PaParams& p, PaCtrl<PaCfg<PANELS>::STAGES>& c, uint8_t* sQ, int chunks,
+                                            int lane) {
+  constexpr int DP = PANELS * 64, COST = NARROW ? PA_NARROW_COST : PA_WIDE_COST;
+  constexpr int ROWS = NARROW ? PA_NARROW_ROWS : PA_WIDE_ROWS;
+  constexpr int SLOT_ROWS = NARROW ? PA_NARROW_ROWS : PA_TILE, SLOT_BYTES = PANELS * SLOT_ROWS * 128;
+  volatile int* abort_flag = &c.abort;
+  PaCursor cur;
+  pa_find<NARROW>(p, reinterpret_cast<const int*>(sQ), chunks, lane, cur);
+  __syncwarp();
+  int* desc = p.part_desc + 8 * blockIdx.x;
+  bool starts = false, ok = true;
+  int q_cnt = 0;
+  for (int i = 0; ok; ++i) {
+    const int slot = i % PA_ITEMS;
+    if (!pa_wait(&c.item_empty[slot], ((i / PA_ITEMS) & 1) ^ 1, abort_flag)) break;
+    PaItem it = {};
+    int lo, hi, tiles = 0;
+    while (cur.left > 0) {  // the next item with a tile in this piece
+      pa_item_keys<NARROW>(p, cur.s.n, cur.s.L, cur.m, lo, hi);
+      tiles = pa_tiles(lo, hi);
+      if (cur.tile < tiles) {
         const int take = min(tiles - cur.tile, cur.left);
         const bool first = cur.tile == 0, last = cur.tile + take == tiles;
-        const int tok0 = cur.m * PA_ITEM_ROWS / p.group;
+        const int tok0 = cur.m * ROWS / p.group;
         it = PaItem{cur.s.row0 + tok0, cur.s.L - cur.s.n + tok0, cur.s.L, cur.seq, cur.hk,
-                    min(cur.s.n * p.group - cur.m * PA_ITEM_ROWS, PA_ITEM_ROWS), cur.m * PA_ITEM_ROWS - tok0 * p.group,
+                    min(cur.s.n * p.group - cur.m * ROWS, ROWS), cur.m * ROWS - tok0 * p.group,
                     lo / PA_TILE + cur.tile, take, lo, hi,
                     first && last ? -1 : 2 * (int)blockIdx.x + (first ? 1 : 0)};
         if (first && !last) {  // the CTA that starts an item names the one that ends it
           starts = true;
           if (lane == 0) {
             desc[1] = it.row0; desc[2] = it.rem; desc[3] = it.hk; desc[4] = it.rows;
-            desc[5] = cur.cut.owner(cur.unit + tiles - 1);
+            desc[5] = cur.cut.owner(cur.place + tiles - 1);
           }
         }
-        cur.left -= take;
-        cur.unit += take;
       }
-      if (lane == 0) {
-        items[slot] = it;
-        sb::mbar_arrive(&item_full[slot]);
-      }
-      if (it.count == 0) break;
-      // queries of the item: one slot, or two of them, as 16-byte chunks in the swizzled K-major layout
-      const int slots = it.rows > PA_TILE ? 2 : 1;
-      for (int x = 0; x < slots; ++x) {
-        const int qs = (q_cnt + x) & 1;
-        ok = pa_wait(&q_empty[qs], (((q_cnt + x) >> 1) & 1) ^ 1, abort_flag);
-        if (!ok) break;
-        constexpr int CH = DP / 8;  // chunks per row
-        const int ch = lane % CH, live = min(it.rows - x * PA_TILE, PA_TILE), end = (live + 31) & ~31;
-        const uint32_t dst = sb::smem_u32(sQ + qs * TILE_BYTES) + (ch >> 3) * PA_PANEL;
-        const uint16_t* base = reinterpret_cast<const uint16_t*>(p.q) + (long)it.row0 * p.q_tok +
-                               (long)it.hk * p.group * p.q_head + ch * 8;
-        // whole warps of rows: lanes without a row read zeros
-#pragma unroll 4
-        for (int r = lane / CH; r < end; r += 32 / CH) {
-          const int row = it.rem + x * PA_TILE + r, t = pa_div(p, row), h = row - t * p.group;
-          const bool take = r < live && ch * 8 < p.D;
-          pa_cp16(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4),
-                  take ? base + (long)t * p.q_tok + (long)h * p.q_head : reinterpret_cast<const uint16_t*>(p.q), take);
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        sb::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) sb::mbar_arrive(&q_full[qs]);
-      }
-      q_cnt += slots;
+      const int used = min(tiles + COST - cur.tile, cur.left);
+      cur.left -= used;
+      cur.place += used;
       cur.tile = 0;
-      if (cur.left > 0 && ++cur.m == pa_items(p, cur.s.n)) {
+      if (cur.left > 0 && ++cur.m == pa_items<NARROW>(p, cur.s.n)) {
         cur.m = 0;
         if (++cur.hk == p.Hkv) {
           cur.hk = 0;
-          do { cur.s = pa_seq(p, ++cur.seq); } while (cur.s.n == 0 && cur.seq + 1 < p.batch);
+          do { cur.s = pa_seq(p, ++cur.seq); } while (pa_items<NARROW>(p, cur.s.n) == 0 && cur.seq + 1 < p.batch);
         }
       }
+      if (it.count) break;
     }
-    if (lane == 0) desc[0] = starts && ok;
-  } else if (warp != 9) {
-    // ------------------------------------------------------------------ K tiles (warp 8), V tiles (warp 11)
-    const bool is_v = warp == 11;
-    const CUtensorMap* tm = is_v ? &tmV : &tmK;
-    if (lane == 0) sb::tma_prefetch_desc(tm);
-    const int page = 1 << p.page_shift;
-    const int box = min(page, PA_TILE), per_tile = PA_TILE / box;  // rows per copy, pages per tile
-    const int bi = lane % per_tile, pn = lane / per_tile;          // this lane's page of the tile, and its panel
-    const int page8 = is_v ? p.v_page8 : p.k_page8, outside = is_v ? p.v_outside : p.k_outside;
-    const uint32_t dst = sb::smem_u32(sRing) + bi * (box >> 3) * p.group_step + pn * p.panel_step;
-    uint32_t ring = 0;
-    bool ok = true;
-    for (int i = 0; ok; ++i) {
-      const int slot = i % PA_ITEMS;
-      if (!pa_wait(&item_full[slot], (i / PA_ITEMS) & 1, abort_flag)) break;
-      const PaItem it = items[slot];
-      __syncwarp();
-      if (lane == 0) sb::mbar_arrive(&item_empty[slot]);
-      if (it.count == 0) break;
-      const int lead = it.rows > PA_TILE ? 1 : 2;
-      const int* trow = p.table + (long)it.seq * p.table_ld;
-      int win = -64, where = 0;  // 32 pages at a time: their first 8-row group in the tensor map
-      for (int t = 0; t < it.count; ++t) {
-        const int key0 = (it.tile0 + t) * PA_TILE, page0 = key0 >> p.page_shift;
-        if (page0 + per_tile > win + 32) {
-          win = page0;
-          const int idx = page0 + lane;
-          where = outside;  // a copy from outside the cache reads zeros
-          if (idx < p.cols && ((idx + 1) << p.page_shift) > it.lo && (idx << p.page_shift) < it.hi) {
-            const int got = trow[idx];
-            if (got >= 0 && got < p.num_pages) where = got * page8;
-            else *p.status = SB_ERR_BAD_ARG;  // a visible page outside the cache: reported, its keys read as zeros
-          }
-        }
-        const int first8 = __shfl_sync(0xffffffffu, where, page0 - win + bi);
-        const uint32_t e = ring + (is_v ? pa_v_place(t, lead, it.count) : pa_k_place(t, lead)), st = e % STAGES;
-        ok = pa_wait(&empty[st], ((e / STAGES) & 1) ^ 1, abort_flag);
-        if (!ok) break;
-        if (lane == 0) sb::mbar_expect_tx(&full[st], TILE_BYTES);
-        __syncwarp();
-        if (pn < p.boxes)
-          pa_tma_5d(dst + st * TILE_BYTES, tm, &full[st], pn * 64, first8 + ((key0 & (page - 1)) >> 3), it.hk);
-      }
-      ring += 2 * it.count;
+    if (lane == 0) {
+      c.items[slot] = it;
+      sb::mbar_arrive(&c.item_full[slot]);
     }
-  } else {
-    // ------------------------------------------------------------------ MMA issue
-    const uint32_t leader = lane == 0;
-    const uint32_t idesc_s = sb::umma_idesc_f16(PA_TILE, PA_TILE, F16 ? 0 : 1, 0, 0);  // K-major both
-    const uint32_t idesc_o = sb::umma_idesc_f16(PA_TILE, DP, F16 ? 0 : 1, 0, 1);       // V is MN-major
-    const uint64_t q_desc = sb::umma_smem_desc(sb::smem_u32(sQ), 16, 1024);
-    const uint64_t k_desc = sb::umma_smem_desc(sb::smem_u32(sRing), 16, p.group_step);
-    const uint64_t v_desc = sb::umma_smem_desc(sb::smem_u32(sRing), p.panel_step, p.group_step);
-    const uint32_t k_panel = p.panel_step >> 4, v_step = (2 * p.group_step) >> 4;  // descriptors count 16-byte units
-    uint32_t ring = 0, p_cnt0 = 0, p_cnt1 = 0;
-    int q_cnt = 0;
-    bool ok = true;
-    for (int i = 0; ok; ++i) {
-      const int slot = i % PA_ITEMS;
-      if (!pa_wait(&item_full[slot], (i / PA_ITEMS) & 1, abort_flag)) break;
-      const int count = __shfl_sync(0xffffffffu, items[slot].count, 0);
-      const int two_q = __shfl_sync(0xffffffffu, items[slot].rows > PA_TILE, 0);
-      if (lane == 0) sb::mbar_arrive(&item_empty[slot]);
-      if (count == 0) break;
-      const int lead = two_q ? 1 : 2, n = two_q ? 2 * count : count;
-      ok = pa_wait(&q_full[q_cnt & 1], (q_cnt >> 1) & 1, abort_flag);
-      if (ok && two_q) ok = pa_wait(&q_full[(q_cnt + 1) & 1], ((q_cnt + 1) >> 1) & 1, abort_flag);
+    if (it.count == 0) break;
+    // queries: one slot, or two of them, as 16-byte chunks in the swizzled K-major layout, rows up to the next full block
+    const int slots = it.rows > SLOT_ROWS ? 2 : 1;
+    for (int x = 0; x < slots; ++x) {
+      const int qs = (q_cnt + x) & 1;
+      ok = pa_wait(&c.q_empty[qs], (((q_cnt + x) >> 1) & 1) ^ 1, abort_flag);
       if (!ok) break;
-      // virtual tile v: group v & 1; key tile v (one query slot) or v / 2 (two)
-      auto issue_s = [&](int v) -> bool {
-        const uint32_t e = ring + pa_k_place(two_q ? v >> 1 : v, lead), st = e % STAGES;
-        if (!pa_wait(&full[st], (e / STAGES) & 1, abort_flag)) return false;
-        sb::tc_fence_after();
-        const int qs = (q_cnt + (two_q ? v & 1 : 0)) & 1;
-        const uint64_t qd = q_desc + qs * (TILE_BYTES >> 4), kd = k_desc + st * (TILE_BYTES >> 4);
-        const uint32_t d = tmem_base + S_COL + (v & 1) * PA_TILE;
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk)
-          pa_umma_ss(leader, d, qd + (kk >> 2) * (PA_PANEL >> 4) + (kk & 3) * 2, kd + (kk >> 2) * k_panel + (kk & 3) * 2,
-                     idesc_s, kk != 0);
-        pa_commit(leader, &s_full[v & 1]);
-        if (!two_q || (v & 1)) pa_commit(leader, &empty[st]);
-        if (two_q ? v >= n - 2 : v == n - 1) pa_commit(leader, &q_empty[qs]);
-        return true;
-      };
-      ok = issue_s(0);
-      if (ok && n > 1) ok = issue_s(1);
-      for (int v = 0; v < n && ok; ++v) {
-        const int x = v & 1;
-        const uint32_t e = ring + pa_v_place(two_q ? v >> 1 : v, lead, count), st = e % STAGES;
-        ok = pa_wait(&p_full[x], (x ? p_cnt1 : p_cnt0) & 1, abort_flag) && pa_wait(&full[st], (e / STAGES) & 1, abort_flag);
-        if (ok && v == 0 && i > 0) ok = pa_wait(epi_done, (i - 1) & 1, abort_flag);  // O of the item before is read
-        if (!ok) break;
-        if (x) ++p_cnt1; else ++p_cnt0;
-        sb::tc_fence_after();
-        const uint64_t vd = v_desc + st * (TILE_BYTES >> 4);
-        const uint32_t pa = tmem_base + S_COL + x * PA_TILE, d = tmem_base + O_COL + x * DP;
-#pragma unroll
-        for (int kk = 0; kk < PA_TILE / 16; ++kk)
-          pa_umma_ts(leader, d, pa + kk * 8, vd + kk * v_step, idesc_o, v > 1 || kk != 0);
-        if (!two_q || x) pa_commit(leader, &empty[st]);
-        if (v + 2 >= n) pa_commit(leader, &o_full[x]);
-        if (v + 2 < n) ok = issue_s(v + 2);
+      constexpr int CH = DP / 8;  // chunks per row
+      const int ch = lane % CH, live = min(it.rows - x * SLOT_ROWS, SLOT_ROWS), end = NARROW ? (live + 15) & ~15 : (live + 31) & ~31;
+      const uint32_t dst = sb::smem_u32(sQ + qs * SLOT_BYTES) + (ch >> 3) * (SLOT_ROWS * 128);
+      const uint16_t* base = reinterpret_cast<const uint16_t*>(p.q) + (long)it.row0 * p.q_tok +
+                             (long)it.hk * p.group * p.q_head + ch * 8;
+#pragma unroll 4
+      for (int r = lane / CH; r < end; r += 32 / CH) {
+        const int row = it.rem + x * SLOT_ROWS + r, t = pa_div(p, row), h = row - t * p.group;
+        const bool take = r < live && ch * 8 < p.D;
+        pa_cp16(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4),
+                take ? base + (long)t * p.q_tok + (long)h * p.q_head : reinterpret_cast<const uint16_t*>(p.q), take);
       }
-      ring += 2 * count;
-      q_cnt += 1 + two_q;
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      sb::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) sb::mbar_arrive(&c.q_full[qs]);
     }
+    q_cnt += slots;
   }
+  if (lane == 0) desc[0] = starts && ok;
+}
+
+// Warps 8 (K) and 11 (V).
+template <bool NARROW, int PANELS>
+__device__ __forceinline__ void pa_load(const PaParams& p, PaCtrl<PaCfg<PANELS>::STAGES>& c, uint8_t* sRing,
+                                        const CUtensorMap* tm, bool is_v, int lane) {
+  constexpr int STAGES = PaCfg<PANELS>::STAGES, TILE_BYTES = PaCfg<PANELS>::TILE_BYTES;
+  volatile int* abort_flag = &c.abort;
+  if (lane == 0) sb::tma_prefetch_desc(tm);
+  const int page = 1 << p.page_shift;
+  const int box = min(page, PA_TILE), per_tile = PA_TILE / box;  // rows per copy, pages per tile
+  const int bi = lane % per_tile, pn = lane / per_tile;          // this lane's page of the tile, and its panel
+  const int page8 = is_v ? p.v_page8 : p.k_page8, outside = is_v ? p.v_outside : p.k_outside;
+  const uint32_t dst = sb::smem_u32(sRing) + bi * (box >> 3) * p.group_step + pn * p.panel_step;
+  uint32_t ring = 0;
+  bool ok = true;
+  for (int i = 0; ok; ++i) {
+    const int slot = i % PA_ITEMS;
+    if (!pa_wait(&c.item_full[slot], (i / PA_ITEMS) & 1, abort_flag)) break;
+    const PaItem it = c.items[slot];
+    __syncwarp();
+    if (lane == 0) sb::mbar_arrive(&c.item_empty[slot]);
+    if (it.count == 0) break;
+    const int lead = pa_lead<NARROW>(it.rows);
+    const int* trow = p.table + (long)it.seq * p.table_ld;
+    int win = -64, where = 0;  // 32 pages at a time: their first 8-row group in the tensor map
+    for (int t = 0; t < it.count; ++t) {
+      const int key0 = (it.tile0 + t) * PA_TILE, page0 = key0 >> p.page_shift;
+      if (page0 + per_tile > win + 32) {
+        win = page0;
+        const int idx = page0 + lane;
+        where = outside;  // a copy from outside the cache reads zeros
+        if (idx < p.cols && ((idx + 1) << p.page_shift) > it.lo && (idx << p.page_shift) < it.hi) {
+          const int got = trow[idx];
+          if (got >= 0 && got < p.num_pages) where = got * page8;
+          else *p.status = SB_ERR_BAD_ARG;  // a visible page outside the cache: reported, its keys read as zeros
+        }
+      }
+      const int first8 = __shfl_sync(0xffffffffu, where, page0 - win + bi);
+      const uint32_t e = ring + (is_v ? pa_v_place(t, lead, it.count) : pa_k_place(t, lead)), st = e % STAGES;
+      ok = pa_wait(&c.empty[st], ((e / STAGES) & 1) ^ 1, abort_flag);
+      if (!ok) break;
+      if (lane == 0) sb::mbar_expect_tx(&c.full[st], TILE_BYTES);
+      __syncwarp();
+      if (pn < p.boxes)
+        pa_tma_5d(dst + st * TILE_BYTES, tm, &c.full[st], pn * 64, first8 + ((key0 & (page - 1)) >> 3), it.hk);
+    }
+    ring += 2 * it.count;
+  }
+}
+
+// Values behind the last visible key may be anything, NaN included, and 0 * NaN is NaN: row r of a V tile in shared memory
+// becomes zeros.
+template <int PANELS> __device__ __forceinline__ void pa_zero_v_row(const PaParams& p, uint8_t* tile, int r) {
+  uint8_t* dst = tile + (r >> 3) * p.group_step + (r & 7) * 128;
+#pragma unroll
+  for (int c = 0; c < PANELS * 8; ++c)
+    *reinterpret_cast<uint4*>(dst + (c >> 3) * p.panel_step + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// Barriers, TMEM and the lengths of 32 sequences at a time (left where the scheduler puts the queries afterwards).
+// Returns false if shared memory does not start on a 1024-byte boundary, as the swizzled tiles need.
+template <bool NARROW, int STAGES>
+__device__ __forceinline__ bool pa_begin(const PaParams& p, PaCtrl<STAGES>& c, uint8_t* smem, int warp, int lane) {
+  if (sb::smem_u32(smem) & 1023) {
+    if (threadIdx.x == 0) *p.status = SB_ERR_BAD_ARG;
+    return false;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      sb::mbar_init(&c.full[i], 1);
+      sb::mbar_init(&c.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      sb::mbar_init(&c.q_full[i], 1);
+      sb::mbar_init(&c.q_empty[i], 1);
+      sb::mbar_init(&c.p_full[i], 4);
+      sb::mbar_init(&c.p_empty[i], 1);
+      sb::mbar_init(&c.o_full[i], 1);
+      sb::mbar_init(&c.vote[i], 4);
+    }
+    for (int i = 0; i < 4; ++i) sb::mbar_init(&c.s_full[i], 1);
+    for (int i = 0; i < 8; ++i) sb::mbar_init(&c.merge[i], 1);
+    sb::mbar_init(&c.fin, 8);
+    sb::mbar_init(&c.epi_done, 8);
+    for (int i = 0; i < PA_ITEMS; ++i) {
+      sb::mbar_init(&c.item_full[i], 1);
+      sb::mbar_init(&c.item_empty[i], 11);  // two loaders, the MMA warp, eight softmax warps
+    }
+    c.abort = 0;
+    sb::mbar_fence_init();
+  }
+  if (warp == 9) {
+    sb::tmem_alloc(&c.tmem_slot, 512);
+    sb::tmem_relinquish();
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  int* sums = reinterpret_cast<int*>(smem);
+  const int chunks = (p.batch + 31) / 32;
+  for (int k = warp; k < chunks; k += PA_WARPS) {
+    PaSeq s;
+    const int t = pa_sum(pa_chunk_cost<NARROW>(p, k, lane, s));
+    if (lane == 0) sums[k] = t;
+  }
+  sb::tc_fence_before();
+  __syncthreads();
+  sb::tc_fence_after();
+  return true;
+}
+template <int STAGES> __device__ __forceinline__ void pa_end(const PaParams& p, PaCtrl<STAGES>& c, int warp) {
+  __syncwarp();
+  volatile int* abort_flag = &c.abort;
+  if (*abort_flag) {
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies and MMAs in flight end
+  }
+  sb::tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    sb::tc_fence_after();
+    sb::tmem_dealloc(c.tmem_slot, 512);
+  }
+  if (threadIdx.x == 0 && *abort_flag) *p.status = SB_ERR_WAIT_TIMEOUT;
+}
+
+// ============================================================================ wide kernel
+template <int PANELS, bool F16>
+__global__ void __launch_bounds__(PA_THREADS, 1)
+    pa_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PaParams p) {
+  using Cfg = PaCfg<PANELS>;
+  constexpr int DP = Cfg::DP, TILE_BYTES = Cfg::TILE_BYTES, STAGES = Cfg::STAGES;
+  constexpr uint32_t S_COL = 0, O_COL = 256;  // two S buffers of 128 columns, two O of DP
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* sQ = smem;  // two slots of 128 rows
+  uint8_t* sRing = smem + Cfg::FRONT;
+  float2* xml = reinterpret_cast<float2*>(smem + Cfg::DATA);  // [group][row]
+  PaCtrl<STAGES>& c = *reinterpret_cast<PaCtrl<STAGES>*>(smem + Cfg::DATA + 2048);
+  volatile int* abort_flag = &c.abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (!pa_begin<false>(p, c, smem, warp, lane)) return;
+  const uint32_t tmem_base = c.tmem_slot;
+
+  if (warp >= 8) {
+    pa_regs_dec<PA_REGS_FEW>();  // one instruction for the whole warpgroup
+    if (warp == 10) {
+      pa_schedule<false, PANELS>(p, c, sQ, (p.batch + 31) / 32, lane);
+    } else if (warp != 9) {
+      pa_load<false, PANELS>(p, c, sRing, warp == 11 ? &tmV : &tmK, warp == 11, lane);
+    } else if (lane == 0) {
+      const uint32_t idesc_s = sb::umma_idesc_f16(PA_TILE, PA_TILE, F16 ? 0 : 1, 0, 0);  // K-major both
+      const uint32_t idesc_o = sb::umma_idesc_f16(PA_TILE, DP, F16 ? 0 : 1, 0, 1);       // V is MN-major
+      const uint64_t q_desc = sb::umma_smem_desc(sb::smem_u32(sQ), 16, 1024);
+      const uint64_t k_desc = sb::umma_smem_desc(sb::smem_u32(sRing), 16, p.group_step);
+      const uint64_t v_desc = sb::umma_smem_desc(sb::smem_u32(sRing), p.panel_step, p.group_step);
+      const uint32_t k_panel = p.panel_step >> 4, v_step = (2 * p.group_step) >> 4;  // descriptors count 16-byte units
+      uint32_t ring = 0, p_cnt0 = 0, p_cnt1 = 0;
+      int q_cnt = 0;
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        const int slot = i % PA_ITEMS;
+        if (!sb::mbar_wait(&c.item_full[slot], (i / PA_ITEMS) & 1, abort_flag)) break;
+        const int count = c.items[slot].count, two_q = c.items[slot].rows > PA_TILE;
+        sb::mbar_arrive(&c.item_empty[slot]);
+        if (count == 0) break;
+        const int lead = two_q ? 1 : 2, n = two_q ? 2 * count : count;
+        ok = sb::mbar_wait(&c.q_full[q_cnt & 1], (q_cnt >> 1) & 1, abort_flag);
+        if (ok && two_q) ok = sb::mbar_wait(&c.q_full[(q_cnt + 1) & 1], ((q_cnt + 1) >> 1) & 1, abort_flag);
+        if (!ok) break;
+        // virtual tile v: group v & 1; key tile v (one query slot) or v / 2 (two)
+        auto k_place = [&](int v) -> uint32_t { return ring + pa_k_place(two_q ? v >> 1 : v, lead); };
+        auto wait_ring = [&](uint32_t e) -> bool { return sb::mbar_wait(&c.full[e % STAGES], (e / STAGES) & 1, abort_flag); };
+        auto issue_s = [&](int v) {
+          const uint32_t st = k_place(v) % STAGES;
+          const int qs = (q_cnt + (two_q ? v & 1 : 0)) & 1;
+          const uint64_t qd = q_desc + qs * (TILE_BYTES >> 4), kd = k_desc + st * (TILE_BYTES >> 4);
+          const uint32_t d = tmem_base + S_COL + (v & 1) * PA_TILE;
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk)
+            sb::umma_f16_ss(d, qd + (kk >> 2) * (PA_PANEL >> 4) + (kk & 3) * 2, kd + (kk >> 2) * k_panel + (kk & 3) * 2,
+                            idesc_s, kk != 0);
+          sb::umma_commit(&c.s_full[v & 1]);
+          if (!two_q || (v & 1)) sb::umma_commit(&c.empty[st]);
+          if (two_q ? v >= n - 2 : v == n - 1) sb::umma_commit(&c.q_empty[qs]);
+        };
+        for (int v = 0; v < min(n, 2) && ok; ++v) {
+          ok = wait_ring(k_place(v));
+          if (!ok) break;
+          sb::tc_fence_after();
+          issue_s(v);
+        }
+        for (int v = 0; v < n && ok; ++v) {
+          const int x = v & 1;
+          const uint32_t e = ring + pa_v_place(two_q ? v >> 1 : v, lead, count), st = e % STAGES;
+          // both tiles first, so that nothing is waited for between the probabilities and the 16 products
+          ok = wait_ring(e);
+          if (ok && v + 2 < n) ok = wait_ring(k_place(v + 2));
+          if (ok && v == 0 && i > 0) ok = sb::mbar_wait(&c.epi_done, (i - 1) & 1, abort_flag);  // O of the item before is read
+          ok = ok && sb::mbar_wait(&c.p_full[x], (x ? p_cnt1 : p_cnt0) & 1, abort_flag);
+          if (!ok) break;
+          if (x) ++p_cnt1; else ++p_cnt0;
+          sb::tc_fence_after();
+          const uint64_t vd = v_desc + st * (TILE_BYTES >> 4);
+          const uint32_t pa = tmem_base + S_COL + x * PA_TILE, d = tmem_base + O_COL + x * DP;
+#pragma unroll
+          for (int kk = 0; kk < PA_TILE / 16; ++kk)
+            pa_umma_ts(d, pa + kk * 8, vd + kk * v_step, idesc_o, v > 1 || kk != 0);
+          if (!two_q || x) sb::umma_commit(&c.empty[st]);
+          if (v + 2 >= n) sb::umma_commit(&c.o_full[x]);
+          if (v + 2 < n) issue_s(v + 2);
+        }
+        ring += 2 * count;
+        q_cnt += 1 + two_q;
+      }
+    }
   } else {
-    // ------------------------------------------------------------------ softmax and output
     pa_regs_inc<PA_REGS_MANY>();
     const int x = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16);
@@ -575,10 +638,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     bool ok = true;
     for (int i = 0; ok; ++i) {
       const int islot = i % PA_ITEMS;
-      if (!pa_wait(&item_full[islot], (i / PA_ITEMS) & 1, abort_flag)) break;
-      const PaItem it = items[islot];
+      if (!pa_wait(&c.item_full[islot], (i / PA_ITEMS) & 1, abort_flag)) break;
+      const PaItem it = c.items[islot];
       __syncwarp();
-      if (lane == 0) sb::mbar_arrive(&item_empty[islot]);
+      if (lane == 0) sb::mbar_arrive(&c.item_empty[islot]);
       if (it.count == 0) break;
       const int rows = it.rows;
       const bool two_q = rows > PA_TILE;
@@ -599,22 +662,22 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       for (int v = x; v < n; v += 2) {
         const int t = two_q ? v >> 1 : v;
         const int key0 = (it.tile0 + t) * PA_TILE;
-        if (!pa_wait(&s_full[x], s_cnt & 1, abort_flag)) { ok = false; break; }
+        if (!pa_wait(&c.s_full[x], s_cnt & 1, abort_flag)) { ok = false; break; }
         ++s_cnt;
         sb::tc_fence_after();
         if (warp_rows > 0) {
           uint32_t s[PA_TILE];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) sb::tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(s + c * 32));
+          for (int ch = 0; ch < 4; ++ch) sb::tmem_ld32(s_addr + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(s + ch * 32));
           sb::tmem_ld_wait();
           if (!__all_sync(0xffffffffu, key0 >= lo && key0 + PA_TILE <= hi)) {
 #pragma unroll
-            for (int c = 0; c < PA_TILE; ++c)
-              if (key0 + c < lo || key0 + c >= hi) s[c] = 0xff800000u;  // -inf, whatever the score was
+            for (int ch = 0; ch < PA_TILE; ++ch)
+              if (key0 + ch < lo || key0 + ch >= hi) s[ch] = 0xff800000u;  // -inf, whatever the score was
           }
           float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < PA_TILE; ++c) m4[c & 3] = fmaxf(m4[c & 3], __uint_as_float(s[c]));
+          for (int ch = 0; ch < PA_TILE; ++ch) m4[ch & 3] = fmaxf(m4[ch & 3], __uint_as_float(s[ch]));
           const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
           const bool move = (mx - ref) * sl2 > 8.f || (ref == -INFINITY && mx > -INFINITY);
           if (__any_sync(0xffffffffu, move)) {
@@ -624,30 +687,30 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             l *= alpha;
             if (v >= 2) {  // O holds the tiles before (complete: their MMAs precede this S)
 #pragma unroll
-              for (int c = 0; c < DP / 32; ++c) {
+              for (int ch = 0; ch < DP / 32; ++ch) {
                 uint32_t o[32];
-                sb::tmem_ld32(o_addr + c * 32, o);
+                sb::tmem_ld32(o_addr + ch * 32, o);
                 sb::tmem_ld_wait();
 #pragma unroll
                 for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-                pa_tmem_st32(o_addr + c * 32, o);
+                pa_tmem_st32(o_addr + ch * 32, o);
               }
             }
           }
           const float neg = ref == -INFINITY ? 0.f : -ref * sl2;
           float sum4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int ch = 0; ch < 2; ++ch) {
             uint32_t pk[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
-              const float a = pa_exp2(fmaf(__uint_as_float(s[c * 64 + 2 * j]), sl2, neg));
-              const float b = pa_exp2(fmaf(__uint_as_float(s[c * 64 + 2 * j + 1]), sl2, neg));
+              const float a = pa_exp2(fmaf(__uint_as_float(s[ch * 64 + 2 * j]), sl2, neg));
+              const float b = pa_exp2(fmaf(__uint_as_float(s[ch * 64 + 2 * j + 1]), sl2, neg));
               sum4[(2 * j) & 3] += a;
               sum4[(2 * j + 1) & 3] += b;
               pk[j] = pa_pack<F16>(a, b);
             }
-            pa_tmem_st32(s_addr + c * 32, pk);
+            pa_tmem_st32(s_addr + ch * 32, pk);
           }
           l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
           sb::tmem_st_wait();
@@ -656,24 +719,21 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           // Values behind the last visible key may be anything, NaN included, and 0 * NaN is NaN: their rows of the
           // V tile are zeroed (twice with two_q, which does no harm).  Thread = key row.
           const uint32_t e = ring + pa_v_place(t, lead, it.count), st = e % STAGES;
-          if (!pa_wait(&full[st], (e / STAGES) & 1, abort_flag)) { ok = false; break; }
+          if (!pa_wait(&c.full[st], (e / STAGES) & 1, abort_flag)) { ok = false; break; }
           if (key0 + r >= it.hi) {
-            uint8_t* dst = sRing + st * TILE_BYTES + (r >> 3) * p.group_step + (r & 7) * 128;
-#pragma unroll
-            for (int c = 0; c < PANELS * 8; ++c)
-              *reinterpret_cast<uint4*>(dst + (c >> 3) * p.panel_step + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+            pa_zero_v_row<PANELS>(p, sRing + st * TILE_BYTES, r);
           }
           sb::fence_proxy_async_smem();
         }
         sb::tc_fence_before();
         __syncwarp();
-        if (lane == 0) sb::mbar_arrive(&p_full[x]);
+        if (lane == 0) sb::mbar_arrive(&c.p_full[x]);
       }
       ring += 2 * it.count;
       if (!ok) break;
       const bool mine = x < n;  // this group had a tile
       if (mine) {
-        if (!pa_wait(&o_full[x], o_cnt & 1, abort_flag)) break;
+        if (!pa_wait(&c.o_full[x], o_cnt & 1, abort_flag)) break;
         ++o_cnt;
         sb::tc_fence_after();
       }
@@ -682,12 +742,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       int c0 = 0, c1 = DP / 32;
       const bool both = !two_q && n > 1;
       if (!two_q) {
-        if (i > 0 && !pa_wait(epi_done, (i - 1) & 1, abort_flag)) break;  // xml of the item before is read
+        if (i > 0 && !pa_wait(&c.epi_done, (i - 1) & 1, abort_flag)) break;  // xml of the item before is read
         xml[x * PA_TILE + r] = make_float2(ref, l);
         sb::tc_fence_before();
         __syncwarp();
-        if (lane == 0) sb::mbar_arrive(&merge[x * 4 + quad]);
-        if (!pa_wait(&merge[(x ^ 1) * 4 + quad], merges & 1, abort_flag)) break;
+        if (lane == 0) sb::mbar_arrive(&c.merge[x * 4 + quad]);
+        if (!pa_wait(&c.merge[(x ^ 1) * 4 + quad], merges & 1, abort_flag)) break;
         ++merges;
         sb::tc_fence_after();
         const float2 a = xml[r], b = xml[PA_TILE + r];
@@ -704,17 +764,17 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const float ga = it.slot < 0 ? fa * inv : fa, gb = it.slot < 0 ? fb * inv : fb;
         uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (long)(it.row0 + tok) * p.o_tok + (long)head * p.o_head;
         const long prow = (long)it.slot * p.part_rows + row;
-        for (int c = c0; c < c1; ++c) {
+        for (int ch = c0; ch < c1; ++ch) {
           uint32_t a[32], b[32];
           float o[32];
           if (both) {
-            sb::tmem_ld32(t_lane + O_COL + c * 32, a);
-            sb::tmem_ld32(t_lane + O_COL + DP + c * 32, b);
+            sb::tmem_ld32(t_lane + O_COL + ch * 32, a);
+            sb::tmem_ld32(t_lane + O_COL + DP + ch * 32, b);
             sb::tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 32; ++j) o[j] = fmaf(__uint_as_float(a[j]), ga, __uint_as_float(b[j]) * gb);
           } else {  // one state: this group's (two_q), or group 0's
-            sb::tmem_ld32((two_q ? o_addr : t_lane + O_COL) + c * 32, a);
+            sb::tmem_ld32((two_q ? o_addr : t_lane + O_COL) + ch * 32, a);
             sb::tmem_ld_wait();
             const float f = two_q && x ? gb : ga;
 #pragma unroll
@@ -724,19 +784,19 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           } else if (it.slot < 0) {
 #pragma unroll
             for (int j = 0; j < 32; j += 8) {
-              if (c * 32 + j < p.D) {
+              if (ch * 32 + j < p.D) {
                 uint4 u;
                 u.x = pa_pack<F16>(o[j], o[j + 1]);
                 u.y = pa_pack<F16>(o[j + 2], o[j + 3]);
                 u.z = pa_pack<F16>(o[j + 4], o[j + 5]);
                 u.w = pa_pack<F16>(o[j + 6], o[j + 7]);
-                *reinterpret_cast<uint4*>(dst + c * 32 + j) = u;
+                *reinterpret_cast<uint4*>(dst + ch * 32 + j) = u;
               }
             }
           } else {
 #pragma unroll
             for (int j = 0; j < 32; j += 4)
-              *reinterpret_cast<float4*>(p.part_o + prow * DP + c * 32 + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+              *reinterpret_cast<float4*>(p.part_o + prow * DP + ch * 32 + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
           }
           __syncwarp();
         }
@@ -745,32 +805,364 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       }
       sb::tc_fence_before();
       __syncwarp();
-      if (lane == 0) sb::mbar_arrive(epi_done);
+      if (lane == 0) sb::mbar_arrive(&c.epi_done);
     }
   }
+  pa_end(p, c, warp);
+}
 
-  __syncwarp();
-  if (*abort_flag) {
-    for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies and MMAs in flight end
+// ============================================================================ narrow kernel
+template <int PANELS, bool F16>
+__global__ void __launch_bounds__(PA_THREADS, 1)
+    pa_narrow_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PaParams p) {
+  using Cfg = PaCfg<PANELS>;
+  constexpr int DP = Cfg::DP, TILE_BYTES = Cfg::TILE_BYTES, STAGES = Cfg::STAGES;
+  constexpr int R = PA_NARROW_ROWS, Q_SLOT = PANELS * R * 128, P_BYTES = PA_TILE * 128;
+  constexpr uint32_t S_COL = 0, O_COL = 256;  // four S^T of 64 columns, two O^T of 64
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* sQ = smem;                    // two slots of 64 rows
+  uint8_t* sP = smem + 2 * 16384;        // [group][key][64 rows], 128-byte swizzle
+  uint8_t* sRing = smem + Cfg::FRONT;
+  float* xrow = reinterpret_cast<float*>(smem + Cfg::DATA);  // [warp][64]: -reference of the rows, later their sums
+  PaCtrl<STAGES>& c = *reinterpret_cast<PaCtrl<STAGES>*>(smem + Cfg::DATA + 2048);
+  volatile int* abort_flag = &c.abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (!pa_begin<true>(p, c, smem, warp, lane)) return;
+  const uint32_t tmem_base = c.tmem_slot;
+
+  if (warp >= 8) {
+    pa_regs_dec<PA_REGS_FEW>();
+    if (warp == 10) {
+      pa_schedule<true, PANELS>(p, c, sQ, (p.batch + 31) / 32, lane);
+    } else if (warp != 9) {
+      pa_load<true, PANELS>(p, c, sRing, warp == 11 ? &tmV : &tmK, warp == 11, lane);
+    } else if (lane == 0) {
+      const uint64_t q_desc = sb::umma_smem_desc(sb::smem_u32(sQ), 16, 1024);
+      const uint64_t k_desc = sb::umma_smem_desc(sb::smem_u32(sRing), 16, p.group_step);
+      // V^T: 128 rows of the product are the columns of the tile; with a head size up to 64 the second half of them reads
+      // the next rows of the tile and goes to lanes that nobody looks at
+      const uint64_t v_desc = sb::umma_smem_desc(sb::smem_u32(sRing), PANELS == 2 ? p.panel_step : 1024, p.group_step);
+      const uint64_t p_desc = sb::umma_smem_desc(sb::smem_u32(sP), 1024, 1024);
+      const uint32_t k_panel = p.panel_step >> 4, v_step = (2 * p.group_step) >> 4;
+      uint32_t ring = 0, p_cnt0 = 0, p_cnt1 = 0;
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        const int slot = i % PA_ITEMS;
+        if (!sb::mbar_wait(&c.item_full[slot], (i / PA_ITEMS) & 1, abort_flag)) break;
+        const int n = c.items[slot].count, cols = (c.items[slot].rows + 15) & ~15;
+        sb::mbar_arrive(&c.item_empty[slot]);
+        if (n == 0) break;
+        const uint32_t idesc_s = sb::umma_idesc_f16(PA_TILE, cols, F16 ? 0 : 1, 0, 0);
+        const uint32_t idesc_o = sb::umma_idesc_f16(PA_TILE, cols, F16 ? 0 : 1, 1, 1);
+        const int qs = i & 1;
+        ok = sb::mbar_wait(&c.q_full[qs], (i >> 1) & 1, abort_flag);
+        auto issue_s = [&](int t) -> bool {
+          const uint32_t e = ring + pa_k_place(t, 4), st = e % STAGES;
+          if (!sb::mbar_wait(&c.full[st], (e / STAGES) & 1, abort_flag)) return false;
+          sb::tc_fence_after();
+          const uint64_t qd = q_desc + qs * (Q_SLOT >> 4), kd = k_desc + st * (TILE_BYTES >> 4);
+          const int buf = (t & 1) * 2 + ((t >> 1) & 1);
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk)
+            sb::umma_f16_ss(tmem_base + S_COL + buf * R, kd + (kk >> 2) * k_panel + (kk & 3) * 2,
+                            qd + (kk >> 2) * (R * 128 >> 4) + (kk & 3) * 2, idesc_s, kk != 0);
+          sb::umma_commit(&c.s_full[buf]);
+          sb::umma_commit(&c.empty[st]);
+          if (t == n - 1) sb::umma_commit(&c.q_empty[qs]);
+          return true;
+        };
+        for (int t = 0; t < min(n, 4) && ok; ++t) ok = issue_s(t);
+        for (int t = 0; t < n && ok; ++t) {
+          const int x = t & 1;
+          const uint32_t e = ring + pa_v_place(t, 4, n), st = e % STAGES;
+          ok = sb::mbar_wait(&c.full[st], (e / STAGES) & 1, abort_flag);
+          if (ok && t == 0 && i > 0) ok = sb::mbar_wait(&c.epi_done, (i - 1) & 1, abort_flag);  // O of the item before is read
+          ok = ok && sb::mbar_wait(&c.p_full[x], (x ? p_cnt1 : p_cnt0) & 1, abort_flag);
+          if (!ok) break;
+          if (x) ++p_cnt1; else ++p_cnt0;
+          sb::tc_fence_after();
+          const uint64_t vd = v_desc + st * (TILE_BYTES >> 4), pd = p_desc + x * (P_BYTES >> 4);
+#pragma unroll
+          for (int kk = 0; kk < PA_TILE / 16; ++kk)
+            sb::umma_f16_ss(tmem_base + O_COL + x * R, vd + kk * v_step, pd + kk * (2048 >> 4), idesc_o, t > 1 || kk != 0);
+          sb::umma_commit(&c.empty[st]);
+          sb::umma_commit(&c.p_empty[x]);
+          if (t + 4 < n) ok = issue_s(t + 4);
+        }
+        ring += 2 * n;
+      }
+    }
+  } else {
+    pa_regs_inc<PA_REGS_MANY>();
+    const int x = warp >> 2, quad = warp & 3, key = quad * 32 + lane;  // thread = key of the tile, later a column of V
+    const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16);
+    const float sl2 = p.sl2;
+    float* nref = xrow + warp * R;                             // this warp's copy: -reference * sl2, +inf where unset
+    float* wmax = reinterpret_cast<float*>(sP + x * P_BYTES);  // [warp of the group][64], while P is not in use
+    uint8_t* prow = sP + x * P_BYTES + key * 128;
+    uint32_t ring = 0, s_cnt0 = 0, s_cnt1 = 0, issued = 0, retired = 0, votes = 0;
+    bool ok = true;
+    // all four warps of the group have come here
+    auto meet = [&]() -> bool {
+      __syncwarp();
+      if (lane == 0) sb::mbar_arrive(&c.vote[x]);
+      return pa_wait(&c.vote[x], votes++ & 1, abort_flag);
+    };
+    for (int i = 0; ok; ++i) {
+      const int islot = i % PA_ITEMS;
+      if (!pa_wait(&c.item_full[islot], (i / PA_ITEMS) & 1, abort_flag)) break;
+      const PaItem it = c.items[islot];
+      __syncwarp();
+      if (lane == 0) sb::mbar_arrive(&c.item_empty[islot]);
+      if (it.count == 0) break;
+      if (i > 0 && !pa_wait(&c.epi_done, (i - 1) & 1, abort_flag)) break;  // xrow of the item before is read
+      const int nb = (it.rows + 15) >> 4, n = it.count;
+      // keys that every row sees: tiles inside need no mask
+      int lo_all = 0, hi_all = 0x7fffffff;
+      {
+        const int pos1 = it.pos0 + pa_div(p, it.rem + it.rows - 1);
+        if (p.window >= 0) lo_all = max(0, pos1 - p.window);
+        hi_all = p.causal ? min(it.pos0 + 1, it.L)
+                          : (p.window >= 0 ? (int)min((long)it.L, (long)it.pos0 + p.window + 1) : it.L);
+      }
+      float ref0 = -INFINITY, ref1 = -INFINITY;  // of rows lane and lane + 32, raw scores
+      float l[R];
+#pragma unroll
+      for (int j = 0; j < R; ++j) l[j] = 0.f;
+      for (int t = x; t < n; t += 2) {
+        const int key0 = (it.tile0 + t) * PA_TILE, buf = (t >> 1) & 1;
+        if (!pa_wait(&c.s_full[x * 2 + buf], (buf ? s_cnt1 : s_cnt0) & 1, abort_flag)) { ok = false; break; }
+        if (buf) ++s_cnt1; else ++s_cnt0;
+        sb::tc_fence_after();
+        float s[R];
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if (b < nb) sb::tmem_ld16(t_lane + S_COL + (x * 2 + buf) * R + b * 16, *reinterpret_cast<uint32_t(*)[16]>(s + b * 16));
+        sb::tmem_ld_wait();
+        const bool inside = key0 >= lo_all && key0 + PA_TILE <= hi_all;
+        if (!inside) {
+          const int j = key0 + key;
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            if (b < nb) {
+#pragma unroll
+              for (int u = 0; u < 16; ++u) {
+                const int pos = it.pos0 + pa_div(p, it.rem + b * 16 + u);
+                const int lo = p.window >= 0 ? pos - p.window : 0;
+                const int hi = p.causal ? min(pos + 1, it.L)
+                                        : (p.window >= 0 ? (int)min((long)it.L, (long)pos + p.window + 1) : it.L);
+                if (b * 16 + u < it.rows && (j < lo || j >= hi)) s[b * 16 + u] = -INFINITY;
+              }
+            }
+        }
+        bool need = t < 2;  // no reference yet
+        if (!need) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            if (b < nb) {
+#pragma unroll
+              for (int u = 0; u < 16; u += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(nref + b * 16 + u);
+                top = fmaxf(top, fmaxf(fmaxf(fmaf(s[b * 16 + u], sl2, f.x), fmaf(s[b * 16 + u + 1], sl2, f.y)),
+                                       fmaxf(fmaf(s[b * 16 + u + 2], sl2, f.z), fmaf(s[b * 16 + u + 3], sl2, f.w))));
+              }
+            }
+          const int mine = __any_sync(0xffffffffu, top > 8.f);
+          int* flags = c.need[x][votes & 1];
+          if (lane == 0) flags[quad] = mine;
+          if (!meet()) { ok = false; break; }
+          const int4 all = *reinterpret_cast<const int4*>(flags);
+          need = (all.x | all.y | all.z | all.w) != 0;
+        }
+        if (retired < issued) {  // P V of this group's tile before: P may be overwritten, O rescaled
+          if (!pa_wait(&c.p_empty[x], retired & 1, abort_flag)) { ok = false; break; }
+          ++retired;
+          sb::tc_fence_after();
+        }
+        if (need) {
+          float m0 = -INFINITY, m1 = -INFINITY;  // maxima over the warp's keys of rows lane and lane + 32
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            if (b < nb) {
+#pragma unroll
+              for (int u = 0; u < 16; ++u) {
+                float m;
+                asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(s[b * 16 + u]));
+                if (lane == (b & 1) * 16 + u) { if (b < 2) m0 = m; else m1 = m; }
+              }
+            }
+          wmax[quad * R + lane] = m0;
+          wmax[quad * R + 32 + lane] = m1;
+          if (!meet()) { ok = false; break; }
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            m0 = fmaxf(m0, wmax[w * R + lane]);
+            m1 = fmaxf(m1, wmax[w * R + 32 + lane]);
+          }
+          m0 = fmaxf(m0, ref0);
+          m1 = fmaxf(m1, ref1);
+          const float a0 = ref0 == -INFINITY ? 0.f : pa_exp2((ref0 - m0) * sl2);
+          const float a1 = ref1 == -INFINITY ? 0.f : pa_exp2((ref1 - m1) * sl2);
+          ref0 = m0;
+          ref1 = m1;
+          nref[lane] = m0 == -INFINITY ? INFINITY : -m0 * sl2;
+          nref[32 + lane] = m1 == -INFINITY ? INFINITY : -m1 * sl2;
+          if (t >= 2) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+              if (b < nb) {
+                uint32_t o[16];
+                sb::tmem_ld16(t_lane + O_COL + x * R + b * 16, o);
+                sb::tmem_ld_wait();
+#pragma unroll
+                for (int u = 0; u < 16; ++u) {
+                  const float a = __shfl_sync(0xffffffffu, b < 2 ? a0 : a1, (b & 1) * 16 + u);
+                  l[b * 16 + u] *= a;
+                  o[u] = __float_as_uint(__uint_as_float(o[u]) * a);
+                }
+                pa_tmem_st16(t_lane + O_COL + x * R + b * 16, o);
+              }
+            sb::tmem_st_wait();
+          }
+          if (!meet()) { ok = false; break; }  // every warp has read the maxima: P goes to the same place
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if (b < nb) {
+            uint32_t pk[8];
+#pragma unroll
+            for (int u = 0; u < 16; u += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(nref + b * 16 + u);
+              const float fs[4] = {f.x, f.y, f.z, f.w};
+              float e[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float v = s[b * 16 + u + k];
+                e[k] = pa_exp2(fmaf(v, sl2, fs[k]));
+                if (!inside && v == -INFINITY) e[k] = 0.f;  // also where the reference is unset
+                l[b * 16 + u + k] += e[k];
+              }
+              pk[u / 2] = pa_pack<F16>(e[0], e[1]);
+              pk[u / 2 + 1] = pa_pack<F16>(e[2], e[3]);
+            }
+            *reinterpret_cast<uint4*>(prow + (((b * 2) ^ (key & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            *reinterpret_cast<uint4*>(prow + (((b * 2 + 1) ^ (key & 7)) << 4)) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+          }
+        if (key0 + PA_TILE > it.hi) {
+          const uint32_t e = ring + pa_v_place(t, 4, n), st = e % STAGES;
+          if (!pa_wait(&c.full[st], (e / STAGES) & 1, abort_flag)) { ok = false; break; }
+          if (key0 + key >= it.hi) pa_zero_v_row<PANELS>(p, sRing + st * TILE_BYTES, key);
+        }
+        sb::fence_proxy_async_smem();
+        sb::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) sb::mbar_arrive(&c.p_full[x]);
+        ++issued;
+      }
+      ring += 2 * n;
+      if (!ok) break;
+      if (retired < issued) {
+        if (!pa_wait(&c.p_empty[x], retired & 1, abort_flag)) break;
+        ++retired;
+        sb::tc_fence_after();
+      }
+      // row sums over the warp's keys: lane r ends with rows r and r + 32
+      float sum[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (h == 0 || nb > 2) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int j = 0; j < o; ++j) {
+              const bool up = lane & o;
+              const float send = up ? l[h * 32 + j] : l[h * 32 + j + o], keep = up ? l[h * 32 + j + o] : l[h * 32 + j];
+              l[h * 32 + j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+            }
+        }
+        sum[h] = l[h * 32];
+      }
+      __syncwarp();
+      nref[lane] = sum[0];
+      nref[32 + lane] = sum[1];
+      if (quad == 0) {  // P of this group is not in use: its place takes the references
+        wmax[lane] = ref0;
+        wmax[32 + lane] = ref1;
+      }
+      sb::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) sb::mbar_arrive(&c.fin);
+      if (!pa_wait(&c.fin, i & 1, abort_flag)) break;
+      sb::tc_fence_after();
+      // factors of both groups' O and the joint reference and sum of rows lane and lane + 32
+      float f0[2], f1[2], top[2], tot[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = h * 32 + lane;
+        const float ra = reinterpret_cast<const float*>(sP)[row], rb = reinterpret_cast<const float*>(sP + P_BYTES)[row];
+        top[h] = fmaxf(ra, rb);
+        f0[h] = ra == -INFINITY ? 0.f : pa_exp2((ra - top[h]) * sl2);
+        f1[h] = rb == -INFINITY ? 0.f : pa_exp2((rb - top[h]) * sl2);
+        const float la = (xrow[row] + xrow[R + row]) + (xrow[2 * R + row] + xrow[3 * R + row]);
+        const float lb = (xrow[4 * R + row] + xrow[5 * R + row]) + (xrow[6 * R + row] + xrow[7 * R + row]);
+        tot[h] = (f0[h] == 0.f ? 0.f : la * f0[h]) + (f1[h] == 0.f ? 0.f : lb * f1[h]);
+        if (it.slot < 0) {
+          const float inv = tot[h] > 0.f ? 1.f / tot[h] : (tot[h] == 0.f ? 0.f : tot[h]);  // no visible key: zeros; NaN stays
+          f0[h] *= inv;
+          f1[h] *= inv;
+        } else if (warp == 0 && row < it.rows) {
+          p.part_ml[(long)it.slot * p.part_rows + row] = make_float2(top[h] == -INFINITY ? -INFINITY : top[h] * sl2, tot[h]);
+        }
+      }
+      // group x writes rows x * 8 nb .. (x + 1) * 8 nb; thread = column of the head
+      const int d = key;
+      for (int j0 = 0; j0 < nb * 8; j0 += 8) {
+        const int row0 = x * nb * 8 + j0;
+        uint32_t a[8], b[8];
+        pa_tmem_ld8(t_lane + O_COL + row0, a, 0);
+        if (n > 1) pa_tmem_ld8(t_lane + O_COL + R + row0, b, 0);
+        sb::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int row = row0 + j;
+          const float ga = __shfl_sync(0xffffffffu, row < 32 ? f0[0] : f0[1], row & 31);
+          const float gb = __shfl_sync(0xffffffffu, row < 32 ? f1[0] : f1[1], row & 31);
+          float v = __uint_as_float(a[j]) * ga;
+          if (n > 1) v = fmaf(__uint_as_float(b[j]), gb, v);
+          if (row < it.rows) {
+            if (it.slot < 0) {
+              const int tok = pa_div(p, it.rem + row), head = it.hk * p.group + (it.rem + row - tok * p.group);
+              if (d < p.D)
+                reinterpret_cast<uint16_t*>(p.out)[(long)(it.row0 + tok) * p.o_tok + (long)head * p.o_head + d] =
+                    (uint16_t)pa_pack<F16>(v, 0.f);
+            } else if (d < DP) {
+              p.part_o[((long)it.slot * p.part_rows + row) * DP + d] = v;
+            }
+          }
+        }
+      }
+      sb::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) sb::mbar_arrive(&c.epi_done);
+    }
   }
-  sb::tc_fence_before();
-  __syncthreads();
-  if (warp == 9) {
-    sb::tc_fence_after();
-    sb::tmem_dealloc(tmem_base, 512);
-  }
-  if (threadIdx.x == 0 && *abort_flag) *p.status = SB_ERR_WAIT_TIMEOUT;
+  pa_end(p, c, warp);
 }
 
 // ============================================================================ joining the partial results
-// blockIdx.x: the CTA that started an item; blockIdx.y strides over the item's rows.  Thread = (part group, four columns):
+// blockIdx.x: the CTA that started an item (first of the narrow kernel, then of the wide one); blockIdx.y strides over the item's rows.  Thread = (part group, four columns):
 // each group runs over every PG-th part with an online reference, the groups are joined in order.
 template <int PANELS, bool F16>
-__global__ void __launch_bounds__(PA_COMBINE_THREADS) pa_combine_kernel(const PaParams p) {
+__global__ void __launch_bounds__(PA_COMBINE_THREADS)
+    pa_combine_kernel(const PaParams first_p, const PaParams second_p, int first_ctas) {
   constexpr int DP = PANELS * 64, QUADS = DP / 4, PG = PA_COMBINE_THREADS / QUADS;
   __shared__ float4 so[PG][QUADS];
   __shared__ float2 sml[PG];
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const bool second = (int)blockIdx.x >= first_ctas;
+  const PaParams& p = second ? second_p : first_p;
+  const int cta = second ? (int)blockIdx.x - first_ctas : (int)blockIdx.x;
   if (p.zero_tail) {  // rows behind the last sequence
     const long first = p.batch > 0 ? min(max(p.cu[p.batch], 0), p.T) : 0, heads = (long)p.Hkv * p.group;
     const long chunks = (p.T - first) * heads * (p.D / 8);
@@ -781,7 +1173,7 @@ __global__ void __launch_bounds__(PA_COMBINE_THREADS) pa_combine_kernel(const Pa
                                 (c - row * (p.D / 8)) * 8) = make_uint4(0, 0, 0, 0);
     }
   }
-  const int* desc = p.part_desc + 8 * blockIdx.x;
+  const int* desc = p.part_desc + 8 * cta;
   if (!desc[0]) return;
   const int row0 = desc[1], rem = desc[2], hk = desc[3], rows = desc[4], last = desc[5];
   const int quad = threadIdx.x % QUADS, pg = threadIdx.x / QUADS;
@@ -789,8 +1181,8 @@ __global__ void __launch_bounds__(PA_COMBINE_THREADS) pa_combine_kernel(const Pa
     float ref = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int c = (int)blockIdx.x + pg; c <= last; c += PG) {
-      const long prow = (long)(2 * c + (c == (int)blockIdx.x ? 1 : 0)) * p.part_rows + row;
+    for (int c = cta + pg; c <= last; c += PG) {
+      const long prow = (long)(2 * c + (c == cta ? 1 : 0)) * p.part_rows + row;
       const float2 ml = p.part_ml[prow];
       const float4 v = *reinterpret_cast<const float4*>(p.part_o + prow * DP + quad * 4);
       if (ml.x == -INFINITY && ml.y == 0.f) continue;  // a part without a visible key
@@ -862,40 +1254,85 @@ int pa_tmap(CUtensorMap* m, const void* base, int D, int heads, int page_size, i
   return r == CUDA_SUCCESS ? SB_OK : SB_ERR_DRIVER;
 }
 
-// CTAs of the main launch: one per SM, fewer when not even the table's full length gives each of them two key tiles
-long pa_ctas(long T, int batch, int Hq, int Hkv, long cap, int sms) {
-  const long items = (T * (Hq / Hkv) + PA_ITEM_ROWS - 1) / PA_ITEM_ROWS + batch;
+// CTAs of a launch: one per SM, fewer when not even the table's full length gives each of them two key tiles
+long pa_ctas(long T, int batch, int Hq, int Hkv, long cap, int item_rows, int sms) {
+  const long items = (T * (Hq / Hkv) + item_rows - 1) / item_rows + batch;
   const long tiles = (cap + PA_TILE - 1) / PA_TILE + 1;
   const long want = (items * Hkv * tiles + 1) / 2;
   return want < 1 ? 1 : want < sms ? want : sms;
 }
-int pa_part_rows(long T, int group) { return T * group < PA_ITEM_ROWS ? (int)(T * group) : PA_ITEM_ROWS; }
 long pa_align(long v) { return (v + 255) & ~255L; }
 
+// Which kernels a call takes, and their places in its workspace.  Sequences with at most 64 rows (new tokens x heads per KV
+// head) are narrow; with no more new tokens than sequences, as in a decoding step, all of them are, whatever their length:
+// the second launch then finds nothing (3 us), and a sequence that does have more rows is read once per 64 of them.
+struct PaPlan {
+  bool wide, narrow;
+  int narrow_max, narrow_ctas, wide_ctas, narrow_rows, wide_rows;
+  long narrow_at, wide_at, bytes;
+};
+PaPlan pa_plan(long T, int batch, int Hq, int Hkv, int D, long cap, int sms) {
+  PaPlan w = {};
+  const long group = Hq / Hkv, rows = T * group, dp = D <= 64 ? 64 : 128;
+  w.narrow = true;
+  w.wide = rows > PA_NARROW_ROWS && T > batch;
+  w.narrow_max = w.wide ? PA_NARROW_ROWS : 0x7fffffff;
+  w.narrow_ctas = (int)pa_ctas(T, batch, Hq, Hkv, cap, PA_NARROW_ROWS, sms);
+  w.wide_ctas = w.wide ? (int)pa_ctas(T, batch, Hq, Hkv, cap, PA_WIDE_ROWS, sms) : 0;
+  w.narrow_rows = (int)(rows < PA_NARROW_ROWS ? rows : PA_NARROW_ROWS);
+  w.wide_rows = (int)(rows < PA_WIDE_ROWS ? rows : PA_WIDE_ROWS);
+  auto size = [&](long ctas, long r) { return pa_align(2 * ctas * r * dp * 4) + pa_align(2 * ctas * r * 8) + pa_align(ctas * 32); };
+  w.narrow_at = 0;
+  w.wide_at = size(w.narrow_ctas, w.narrow_rows);
+  w.bytes = w.wide_at + (w.wide ? size(w.wide_ctas, w.wide_rows) : 0);
+  return w;
+}
+void pa_place(PaParams* p, uint8_t* ws, long ctas, int rows, long dp) {
+  p->part_rows = rows;
+  p->part_o = reinterpret_cast<float*>(ws);
+  ws += pa_align(2 * ctas * rows * dp * 4);
+  p->part_ml = reinterpret_cast<float2*>(ws);
+  ws += pa_align(2 * ctas * rows * 8);
+  p->part_desc = reinterpret_cast<int*>(ws);
+}
+
 template <int PANELS, bool F16>
-int pa_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const PaParams& p, int ctas, cudaStream_t stream) {
+int pa_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, PaParams p, const PaPlan& w, uint8_t* ws, cudaStream_t stream) {
+  constexpr int SMEM = PaCfg<PANELS>::SMEM;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
   static bool set[64] = {};  // the attribute belongs to a device
   if (dev >= 64 || !set[dev]) {
-    e = cudaFuncSetAttribute(pa_kernel<PANELS, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, PaCfg<PANELS>::SMEM);
+    e = cudaFuncSetAttribute(pa_wide_kernel<PANELS, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(pa_narrow_kernel<PANELS, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return (int)e;
     if (dev < 64) set[dev] = true;
   }
-  pa_kernel<PANELS, F16><<<ctas, PA_THREADS, PaCfg<PANELS>::SMEM, stream>>>(tmK, tmV, p);
+  p.narrow_max = w.narrow_max;
+  PaParams pn = p, pw = p;
+  pa_place(&pn, ws + w.narrow_at, w.narrow_ctas, w.narrow_rows, PaCfg<PANELS>::DP);
+  if (w.wide) {
+    pa_place(&pw, ws + w.wide_at, w.wide_ctas, w.wide_rows, PaCfg<PANELS>::DP);
+    pa_wide_kernel<PANELS, F16><<<w.wide_ctas, PA_THREADS, SMEM, stream>>>(tmK, tmV, pw);
+    SB_CHECK_LAUNCH();
+  }
+  pa_narrow_kernel<PANELS, F16><<<w.narrow_ctas, PA_THREADS, SMEM, stream>>>(tmK, tmV, pn);
   SB_CHECK_LAUNCH();
-  // launched while the main kernel still runs; waits for it on the device
+  // launched while the kernel before still runs; waits for it on the device
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, p.part_rows < 16 ? p.part_rows : 16);
+  const int rows = w.wide ? w.wide_rows : w.narrow_rows;
+  cfg.gridDim = dim3(w.narrow_ctas + w.wide_ctas, rows < 16 ? rows : 16);
   cfg.blockDim = dim3(PA_COMBINE_THREADS);
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, pa_combine_kernel<PANELS, F16>, p);
+  const PaParams second = w.wide ? pw : pn;
+  e = cudaLaunchKernelEx(&cfg, pa_combine_kernel<PANELS, F16>, pn, second, w.narrow_ctas);
   return e == cudaSuccess ? SB_OK : (int)e;
 }
 
@@ -904,8 +1341,7 @@ int pa_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const PaParams& p,
 // Bytes of workspace of one call (contents need not be initialised); `cap` = positions that the page table can hold.
 SB_API long sb200_paged_attention_workspace(int T, int batch, int Hq, int Hkv, int D, long cap, int sms) {
   if (T <= 0 || batch < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || D <= 0 || sms <= 0) return 0;
-  const long slots = 2 * pa_ctas(T, batch, Hq, Hkv, cap, sms), rows = pa_part_rows(T, Hq / Hkv), dp = D <= 64 ? 64 : 128;
-  return pa_align(slots * rows * dp * 4) + pa_align(slots * rows * 8) + slots / 2 * 32;
+  return pa_plan(T, batch, Hq, Hkv, D, cap, sms).bytes;
 }
 
 // out[t, h] for the new tokens of `batch` sequences, q / out [T, Hq, D] (token and head strides in elements), caches
@@ -944,7 +1380,7 @@ SB_API int sb200_paged_attention(const void* q, const void* k_cache, const void*
   p.group_step = joined ? 2048 : 1024;
   p.panel_step = joined ? 1024 : PA_PANEL;
   p.boxes = joined || D <= 64 ? 1 : 2;
-  const int ctas = (int)pa_ctas(T, batch, Hq, Hkv, cap, sms), dp = D <= 64 ? 64 : 128;
+  const PaPlan w = pa_plan(T, batch, Hq, Hkv, D, cap, sms);
   p.q = q; p.out = out; p.table = table; p.cu = cu; p.lens = lens;
   p.table_ld = table_ld; p.q_tok = q_tok; p.q_head = q_head; p.o_tok = o_tok; p.o_head = o_head;
   p.T = T; p.batch = batch; p.Hkv = Hkv; p.group = Hq / Hkv;
@@ -952,14 +1388,8 @@ SB_API int sb200_paged_attention(const void* q, const void* k_cache, const void*
   p.D = D; p.cols = cols; p.num_pages = num_pages;
   while ((1 << p.page_shift) < page_size) ++p.page_shift;
   p.causal = causal; p.window = window < (1 << 30) ? window : 1 << 30; p.sl2 = scale * 1.4426950408889634f;
-  p.part_rows = pa_part_rows(T, p.group);
-  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
-  p.part_o = reinterpret_cast<float*>(ws);
-  ws += pa_align(2L * ctas * p.part_rows * dp * 4);
-  p.part_ml = reinterpret_cast<float2*>(ws);
-  ws += pa_align(2L * ctas * p.part_rows * 8);
-  p.part_desc = reinterpret_cast<int*>(ws);
   p.zero_tail = zero_tail; p.status = status;
-  if (D <= 64) return f16 ? pa_launch<1, true>(tmK, tmV, p, ctas, stream) : pa_launch<1, false>(tmK, tmV, p, ctas, stream);
-  return f16 ? pa_launch<2, true>(tmK, tmV, p, ctas, stream) : pa_launch<2, false>(tmK, tmV, p, ctas, stream);
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  if (D <= 64) return f16 ? pa_launch<1, true>(tmK, tmV, p, w, ws, stream) : pa_launch<1, false>(tmK, tmV, p, w, ws, stream);
+  return f16 ? pa_launch<2, true>(tmK, tmV, p, w, ws, stream) : pa_launch<2, false>(tmK, tmV, p, w, ws, stream);
 }
