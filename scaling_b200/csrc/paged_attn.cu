@@ -38,7 +38,7 @@
 namespace {
 
 constexpr int PA_TILE = 128;
-constexpr int PA_WIDE_ROWS = 256, PA_NARROW_ROWS = 64;  // rows per item
+constexpr int PA_WIDE_ROWS = 256, PA_NARROW_ROWS = 64;  // rows per item (narrow: at most)
 constexpr int PA_WARPS = 12;
 constexpr int PA_THREADS = PA_WARPS * 32;
 // registers per thread after the roles part: 128 x 80 + 256 x 208 = 63488 of the 384 x 168 that the launch holds
@@ -48,6 +48,12 @@ constexpr int PA_ITEMS = 4;       // descriptors in flight
 constexpr int PA_COMBINE_THREADS = 256;
 // What the start and the end of an item cost, in tiles: added to its length on the work line.
 constexpr int PA_WIDE_COST = 2, PA_NARROW_COST = 1;
+// ROWS (rows per item) tells the kernels apart in the functions that they share.
+template <int ROWS> struct PaKind {
+  static constexpr bool NARROW = ROWS <= PA_NARROW_ROWS;
+  static constexpr int COST = NARROW ? PA_NARROW_COST : PA_WIDE_COST;
+  static constexpr int SLOT_ROWS = NARROW ? ROWS : PA_TILE;  // rows per query slot
+};
 
 struct PaParams {
   const void* q;
@@ -195,8 +201,7 @@ __device__ __forceinline__ PaSeq pa_seq(const PaParams& p, int b) {
 // n / group for n < group + 256
 __device__ __forceinline__ int pa_div(const PaParams& p, int n) { return p.group == 1 ? n : (int)__umulhi(n, p.group_inv); }
 // keys that some row of item m sees
-template <bool NARROW> __device__ __forceinline__ void pa_item_keys(const PaParams& p, int n, int L, int m, int& lo, int& hi) {
-  constexpr int ROWS = NARROW ? PA_NARROW_ROWS : PA_WIDE_ROWS;
+template <int ROWS> __device__ __forceinline__ void pa_item_keys(const PaParams& p, int n, int L, int m, int& lo, int& hi) {
   const int rows = n * p.group;
   const int first = m * ROWS / p.group, last = (min(rows, (m + 1) * ROWS) - 1) / p.group;
   const int pos0 = L - n + first, pos1 = L - n + last;
@@ -207,16 +212,15 @@ template <bool NARROW> __device__ __forceinline__ void pa_item_keys(const PaPara
 // key tiles between lo and hi, at least one: a row without keys still has to be written
 __device__ __forceinline__ int pa_tiles(int lo, int hi) { return max((hi + PA_TILE - 1) / PA_TILE - lo / PA_TILE, 1); }
 // length of item m on the line
-template <bool NARROW> __device__ __forceinline__ int pa_item_cost(const PaParams& p, int n, int L, int m) {
+template <int ROWS> __device__ __forceinline__ int pa_item_cost(const PaParams& p, int n, int L, int m) {
   int lo, hi;
-  pa_item_keys<NARROW>(p, n, L, m, lo, hi);
-  return pa_tiles(lo, hi) + (NARROW ? PA_NARROW_COST : PA_WIDE_COST);
+  pa_item_keys<ROWS>(p, n, L, m, lo, hi);
+  return pa_tiles(lo, hi) + PaKind<ROWS>::COST;
 }
 // items of a sequence of n new tokens in this kernel, per KV head
-template <bool NARROW> __device__ __forceinline__ int pa_items(const PaParams& p, int n) {
-  constexpr int ROWS = NARROW ? PA_NARROW_ROWS : PA_WIDE_ROWS;
+template <int ROWS> __device__ __forceinline__ int pa_items(const PaParams& p, int n) {
   const int rows = n * p.group;
-  return (rows <= p.narrow_max) == NARROW ? (rows + ROWS - 1) / ROWS : 0;
+  return (rows <= p.narrow_max) == PaKind<ROWS>::NARROW ? (rows + ROWS - 1) / ROWS : 0;
 }
 __device__ __forceinline__ int pa_scan(int v, int lane) {
 #pragma unroll
@@ -228,20 +232,20 @@ __device__ __forceinline__ int pa_scan(int v, int lane) {
 }
 __device__ __forceinline__ int pa_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
 // Length of all items of one KV head of sequence 32 * chunk + lane (0 beyond the last sequence); the whole warp calls.
-template <bool NARROW> __device__ __forceinline__ int pa_chunk_cost(const PaParams& p, int chunk, int lane, PaSeq& s) {
+template <int ROWS> __device__ __forceinline__ int pa_chunk_cost(const PaParams& p, int chunk, int lane, PaSeq& s) {
   const int b = chunk * 32 + lane;
   s = PaSeq{0, 0, 0};
   if (b < p.batch) s = pa_seq(p, b);
-  const int items = pa_items<NARROW>(p, s.n);
-  int cost = items == 1 ? pa_item_cost<NARROW>(p, s.n, s.L, 0) : 0;
+  const int items = pa_items<ROWS>(p, s.n);
+  int cost = items == 1 ? pa_item_cost<ROWS>(p, s.n, s.L, 0) : 0;
   unsigned many = __ballot_sync(0xffffffffu, items > 1);
   while (many) {  // the warp shares the items of one sequence
     const int src = __ffs(many) - 1;
     many &= many - 1;
     const int n = __shfl_sync(0xffffffffu, s.n, src), L = __shfl_sync(0xffffffffu, s.L, src);
-    const int cnt = pa_items<NARROW>(p, n);
+    const int cnt = pa_items<ROWS>(p, n);
     int sum = 0;
-    for (int m = lane; m < cnt; m += 32) sum += pa_item_cost<NARROW>(p, n, L, m);
+    for (int m = lane; m < cnt; m += 32) sum += pa_item_cost<ROWS>(p, n, L, m);
     sum = pa_sum(sum);
     if (lane == src) cost = sum;
   }
@@ -264,7 +268,7 @@ struct PaCursor {  // where a CTA's piece of the line starts, and how long it is
 };
 
 // The whole warp; sums[c] = length per KV head of sequences 32 c .. 32 c + 31.
-template <bool NARROW>
+template <int ROWS>
 __device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int chunks, int lane, PaCursor& c) {
   long long all = 0;
   for (int i = lane; i < chunks; i += 32) all += sums[i];
@@ -279,7 +283,7 @@ __device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int 
   PaCut& cut = c.cut;
   const int total = (int)all;
   // two tiles per CTA at least, one for each softmax group
-  cut.ctas = min((int)gridDim.x, (total + 1) / (2 + (NARROW ? PA_NARROW_COST : PA_WIDE_COST)));
+  cut.ctas = min((int)gridDim.x, (total + 1) / (2 + PaKind<ROWS>::COST));
   if (total > 0) cut.ctas = max(cut.ctas, 1);
   if ((int)blockIdx.x >= cut.ctas) return;
   cut.per = total / cut.ctas;
@@ -301,7 +305,7 @@ __device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int 
     }
   }
   PaSeq s;
-  const int cost = pa_chunk_cost<NARROW>(p, chunk, lane, s), v = cost * p.Hkv, inc = pa_scan(v, lane);
+  const int cost = pa_chunk_cost<ROWS>(p, chunk, lane, s), v = cost * p.Hkv, inc = pa_scan(v, lane);
   const int k = __ffs(__ballot_sync(0xffffffffu, inc > off)) - 1;
   off -= __shfl_sync(0xffffffffu, inc - v, k);
   const int per_head = __shfl_sync(0xffffffffu, cost, k);
@@ -309,11 +313,11 @@ __device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int 
   c.seq = chunk * 32 + k;
   c.hk = off / per_head;
   off -= c.hk * per_head;
-  const int items = pa_items<NARROW>(p, c.s.n);
+  const int items = pa_items<ROWS>(p, c.s.n);
   c.tile = off;
   if (items > 1) {
     for (int base = 0; base < items; base += 32) {
-      const int t = base + lane < items ? pa_item_cost<NARROW>(p, c.s.n, c.s.L, base + lane) : 0, ti = pa_scan(t, lane);
+      const int t = base + lane < items ? pa_item_cost<ROWS>(p, c.s.n, c.s.L, base + lane) : 0, ti = pa_scan(t, lane);
       const unsigned hit = __ballot_sync(0xffffffffu, ti > off);
       if (hit) {
         const int j = __ffs(hit) - 1;
@@ -330,19 +334,18 @@ __device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int 
 // the MMA warp takes them (narrow: 4; wide: 1 with two_q, else 2, the first S of both groups).
 __device__ __forceinline__ uint32_t pa_k_place(int t, int lead) { return t < lead ? t : 2 * t - lead + 1; }
 __device__ __forceinline__ uint32_t pa_v_place(int t, int lead, int count) { return t + min(t + lead, count); }
-template <bool NARROW> __device__ __forceinline__ int pa_lead(int rows) { return NARROW ? 4 : rows > PA_TILE ? 1 : 2; }
+template <int ROWS> __device__ __forceinline__ int pa_lead(int rows) { return PaKind<ROWS>::NARROW ? 4 : rows > PA_TILE ? 1 : 2; }
 
 // ============================================================================ roles that both kernels share
 // Warp 10: cuts the piece into items, publishes their descriptors and copies their queries.
-template <bool NARROW, int PANELS>
+template <int ROWS, int PANELS>
 __device__ __forceinline__ void pa_schedule(const PaParams& p, PaCtrl<PaCfg<PANELS>::STAGES>& c, uint8_t* sQ, int chunks,
                                             int lane) {
-  constexpr int DP = PANELS * 64, COST = NARROW ? PA_NARROW_COST : PA_WIDE_COST;
-  constexpr int ROWS = NARROW ? PA_NARROW_ROWS : PA_WIDE_ROWS;
-  constexpr int SLOT_ROWS = NARROW ? PA_NARROW_ROWS : PA_TILE, SLOT_BYTES = PANELS * SLOT_ROWS * 128;
+  constexpr int DP = PANELS * 64, COST = PaKind<ROWS>::COST;
+  constexpr int SLOT_ROWS = PaKind<ROWS>::SLOT_ROWS, SLOT_BYTES = PANELS * SLOT_ROWS * 128;
   volatile int* abort_flag = &c.abort;
   PaCursor cur;
-  pa_find<NARROW>(p, reinterpret_cast<const int*>(sQ), chunks, lane, cur);
+  pa_find<ROWS>(p, reinterpret_cast<const int*>(sQ), chunks, lane, cur);
   __syncwarp();
   int* desc = p.part_desc + 8 * blockIdx.x;
   bool starts = false, ok = true;
@@ -353,7 +356,7 @@ __device__ __forceinline__ void pa_schedule(const PaParams& p, PaCtrl<PaCfg<PANE
     PaItem it = {};
     int lo, hi, tiles = 0;
     while (cur.left > 0) {  // the next item with a tile in this piece
-      pa_item_keys<NARROW>(p, cur.s.n, cur.s.L, cur.m, lo, hi);
+      pa_item_keys<ROWS>(p, cur.s.n, cur.s.L, cur.m, lo, hi);
       tiles = pa_tiles(lo, hi);
       if (cur.tile < tiles) {
         const int take = min(tiles - cur.tile, cur.left);
@@ -375,11 +378,11 @@ __device__ __forceinline__ void pa_schedule(const PaParams& p, PaCtrl<PaCfg<PANE
       cur.left -= used;
       cur.place += used;
       cur.tile = 0;
-      if (cur.left > 0 && ++cur.m == pa_items<NARROW>(p, cur.s.n)) {
+      if (cur.left > 0 && ++cur.m == pa_items<ROWS>(p, cur.s.n)) {
         cur.m = 0;
         if (++cur.hk == p.Hkv) {
           cur.hk = 0;
-          do { cur.s = pa_seq(p, ++cur.seq); } while (pa_items<NARROW>(p, cur.s.n) == 0 && cur.seq + 1 < p.batch);
+          do { cur.s = pa_seq(p, ++cur.seq); } while (pa_items<ROWS>(p, cur.s.n) == 0 && cur.seq + 1 < p.batch);
         }
       }
       if (it.count) break;
@@ -396,11 +399,11 @@ __device__ __forceinline__ void pa_schedule(const PaParams& p, PaCtrl<PaCfg<PANE
       ok = pa_wait(&c.q_empty[qs], (((q_cnt + x) >> 1) & 1) ^ 1, abort_flag);
       if (!ok) break;
       constexpr int CH = DP / 8;  // chunks per row
-      const int ch = lane % CH, live = min(it.rows - x * SLOT_ROWS, SLOT_ROWS), end = NARROW ? (live + 15) & ~15 : (live + 31) & ~31;
+      const int ch = lane % CH, live = min(it.rows - x * SLOT_ROWS, SLOT_ROWS), end = PaKind<ROWS>::NARROW ? (live + 15) & ~15 : (live + 31) & ~31;
       const uint32_t dst = sb::smem_u32(sQ + qs * SLOT_BYTES) + (ch >> 3) * (SLOT_ROWS * 128);
       const uint16_t* base = reinterpret_cast<const uint16_t*>(p.q) + (long)it.row0 * p.q_tok +
                              (long)it.hk * p.group * p.q_head + ch * 8;
-#pragma unroll 4
+#pragma unroll 1  // short code: it runs once per item and is fetched each time
       for (int r = lane / CH; r < end; r += 32 / CH) {
         const int row = it.rem + x * SLOT_ROWS + r, t = pa_div(p, row), h = row - t * p.group;
         const bool take = r < live && ch * 8 < p.D;
@@ -418,7 +421,7 @@ __device__ __forceinline__ void pa_schedule(const PaParams& p, PaCtrl<PaCfg<PANE
 }
 
 // Warps 8 (K) and 11 (V).
-template <bool NARROW, int PANELS>
+template <int ROWS, int PANELS>
 __device__ __forceinline__ void pa_load(const PaParams& p, PaCtrl<PaCfg<PANELS>::STAGES>& c, uint8_t* sRing,
                                         const CUtensorMap* tm, bool is_v, int lane) {
   constexpr int STAGES = PaCfg<PANELS>::STAGES, TILE_BYTES = PaCfg<PANELS>::TILE_BYTES;
@@ -438,7 +441,7 @@ __device__ __forceinline__ void pa_load(const PaParams& p, PaCtrl<PaCfg<PANELS>:
     __syncwarp();
     if (lane == 0) sb::mbar_arrive(&c.item_empty[slot]);
     if (it.count == 0) break;
-    const int lead = pa_lead<NARROW>(it.rows);
+    const int lead = pa_lead<ROWS>(it.rows);
     const int* trow = p.table + (long)it.seq * p.table_ld;
     int win = -64, where = 0;  // 32 pages at a time: their first 8-row group in the tensor map
     for (int t = 0; t < it.count; ++t) {
@@ -477,7 +480,7 @@ template <int PANELS> __device__ __forceinline__ void pa_zero_v_row(const PaPara
 
 // Barriers, TMEM and the lengths of 32 sequences at a time (left where the scheduler puts the queries afterwards).
 // Returns false if shared memory does not start on a 1024-byte boundary, as the swizzled tiles need.
-template <bool NARROW, int STAGES>
+template <int ROWS, int STAGES>
 __device__ __forceinline__ bool pa_begin(const PaParams& p, PaCtrl<STAGES>& c, uint8_t* smem, int warp, int lane) {
   if (sb::smem_u32(smem) & 1023) {
     if (threadIdx.x == 0) *p.status = SB_ERR_BAD_ARG;
@@ -516,7 +519,7 @@ __device__ __forceinline__ bool pa_begin(const PaParams& p, PaCtrl<STAGES>& c, u
   const int chunks = (p.batch + 31) / 32;
   for (int k = warp; k < chunks; k += PA_WARPS) {
     PaSeq s;
-    const int t = pa_sum(pa_chunk_cost<NARROW>(p, k, lane, s));
+    const int t = pa_sum(pa_chunk_cost<ROWS>(p, k, lane, s));
     if (lane == 0) sums[k] = t;
   }
   sb::tc_fence_before();
@@ -553,15 +556,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   PaCtrl<STAGES>& c = *reinterpret_cast<PaCtrl<STAGES>*>(smem + Cfg::DATA + 2048);
   volatile int* abort_flag = &c.abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (!pa_begin<false>(p, c, smem, warp, lane)) return;
+  if (!pa_begin<PA_WIDE_ROWS>(p, c, smem, warp, lane)) return;
   const uint32_t tmem_base = c.tmem_slot;
 
   if (warp >= 8) {
     pa_regs_dec<PA_REGS_FEW>();  // one instruction for the whole warpgroup
     if (warp == 10) {
-      pa_schedule<false, PANELS>(p, c, sQ, (p.batch + 31) / 32, lane);
+      pa_schedule<PA_WIDE_ROWS, PANELS>(p, c, sQ, (p.batch + 31) / 32, lane);
     } else if (warp != 9) {
-      pa_load<false, PANELS>(p, c, sRing, warp == 11 ? &tmV : &tmK, warp == 11, lane);
+      pa_load<PA_WIDE_ROWS, PANELS>(p, c, sRing, warp == 11 ? &tmV : &tmK, warp == 11, lane);
     } else if (lane == 0) {
       const uint32_t idesc_s = sb::umma_idesc_f16(PA_TILE, PA_TILE, F16 ? 0 : 1, 0, 0);  // K-major both
       const uint32_t idesc_o = sb::umma_idesc_f16(PA_TILE, DP, F16 ? 0 : 1, 0, 1);       // V is MN-major
@@ -812,30 +815,49 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 }
 
 // ============================================================================ narrow kernel
-template <int PANELS, bool F16>
+// v[j] of lane i is the value of row j; lane r ends with the result over all lanes of row r (NV = 16: and so does r + 16).
+template <int NV, typename F> __device__ __forceinline__ float pa_transpose_reduce(float (&v)[NV], int lane, F f) {
+  if (NV == 16) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] = f(v[j], __shfl_xor_sync(0xffffffffu, v[j], 16));
+  }
+#pragma unroll
+  for (int o = NV / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int j = 0; j < o; ++j) {
+      const bool up = lane & o;
+      const float send = up ? v[j] : v[j + o], keep = up ? v[j + o] : v[j];
+      v[j] = f(keep, __shfl_xor_sync(0xffffffffu, send, o));
+    }
+  return v[0];
+}
+
+// NB: blocks of 16 rows that an item may have (1 or 4).
+template <int PANELS, bool F16, int NB>
 __global__ void __launch_bounds__(PA_THREADS, 1)
     pa_narrow_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PaParams p) {
   using Cfg = PaCfg<PANELS>;
   constexpr int DP = Cfg::DP, TILE_BYTES = Cfg::TILE_BYTES, STAGES = Cfg::STAGES;
-  constexpr int R = PA_NARROW_ROWS, Q_SLOT = PANELS * R * 128, P_BYTES = PA_TILE * 128;
-  constexpr uint32_t S_COL = 0, O_COL = 256;  // four S^T of 64 columns, two O^T of 64
+  constexpr int R = 16 * NB, H = (NB + 1) / 2, Q_SLOT = PANELS * R * 128, P_BYTES = PA_TILE * 128;
+  constexpr int HV = R < 32 ? R : 32;         // rows of a half: row h * 32 + r belongs to lane r
+  constexpr uint32_t S_COL = 0, O_COL = 256;  // four S^T of R columns, two O^T of R
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;                    // two slots of 64 rows
   uint8_t* sP = smem + 2 * 16384;        // [group][key][64 rows], 128-byte swizzle
   uint8_t* sRing = smem + Cfg::FRONT;
-  float* xrow = reinterpret_cast<float*>(smem + Cfg::DATA);  // [warp][64]: -reference of the rows, later their sums
+  float* xrow = reinterpret_cast<float*>(smem + Cfg::DATA);  // [warp][R]: -reference of the rows, later their sums
   PaCtrl<STAGES>& c = *reinterpret_cast<PaCtrl<STAGES>*>(smem + Cfg::DATA + 2048);
   volatile int* abort_flag = &c.abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (!pa_begin<true>(p, c, smem, warp, lane)) return;
+  if (!pa_begin<R>(p, c, smem, warp, lane)) return;
   const uint32_t tmem_base = c.tmem_slot;
 
   if (warp >= 8) {
     pa_regs_dec<PA_REGS_FEW>();
     if (warp == 10) {
-      pa_schedule<true, PANELS>(p, c, sQ, (p.batch + 31) / 32, lane);
+      pa_schedule<R, PANELS>(p, c, sQ, (p.batch + 31) / 32, lane);
     } else if (warp != 9) {
-      pa_load<true, PANELS>(p, c, sRing, warp == 11 ? &tmV : &tmK, warp == 11, lane);
+      pa_load<R, PANELS>(p, c, sRing, warp == 11 ? &tmV : &tmK, warp == 11, lane);
     } else if (lane == 0) {
       const uint64_t q_desc = sb::umma_smem_desc(sb::smem_u32(sQ), 16, 1024);
       const uint64_t k_desc = sb::umma_smem_desc(sb::smem_u32(sRing), 16, p.group_step);
@@ -898,7 +920,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16);
     const float sl2 = p.sl2;
     float* nref = xrow + warp * R;                             // this warp's copy: -reference * sl2, +inf where unset
-    float* wmax = reinterpret_cast<float*>(sP + x * P_BYTES);  // [warp of the group][64], while P is not in use
+    float* wmax = reinterpret_cast<float*>(sP + x * P_BYTES);  // [warp of the group][64], where P is not in use
     uint8_t* prow = sP + x * P_BYTES + key * 128;
     uint32_t ring = 0, s_cnt0 = 0, s_cnt1 = 0, issued = 0, retired = 0, votes = 0;
     bool ok = true;
@@ -916,7 +938,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       if (lane == 0) sb::mbar_arrive(&c.item_empty[islot]);
       if (it.count == 0) break;
       if (i > 0 && !pa_wait(&c.epi_done, (i - 1) & 1, abort_flag)) break;  // xrow of the item before is read
-      const int nb = (it.rows + 15) >> 4, n = it.count;
+      const int nb = NB == 1 ? 1 : (it.rows + 15) >> 4, n = it.count;
       // keys that every row sees: tiles inside need no mask
       int lo_all = 0, hi_all = 0x7fffffff;
       {
@@ -925,7 +947,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         hi_all = p.causal ? min(it.pos0 + 1, it.L)
                           : (p.window >= 0 ? (int)min((long)it.L, (long)it.pos0 + p.window + 1) : it.L);
       }
-      float ref0 = -INFINITY, ref1 = -INFINITY;  // of rows lane and lane + 32, raw scores
+      float ref[H];  // raw reference of rows lane and lane + 32
+#pragma unroll
+      for (int h = 0; h < H; ++h) ref[h] = -INFINITY;
       float l[R];
 #pragma unroll
       for (int j = 0; j < R; ++j) l[j] = 0.f;
@@ -936,14 +960,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         sb::tc_fence_after();
         float s[R];
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int b = 0; b < NB; ++b)
           if (b < nb) sb::tmem_ld16(t_lane + S_COL + (x * 2 + buf) * R + b * 16, *reinterpret_cast<uint32_t(*)[16]>(s + b * 16));
         sb::tmem_ld_wait();
         const bool inside = key0 >= lo_all && key0 + PA_TILE <= hi_all;
         if (!inside) {
           const int j = key0 + key;
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
+          for (int b = 0; b < NB; ++b)
             if (b < nb) {
 #pragma unroll
               for (int u = 0; u < 16; ++u) {
@@ -959,7 +983,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         if (!need) {
           float top = -INFINITY;
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
+          for (int b = 0; b < NB; ++b)
             if (b < nb) {
 #pragma unroll
               for (int u = 0; u < 16; u += 4) {
@@ -981,43 +1005,35 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           sb::tc_fence_after();
         }
         if (need) {
-          float m0 = -INFINITY, m1 = -INFINITY;  // maxima over the warp's keys of rows lane and lane + 32
+          float alpha[H];
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
-            if (b < nb) {
+          for (int h = 0; h < H; ++h) {  // maxima over the warp's keys
+            float v[HV];
 #pragma unroll
-              for (int u = 0; u < 16; ++u) {
-                float m;
-                asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(s[b * 16 + u]));
-                if (lane == (b & 1) * 16 + u) { if (b < 2) m0 = m; else m1 = m; }
-              }
-            }
-          wmax[quad * R + lane] = m0;
-          wmax[quad * R + 32 + lane] = m1;
+            for (int j = 0; j < HV; ++j) v[j] = h * 2 + j / 16 < nb ? s[h * 32 + j] : -INFINITY;
+            alpha[h] = pa_transpose_reduce<HV>(v, lane, [](float a, float b) { return fmaxf(a, b); });
+            wmax[quad * 64 + h * 32 + lane] = alpha[h];
+          }
           if (!meet()) { ok = false; break; }
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            m0 = fmaxf(m0, wmax[w * R + lane]);
-            m1 = fmaxf(m1, wmax[w * R + 32 + lane]);
+          for (int h = 0; h < H; ++h) {
+            float m = ref[h];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) m = fmaxf(m, wmax[w * 64 + h * 32 + lane]);
+            alpha[h] = ref[h] == -INFINITY ? 0.f : pa_exp2((ref[h] - m) * sl2);
+            ref[h] = m;
+            if (HV == 32 || lane < HV) nref[h * 32 + lane] = m == -INFINITY ? INFINITY : -m * sl2;
           }
-          m0 = fmaxf(m0, ref0);
-          m1 = fmaxf(m1, ref1);
-          const float a0 = ref0 == -INFINITY ? 0.f : pa_exp2((ref0 - m0) * sl2);
-          const float a1 = ref1 == -INFINITY ? 0.f : pa_exp2((ref1 - m1) * sl2);
-          ref0 = m0;
-          ref1 = m1;
-          nref[lane] = m0 == -INFINITY ? INFINITY : -m0 * sl2;
-          nref[32 + lane] = m1 == -INFINITY ? INFINITY : -m1 * sl2;
           if (t >= 2) {
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
+            for (int b = 0; b < NB; ++b)
               if (b < nb) {
                 uint32_t o[16];
                 sb::tmem_ld16(t_lane + O_COL + x * R + b * 16, o);
                 sb::tmem_ld_wait();
 #pragma unroll
                 for (int u = 0; u < 16; ++u) {
-                  const float a = __shfl_sync(0xffffffffu, b < 2 ? a0 : a1, (b & 1) * 16 + u);
+                  const float a = __shfl_sync(0xffffffffu, alpha[b / 2], (b & 1) * 16 + u);
                   l[b * 16 + u] *= a;
                   o[u] = __float_as_uint(__uint_as_float(o[u]) * a);
                 }
@@ -1028,7 +1044,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           if (!meet()) { ok = false; break; }  // every warp has read the maxima: P goes to the same place
         }
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int b = 0; b < NB; ++b)
           if (b < nb) {
             uint32_t pk[8];
 #pragma unroll
@@ -1067,28 +1083,18 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         ++retired;
         sb::tc_fence_after();
       }
-      // row sums over the warp's keys: lane r ends with rows r and r + 32
-      float sum[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (h == 0 || nb > 2) {
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-            for (int j = 0; j < o; ++j) {
-              const bool up = lane & o;
-              const float send = up ? l[h * 32 + j] : l[h * 32 + j + o], keep = up ? l[h * 32 + j + o] : l[h * 32 + j];
-              l[h * 32 + j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-            }
-        }
-        sum[h] = l[h * 32];
-      }
+      // row sums over the warp's keys and the references, for both groups to see (P is not in use)
       __syncwarp();
-      nref[lane] = sum[0];
-      nref[32 + lane] = sum[1];
-      if (quad == 0) {  // P of this group is not in use: its place takes the references
-        wmax[lane] = ref0;
-        wmax[32 + lane] = ref1;
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        float v[HV];
+#pragma unroll
+        for (int j = 0; j < HV; ++j) v[j] = l[h * 32 + j];
+        const float sum = pa_transpose_reduce<HV>(v, lane, [](float a, float b) { return a + b; });
+        if (HV == 32 || lane < HV) {
+          nref[h * 32 + lane] = sum;
+          if (quad == 0) wmax[h * 32 + lane] = ref[h];
+        }
       }
       sb::tc_fence_before();
       __syncwarp();
@@ -1096,27 +1102,32 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       if (!pa_wait(&c.fin, i & 1, abort_flag)) break;
       sb::tc_fence_after();
       // factors of both groups' O and the joint reference and sum of rows lane and lane + 32
-      float f0[2], f1[2], top[2], tot[2];
+      float f0[H], f1[H];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = h * 32 + lane;
+      for (int h = 0; h < H; ++h) {
+        const int row = h * 32 + (lane & (HV - 1));
         const float ra = reinterpret_cast<const float*>(sP)[row], rb = reinterpret_cast<const float*>(sP + P_BYTES)[row];
-        top[h] = fmaxf(ra, rb);
-        f0[h] = ra == -INFINITY ? 0.f : pa_exp2((ra - top[h]) * sl2);
-        f1[h] = rb == -INFINITY ? 0.f : pa_exp2((rb - top[h]) * sl2);
-        const float la = (xrow[row] + xrow[R + row]) + (xrow[2 * R + row] + xrow[3 * R + row]);
-        const float lb = (xrow[4 * R + row] + xrow[5 * R + row]) + (xrow[6 * R + row] + xrow[7 * R + row]);
-        tot[h] = (f0[h] == 0.f ? 0.f : la * f0[h]) + (f1[h] == 0.f ? 0.f : lb * f1[h]);
+        const float top = fmaxf(ra, rb);
+        f0[h] = ra == -INFINITY ? 0.f : pa_exp2((ra - top) * sl2);
+        f1[h] = rb == -INFINITY ? 0.f : pa_exp2((rb - top) * sl2);
+        float la = 0.f, lb = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          la += xrow[w * R + row];
+          lb += xrow[(4 + w) * R + row];
+        }
+        const float tot = (f0[h] == 0.f ? 0.f : la * f0[h]) + (f1[h] == 0.f ? 0.f : lb * f1[h]);
         if (it.slot < 0) {
-          const float inv = tot[h] > 0.f ? 1.f / tot[h] : (tot[h] == 0.f ? 0.f : tot[h]);  // no visible key: zeros; NaN stays
+          const float inv = tot > 0.f ? 1.f / tot : (tot == 0.f ? 0.f : tot);  // no visible key: zeros; NaN stays
           f0[h] *= inv;
           f1[h] *= inv;
         } else if (warp == 0 && row < it.rows) {
-          p.part_ml[(long)it.slot * p.part_rows + row] = make_float2(top[h] == -INFINITY ? -INFINITY : top[h] * sl2, tot[h]);
+          p.part_ml[(long)it.slot * p.part_rows + row] = make_float2(top == -INFINITY ? -INFINITY : top * sl2, tot);
         }
       }
       // group x writes rows x * 8 nb .. (x + 1) * 8 nb; thread = column of the head
       const int d = key;
+#pragma unroll 1
       for (int j0 = 0; j0 < nb * 8; j0 += 8) {
         const int row0 = x * nb * 8 + j0;
         uint32_t a[8], b[8];
@@ -1126,8 +1137,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int row = row0 + j;
-          const float ga = __shfl_sync(0xffffffffu, row < 32 ? f0[0] : f0[1], row & 31);
-          const float gb = __shfl_sync(0xffffffffu, row < 32 ? f1[0] : f1[1], row & 31);
+          const float ga = __shfl_sync(0xffffffffu, row < 32 ? f0[0] : f0[H - 1], row & 31);
+          const float gb = __shfl_sync(0xffffffffu, row < 32 ? f1[0] : f1[H - 1], row & 31);
           float v = __uint_as_float(a[j]) * ga;
           if (n > 1) v = fmaf(__uint_as_float(b[j]), gb, v);
           if (row < it.rows) {
@@ -1151,72 +1162,108 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 }
 
 // ============================================================================ joining the partial results
-// blockIdx.x: the CTA that started an item (first of the narrow kernel, then of the wide one); blockIdx.y strides over the item's rows.  Thread = (part group, four columns):
-// each group runs over every PG-th part with an online reference, the groups are joined in order.
+// A task is a block of rows of an item that several CTAs worked on: eight rows with a thread per four columns, or, with many
+// parts, one row whose parts are dealt to eight groups of threads that are joined in order.  Every block lists the tasks
+// (one descriptor per CTA) and takes every gridDim-th, so the launch is one wave whatever the items are.
 template <int PANELS, bool F16>
-__global__ void __launch_bounds__(PA_COMBINE_THREADS)
-    pa_combine_kernel(const PaParams first_p, const PaParams second_p, int first_ctas) {
-  constexpr int DP = PANELS * 64, QUADS = DP / 4, PG = PA_COMBINE_THREADS / QUADS;
+__global__ void __launch_bounds__(PA_COMBINE_THREADS, 4)
+    pa_combine_kernel(const __grid_constant__ PaParams pn, const __grid_constant__ PaParams pw, int narrow_ctas, int ctas) {
+  constexpr int DP = PANELS * 64, QUADS = DP / 4, PG = PA_COMBINE_THREADS / QUADS, WARPS = PA_COMBINE_THREADS / 32;
   __shared__ float4 so[PG][QUADS];
   __shared__ float2 sml[PG];
+  __shared__ int swarp[WARPS];
+  __shared__ int stask[3];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const bool second = (int)blockIdx.x >= first_ctas;
-  const PaParams& p = second ? second_p : first_p;
-  const int cta = second ? (int)blockIdx.x - first_ctas : (int)blockIdx.x;
-  if (p.zero_tail) {  // rows behind the last sequence
-    const long first = p.batch > 0 ? min(max(p.cu[p.batch], 0), p.T) : 0, heads = (long)p.Hkv * p.group;
-    const long chunks = (p.T - first) * heads * (p.D / 8);
-    const long step = (long)gridDim.x * gridDim.y * PA_COMBINE_THREADS;
-    for (long c = ((long)blockIdx.y * gridDim.x + blockIdx.x) * PA_COMBINE_THREADS + threadIdx.x; c < chunks; c += step) {
-      const long row = c / (p.D / 8), t = row / heads;
-      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + (first + t) * p.o_tok + (row - t * heads) * p.o_head +
-                                (c - row * (p.D / 8)) * 8) = make_uint4(0, 0, 0, 0);
+  if (pn.zero_tail) {  // rows behind the last sequence
+    const long first = pn.batch > 0 ? min(max(pn.cu[pn.batch], 0), pn.T) : 0, heads = (long)pn.Hkv * pn.group;
+    const long chunks = (pn.T - first) * heads * (pn.D / 8);
+    for (long c = (long)blockIdx.x * PA_COMBINE_THREADS + threadIdx.x; c < chunks; c += (long)gridDim.x * PA_COMBINE_THREADS) {
+      const long row = c / (pn.D / 8), t = row / heads;
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(pn.out) + (first + t) * pn.o_tok + (row - t * heads) * pn.o_head +
+                                (c - row * (pn.D / 8)) * 8) = make_uint4(0, 0, 0, 0);
     }
   }
-  const int* desc = p.part_desc + 8 * cta;
-  if (!desc[0]) return;
-  const int row0 = desc[1], rem = desc[2], hk = desc[3], rows = desc[4], last = desc[5];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int quad = threadIdx.x % QUADS, pg = threadIdx.x / QUADS;
-  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
-    float ref = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  int before = 0;  // tasks of the descriptors before `base`
+  for (int base = 0; base < ctas; base += PA_COMBINE_THREADS) {
+    const int mine = base + threadIdx.x;
+    int tasks = 0;
+    if (mine < ctas) {
+      const int local = mine < narrow_ctas ? mine : mine - narrow_ctas;
+      const int* desc = (mine < narrow_ctas ? pn : pw).part_desc + 8 * local;
+      if (desc[0]) tasks = desc[5] - local < PG ? (desc[4] + PG - 1) / PG : desc[4];
+    }
+    const int inc = pa_scan(tasks, lane);
+    __syncthreads();
+    if (lane == 31) swarp[warp] = inc;
+    __syncthreads();
+    int lo = before + inc - tasks, all = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) lo += swarp[w];
+      all += swarp[w];
+    }
+    // tasks of this block inside [before, before + all)
+    int task = (int)blockIdx.x + (before > (int)blockIdx.x ? (before - (int)blockIdx.x + gridDim.x - 1) / gridDim.x * gridDim.x : 0);
+    for (; task < before + all; task += gridDim.x) {
+      __syncthreads();
+      if (task >= lo && task < lo + tasks) {
+        stask[0] = mine;
+        stask[1] = task - lo;
+      }
+      __syncthreads();
+      const bool wide = stask[0] >= narrow_ctas;
+      const int cta = wide ? stask[0] - narrow_ctas : stask[0], block = stask[1];
+      const PaParams& p = wide ? pw : pn;
+      const int* desc = p.part_desc + 8 * cta;
+      const int row0 = desc[1], rem = desc[2], hk = desc[3], rows = desc[4], last = desc[5];
+      const bool few = last - cta < PG;
+      const int row = few ? block * PG + pg : block, step = few ? 1 : PG;
+      float ref = -INFINITY, l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < rows) {
 #pragma unroll 4
-    for (int c = cta + pg; c <= last; c += PG) {
-      const long prow = (long)(2 * c + (c == cta ? 1 : 0)) * p.part_rows + row;
-      const float2 ml = p.part_ml[prow];
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + prow * DP + quad * 4);
-      if (ml.x == -INFINITY && ml.y == 0.f) continue;  // a part without a visible key
-      const float next = fmaxf(ref, ml.x);
-      const float a = ref == -INFINITY ? 0.f : exp2f(ref - next), b = exp2f(ml.x - next);
-      l = l * a + ml.y * b;
-      o.x = o.x * a + v.x * b; o.y = o.y * a + v.y * b; o.z = o.z * a + v.z * b; o.w = o.w * a + v.w * b;
-      ref = next;
-    }
-    __syncthreads();
-    so[pg][quad] = o;
-    if (quad == 0) sml[pg] = make_float2(ref, l);
-    __syncthreads();
-    if (pg == 0) {
-      float top = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int g = 0; g < PG; ++g) top = fmaxf(top, sml[g].x);
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int g = 0; g < PG; ++g) {
-        const float2 ml = sml[g];
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;
-        const float f = exp2f(ml.x - top);
-        const float4 v = so[g][quad];
-        sum += ml.y * f;
-        acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+        for (int c = few ? cta : cta + pg; c <= last; c += step) {
+          const long prow = (long)(2 * c + (c == cta ? 1 : 0)) * p.part_rows + row;
+          const float2 ml = p.part_ml[prow];
+          const float4 v = *reinterpret_cast<const float4*>(p.part_o + prow * DP + quad * 4);
+          if (ml.x == -INFINITY && ml.y == 0.f) continue;  // a part without a visible key
+          const float next = fmaxf(ref, ml.x);
+          const float a = ref == -INFINITY ? 0.f : exp2f(ref - next), b = exp2f(ml.x - next);
+          l = l * a + ml.y * b;
+          o.x = o.x * a + v.x * b; o.y = o.y * a + v.y * b; o.z = o.z * a + v.z * b; o.w = o.w * a + v.w * b;
+          ref = next;
+        }
       }
-      const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-      const int tok = pa_div(p, rem + row), head = hk * p.group + (rem + row - tok * p.group);
-      if (quad * 4 < p.D) {
+      if (!few) {
+        so[pg][quad] = o;
+        if (quad == 0) sml[pg] = make_float2(ref, l);
+        __syncthreads();
+        if (pg > 0) continue;
+        ref = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < PG; ++g) ref = fmaxf(ref, sml[g].x);
+        l = 0.f;
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int g = 0; g < PG; ++g) {
+          const float2 ml = sml[g];
+          if (ml.x == -INFINITY && ml.y == 0.f) continue;
+          const float f = exp2f(ml.x - ref);
+          const float4 v = so[g][quad];
+          l += ml.y * f;
+          o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
+        }
+      }
+      if (row < rows && quad * 4 < p.D) {
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        const int tok = pa_div(p, rem + row), head = hk * p.group + (rem + row - tok * p.group);
         uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (long)(row0 + tok) * p.o_tok + (long)head * p.o_head + quad * 4;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pa_pack<F16>(acc.x * inv, acc.y * inv), pa_pack<F16>(acc.z * inv, acc.w * inv));
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pa_pack<F16>(o.x * inv, o.y * inv), pa_pack<F16>(o.z * inv, o.w * inv));
       }
     }
+    before += all;
   }
 }
 
@@ -1267,24 +1314,23 @@ long pa_align(long v) { return (v + 255) & ~255L; }
 // head) are narrow; with no more new tokens than sequences, as in a decoding step, all of them are, whatever their length:
 // the second launch then finds nothing (3 us), and a sequence that does have more rows is read once per 64 of them.
 struct PaPlan {
-  bool wide, narrow;
-  int narrow_max, narrow_ctas, wide_ctas, narrow_rows, wide_rows;
+  bool wide;
+  int narrow_max, narrow_rows, narrow_ctas, wide_ctas;
   long narrow_at, wide_at, bytes;
 };
 PaPlan pa_plan(long T, int batch, int Hq, int Hkv, int D, long cap, int sms) {
   PaPlan w = {};
   const long group = Hq / Hkv, rows = T * group, dp = D <= 64 ? 64 : 128;
-  w.narrow = true;
   w.wide = rows > PA_NARROW_ROWS && T > batch;
   w.narrow_max = w.wide ? PA_NARROW_ROWS : 0x7fffffff;
-  w.narrow_ctas = (int)pa_ctas(T, batch, Hq, Hkv, cap, PA_NARROW_ROWS, sms);
+  // decoding steps whose heads per KV head fit 16 rows take the kernel with the shorter code
+  w.narrow_rows = w.wide || group > 16 ? PA_NARROW_ROWS : 16;
+  w.narrow_ctas = (int)pa_ctas(T, batch, Hq, Hkv, cap, w.narrow_rows, sms);
   w.wide_ctas = w.wide ? (int)pa_ctas(T, batch, Hq, Hkv, cap, PA_WIDE_ROWS, sms) : 0;
-  w.narrow_rows = (int)(rows < PA_NARROW_ROWS ? rows : PA_NARROW_ROWS);
-  w.wide_rows = (int)(rows < PA_WIDE_ROWS ? rows : PA_WIDE_ROWS);
   auto size = [&](long ctas, long r) { return pa_align(2 * ctas * r * dp * 4) + pa_align(2 * ctas * r * 8) + pa_align(ctas * 32); };
   w.narrow_at = 0;
   w.wide_at = size(w.narrow_ctas, w.narrow_rows);
-  w.bytes = w.wide_at + (w.wide ? size(w.wide_ctas, w.wide_rows) : 0);
+  w.bytes = w.wide_at + (w.wide ? size(w.wide_ctas, PA_WIDE_ROWS) : 0);
   return w;
 }
 void pa_place(PaParams* p, uint8_t* ws, long ctas, int rows, long dp) {
@@ -1306,7 +1352,9 @@ int pa_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, PaParams p, const 
   if (dev >= 64 || !set[dev]) {
     e = cudaFuncSetAttribute(pa_wide_kernel<PANELS, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(pa_narrow_kernel<PANELS, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+      e = cudaFuncSetAttribute(pa_narrow_kernel<PANELS, F16, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(pa_narrow_kernel<PANELS, F16, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return (int)e;
     if (dev < 64) set[dev] = true;
   }
@@ -1314,25 +1362,25 @@ int pa_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, PaParams p, const 
   PaParams pn = p, pw = p;
   pa_place(&pn, ws + w.narrow_at, w.narrow_ctas, w.narrow_rows, PaCfg<PANELS>::DP);
   if (w.wide) {
-    pa_place(&pw, ws + w.wide_at, w.wide_ctas, w.wide_rows, PaCfg<PANELS>::DP);
+    pa_place(&pw, ws + w.wide_at, w.wide_ctas, PA_WIDE_ROWS, PaCfg<PANELS>::DP);
     pa_wide_kernel<PANELS, F16><<<w.wide_ctas, PA_THREADS, SMEM, stream>>>(tmK, tmV, pw);
     SB_CHECK_LAUNCH();
   }
-  pa_narrow_kernel<PANELS, F16><<<w.narrow_ctas, PA_THREADS, SMEM, stream>>>(tmK, tmV, pn);
+  if (w.narrow_rows == 16) pa_narrow_kernel<PANELS, F16, 1><<<w.narrow_ctas, PA_THREADS, SMEM, stream>>>(tmK, tmV, pn);
+  else pa_narrow_kernel<PANELS, F16, 4><<<w.narrow_ctas, PA_THREADS, SMEM, stream>>>(tmK, tmV, pn);
   SB_CHECK_LAUNCH();
   // launched while the kernel before still runs; waits for it on the device
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  const int rows = w.wide ? w.wide_rows : w.narrow_rows;
-  cfg.gridDim = dim3(w.narrow_ctas + w.wide_ctas, rows < 16 ? rows : 16);
+  const int ctas = w.narrow_ctas + w.wide_ctas;
+  cfg.gridDim = dim3(w.wide || ctas >= 128 ? 4 * 148 : 4 * ctas);
   cfg.blockDim = dim3(PA_COMBINE_THREADS);
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const PaParams second = w.wide ? pw : pn;
-  e = cudaLaunchKernelEx(&cfg, pa_combine_kernel<PANELS, F16>, pn, second, w.narrow_ctas);
+  e = cudaLaunchKernelEx(&cfg, pa_combine_kernel<PANELS, F16>, pn, pw, w.narrow_ctas, ctas);
   return e == cudaSuccess ? SB_OK : (int)e;
 }
 
