@@ -270,12 +270,19 @@ struct PaCursor {  // where a CTA's piece of the line starts, and how long it is
 // The whole warp; sums[c] = length per KV head of sequences 32 c .. 32 c + 31.
 template <int ROWS>
 __device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int chunks, int lane, PaCursor& c) {
+  c = PaCursor{};
+  PaSeq s = {0, 0, 0};
+  int cost = 0;  // of sequence 32 chunk + lane
   long long all = 0;
-  for (int i = lane; i < chunks; i += 32) all += sums[i];
+  if (chunks > 1) {
+    for (int i = lane; i < chunks; i += 32) all += sums[i];
+  } else {
+    cost = pa_chunk_cost<ROWS>(p, 0, lane, s);
+    all = cost;
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   all *= p.Hkv;
-  c = PaCursor{};
   if (all > 0x7fffffff) {  // months of work
     if (lane == 0) *p.status = SB_ERR_TOO_LARGE;
     return;
@@ -303,9 +310,9 @@ __device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int 
       }
       off -= __shfl_sync(0xffffffffu, inc, 31);
     }
+    cost = pa_chunk_cost<ROWS>(p, chunk, lane, s);
   }
-  PaSeq s;
-  const int cost = pa_chunk_cost<ROWS>(p, chunk, lane, s), v = cost * p.Hkv, inc = pa_scan(v, lane);
+  const int v = cost * p.Hkv, inc = pa_scan(v, lane);
   const int k = __ffs(__ballot_sync(0xffffffffu, inc > off)) - 1;
   off -= __shfl_sync(0xffffffffu, inc - v, k);
   const int per_head = __shfl_sync(0xffffffffu, cost, k);
@@ -398,17 +405,26 @@ __device__ __forceinline__ void pa_schedule(const PaParams& p, PaCtrl<PaCfg<PANE
       const int qs = (q_cnt + x) & 1;
       ok = pa_wait(&c.q_empty[qs], (((q_cnt + x) >> 1) & 1) ^ 1, abort_flag);
       if (!ok) break;
-      constexpr int CH = DP / 8;  // chunks per row
+      constexpr int CH = DP / 8, STEP = 32 / CH;  // chunks per row, rows per instruction
       const int ch = lane % CH, live = min(it.rows - x * SLOT_ROWS, SLOT_ROWS), end = PaKind<ROWS>::NARROW ? (live + 15) & ~15 : (live + 31) & ~31;
       const uint32_t dst = sb::smem_u32(sQ + qs * SLOT_BYTES) + (ch >> 3) * (SLOT_ROWS * 128);
-      const uint16_t* base = reinterpret_cast<const uint16_t*>(p.q) + (long)it.row0 * p.q_tok +
-                             (long)it.hk * p.group * p.q_head + ch * 8;
-#pragma unroll 1  // short code: it runs once per item and is fetched each time
-      for (int r = lane / CH; r < end; r += 32 / CH) {
-        const int row = it.rem + x * SLOT_ROWS + r, t = pa_div(p, row), h = row - t * p.group;
+      // row -> (token, head) by steps, without a division per row
+      const int row = it.rem + x * SLOT_ROWS + lane / CH, t0 = pa_div(p, row);
+      int h = row - t0 * p.group;
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (long)(it.row0 + t0) * p.q_tok +
+                            (long)(it.hk * p.group + h) * p.q_head + ch * 8;
+      const int dt = pa_div(p, STEP), dh = STEP - dt * p.group;
+      const long go = dt * p.q_tok + dh * p.q_head, wrap = p.q_tok - p.group * p.q_head;
+#pragma unroll 2
+      for (int r = lane / CH; r < end; r += STEP) {
         const bool take = r < live && ch * 8 < p.D;
-        pa_cp16(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4),
-                take ? base + (long)t * p.q_tok + (long)h * p.q_head : reinterpret_cast<const uint16_t*>(p.q), take);
+        pa_cp16(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4), take ? src : reinterpret_cast<const uint16_t*>(p.q), take);
+        src += go;
+        h += dh;
+        if (h >= p.group) {
+          h -= p.group;
+          src += wrap;
+        }
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
       sb::fence_proxy_async_smem();
@@ -478,7 +494,8 @@ template <int PANELS> __device__ __forceinline__ void pa_zero_v_row(const PaPara
     *reinterpret_cast<uint4*>(dst + (c >> 3) * p.panel_step + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
 }
 
-// Barriers, TMEM and the lengths of 32 sequences at a time (left where the scheduler puts the queries afterwards).
+// Barriers, TMEM and the lengths of 32 sequences at a time (left where the scheduler puts the queries
+// afterwards; with one such group the scheduler works it out alone).
 // Returns false if shared memory does not start on a 1024-byte boundary, as the swizzled tiles need.
 template <int ROWS, int STAGES>
 __device__ __forceinline__ bool pa_begin(const PaParams& p, PaCtrl<STAGES>& c, uint8_t* smem, int warp, int lane) {
@@ -517,7 +534,7 @@ __device__ __forceinline__ bool pa_begin(const PaParams& p, PaCtrl<STAGES>& c, u
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int* sums = reinterpret_cast<int*>(smem);
   const int chunks = (p.batch + 31) / 32;
-  for (int k = warp; k < chunks; k += PA_WARPS) {
+  for (int k = chunks > 1 ? warp : chunks; k < chunks; k += PA_WARPS) {
     PaSeq s;
     const int t = pa_sum(pa_chunk_cost<ROWS>(p, k, lane, s));
     if (lane == 0) sums[k] = t;
@@ -539,6 +556,8 @@ template <int STAGES> __device__ __forceinline__ void pa_end(const PaParams& p, 
     sb::tc_fence_after();
     sb::tmem_dealloc(c.tmem_slot, 512);
   }
+  // the narrow kernel may have started before the wide one ended: it does not end before it
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (threadIdx.x == 0 && *abort_flag) *p.status = SB_ERR_WAIT_TIMEOUT;
 }
 
@@ -1127,6 +1146,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       }
       // group x writes rows x * 8 nb .. (x + 1) * 8 nb; thread = column of the head
       const int d = key;
+      const bool store = it.slot < 0 ? d < p.D : d < DP;
+      long at[H];  // where rows lane and lane + 32 go, -1: nowhere
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const int row = h * 32 + (lane & (HV - 1)), tok = pa_div(p, it.rem + row);
+        at[h] = it.slot < 0 ? (long)(it.row0 + tok) * p.o_tok + (long)(it.hk * p.group + it.rem + row - tok * p.group) * p.o_head
+                            : ((long)it.slot * p.part_rows + row) * DP;
+        if (row >= it.rows) at[h] = -1;
+      }
 #pragma unroll 1
       for (int j0 = 0; j0 < nb * 8; j0 += 8) {
         const int row0 = x * nb * 8 + j0;
@@ -1141,15 +1169,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           const float gb = __shfl_sync(0xffffffffu, row < 32 ? f1[0] : f1[H - 1], row & 31);
           float v = __uint_as_float(a[j]) * ga;
           if (n > 1) v = fmaf(__uint_as_float(b[j]), gb, v);
-          if (row < it.rows) {
-            if (it.slot < 0) {
-              const int tok = pa_div(p, it.rem + row), head = it.hk * p.group + (it.rem + row - tok * p.group);
-              if (d < p.D)
-                reinterpret_cast<uint16_t*>(p.out)[(long)(it.row0 + tok) * p.o_tok + (long)head * p.o_head + d] =
-                    (uint16_t)pa_pack<F16>(v, 0.f);
-            } else if (d < DP) {
-              p.part_o[((long)it.slot * p.part_rows + row) * DP + d] = v;
-            }
+          const long to = __shfl_sync(0xffffffffu, row < 32 ? at[0] : at[H - 1], row & 31);
+          if (to >= 0 && store) {
+            if (it.slot < 0) reinterpret_cast<uint16_t*>(p.out)[to + d] = (uint16_t)pa_pack<F16>(v, 0.f);
+            else p.part_o[to + d] = v;
           }
         }
       }
@@ -1366,19 +1389,25 @@ int pa_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, PaParams p, const 
     pa_wide_kernel<PANELS, F16><<<w.wide_ctas, PA_THREADS, SMEM, stream>>>(tmK, tmV, pw);
     SB_CHECK_LAUNCH();
   }
-  if (w.narrow_rows == 16) pa_narrow_kernel<PANELS, F16, 1><<<w.narrow_ctas, PA_THREADS, SMEM, stream>>>(tmK, tmV, pn);
-  else pa_narrow_kernel<PANELS, F16, 4><<<w.narrow_ctas, PA_THREADS, SMEM, stream>>>(tmK, tmV, pn);
-  SB_CHECK_LAUNCH();
-  // launched while the kernel before still runs; waits for it on the device
+  // Launches that may start while the kernel before still runs: the narrow kernel reads nothing that the wide one writes,
+  // its CTAs follow as SMs become free; the last kernel waits on the device.
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(w.narrow_ctas);
+  cfg.blockDim = dim3(PA_THREADS);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = w.wide ? 1 : 0;
+  e = w.narrow_rows == 16 ? cudaLaunchKernelEx(&cfg, pa_narrow_kernel<PANELS, F16, 1>, tmK, tmV, pn)
+                          : cudaLaunchKernelEx(&cfg, pa_narrow_kernel<PANELS, F16, 4>, tmK, tmV, pn);
+  if (e != cudaSuccess) return (int)e;
   const int ctas = w.narrow_ctas + w.wide_ctas;
   cfg.gridDim = dim3(w.wide || ctas >= 128 ? 4 * 148 : 4 * ctas);
   cfg.blockDim = dim3(PA_COMBINE_THREADS);
-  cfg.stream = stream;
-  cfg.attrs = &attr;
+  cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, pa_combine_kernel<PANELS, F16>, pn, pw, w.narrow_ctas, ctas);
   return e == cudaSuccess ? SB_OK : (int)e;
