@@ -23,8 +23,8 @@
 // Narrow (at most 64 rows: decoding): a stream over K and V, so everything else has to be small against the tile's bytes.
 //   Rows in lanes would leave most lanes and three of four warps idle; here the keys are in the lanes: S^T = K Q^T
 //   [128 keys x rows], a thread takes the exponentials of one key for all rows, and O^T += V^T P [D x rows].  S^T of four
-//   tiles is in flight.  A thread keeps the row sums over its own keys; the rows' references are shared by the four warps
-//   of a group, which agree once per tile whether any score has outgrown them.
+//   tiles is in flight.  The rows' references are shared by the four warps of a group, which agree once per tile whether
+//   any score has outgrown them (then the tile's P is written again).
 //
 // Warp roles: 0-3 and 4-7 softmax groups, 8 and 11 TMA loaders of K and of V (a page of 16 tokens is a copy of its own, and
 // one warp alone issues them no faster than the memory delivers), 9 MMA issuer, 10 scheduler, which also copies the queries.
@@ -47,7 +47,7 @@ constexpr int PA_PANEL = 16384;   // 128 rows x 128 bytes
 constexpr int PA_ITEMS = 4;       // descriptors in flight
 constexpr int PA_COMBINE_THREADS = 256;
 // What the start and the end of an item cost, in tiles: added to its length on the work line.
-constexpr int PA_WIDE_COST = 2, PA_NARROW_COST = 1;
+constexpr int PA_WIDE_COST = 2, PA_NARROW_COST = 3;
 // ROWS (rows per item) tells the kernels apart in the functions that they share.
 template <int ROWS> struct PaKind {
   static constexpr bool NARROW = ROWS <= PA_NARROW_ROWS;
@@ -834,14 +834,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 }
 
 // ============================================================================ narrow kernel
-// v[j] of lane i is the value of row j; lane r ends with the result over all lanes of row r (NV = 16: and so does r + 16).
-template <int NV, typename F> __device__ __forceinline__ float pa_transpose_reduce(float (&v)[NV], int lane, F f) {
-  if (NV == 16) {
+// v[j] of all lanes joined by f: lanes r and r + 16 end with the result of j = r.
+template <typename F> __device__ __forceinline__ float pa_transpose_reduce(float (&v)[16], int lane, F f) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) v[j] = f(v[j], __shfl_xor_sync(0xffffffffu, v[j], 16));
-  }
+  for (int j = 0; j < 16; ++j) v[j] = f(v[j], __shfl_xor_sync(0xffffffffu, v[j], 16));
 #pragma unroll
-  for (int o = NV / 2; o > 0; o >>= 1)
+  for (int o = 8; o > 0; o >>= 1)
 #pragma unroll
     for (int j = 0; j < o; ++j) {
       const bool up = lane & o;
@@ -851,33 +849,33 @@ template <int NV, typename F> __device__ __forceinline__ float pa_transpose_redu
   return v[0];
 }
 
-// NB: blocks of 16 rows that an item may have (1 or 4).
-template <int PANELS, bool F16, int NB>
+// All loops over the rows go by blocks of 16 and are not unrolled further: code that does not fit the instruction caches
+// costs more than the work here (unrolled over 64 rows the kernel took 48 us where it now takes less than half).  So what a
+// thread keeps of the rows between tiles has to be little: row r is kept by lane r % 32 of every warp.
+template <int PANELS, bool F16>
 __global__ void __launch_bounds__(PA_THREADS, 1)
     pa_narrow_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PaParams p) {
   using Cfg = PaCfg<PANELS>;
   constexpr int DP = Cfg::DP, TILE_BYTES = Cfg::TILE_BYTES, STAGES = Cfg::STAGES;
-  constexpr int R = 16 * NB, H = (NB + 1) / 2, Q_SLOT = PANELS * R * 128, P_BYTES = PA_TILE * 128;
-  constexpr int HV = R < 32 ? R : 32;         // rows of a half: row h * 32 + r belongs to lane r
-  constexpr uint32_t S_COL = 0, O_COL = 256;  // four S^T of R columns, two O^T of R
+  constexpr int R = PA_NARROW_ROWS, Q_SLOT = PANELS * R * 128, P_BYTES = PA_TILE * 128;
+  constexpr uint32_t S_COL = 0, O_COL = 256;  // four S^T and two O^T of 64 columns
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;                    // two slots of 64 rows
   uint8_t* sP = smem + 2 * 16384;        // [group][key][64 rows], 128-byte swizzle
   uint8_t* sRing = smem + Cfg::FRONT;
-  float* xrow = reinterpret_cast<float*>(smem + Cfg::DATA);  // [warp][R]: -reference of the rows, later their sums
+  float* sRef = reinterpret_cast<float*>(smem + Cfg::DATA);  // [group][old / new][row]: -reference, +inf where unset
   PaCtrl<STAGES>& c = *reinterpret_cast<PaCtrl<STAGES>*>(smem + Cfg::DATA + 2048);
   volatile int* abort_flag = &c.abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (!pa_begin<R>(p, c, smem, warp, lane)) return;
   const uint32_t tmem_base = c.tmem_slot;
 
-  if (warp >= 8) {
-    pa_regs_dec<PA_REGS_FEW>();
-    if (warp == 10) {
-      pa_schedule<R, PANELS>(p, c, sQ, (p.batch + 31) / 32, lane);
-    } else if (warp != 9) {
-      pa_load<R, PANELS>(p, c, sRing, warp == 11 ? &tmV : &tmK, warp == 11, lane);
-    } else if (lane == 0) {
+  if (warp == 10) {
+    pa_schedule<R, PANELS>(p, c, sQ, (p.batch + 31) / 32, lane);
+  } else if (warp == 8 || warp == 11) {
+    pa_load<R, PANELS>(p, c, sRing, warp == 11 ? &tmV : &tmK, warp == 11, lane);
+  } else if (warp == 9) {
+    if (lane == 0) {
       const uint64_t q_desc = sb::umma_smem_desc(sb::smem_u32(sQ), 16, 1024);
       const uint64_t k_desc = sb::umma_smem_desc(sb::smem_u32(sRing), 16, p.group_step);
       // V^T: 128 rows of the product are the columns of the tile; with a head size up to 64 the second half of them reads
@@ -912,33 +910,33 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           if (t == n - 1) sb::umma_commit(&c.q_empty[qs]);
           return true;
         };
-        for (int t = 0; t < min(n, 4) && ok; ++t) ok = issue_s(t);
-        for (int t = 0; t < n && ok; ++t) {
-          const int x = t & 1;
-          const uint32_t e = ring + pa_v_place(t, 4, n), st = e % STAGES;
-          ok = sb::mbar_wait(&c.full[st], (e / STAGES) & 1, abort_flag);
-          if (ok && t == 0 && i > 0) ok = sb::mbar_wait(&c.epi_done, (i - 1) & 1, abort_flag);  // O of the item before is read
-          ok = ok && sb::mbar_wait(&c.p_full[x], (x ? p_cnt1 : p_cnt0) & 1, abort_flag);
-          if (!ok) break;
-          if (x) ++p_cnt1; else ++p_cnt0;
-          sb::tc_fence_after();
-          const uint64_t vd = v_desc + st * (TILE_BYTES >> 4), pd = p_desc + x * (P_BYTES >> 4);
+#pragma unroll 1
+        for (int t = -4; t < n && ok; ++t) {
+          if (t >= 0) {
+            const int x = t & 1;
+            const uint32_t e = ring + pa_v_place(t, 4, n), st = e % STAGES;
+            ok = sb::mbar_wait(&c.full[st], (e / STAGES) & 1, abort_flag);
+            if (ok && t == 0 && i > 0) ok = sb::mbar_wait(&c.epi_done, (i - 1) & 1, abort_flag);  // O of the item before is read
+            ok = ok && sb::mbar_wait(&c.p_full[x], (x ? p_cnt1 : p_cnt0) & 1, abort_flag);
+            if (!ok) break;
+            if (x) ++p_cnt1; else ++p_cnt0;
+            sb::tc_fence_after();
+            const uint64_t vd = v_desc + st * (TILE_BYTES >> 4), pd = p_desc + x * (P_BYTES >> 4);
 #pragma unroll
-          for (int kk = 0; kk < PA_TILE / 16; ++kk)
-            sb::umma_f16_ss(tmem_base + O_COL + x * R, vd + kk * v_step, pd + kk * (2048 >> 4), idesc_o, t > 1 || kk != 0);
-          sb::umma_commit(&c.empty[st]);
-          sb::umma_commit(&c.p_empty[x]);
+            for (int kk = 0; kk < PA_TILE / 16; ++kk)
+              sb::umma_f16_ss(tmem_base + O_COL + x * R, vd + kk * v_step, pd + kk * (2048 >> 4), idesc_o, t > 1 || kk != 0);
+            sb::umma_commit(&c.empty[st]);
+            sb::umma_commit(&c.p_empty[x]);
+          }
           if (t + 4 < n) ok = issue_s(t + 4);
         }
         ring += 2 * n;
       }
     }
   } else {
-    pa_regs_inc<PA_REGS_MANY>();
     const int x = warp >> 2, quad = warp & 3, key = quad * 32 + lane;  // thread = key of the tile, later a column of V
     const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16);
     const float sl2 = p.sl2;
-    float* nref = xrow + warp * R;                             // this warp's copy: -reference * sl2, +inf where unset
     float* wmax = reinterpret_cast<float*>(sP + x * P_BYTES);  // [warp of the group][64], where P is not in use
     uint8_t* prow = sP + x * P_BYTES + key * 128;
     uint32_t ring = 0, s_cnt0 = 0, s_cnt1 = 0, issued = 0, retired = 0, votes = 0;
@@ -956,134 +954,132 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       __syncwarp();
       if (lane == 0) sb::mbar_arrive(&c.item_empty[islot]);
       if (it.count == 0) break;
-      if (i > 0 && !pa_wait(&c.epi_done, (i - 1) & 1, abort_flag)) break;  // xrow of the item before is read
-      const int nb = NB == 1 ? 1 : (it.rows + 15) >> 4, n = it.count;
+      if (i > 0 && !pa_wait(&c.epi_done, (i - 1) & 1, abort_flag)) break;  // sRef of the item before is read
+      const int nb = (it.rows + 15) >> 4, n = it.count;
       // keys that every row sees: tiles inside need no mask
-      int lo_all = 0, hi_all = 0x7fffffff;
-      {
-        const int pos1 = it.pos0 + pa_div(p, it.rem + it.rows - 1);
-        if (p.window >= 0) lo_all = max(0, pos1 - p.window);
-        hi_all = p.causal ? min(it.pos0 + 1, it.L)
-                          : (p.window >= 0 ? (int)min((long)it.L, (long)it.pos0 + p.window + 1) : it.L);
-      }
-      float ref[H];  // raw reference of rows lane and lane + 32
-#pragma unroll
-      for (int h = 0; h < H; ++h) ref[h] = -INFINITY;
-      float l[R];
-#pragma unroll
-      for (int j = 0; j < R; ++j) l[j] = 0.f;
+      const int pos1 = it.pos0 + pa_div(p, it.rem + it.rows - 1);
+      const int lo_all = p.window >= 0 ? max(0, pos1 - p.window) : 0;
+      const int hi_all = p.causal ? min(it.pos0 + 1, it.L)
+                                  : (p.window >= 0 ? (int)min((long)it.L, (long)it.pos0 + p.window + 1) : it.L);
+      int cur = 0;
+      float* ref = sRef + x * 2 * R;
+      float l0 = 0.f, l1 = 0.f;  // sums of rows lane and lane + 32 over this warp's keys
       for (int t = x; t < n; t += 2) {
         const int key0 = (it.tile0 + t) * PA_TILE, buf = (t >> 1) & 1;
+        if (retired < issued) {  // P V of this group's tile before: P may be overwritten, O rescaled
+          if (!pa_wait(&c.p_empty[x], retired & 1, abort_flag)) { ok = false; break; }
+          ++retired;
+        }
         if (!pa_wait(&c.s_full[x * 2 + buf], (buf ? s_cnt1 : s_cnt0) & 1, abort_flag)) { ok = false; break; }
         if (buf) ++s_cnt1; else ++s_cnt0;
         sb::tc_fence_after();
-        float s[R];
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-          if (b < nb) sb::tmem_ld16(t_lane + S_COL + (x * 2 + buf) * R + b * 16, *reinterpret_cast<uint32_t(*)[16]>(s + b * 16));
-        sb::tmem_ld_wait();
+        const uint32_t s_addr = t_lane + S_COL + (x * 2 + buf) * R;
         const bool inside = key0 >= lo_all && key0 + PA_TILE <= hi_all;
-        if (!inside) {
-          const int j = key0 + key;
+        // scores of a block of 16 rows, -inf where a row does not see the thread's key
+        auto scores = [&](int b, float (&s)[16]) {
+          sb::tmem_ld16(s_addr + b * 16, reinterpret_cast<uint32_t(&)[16]>(s));
+          sb::tmem_ld_wait();
+          if (!inside) {
+            const int j = key0 + key, tok = pa_div(p, it.rem + b * 16);
+            int pos = it.pos0 + tok, h = it.rem + b * 16 - tok * p.group;
 #pragma unroll
-          for (int b = 0; b < NB; ++b)
-            if (b < nb) {
-#pragma unroll
-              for (int u = 0; u < 16; ++u) {
-                const int pos = it.pos0 + pa_div(p, it.rem + b * 16 + u);
-                const int lo = p.window >= 0 ? pos - p.window : 0;
-                const int hi = p.causal ? min(pos + 1, it.L)
-                                        : (p.window >= 0 ? (int)min((long)it.L, (long)pos + p.window + 1) : it.L);
-                if (b * 16 + u < it.rows && (j < lo || j >= hi)) s[b * 16 + u] = -INFINITY;
+            for (int u = 0; u < 16; ++u) {
+              const int lo = p.window >= 0 ? pos - p.window : 0;
+              const int hi = p.causal ? min(pos + 1, it.L)
+                                      : (p.window >= 0 ? (int)min((long)it.L, (long)pos + p.window + 1) : it.L);
+              if (b * 16 + u < it.rows && (j < lo || j >= hi)) s[u] = -INFINITY;
+              if (++h == p.group) {
+                h = 0;
+                ++pos;
               }
             }
-        }
+          }
+        };
+        // P of the tile against the current references and its row sums; returns the largest exponent
+        float t0 = 0.f, t1 = 0.f;
+        auto probabilities = [&]() -> float {
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int b = 0; b < nb; ++b) {
+            float s[16];
+            scores(b, s);
+            uint32_t pk[8];
+#pragma unroll
+            for (int u = 0; u < 16; u += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(ref + cur * R + b * 16 + u);
+              const float fs[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                float z = fmaf(s[u + k], sl2, fs[k]);
+                if (!inside && s[u + k] == -INFINITY) z = -INFINITY;  // also where the reference is unset
+                top = fmaxf(top, z);
+                s[u + k] = pa_exp2(z);
+              }
+              pk[u / 2] = pa_pack<F16>(s[u], s[u + 1]);
+              pk[u / 2 + 1] = pa_pack<F16>(s[u + 2], s[u + 3]);
+            }
+            *reinterpret_cast<uint4*>(prow + (((b * 2) ^ (key & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            *reinterpret_cast<uint4*>(prow + (((b * 2 + 1) ^ (key & 7)) << 4)) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+            const float sum = pa_transpose_reduce(s, lane, [](float a, float b) { return a + b; });
+            if (lane >> 4 == (b & 1)) {
+              if (b < 2) t0 = sum; else t1 = sum;
+            }
+          }
+          return top;
+        };
         bool need = t < 2;  // no reference yet
         if (!need) {
-          float top = -INFINITY;
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-            if (b < nb) {
-#pragma unroll
-              for (int u = 0; u < 16; u += 4) {
-                const float4 f = *reinterpret_cast<const float4*>(nref + b * 16 + u);
-                top = fmaxf(top, fmaxf(fmaxf(fmaf(s[b * 16 + u], sl2, f.x), fmaf(s[b * 16 + u + 1], sl2, f.y)),
-                                       fmaxf(fmaf(s[b * 16 + u + 2], sl2, f.z), fmaf(s[b * 16 + u + 3], sl2, f.w))));
-              }
-            }
-          const int mine = __any_sync(0xffffffffu, top > 8.f);
+          const int mine = __any_sync(0xffffffffu, probabilities() > 8.f);
           int* flags = c.need[x][votes & 1];
           if (lane == 0) flags[quad] = mine;
           if (!meet()) { ok = false; break; }
           const int4 all = *reinterpret_cast<const int4*>(flags);
           need = (all.x | all.y | all.z | all.w) != 0;
         }
-        if (retired < issued) {  // P V of this group's tile before: P may be overwritten, O rescaled
-          if (!pa_wait(&c.p_empty[x], retired & 1, abort_flag)) { ok = false; break; }
-          ++retired;
-          sb::tc_fence_after();
-        }
         if (need) {
-          float alpha[H];
-#pragma unroll
-          for (int h = 0; h < H; ++h) {  // maxima over the warp's keys
-            float v[HV];
-#pragma unroll
-            for (int j = 0; j < HV; ++j) v[j] = h * 2 + j / 16 < nb ? s[h * 32 + j] : -INFINITY;
-            alpha[h] = pa_transpose_reduce<HV>(v, lane, [](float a, float b) { return fmaxf(a, b); });
-            wmax[quad * 64 + h * 32 + lane] = alpha[h];
+#pragma unroll 1
+          for (int b = 0; b < nb; ++b) {  // maxima over the warp's keys
+            float s[16];
+            scores(b, s);
+            const float m = pa_transpose_reduce(s, lane, [](float a, float b) { return fmaxf(a, b); });
+            if (lane < 16) wmax[quad * R + b * 16 + lane] = m;
           }
           if (!meet()) { ok = false; break; }
+          float alpha[2];  // of rows lane and lane + 32; every warp works them out
 #pragma unroll
-          for (int h = 0; h < H; ++h) {
-            float m = ref[h];
+          for (int h = 0; h < 2; ++h) {
+            const int row = h * 32 + lane;
+            float m = wmax[row];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) m = fmaxf(m, wmax[w * 64 + h * 32 + lane]);
-            alpha[h] = ref[h] == -INFINITY ? 0.f : pa_exp2((ref[h] - m) * sl2);
-            ref[h] = m;
-            if (HV == 32 || lane < HV) nref[h * 32 + lane] = m == -INFINITY ? INFINITY : -m * sl2;
+            for (int w = 1; w < 4; ++w) m = fmaxf(m, wmax[w * R + row]);
+            const float old = t < 2 ? INFINITY : ref[cur * R + row];
+            const float next = m == -INFINITY ? old : fminf(old, -m * sl2);
+            alpha[h] = old == INFINITY ? 0.f : pa_exp2(next - old);
+            if (row < nb * 16) ref[(cur ^ 1) * R + row] = next;
           }
+          cur ^= 1;
+          l0 *= alpha[0];
+          l1 *= alpha[1];
           if (t >= 2) {
+#pragma unroll 1
+            for (int b = 0; b < nb; ++b) {
+              uint32_t o[16];
+              sb::tmem_ld16(t_lane + O_COL + x * R + b * 16, o);
+              sb::tmem_ld_wait();
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-              if (b < nb) {
-                uint32_t o[16];
-                sb::tmem_ld16(t_lane + O_COL + x * R + b * 16, o);
-                sb::tmem_ld_wait();
-#pragma unroll
-                for (int u = 0; u < 16; ++u) {
-                  const float a = __shfl_sync(0xffffffffu, alpha[b / 2], (b & 1) * 16 + u);
-                  l[b * 16 + u] *= a;
-                  o[u] = __float_as_uint(__uint_as_float(o[u]) * a);
-                }
-                pa_tmem_st16(t_lane + O_COL + x * R + b * 16, o);
+              for (int u = 0; u < 16; ++u) {
+                const float a = __shfl_sync(0xffffffffu, b < 2 ? alpha[0] : alpha[1], (b & 1) * 16 + u);
+                o[u] = __float_as_uint(__uint_as_float(o[u]) * a);
               }
+              pa_tmem_st16(t_lane + O_COL + x * R + b * 16, o);
+            }
             sb::tmem_st_wait();
           }
           if (!meet()) { ok = false; break; }  // every warp has read the maxima: P goes to the same place
+          probabilities();
         }
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-          if (b < nb) {
-            uint32_t pk[8];
-#pragma unroll
-            for (int u = 0; u < 16; u += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(nref + b * 16 + u);
-              const float fs[4] = {f.x, f.y, f.z, f.w};
-              float e[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float v = s[b * 16 + u + k];
-                e[k] = pa_exp2(fmaf(v, sl2, fs[k]));
-                if (!inside && v == -INFINITY) e[k] = 0.f;  // also where the reference is unset
-                l[b * 16 + u + k] += e[k];
-              }
-              pk[u / 2] = pa_pack<F16>(e[0], e[1]);
-              pk[u / 2 + 1] = pa_pack<F16>(e[2], e[3]);
-            }
-            *reinterpret_cast<uint4*>(prow + (((b * 2) ^ (key & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-            *reinterpret_cast<uint4*>(prow + (((b * 2 + 1) ^ (key & 7)) << 4)) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
-          }
+        l0 += t0;
+        l1 += t1;
         if (key0 + PA_TILE > it.hi) {
           const uint32_t e = ring + pa_v_place(t, 4, n), st = e % STAGES;
           if (!pa_wait(&c.full[st], (e / STAGES) & 1, abort_flag)) { ok = false; break; }
@@ -1100,79 +1096,61 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       if (retired < issued) {
         if (!pa_wait(&c.p_empty[x], retired & 1, abort_flag)) break;
         ++retired;
-        sb::tc_fence_after();
       }
-      // row sums over the warp's keys and the references, for both groups to see (P is not in use)
-      __syncwarp();
-#pragma unroll
-      for (int h = 0; h < H; ++h) {
-        float v[HV];
-#pragma unroll
-        for (int j = 0; j < HV; ++j) v[j] = l[h * 32 + j];
-        const float sum = pa_transpose_reduce<HV>(v, lane, [](float a, float b) { return a + b; });
-        if (HV == 32 || lane < HV) {
-          nref[h * 32 + lane] = sum;
-          if (quad == 0) wmax[h * 32 + lane] = ref[h];
-        }
-      }
-      sb::tc_fence_before();
+      wmax[quad * R + lane] = l0;  // P of this group is not in use: its place takes the warps' sums
+      wmax[quad * R + 32 + lane] = l1;
+      if (quad == 0 && lane == 0) c.need[x][0][0] = cur;  // no vote is under way
       __syncwarp();
       if (lane == 0) sb::mbar_arrive(&c.fin);
       if (!pa_wait(&c.fin, i & 1, abort_flag)) break;
       sb::tc_fence_after();
-      // factors of both groups' O and the joint reference and sum of rows lane and lane + 32
-      float f0[H], f1[H];
-#pragma unroll
-      for (int h = 0; h < H; ++h) {
-        const int row = h * 32 + (lane & (HV - 1));
-        const float ra = reinterpret_cast<const float*>(sP)[row], rb = reinterpret_cast<const float*>(sP + P_BYTES)[row];
-        const float top = fmaxf(ra, rb);
-        f0[h] = ra == -INFINITY ? 0.f : pa_exp2((ra - top) * sl2);
-        f1[h] = rb == -INFINITY ? 0.f : pa_exp2((rb - top) * sl2);
-        float la = 0.f, lb = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          la += xrow[w * R + row];
-          lb += xrow[(4 + w) * R + row];
-        }
-        const float tot = (f0[h] == 0.f ? 0.f : la * f0[h]) + (f1[h] == 0.f ? 0.f : lb * f1[h]);
+      // Both groups' states are joined: group x writes rows x * 8 nb .. (x + 1) * 8 nb, thread = column of the head.
+      // Lane r works out the factors of row first + r, so that their chain of loads and exponentials is waited for once.
+      const int first = x * nb * 8, mine = min(first + lane, R - 1);
+      float g0, g1;
+      {
+        const float* sum0 = reinterpret_cast<const float*>(sP);
+        const float* sum1 = reinterpret_cast<const float*>(sP + P_BYTES);
+        const float r0 = sRef[c.need[0][0][0] * R + mine];
+        const float r1 = n > 1 ? sRef[(2 + c.need[1][0][0]) * R + mine] : INFINITY;
+        const float a0 = (sum0[mine] + sum0[R + mine]) + (sum0[2 * R + mine] + sum0[3 * R + mine]);
+        const float a1 = (sum1[mine] + sum1[R + mine]) + (sum1[2 * R + mine] + sum1[3 * R + mine]);
+        const float top = fminf(r0, r1);
+        g0 = r0 == INFINITY ? 0.f : pa_exp2(top - r0);
+        g1 = r1 == INFINITY ? 0.f : pa_exp2(top - r1);
+        const float sum = (g0 == 0.f ? 0.f : a0 * g0) + (g1 == 0.f ? 0.f : a1 * g1);
         if (it.slot < 0) {
-          const float inv = tot > 0.f ? 1.f / tot : (tot == 0.f ? 0.f : tot);  // no visible key: zeros; NaN stays
-          f0[h] *= inv;
-          f1[h] *= inv;
-        } else if (warp == 0 && row < it.rows) {
-          p.part_ml[(long)it.slot * p.part_rows + row] = make_float2(top == -INFINITY ? -INFINITY : top * sl2, tot);
+          const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // no visible key: zeros; NaN stays
+          g0 *= inv;
+          g1 *= inv;
+        } else if (quad == 0 && lane < nb * 8 && mine < it.rows) {
+          p.part_ml[(long)it.slot * p.part_rows + mine] = make_float2(-top, sum);
         }
       }
-      // group x writes rows x * 8 nb .. (x + 1) * 8 nb; thread = column of the head
       const int d = key;
-      const bool store = it.slot < 0 ? d < p.D : d < DP;
-      long at[H];  // where rows lane and lane + 32 go, -1: nowhere
-#pragma unroll
-      for (int h = 0; h < H; ++h) {
-        const int row = h * 32 + (lane & (HV - 1)), tok = pa_div(p, it.rem + row);
-        at[h] = it.slot < 0 ? (long)(it.row0 + tok) * p.o_tok + (long)(it.hk * p.group + it.rem + row - tok * p.group) * p.o_head
-                            : ((long)it.slot * p.part_rows + row) * DP;
-        if (row >= it.rows) at[h] = -1;
-      }
+      const bool whole = it.slot < 0, store = whole ? d < p.D : d < DP;
+      int row = first, tok = pa_div(p, it.rem + row), h = it.rem + row - tok * p.group;
+      long at = whole ? (long)(it.row0 + tok) * p.o_tok + (long)(it.hk * p.group + h) * p.o_head + d
+                      : ((long)it.slot * p.part_rows + row) * DP + d;
+      const long go = whole ? p.o_head : DP, wrap = whole ? p.o_tok - p.group * p.o_head : 0;
 #pragma unroll 1
-      for (int j0 = 0; j0 < nb * 8; j0 += 8) {
-        const int row0 = x * nb * 8 + j0;
-        uint32_t a[8], b[8];
-        pa_tmem_ld8(t_lane + O_COL + row0, a, 0);
-        if (n > 1) pa_tmem_ld8(t_lane + O_COL + R + row0, b, 0);
+      for (int j0 = 0; j0 < nb * 8 && row < it.rows; j0 += 8) {
+        uint32_t o0[8], o1[8] = {};
+        pa_tmem_ld8(t_lane + O_COL + row, o0, 0);
+        if (n > 1) pa_tmem_ld8(t_lane + O_COL + R + row, o1, 0);
         sb::tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int row = row0 + j;
-          const float ga = __shfl_sync(0xffffffffu, row < 32 ? f0[0] : f0[H - 1], row & 31);
-          const float gb = __shfl_sync(0xffffffffu, row < 32 ? f1[0] : f1[H - 1], row & 31);
-          float v = __uint_as_float(a[j]) * ga;
-          if (n > 1) v = fmaf(__uint_as_float(b[j]), gb, v);
-          const long to = __shfl_sync(0xffffffffu, row < 32 ? at[0] : at[H - 1], row & 31);
-          if (to >= 0 && store) {
-            if (it.slot < 0) reinterpret_cast<uint16_t*>(p.out)[to + d] = (uint16_t)pa_pack<F16>(v, 0.f);
-            else p.part_o[to + d] = v;
+        for (int j = 0; j < 8; ++j, ++row) {
+          const float ga = __shfl_sync(0xffffffffu, g0, j0 + j), gb = __shfl_sync(0xffffffffu, g1, j0 + j);
+          const float v = fmaf(__uint_as_float(o0[j]), ga, __uint_as_float(o1[j]) * gb);
+          if (row < it.rows && store) {
+            if (whole) reinterpret_cast<uint16_t*>(p.out)[at] = (uint16_t)pa_pack<F16>(v, 0.f);
+            else p.part_o[at] = v;
+          }
+          at += go;
+          if (++h == p.group) {
+            h = 0;
+            at += wrap;
           }
         }
       }
@@ -1343,12 +1321,11 @@ struct PaPlan {
 };
 PaPlan pa_plan(long T, int batch, int Hq, int Hkv, int D, long cap, int sms) {
   PaPlan w = {};
-  const long group = Hq / Hkv, rows = T * group, dp = D <= 64 ? 64 : 128;
+  const long rows = T * (Hq / Hkv), dp = D <= 64 ? 64 : 128;
   w.wide = rows > PA_NARROW_ROWS && T > batch;
   w.narrow_max = w.wide ? PA_NARROW_ROWS : 0x7fffffff;
-  // decoding steps whose heads per KV head fit 16 rows take the kernel with the shorter code
-  w.narrow_rows = w.wide || group > 16 ? PA_NARROW_ROWS : 16;
-  w.narrow_ctas = (int)pa_ctas(T, batch, Hq, Hkv, cap, w.narrow_rows, sms);
+  w.narrow_rows = (int)(rows < PA_NARROW_ROWS ? rows : PA_NARROW_ROWS);
+  w.narrow_ctas = (int)pa_ctas(T, batch, Hq, Hkv, cap, PA_NARROW_ROWS, sms);
   w.wide_ctas = w.wide ? (int)pa_ctas(T, batch, Hq, Hkv, cap, PA_WIDE_ROWS, sms) : 0;
   auto size = [&](long ctas, long r) { return pa_align(2 * ctas * r * dp * 4) + pa_align(2 * ctas * r * 8) + pa_align(ctas * 32); };
   w.narrow_at = 0;
@@ -1375,9 +1352,7 @@ int pa_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, PaParams p, const 
   if (dev >= 64 || !set[dev]) {
     e = cudaFuncSetAttribute(pa_wide_kernel<PANELS, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(pa_narrow_kernel<PANELS, F16, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(pa_narrow_kernel<PANELS, F16, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+      e = cudaFuncSetAttribute(pa_narrow_kernel<PANELS, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return (int)e;
     if (dev < 64) set[dev] = true;
   }
@@ -1401,8 +1376,7 @@ int pa_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, PaParams p, const 
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = w.wide ? 1 : 0;
-  e = w.narrow_rows == 16 ? cudaLaunchKernelEx(&cfg, pa_narrow_kernel<PANELS, F16, 1>, tmK, tmV, pn)
-                          : cudaLaunchKernelEx(&cfg, pa_narrow_kernel<PANELS, F16, 4>, tmK, tmV, pn);
+  e = cudaLaunchKernelEx(&cfg, pa_narrow_kernel<PANELS, F16>, tmK, tmV, pn);
   if (e != cudaSuccess) return (int)e;
   const int ctas = w.narrow_ctas + w.wide_ctas;
   cfg.gridDim = dim3(w.wide || ctas >= 128 ? 4 * 148 : 4 * ctas);
