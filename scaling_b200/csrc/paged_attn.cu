@@ -47,7 +47,7 @@ constexpr int PA_PANEL = 16384;   // 128 rows x 128 bytes
 constexpr int PA_ITEMS = 4;       // descriptors in flight
 constexpr int PA_COMBINE_THREADS = 256;
 // What the start and the end of an item cost, in tiles: added to its length on the work line.
-constexpr int PA_WIDE_COST = 2, PA_NARROW_COST = 3;
+constexpr int PA_WIDE_COST = 2, PA_NARROW_COST = 2;
 // ROWS (rows per item) tells the kernels apart in the functions that they share.
 template <int ROWS> struct PaKind {
   static constexpr bool NARROW = ROWS <= PA_NARROW_ROWS;
@@ -963,7 +963,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                                   : (p.window >= 0 ? (int)min((long)it.L, (long)it.pos0 + p.window + 1) : it.L);
       int cur = 0;
       float* ref = sRef + x * 2 * R;
-      float l0 = 0.f, l1 = 0.f;  // sums of rows lane and lane + 32 over this warp's keys
+      // row sums: of the first 16 rows per key in every thread, of the others over the warp's keys in lane row % 32
+      float l[16], l0 = 0.f, l1 = 0.f;
+#pragma unroll
+      for (int u = 0; u < 16; ++u) l[u] = 0.f;
       for (int t = x; t < n; t += 2) {
         const int key0 = (it.tile0 + t) * PA_TILE, buf = (t >> 1) & 1;
         if (retired < issued) {  // P V of this group's tile before: P may be overwritten, O rescaled
@@ -996,7 +999,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           }
         };
         // P of the tile against the current references and its row sums; returns the largest exponent
-        float t0 = 0.f, t1 = 0.f;
+        float t0 = 0.f, t1 = 0.f, first[16];
         auto probabilities = [&]() -> float {
           float top = -INFINITY;
 #pragma unroll 1
@@ -1020,9 +1023,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             }
             *reinterpret_cast<uint4*>(prow + (((b * 2) ^ (key & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
             *reinterpret_cast<uint4*>(prow + (((b * 2 + 1) ^ (key & 7)) << 4)) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
-            const float sum = pa_transpose_reduce(s, lane, [](float a, float b) { return a + b; });
-            if (lane >> 4 == (b & 1)) {
-              if (b < 2) t0 = sum; else t1 = sum;
+            if (b == 0) {
+#pragma unroll
+              for (int u = 0; u < 16; ++u) first[u] = s[u];
+            } else {
+              const float sum = pa_transpose_reduce(s, lane, [](float a, float b) { return a + b; });
+              if (lane >> 4 == (b & 1)) {
+                if (b < 2) t0 = sum; else t1 = sum;
+              }
             }
           }
           return top;
@@ -1060,6 +1068,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           cur ^= 1;
           l0 *= alpha[0];
           l1 *= alpha[1];
+#pragma unroll
+          for (int u = 0; u < 16; ++u) l[u] *= __shfl_sync(0xffffffffu, alpha[0], u);
           if (t >= 2) {
 #pragma unroll 1
             for (int b = 0; b < nb; ++b) {
@@ -1080,6 +1090,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
         l0 += t0;
         l1 += t1;
+#pragma unroll
+        for (int u = 0; u < 16; ++u) l[u] += first[u];
         if (key0 + PA_TILE > it.hi) {
           const uint32_t e = ring + pa_v_place(t, 4, n), st = e % STAGES;
           if (!pa_wait(&c.full[st], (e / STAGES) & 1, abort_flag)) { ok = false; break; }
@@ -1097,6 +1109,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         if (!pa_wait(&c.p_empty[x], retired & 1, abort_flag)) break;
         ++retired;
       }
+      const float sum16 = pa_transpose_reduce(l, lane, [](float a, float b) { return a + b; });
+      if (lane < 16) l0 = sum16;
       wmax[quad * R + lane] = l0;  // P of this group is not in use: its place takes the warps' sums
       wmax[quad * R + 32 + lane] = l1;
       if (quad == 0 && lane == 0) c.need[x][0][0] = cur;  // no vote is under way
