@@ -15,19 +15,21 @@
 // K and V tiles come by TMA through a ring that does not know items: the loaders run ahead into the next ones.
 //
 // Wide (sequences with more than 64 rows): matrix products.  Items of 256 rows, S = Q K^T with query rows in the 128 TMEM
-//   lanes.  Two groups of four softmax warps (thread = query row = lane) work on different S at any time, so that the
+//   lanes.  Two groups of four softmax warps (thread = query row = lane), each with an MMA warp of its own, so that the
 //   tensor core computes for one while the other takes exponentials.  Items of more than 128 rows give each group 128
-//   rows of its own ("two_q"); smaller items give both the same rows and every second key tile, and join the two states at
-//   the end.  The probabilities overwrite the first half of S as packed 16-bit values and are the TMEM operand of
-//   O += P V; O stays in TMEM over the whole item.
+//   rows of its own ("two_q"); smaller items give both the same rows and half the keys of each tile, and join the two
+//   states at the end.  A group works on half tiles of 64 keys with two S in TMEM, so it never waits for the product that follows its
+//   own probabilities; these overwrite the first half of their S as packed 16-bit values and are the TMEM operand of
+//   O += P V.  O stays in TMEM over the whole item.
 // Narrow (at most 64 rows: decoding): a stream over K and V, so everything else has to be small against the tile's bytes.
 //   Rows in lanes would leave most lanes and three of four warps idle; here the keys are in the lanes: S^T = K Q^T
 //   [128 keys x rows], a thread takes the exponentials of one key for all rows, and O^T += V^T P [D x rows].  S^T of four
 //   tiles is in flight.  The rows' references are shared by the four warps of a group, which agree once per tile whether
 //   any score has outgrown them (then the tile's P is written again).
 //
-// Warp roles: 0-3 and 4-7 softmax groups, 8 and 11 TMA loaders of K and of V (a page of 16 tokens is a copy of its own, and
-// one warp alone issues them no faster than the memory delivers), 9 MMA issuer, 10 scheduler, which also copies the queries.
+// Warp roles: 0-3 and 4-7 softmax groups, 10 scheduler, which also copies the queries.  Narrow: 8 and 11 TMA loaders of K and
+// of V (a page of 16 tokens is a copy of its own, and one warp alone issues them no faster than the memory delivers), 9 MMA
+// issuer.  Wide: 8 loader of both, 9 and 11 MMA issuers of the two groups.
 //
 // Rounding: scores, sums and outputs are fp32; P is rounded to the 16-bit element type for the second product (half a
 // step per probability, averaged over the row), the output once.
@@ -38,6 +40,7 @@
 namespace {
 
 constexpr int PA_TILE = 128;
+constexpr int PA_HALF = 64;  // keys per step of the wide kernel
 constexpr int PA_WIDE_ROWS = 256, PA_NARROW_ROWS = 64;  // rows per item (narrow: at most)
 constexpr int PA_WARPS = 12;
 constexpr int PA_THREADS = PA_WARPS * 32;
@@ -102,7 +105,7 @@ template <int PANELS> struct PaCfg {
 template <int STAGES> struct PaCtrl {
   uint64_t full[STAGES], empty[STAGES];  // ring
   uint64_t q_full[2], q_empty[2];
-  uint64_t s_full[4], p_full[2], p_empty[2], o_full[2], merge[8], vote[2], fin, epi_done;
+  uint64_t s_full[4], p_full[4], p_empty[2], merge[8], vote[2], fin, epi_done;
   uint64_t item_full[PA_ITEMS], item_empty[PA_ITEMS];
   PaItem items[PA_ITEMS];
   alignas(16) int need[2][2][4];  // narrow: [group][round parity][warp]
@@ -131,6 +134,27 @@ __device__ __forceinline__ void pa_tma_5d(uint32_t dst, const void* tmap, uint64
       "[%0], [%1, {%3, %4, %4, %5, %6}], [%2];"
       ::"r"(dst), "l"(tmap), "r"(sb::smem_u32(bar)), "r"(x), "r"(0), "r"(group8), "r"(head)
       : "memory");
+}
+__device__ __forceinline__ float pa_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 pa_fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 x, y, z, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\n"
+      "fma.rn.f32x2 w, x, y, z;\nmov.b64 {%0, %1}, w;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 pa_add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 x, y, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 w, x, y;\nmov.b64 {%0, %1}, w;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 // Bounded wait of a whole warp: every lane gets the same answer, also when the wait gives up, so that no lane is missing
 // from the warp-wide instructions that follow.
@@ -436,17 +460,19 @@ __device__ __forceinline__ void pa_schedule(const PaParams& p, PaCtrl<PaCfg<PANE
   if (lane == 0) desc[0] = starts && ok;
 }
 
-// Warps 8 (K) and 11 (V).
-template <int ROWS, int PANELS>
+// K tiles, V tiles, or both in the order of the ring.
+template <int ROWS, int PANELS, bool K, bool V>
 __device__ __forceinline__ void pa_load(const PaParams& p, PaCtrl<PaCfg<PANELS>::STAGES>& c, uint8_t* sRing,
-                                        const CUtensorMap* tm, bool is_v, int lane) {
+                                        const CUtensorMap* tmK, const CUtensorMap* tmV, int lane) {
   constexpr int STAGES = PaCfg<PANELS>::STAGES, TILE_BYTES = PaCfg<PANELS>::TILE_BYTES;
   volatile int* abort_flag = &c.abort;
-  if (lane == 0) sb::tma_prefetch_desc(tm);
+  if (lane == 0) {
+    if (K) sb::tma_prefetch_desc(tmK);
+    if (V) sb::tma_prefetch_desc(tmV);
+  }
   const int page = 1 << p.page_shift;
   const int box = min(page, PA_TILE), per_tile = PA_TILE / box;  // rows per copy, pages per tile
   const int bi = lane % per_tile, pn = lane / per_tile;          // this lane's page of the tile, and its panel
-  const int page8 = is_v ? p.v_page8 : p.k_page8, outside = is_v ? p.v_outside : p.k_outside;
   const uint32_t dst = sb::smem_u32(sRing) + bi * (box >> 3) * p.group_step + pn * p.panel_step;
   uint32_t ring = 0;
   bool ok = true;
@@ -459,27 +485,32 @@ __device__ __forceinline__ void pa_load(const PaParams& p, PaCtrl<PaCfg<PANELS>:
     if (it.count == 0) break;
     const int lead = pa_lead<ROWS>(it.rows);
     const int* trow = p.table + (long)it.seq * p.table_ld;
-    int win = -64, where = 0;  // 32 pages at a time: their first 8-row group in the tensor map
-    for (int t = 0; t < it.count; ++t) {
+    int win[2] = {-64, -64}, where[2] = {0, 0};  // 32 pages at a time, for K and V: their first 8-row group in the tensor map
+    auto load = [&](int t, int kv) -> bool {
       const int key0 = (it.tile0 + t) * PA_TILE, page0 = key0 >> p.page_shift;
-      if (page0 + per_tile > win + 32) {
-        win = page0;
+      if (page0 + per_tile > win[kv] + 32) {
+        win[kv] = page0;
         const int idx = page0 + lane;
-        where = outside;  // a copy from outside the cache reads zeros
+        int at = kv ? p.v_outside : p.k_outside;  // a copy from outside the cache reads zeros
         if (idx < p.cols && ((idx + 1) << p.page_shift) > it.lo && (idx << p.page_shift) < it.hi) {
           const int got = trow[idx];
-          if (got >= 0 && got < p.num_pages) where = got * page8;
+          if (got >= 0 && got < p.num_pages) at = got * (kv ? p.v_page8 : p.k_page8);
           else *p.status = SB_ERR_BAD_ARG;  // a visible page outside the cache: reported, its keys read as zeros
         }
+        where[kv] = at;
       }
-      const int first8 = __shfl_sync(0xffffffffu, where, page0 - win + bi);
-      const uint32_t e = ring + (is_v ? pa_v_place(t, lead, it.count) : pa_k_place(t, lead)), st = e % STAGES;
-      ok = pa_wait(&c.empty[st], ((e / STAGES) & 1) ^ 1, abort_flag);
-      if (!ok) break;
+      const int first8 = __shfl_sync(0xffffffffu, where[kv], page0 - win[kv] + bi);
+      const uint32_t e = ring + (kv ? pa_v_place(t, lead, it.count) : pa_k_place(t, lead)), st = e % STAGES;
+      if (!pa_wait(&c.empty[st], ((e / STAGES) & 1) ^ 1, abort_flag)) return false;
       if (lane == 0) sb::mbar_expect_tx(&c.full[st], TILE_BYTES);
       __syncwarp();
       if (pn < p.boxes)
-        pa_tma_5d(dst + st * TILE_BYTES, tm, &c.full[st], pn * 64, first8 + ((key0 & (page - 1)) >> 3), it.hk);
+        pa_tma_5d(dst + st * TILE_BYTES, kv ? tmV : tmK, &c.full[st], pn * 64, first8 + ((key0 & (page - 1)) >> 3), it.hk);
+      return true;
+    };
+    for (int t = -lead; t < it.count && ok; ++t) {
+      if (V && t >= 0) ok = load(t, 1);
+      if (K && ok && t + lead < it.count) ok = load(t + lead, 0);
     }
     ring += 2 * it.count;
   }
@@ -499,6 +530,7 @@ template <int PANELS> __device__ __forceinline__ void pa_zero_v_row(const PaPara
 // Returns false if shared memory does not start on a 1024-byte boundary, as the swizzled tiles need.
 template <int ROWS, int STAGES>
 __device__ __forceinline__ bool pa_begin(const PaParams& p, PaCtrl<STAGES>& c, uint8_t* smem, int warp, int lane) {
+  constexpr int ISSUERS = PaKind<ROWS>::NARROW ? 1 : 2;  // warps that issue MMAs: each releases what the MMAs read
   if (sb::smem_u32(smem) & 1023) {
     if (threadIdx.x == 0) *p.status = SB_ERR_BAD_ARG;
     return false;
@@ -506,23 +538,24 @@ __device__ __forceinline__ bool pa_begin(const PaParams& p, PaCtrl<STAGES>& c, u
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
       sb::mbar_init(&c.full[i], 1);
-      sb::mbar_init(&c.empty[i], 1);
+      sb::mbar_init(&c.empty[i], ISSUERS);
     }
     for (int i = 0; i < 2; ++i) {
       sb::mbar_init(&c.q_full[i], 1);
-      sb::mbar_init(&c.q_empty[i], 1);
-      sb::mbar_init(&c.p_full[i], 4);
+      sb::mbar_init(&c.q_empty[i], ISSUERS);
       sb::mbar_init(&c.p_empty[i], 1);
-      sb::mbar_init(&c.o_full[i], 1);
       sb::mbar_init(&c.vote[i], 4);
     }
-    for (int i = 0; i < 4; ++i) sb::mbar_init(&c.s_full[i], 1);
+    for (int i = 0; i < 4; ++i) {
+      sb::mbar_init(&c.s_full[i], 1);
+      sb::mbar_init(&c.p_full[i], 4);
+    }
     for (int i = 0; i < 8; ++i) sb::mbar_init(&c.merge[i], 1);
     sb::mbar_init(&c.fin, 8);
     sb::mbar_init(&c.epi_done, 8);
     for (int i = 0; i < PA_ITEMS; ++i) {
       sb::mbar_init(&c.item_full[i], 1);
-      sb::mbar_init(&c.item_empty[i], 11);  // two loaders, the MMA warp, eight softmax warps
+      sb::mbar_init(&c.item_empty[i], 11);  // loaders and MMA warps (three in all), eight softmax warps
     }
     c.abort = 0;
     sb::mbar_fence_init();
@@ -567,7 +600,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     pa_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PaParams p) {
   using Cfg = PaCfg<PANELS>;
   constexpr int DP = Cfg::DP, TILE_BYTES = Cfg::TILE_BYTES, STAGES = Cfg::STAGES;
-  constexpr uint32_t S_COL = 0, O_COL = 256;  // two S buffers of 128 columns, two O of DP
+  constexpr uint32_t S_COL = 0, O_COL = 256;  // two S of 64 columns per group, two O of DP
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;  // two slots of 128 rows
   uint8_t* sRing = smem + Cfg::FRONT;
@@ -582,15 +615,19 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     pa_regs_dec<PA_REGS_FEW>();  // one instruction for the whole warpgroup
     if (warp == 10) {
       pa_schedule<PA_WIDE_ROWS, PANELS>(p, c, sQ, (p.batch + 31) / 32, lane);
-    } else if (warp != 9) {
-      pa_load<PA_WIDE_ROWS, PANELS>(p, c, sRing, warp == 11 ? &tmV : &tmK, warp == 11, lane);
+    } else if (warp == 8) {
+      pa_load<PA_WIDE_ROWS, PANELS, true, true>(p, c, sRing, &tmK, &tmV, lane);
     } else if (lane == 0) {
-      const uint32_t idesc_s = sb::umma_idesc_f16(PA_TILE, PA_TILE, F16 ? 0 : 1, 0, 0);  // K-major both
+      // MMAs of one group.  Half tiles of 64 keys: S(u) goes to buffer u & 1, P(u) overwrites its first 32 columns, and
+      // S(u + 2) follows P(u) V in the same buffer while the softmax warps work on S(u + 1).
+      const int x = warp == 11;
+      const uint32_t idesc_s = sb::umma_idesc_f16(PA_TILE, PA_HALF, F16 ? 0 : 1, 0, 0);  // K-major both
       const uint32_t idesc_o = sb::umma_idesc_f16(PA_TILE, DP, F16 ? 0 : 1, 0, 1);       // V is MN-major
       const uint64_t q_desc = sb::umma_smem_desc(sb::smem_u32(sQ), 16, 1024);
       const uint64_t k_desc = sb::umma_smem_desc(sb::smem_u32(sRing), 16, p.group_step);
       const uint64_t v_desc = sb::umma_smem_desc(sb::smem_u32(sRing), p.panel_step, p.group_step);
-      const uint32_t k_panel = p.panel_step >> 4, v_step = (2 * p.group_step) >> 4;  // descriptors count 16-byte units
+      const uint32_t k_panel = p.panel_step >> 4, half_step = (8 * p.group_step) >> 4, v_step = (2 * p.group_step) >> 4;
+      const uint32_t s_col = tmem_base + S_COL + x * PA_TILE, o_col = tmem_base + O_COL + x * DP;
       uint32_t ring = 0, p_cnt0 = 0, p_cnt1 = 0;
       int q_cnt = 0;
       bool ok = true;
@@ -600,51 +637,55 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const int count = c.items[slot].count, two_q = c.items[slot].rows > PA_TILE;
         sb::mbar_arrive(&c.item_empty[slot]);
         if (count == 0) break;
-        const int lead = two_q ? 1 : 2, n = two_q ? 2 * count : count;
-        ok = sb::mbar_wait(&c.q_full[q_cnt & 1], (q_cnt >> 1) & 1, abort_flag);
-        if (ok && two_q) ok = sb::mbar_wait(&c.q_full[(q_cnt + 1) & 1], ((q_cnt + 1) >> 1) & 1, abort_flag);
-        if (!ok) break;
-        // virtual tile v: group v & 1; key tile v (one query slot) or v / 2 (two)
-        auto k_place = [&](int v) -> uint32_t { return ring + pa_k_place(two_q ? v >> 1 : v, lead); };
-        auto wait_ring = [&](uint32_t e) -> bool { return sb::mbar_wait(&c.full[e % STAGES], (e / STAGES) & 1, abort_flag); };
-        auto issue_s = [&](int v) {
-          const uint32_t st = k_place(v) % STAGES;
-          const int qs = (q_cnt + (two_q ? v & 1 : 0)) & 1;
-          const uint64_t qd = q_desc + qs * (TILE_BYTES >> 4), kd = k_desc + st * (TILE_BYTES >> 4);
-          const uint32_t d = tmem_base + S_COL + (v & 1) * PA_TILE;
-#pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk)
-            sb::umma_f16_ss(d, qd + (kk >> 2) * (PA_PANEL >> 4) + (kk & 3) * 2, kd + (kk >> 2) * k_panel + (kk & 3) * 2,
-                            idesc_s, kk != 0);
-          sb::umma_commit(&c.s_full[v & 1]);
-          if (!two_q || (v & 1)) sb::umma_commit(&c.empty[st]);
-          if (two_q ? v >= n - 2 : v == n - 1) sb::umma_commit(&c.q_empty[qs]);
-        };
-        for (int v = 0; v < min(n, 2) && ok; ++v) {
-          ok = wait_ring(k_place(v));
+        // step u: with two_q tile u / 2 and its halves in turn, else tile u and half x.  Both groups take every tile in
+        // the ring's order: the parity of a barrier that a warp has not followed phase by phase says nothing.
+        const int lead = two_q ? 1 : 2, n = two_q ? 2 * count : count, shift = two_q;
+        const int qu = q_cnt + (two_q ? x : 0), qs = qu & 1;
+        ok = sb::mbar_wait(&c.q_full[qs], (qu >> 1) & 1, abort_flag);
+#pragma unroll 1
+        for (int u = -2; u < n && ok; ++u) {
+          const int b = u & 1;
+          const bool next = u + 2 < n;
+          const int half = two_q ? b : x;
+          const uint32_t ke = ring + pa_k_place((u + 2) >> shift, lead), ks = ke % STAGES;
+          const uint32_t ve = ring + pa_v_place(u >> shift, lead, count), vs = ve % STAGES;
+          // All that this step needs is asked for together, because each answer takes some 180 cycles.  The first step on a
+          // tile waits for its copy, the last one releases it.
+          const bool opens = !two_q || b == 0, closes = !two_q || b, need_k = next && opens, need_v = u >= 0 && opens;
+          const uint32_t pc = b ? p_cnt1 : p_cnt0;
+          const uint32_t got_k = need_k ? sb::mbar_try_wait(&c.full[ks], (ke / STAGES) & 1) : 1;
+          const uint32_t got_v = need_v ? sb::mbar_try_wait(&c.full[vs], (ve / STAGES) & 1) : 1;
+          const uint32_t got_p = u >= 0 ? sb::mbar_try_wait(&c.p_full[x * 2 + b], pc & 1) : 1;
+          if (!(got_k & got_v & got_p)) {
+            if (need_v) ok = sb::mbar_wait(&c.full[vs], (ve / STAGES) & 1, abort_flag);
+            if (ok && need_k) ok = sb::mbar_wait(&c.full[ks], (ke / STAGES) & 1, abort_flag);
+            if (ok && u >= 0) ok = sb::mbar_wait(&c.p_full[x * 2 + b], pc & 1, abort_flag);
+          }
+          if (ok && u == 0 && i > 0) ok = sb::mbar_wait(&c.epi_done, (i - 1) & 1, abort_flag);  // O of the item before is read
           if (!ok) break;
           sb::tc_fence_after();
-          issue_s(v);
-        }
-        for (int v = 0; v < n && ok; ++v) {
-          const int x = v & 1;
-          const uint32_t e = ring + pa_v_place(two_q ? v >> 1 : v, lead, count), st = e % STAGES;
-          // both tiles first, so that nothing is waited for between the probabilities and the 16 products
-          ok = wait_ring(e);
-          if (ok && v + 2 < n) ok = wait_ring(k_place(v + 2));
-          if (ok && v == 0 && i > 0) ok = sb::mbar_wait(&c.epi_done, (i - 1) & 1, abort_flag);  // O of the item before is read
-          ok = ok && sb::mbar_wait(&c.p_full[x], (x ? p_cnt1 : p_cnt0) & 1, abort_flag);
-          if (!ok) break;
-          if (x) ++p_cnt1; else ++p_cnt0;
-          sb::tc_fence_after();
-          const uint64_t vd = v_desc + st * (TILE_BYTES >> 4);
-          const uint32_t pa = tmem_base + S_COL + x * PA_TILE, d = tmem_base + O_COL + x * DP;
+          if (u >= 0) {
+            if (b) ++p_cnt1; else ++p_cnt0;
+            const uint64_t vd = v_desc + vs * (TILE_BYTES >> 4) + half * half_step;
 #pragma unroll
-          for (int kk = 0; kk < PA_TILE / 16; ++kk)
-            pa_umma_ts(d, pa + kk * 8, vd + kk * v_step, idesc_o, v > 1 || kk != 0);
-          if (!two_q || x) sb::umma_commit(&c.empty[st]);
-          if (v + 2 >= n) sb::umma_commit(&c.o_full[x]);
-          if (v + 2 < n) issue_s(v + 2);
+            for (int kk = 0; kk < PA_HALF / 16; ++kk)
+              pa_umma_ts(o_col, s_col + b * PA_HALF + kk * 8, vd + kk * v_step, idesc_o, u > 0 || kk != 0);
+            sb::umma_commit(&c.p_empty[x]);
+            if (closes) sb::umma_commit(&c.empty[vs]);
+          }
+          if (next) {
+            const uint64_t qd = q_desc + qs * (TILE_BYTES >> 4), kd = k_desc + ks * (TILE_BYTES >> 4) + half * half_step;
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk)
+              sb::umma_f16_ss(s_col + b * PA_HALF, qd + (kk >> 2) * (PA_PANEL >> 4) + (kk & 3) * 2,
+                              kd + (kk >> 2) * k_panel + (kk & 3) * 2, idesc_s, kk != 0);
+            sb::umma_commit(&c.s_full[x * 2 + b]);
+            if (closes) sb::umma_commit(&c.empty[ks]);
+            if (u + 3 == n) {  // the slot's two releases come from both groups, or from the one that reads it
+              sb::umma_commit(&c.q_empty[qs]);
+              if (two_q) sb::umma_commit(&c.q_empty[qs]);
+            }
+          }
         }
         ring += 2 * count;
         q_cnt += 1 + two_q;
@@ -654,9 +695,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     pa_regs_inc<PA_REGS_MANY>();
     const int x = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16);
-    const uint32_t s_addr = t_lane + S_COL + x * PA_TILE, o_addr = t_lane + O_COL + x * DP;
+    const uint32_t o_addr = t_lane + O_COL + x * DP;
     const float sl2 = p.sl2;
-    uint32_t ring = 0, s_cnt = 0, o_cnt = 0, merges = 0;
+    uint32_t ring = 0, s_cnt0 = 0, s_cnt1 = 0, o_cnt = 0, merges = 0;
     bool ok = true;
     for (int i = 0; ok; ++i) {
       const int islot = i % PA_ITEMS;
@@ -680,34 +721,38 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         hi = p.causal ? min(pos + 1, it.L) : (p.window >= 0 ? (int)min((long)it.L, (long)pos + p.window + 1) : it.L);
       }
       float ref = -INFINITY, l = 0.f;
-      const int n = two_q ? 2 * it.count : it.count;
-      for (int v = x; v < n; v += 2) {
-        const int t = two_q ? v >> 1 : v;
-        const int key0 = (it.tile0 + t) * PA_TILE;
-        if (!pa_wait(&c.s_full[x], s_cnt & 1, abort_flag)) { ok = false; break; }
-        ++s_cnt;
+      const int n = two_q ? 2 * it.count : it.count;  // half tiles of this group
+      for (int u = 0; u < n; ++u) {
+        const int t = two_q ? u >> 1 : u, b = u & 1, half = two_q ? b : x;
+        const int key0 = (it.tile0 + t) * PA_TILE + half * PA_HALF;
+        if (!pa_wait(&c.s_full[x * 2 + b], (b ? s_cnt1 : s_cnt0) & 1, abort_flag)) { ok = false; break; }
+        if (b) ++s_cnt1; else ++s_cnt0;
         sb::tc_fence_after();
+        const uint32_t s_addr = t_lane + S_COL + x * PA_TILE + b * PA_HALF;
         if (warp_rows > 0) {
-          uint32_t s[PA_TILE];
+          uint32_t s[PA_HALF];
 #pragma unroll
-          for (int ch = 0; ch < 4; ++ch) sb::tmem_ld32(s_addr + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(s + ch * 32));
+          for (int ch = 0; ch < 2; ++ch) sb::tmem_ld32(s_addr + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(s + ch * 32));
           sb::tmem_ld_wait();
-          if (!__all_sync(0xffffffffu, key0 >= lo && key0 + PA_TILE <= hi)) {
+          if (!__all_sync(0xffffffffu, key0 >= lo && key0 + PA_HALF <= hi)) {
 #pragma unroll
-            for (int ch = 0; ch < PA_TILE; ++ch)
-              if (key0 + ch < lo || key0 + ch >= hi) s[ch] = 0xff800000u;  // -inf, whatever the score was
+            for (int j = 0; j < PA_HALF; ++j)
+              if (key0 + j < lo || key0 + j >= hi) s[j] = 0xff800000u;  // -inf, whatever the score was
           }
           float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int ch = 0; ch < PA_TILE; ++ch) m4[ch & 3] = fmaxf(m4[ch & 3], __uint_as_float(s[ch]));
-          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          for (int j = 0; j < PA_HALF; j += 2)
+            m4[(j >> 1) & 3] = pa_max3(m4[(j >> 1) & 3], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+          const float mx = pa_max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
           const bool move = (mx - ref) * sl2 > 8.f || (ref == -INFINITY && mx > -INFINITY);
           if (__any_sync(0xffffffffu, move)) {
             const float next = move ? mx : ref;
             const float alpha = move ? (ref == -INFINITY ? 0.f : pa_exp2((ref - next) * sl2)) : 1.f;
             ref = next;
             l *= alpha;
-            if (v >= 2) {  // O holds the tiles before (complete: their MMAs precede this S)
+            if (u > 0) {  // O holds the half tiles before, once the last product is complete (the one before it precedes this S)
+              if (!pa_wait(&c.p_empty[x], (o_cnt - 1) & 1, abort_flag)) { ok = false; break; }
+              sb::tc_fence_after();
 #pragma unroll
               for (int ch = 0; ch < DP / 32; ++ch) {
                 uint32_t o[32];
@@ -720,49 +765,40 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             }
           }
           const float neg = ref == -INFINITY ? 0.f : -ref * sl2;
-          float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+          const float2 scale2 = make_float2(sl2, sl2), neg2 = make_float2(neg, neg);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          uint32_t pk[32];
 #pragma unroll
-          for (int ch = 0; ch < 2; ++ch) {
-            uint32_t pk[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float a = pa_exp2(fmaf(__uint_as_float(s[ch * 64 + 2 * j]), sl2, neg));
-              const float b = pa_exp2(fmaf(__uint_as_float(s[ch * 64 + 2 * j + 1]), sl2, neg));
-              sum4[(2 * j) & 3] += a;
-              sum4[(2 * j + 1) & 3] += b;
-              pk[j] = pa_pack<F16>(a, b);
-            }
-            pa_tmem_st32(s_addr + ch * 32, pk);
+          for (int j = 0; j < 32; ++j) {
+            const float2 z = pa_fma2(make_float2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), scale2, neg2);
+            const float2 e = make_float2(pa_exp2(z.x), pa_exp2(z.y));
+            sum[j & 1] = pa_add2(sum[j & 1], e);
+            pk[j] = pa_pack<F16>(e.x, e.y);
           }
-          l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+          pa_tmem_st32(s_addr, pk);
+          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           sb::tmem_st_wait();
         }
-        if (key0 + PA_TILE > it.hi) {
-          // Values behind the last visible key may be anything, NaN included, and 0 * NaN is NaN: their rows of the
-          // V tile are zeroed (twice with two_q, which does no harm).  Thread = key row.
+        if (key0 + PA_HALF > it.hi) {  // rows of V behind the last visible key (by both groups with two_q, which does no harm)
           const uint32_t e = ring + pa_v_place(t, lead, it.count), st = e % STAGES;
           if (!pa_wait(&c.full[st], (e / STAGES) & 1, abort_flag)) { ok = false; break; }
-          if (key0 + r >= it.hi) {
-            pa_zero_v_row<PANELS>(p, sRing + st * TILE_BYTES, r);
-          }
+          if (r < PA_HALF && key0 + r >= it.hi) pa_zero_v_row<PANELS>(p, sRing + st * TILE_BYTES, half * PA_HALF + r);
           sb::fence_proxy_async_smem();
         }
         sb::tc_fence_before();
         __syncwarp();
-        if (lane == 0) sb::mbar_arrive(&c.p_full[x]);
+        if (lane == 0) sb::mbar_arrive(&c.p_full[x * 2 + b]);
+        ++o_cnt;
       }
       ring += 2 * it.count;
       if (!ok) break;
-      const bool mine = x < n;  // this group had a tile
-      if (mine) {
-        if (!pa_wait(&c.o_full[x], o_cnt & 1, abort_flag)) break;
-        ++o_cnt;
-        sb::tc_fence_after();
-      }
+      // the last two products, one phase after the other
+      if (o_cnt > 1 && !pa_wait(&c.p_empty[x], (o_cnt - 2) & 1, abort_flag)) break;
+      if (!pa_wait(&c.p_empty[x], (o_cnt - 1) & 1, abort_flag)) break;
+      sb::tc_fence_after();
       // the two states of a row: fa, fb scale the groups' outputs to a common reference
       float fa = x == 0 ? 1.f : 0.f, fb = 1.f - fa;
       int c0 = 0, c1 = DP / 32;
-      const bool both = !two_q && n > 1;
       if (!two_q) {
         if (i > 0 && !pa_wait(&c.epi_done, (i - 1) & 1, abort_flag)) break;  // xml of the item before is read
         xml[x * PA_TILE + r] = make_float2(ref, l);
@@ -789,16 +825,16 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         for (int ch = c0; ch < c1; ++ch) {
           uint32_t a[32], b[32];
           float o[32];
-          if (both) {
+          if (!two_q) {
             sb::tmem_ld32(t_lane + O_COL + ch * 32, a);
             sb::tmem_ld32(t_lane + O_COL + DP + ch * 32, b);
             sb::tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 32; ++j) o[j] = fmaf(__uint_as_float(a[j]), ga, __uint_as_float(b[j]) * gb);
-          } else {  // one state: this group's (two_q), or group 0's
-            sb::tmem_ld32((two_q ? o_addr : t_lane + O_COL) + ch * 32, a);
+          } else {
+            sb::tmem_ld32(o_addr + ch * 32, a);
             sb::tmem_ld_wait();
-            const float f = two_q && x ? gb : ga;
+            const float f = x ? gb : ga;
 #pragma unroll
             for (int j = 0; j < 32; ++j) o[j] = __uint_as_float(a[j]) * f;
           }
@@ -872,8 +908,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 
   if (warp == 10) {
     pa_schedule<R, PANELS>(p, c, sQ, (p.batch + 31) / 32, lane);
-  } else if (warp == 8 || warp == 11) {
-    pa_load<R, PANELS>(p, c, sRing, warp == 11 ? &tmV : &tmK, warp == 11, lane);
+  } else if (warp == 8) {
+    pa_load<R, PANELS, true, false>(p, c, sRing, &tmK, &tmV, lane);
+  } else if (warp == 11) {
+    pa_load<R, PANELS, false, true>(p, c, sRing, &tmK, &tmV, lane);
   } else if (warp == 9) {
     if (lane == 0) {
       const uint64_t q_desc = sb::umma_smem_desc(sb::smem_u32(sQ), 16, 1024);
