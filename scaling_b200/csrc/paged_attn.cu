@@ -49,6 +49,7 @@ constexpr int PA_REGS_FEW = 80, PA_REGS_MANY = 208;
 constexpr int PA_PANEL = 16384;   // 128 rows x 128 bytes
 constexpr int PA_ITEMS = 4;       // descriptors in flight
 constexpr int PA_COMBINE_THREADS = 256;
+constexpr unsigned long long PA_WAIT_NS = 4000000000ull;
 // What the start and the end of an item cost, in tiles: added to its length on the work line.
 constexpr int PA_WIDE_COST = 2, PA_NARROW_COST = 2;
 // ROWS (rows per item) tells the kernels apart in the functions that they share.
@@ -105,7 +106,7 @@ template <int PANELS> struct PaCfg {
 template <int STAGES> struct PaCtrl {
   uint64_t full[STAGES], empty[STAGES];  // ring
   uint64_t q_full[2], q_empty[2];
-  uint64_t s_full[4], p_full[4], p_empty[2], merge[8], vote[2], fin, epi_done;
+  uint64_t s_full[4], p_full[4], p_empty[4], merge[8], vote[2], fin, epi_done;
   uint64_t item_full[PA_ITEMS], item_empty[PA_ITEMS];
   PaItem items[PA_ITEMS];
   alignas(16) int need[2][2][4];  // narrow: [group][round parity][warp]
@@ -156,10 +157,25 @@ __device__ __forceinline__ float2 pa_add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+// Bounded wait: up to PA_WAIT_NS, then the flag is raised and every other wait of the CTA ends as well.
+__device__ __forceinline__ bool pa_wait_lane(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (sb::mbar_try_wait(bar, parity)) return true;
+  const unsigned long long start = sb::globaltimer_ns();
+  for (uint32_t i = 1;; ++i) {
+    if (sb::mbar_try_wait(bar, parity)) return true;
+    if ((i & 63) == 0) {
+      if (*abort_flag) return false;
+      if (sb::globaltimer_ns() - start > PA_WAIT_NS) {
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+}
 // Bounded wait of a whole warp: every lane gets the same answer, also when the wait gives up, so that no lane is missing
 // from the warp-wide instructions that follow.
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  return __all_sync(0xffffffffu, sb::mbar_wait(bar, parity, abort_flag));
+  return __all_sync(0xffffffffu, pa_wait_lane(bar, parity, abort_flag));
 }
 // D[tmem] (+)= A[tmem] * B[smem]: A holds two 16-bit values of a row per 32-bit column
 __device__ __forceinline__ void pa_umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -543,10 +559,10 @@ __device__ __forceinline__ bool pa_begin(const PaParams& p, PaCtrl<STAGES>& c, u
     for (int i = 0; i < 2; ++i) {
       sb::mbar_init(&c.q_full[i], 1);
       sb::mbar_init(&c.q_empty[i], ISSUERS);
-      sb::mbar_init(&c.p_empty[i], 1);
       sb::mbar_init(&c.vote[i], 4);
     }
     for (int i = 0; i < 4; ++i) {
+      sb::mbar_init(&c.p_empty[i], 1);
       sb::mbar_init(&c.s_full[i], 1);
       sb::mbar_init(&c.p_full[i], 4);
     }
@@ -633,7 +649,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       bool ok = true;
       for (int i = 0; ok; ++i) {
         const int slot = i % PA_ITEMS;
-        if (!sb::mbar_wait(&c.item_full[slot], (i / PA_ITEMS) & 1, abort_flag)) break;
+        if (!pa_wait_lane(&c.item_full[slot], (i / PA_ITEMS) & 1, abort_flag)) break;
         const int count = c.items[slot].count, two_q = c.items[slot].rows > PA_TILE;
         sb::mbar_arrive(&c.item_empty[slot]);
         if (count == 0) break;
@@ -641,37 +657,42 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         // the ring's order: the parity of a barrier that a warp has not followed phase by phase says nothing.
         const int lead = two_q ? 1 : 2, n = two_q ? 2 * count : count, shift = two_q;
         const int qu = q_cnt + (two_q ? x : 0), qs = qu & 1;
-        ok = sb::mbar_wait(&c.q_full[qs], (qu >> 1) & 1, abort_flag);
+        ok = pa_wait_lane(&c.q_full[qs], (qu >> 1) & 1, abort_flag);
+        // ring places of the next K and V tile, as stage and parity
+        uint32_t ks = ring % STAGES, kp = (ring / STAGES) & 1, ve = ring + pa_v_place(0, lead, count), vs = ve % STAGES,
+                 vp = (ve / STAGES) & 1;
+        auto advance = [](uint32_t& st, uint32_t& parity, uint32_t by) {
+          st += by;
+          if (st >= STAGES) {
+            st -= STAGES;
+            parity ^= 1;
+          }
+        };
+        int kt = 0, vt = 0;
 #pragma unroll 1
         for (int u = -2; u < n && ok; ++u) {
-          const int b = u & 1;
+          const int b = u & 1, half = two_q ? b : x;
           const bool next = u + 2 < n;
-          const int half = two_q ? b : x;
-          const uint32_t ke = ring + pa_k_place((u + 2) >> shift, lead), ks = ke % STAGES;
-          const uint32_t ve = ring + pa_v_place(u >> shift, lead, count), vs = ve % STAGES;
           // All that this step needs is asked for together, because each answer takes some 180 cycles.  The first step on a
           // tile waits for its copy, the last one releases it.
           const bool opens = !two_q || b == 0, closes = !two_q || b, need_k = next && opens, need_v = u >= 0 && opens;
-          const uint32_t pc = b ? p_cnt1 : p_cnt0;
-          const uint32_t got_k = need_k ? sb::mbar_try_wait(&c.full[ks], (ke / STAGES) & 1) : 1;
-          const uint32_t got_v = need_v ? sb::mbar_try_wait(&c.full[vs], (ve / STAGES) & 1) : 1;
-          const uint32_t got_p = u >= 0 ? sb::mbar_try_wait(&c.p_full[x * 2 + b], pc & 1) : 1;
+          const uint32_t pc = (b ? p_cnt1 : p_cnt0) & 1;
+          const uint32_t got_k = need_k ? sb::mbar_try_wait(&c.full[ks], kp) : 1;
+          const uint32_t got_v = need_v ? sb::mbar_try_wait(&c.full[vs], vp) : 1;
+          const uint32_t got_p = u >= 0 ? sb::mbar_try_wait(&c.p_full[x * 2 + b], pc) : 1;
           if (!(got_k & got_v & got_p)) {
-            if (need_v) ok = sb::mbar_wait(&c.full[vs], (ve / STAGES) & 1, abort_flag);
-            if (ok && need_k) ok = sb::mbar_wait(&c.full[ks], (ke / STAGES) & 1, abort_flag);
-            if (ok && u >= 0) ok = sb::mbar_wait(&c.p_full[x * 2 + b], pc & 1, abort_flag);
+            if (need_v) ok = pa_wait_lane(&c.full[vs], vp, abort_flag);
+            if (ok && need_k) ok = pa_wait_lane(&c.full[ks], kp, abort_flag);
+            if (ok && u >= 0) ok = pa_wait_lane(&c.p_full[x * 2 + b], pc, abort_flag);
           }
-          if (ok && u == 0 && i > 0) ok = sb::mbar_wait(&c.epi_done, (i - 1) & 1, abort_flag);  // O of the item before is read
+          if (ok && u == 0 && i > 0) ok = pa_wait_lane(&c.epi_done, (i - 1) & 1, abort_flag);  // O of the item before is read
           if (!ok) break;
           sb::tc_fence_after();
           if (u >= 0) {
-            if (b) ++p_cnt1; else ++p_cnt0;
             const uint64_t vd = v_desc + vs * (TILE_BYTES >> 4) + half * half_step;
 #pragma unroll
             for (int kk = 0; kk < PA_HALF / 16; ++kk)
               pa_umma_ts(o_col, s_col + b * PA_HALF + kk * 8, vd + kk * v_step, idesc_o, u > 0 || kk != 0);
-            sb::umma_commit(&c.p_empty[x]);
-            if (closes) sb::umma_commit(&c.empty[vs]);
           }
           if (next) {
             const uint64_t qd = q_desc + qs * (TILE_BYTES >> 4), kd = k_desc + ks * (TILE_BYTES >> 4) + half * half_step;
@@ -679,11 +700,24 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             for (int kk = 0; kk < DP / 16; ++kk)
               sb::umma_f16_ss(s_col + b * PA_HALF, qd + (kk >> 2) * (PA_PANEL >> 4) + (kk & 3) * 2,
                               kd + (kk >> 2) * k_panel + (kk & 3) * 2, idesc_s, kk != 0);
-            sb::umma_commit(&c.s_full[x * 2 + b]);
-            if (closes) sb::umma_commit(&c.empty[ks]);
+            sb::umma_commit(&c.s_full[x * 2 + b]);  // also says that P(u) V is complete
             if (u + 3 == n) {  // the slot's two releases come from both groups, or from the one that reads it
               sb::umma_commit(&c.q_empty[qs]);
               if (two_q) sb::umma_commit(&c.q_empty[qs]);
+            }
+            if (closes) {
+              sb::umma_commit(&c.empty[ks]);
+              advance(ks, kp, ++kt < lead ? 1 : 2);
+            }
+          } else {
+            // the last two products of the item, no S after them: a barrier each, one phase per item
+            sb::umma_commit(&c.p_empty[x * 2 + (u + 1 == n)]);
+          }
+          if (u >= 0) {
+            if (b) ++p_cnt1; else ++p_cnt0;
+            if (closes) {
+              sb::umma_commit(&c.empty[vs]);
+              advance(vs, vp, vt++ + lead < count ? 2 : 1);
             }
           }
         }
@@ -697,7 +731,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16);
     const uint32_t o_addr = t_lane + O_COL + x * DP;
     const float sl2 = p.sl2;
-    uint32_t ring = 0, s_cnt0 = 0, s_cnt1 = 0, o_cnt = 0, merges = 0;
+    uint32_t ring = 0, s_cnt0 = 0, s_cnt1 = 0, merges = 0;  // s_cnt: steps taken on each buffer
     bool ok = true;
     for (int i = 0; ok; ++i) {
       const int islot = i % PA_ITEMS;
@@ -750,8 +784,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             const float alpha = move ? (ref == -INFINITY ? 0.f : pa_exp2((ref - next) * sl2)) : 1.f;
             ref = next;
             l *= alpha;
-            if (u > 0) {  // O holds the half tiles before, once the last product is complete (the one before it precedes this S)
-              if (!pa_wait(&c.p_empty[x], (o_cnt - 1) & 1, abort_flag)) { ok = false; break; }
+            if (u > 0) {
+              // O holds the half tiles before, once their last product is complete: S(u + 1) follows it (and S(u) the one
+              // before it); at the item's end it has a barrier of its own
+              if (u + 1 < n ? !pa_wait(&c.s_full[x * 2 + (b ^ 1)], (b ? s_cnt0 : s_cnt1) & 1, abort_flag)
+                            : !pa_wait(&c.p_empty[x * 2], i & 1, abort_flag)) { ok = false; break; }
               sb::tc_fence_after();
 #pragma unroll
               for (int ch = 0; ch < DP / 32; ++ch) {
@@ -788,13 +825,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         sb::tc_fence_before();
         __syncwarp();
         if (lane == 0) sb::mbar_arrive(&c.p_full[x * 2 + b]);
-        ++o_cnt;
       }
       ring += 2 * it.count;
       if (!ok) break;
-      // the last two products, one phase after the other
-      if (o_cnt > 1 && !pa_wait(&c.p_empty[x], (o_cnt - 2) & 1, abort_flag)) break;
-      if (!pa_wait(&c.p_empty[x], (o_cnt - 1) & 1, abort_flag)) break;
+      if (!pa_wait(&c.p_empty[x * 2 + 1], i & 1, abort_flag)) break;  // the last product
       sb::tc_fence_after();
       // the two states of a row: fa, fb scale the groups' outputs to a common reference
       float fa = x == 0 ? 1.f : 0.f, fb = 1.f - fa;
@@ -925,17 +959,17 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       bool ok = true;
       for (int i = 0; ok; ++i) {
         const int slot = i % PA_ITEMS;
-        if (!sb::mbar_wait(&c.item_full[slot], (i / PA_ITEMS) & 1, abort_flag)) break;
+        if (!pa_wait_lane(&c.item_full[slot], (i / PA_ITEMS) & 1, abort_flag)) break;
         const int n = c.items[slot].count, cols = (c.items[slot].rows + 15) & ~15;
         sb::mbar_arrive(&c.item_empty[slot]);
         if (n == 0) break;
         const uint32_t idesc_s = sb::umma_idesc_f16(PA_TILE, cols, F16 ? 0 : 1, 0, 0);
         const uint32_t idesc_o = sb::umma_idesc_f16(PA_TILE, cols, F16 ? 0 : 1, 1, 1);
         const int qs = i & 1;
-        ok = sb::mbar_wait(&c.q_full[qs], (i >> 1) & 1, abort_flag);
+        ok = pa_wait_lane(&c.q_full[qs], (i >> 1) & 1, abort_flag);
         auto issue_s = [&](int t) -> bool {
           const uint32_t e = ring + pa_k_place(t, 4), st = e % STAGES;
-          if (!sb::mbar_wait(&c.full[st], (e / STAGES) & 1, abort_flag)) return false;
+          if (!pa_wait_lane(&c.full[st], (e / STAGES) & 1, abort_flag)) return false;
           sb::tc_fence_after();
           const uint64_t qd = q_desc + qs * (Q_SLOT >> 4), kd = k_desc + st * (TILE_BYTES >> 4);
           const int buf = (t & 1) * 2 + ((t >> 1) & 1);
@@ -953,9 +987,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           if (t >= 0) {
             const int x = t & 1;
             const uint32_t e = ring + pa_v_place(t, 4, n), st = e % STAGES;
-            ok = sb::mbar_wait(&c.full[st], (e / STAGES) & 1, abort_flag);
-            if (ok && t == 0 && i > 0) ok = sb::mbar_wait(&c.epi_done, (i - 1) & 1, abort_flag);  // O of the item before is read
-            ok = ok && sb::mbar_wait(&c.p_full[x], (x ? p_cnt1 : p_cnt0) & 1, abort_flag);
+            ok = pa_wait_lane(&c.full[st], (e / STAGES) & 1, abort_flag);
+            if (ok && t == 0 && i > 0) ok = pa_wait_lane(&c.epi_done, (i - 1) & 1, abort_flag);  // O of the item before is read
+            ok = ok && pa_wait_lane(&c.p_full[x], (x ? p_cnt1 : p_cnt0) & 1, abort_flag);
             if (!ok) break;
             if (x) ++p_cnt1; else ++p_cnt0;
             sb::tc_fence_after();
