@@ -19,13 +19,16 @@
 // base^(-2 i / rot) / (2 pi) in fp64; a thread multiplies by the position, drops the whole turns in fp64 and takes
 // sincospi of what is left in fp32.  One thread per (token, pair) fills a table in shared memory that all heads of the
 // token read.
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 
 namespace {
 
 constexpr int QN_THREADS = 256;
+constexpr int QN_FWD_BLOCKS = 3;          // per SM
 constexpr int QN_MAX_D = 256;
 constexpr int QN_MAX_SLOTS = 64;          // tokens per tile
 constexpr int QN_TABLE_BYTES = 24 * 1024; // sine table of a tile
@@ -38,6 +41,7 @@ struct QnRows {  // one of q, k, v: the heads of every token
   const void* b;
   long x_tok, x_head, y_tok, y_head, dy_tok, dy_head;
   int heads;
+  uint32_t inv;  // floor(2^32 / heads) + 1 (heads > 1): (n * inv) >> 32 = n / heads for the row numbers of a tile
 };
 
 struct QnParams {
@@ -45,7 +49,7 @@ struct QnParams {
   const int* pos;   // [T], or null in the paged form: the token's place in its sequence
   int T, D, rot, interleaved, rms, w_dtype;
   float eps;
-  int tile;         // tokens per tile
+  int tile, tile_k; // tokens per tile (backward: of q and of k)
   int log_g;        // lanes per row, as a power of two
   // paged form: k.y / v.y are the caches, y_head the stride between heads of a slot
   const int* table;
@@ -65,6 +69,8 @@ __device__ __forceinline__ float qn_load_any(const void* p, int i, int dtype) {
   if (dtype == SB_DT_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
   return __half2float(reinterpret_cast<const __half*>(p)[i]);
 }
+
+__device__ __forceinline__ int qn_token(const QnRows& r, int row) { return r.heads == 1 ? row : (int)__umulhi(row, r.inv); }
 
 // N consecutive elements as one access
 template <typename T, int N> struct alignas(sizeof(T) * N) QnVec { T e[N]; };
@@ -199,7 +205,7 @@ __device__ __forceinline__ void qn_stats(const float (&a)[NP][V], const float (&
 // ============================================================================ forward
 // One CTA per tile of tokens.  PAGED: k and v go to their slots of the cache, positions come from the sequence lengths.
 template <typename T, int V, int NP, bool PAGED>
-__global__ void __launch_bounds__(QN_THREADS, 4) qn_fwd_kernel(const __grid_constant__ QnParams p) {
+__global__ void __launch_bounds__(QN_THREADS, QN_FWD_BLOCKS) qn_fwd_kernel(const __grid_constant__ QnParams p) {
   extern __shared__ __align__(16) float smem[];
   using Vec = QnVec<T, V>;
   const int D = p.D, chunks = (D + V - 1) / V, np = (p.rot + 2 * V - 1) / (2 * V);
@@ -245,12 +251,6 @@ __global__ void __launch_bounds__(QN_THREADS, 4) qn_fwd_kernel(const __grid_cons
       spos[threadIdx.x] = p.pos ? p.pos[t] : 0;
     }
   }
-  __syncthreads();
-  if (p.rot) {
-    qn_fill_table<V>(p, tbl, spos, n_tok, np);
-    __syncthreads();
-  }
-
   int ca[NP], cb[NP];
   bool ha[NP], hb[NP];
 #pragma unroll
@@ -259,103 +259,122 @@ __global__ void __launch_bounds__(QN_THREADS, 4) qn_fwd_kernel(const __grid_cons
     ca[i] = c.a; cb[i] = c.b;
     ha[i] = c.a < chunks; hb[i] = c.b < chunks;
   }
-#pragma unroll 1
-  for (int kind = 0; kind < (PAGED ? 3 : 2); ++kind) {
+  // Rounds of the row groups over q, then k, then v; the loads of a round are issued a round ahead.
+  const int rounds[3] = {(n_tok * p.q.heads + n_grp - 1) / n_grp, (n_tok * p.k.heads + n_grp - 1) / n_grp,
+                         PAGED ? (n_tok * p.v.heads + n_grp - 1) / n_grp : 0};
+  const int first_k = rounds[0], first_v = first_k + rounds[1], total = first_v + rounds[2];
+  Vec na[NP], nb[NP];
+  auto load = [&](int it) {
+    const int kind = it < first_k ? 0 : it < first_v ? 1 : 2;
     const QnRows& R = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
-    const int rows = n_tok * R.heads, iters = (rows + n_grp - 1) / n_grp;
-    const float* w = sw + kind * 2 * QN_MAX_D;
-    const float* bias = w + QN_MAX_D;
-    const bool plain = kind == 2 || (!R.w && !p.rot);  // a copy, bit by bit
-#pragma unroll 1
-    for (int it = 0; it < iters; ++it) {  // the same trip count for every lane: the shuffles name all of them
-      const int row = grp + it * n_grp;
-      const bool live = row < rows;
-      const int tl = live ? row / R.heads : 0, h = row - tl * R.heads;
+    const int row = grp + (it - (kind == 0 ? 0 : kind == 1 ? first_k : first_v)) * n_grp;
+    if (row < n_tok * R.heads) {
+      const int tl = qn_token(R, row), h = row - tl * R.heads;
       const T* x = reinterpret_cast<const T*>(R.x) + (long)(t0 + tl) * R.x_tok + (long)h * R.x_head;
-      Vec va[NP], vb[NP];
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        if (live && ha[i]) va[i] = *reinterpret_cast<const Vec*>(x + ca[i] * V);
-        if (live && hb[i]) vb[i] = *reinterpret_cast<const Vec*>(x + cb[i] * V);
+        if (ha[i]) na[i] = *reinterpret_cast<const Vec*>(x + ca[i] * V);
+        if (hb[i]) nb[i] = *reinterpret_cast<const Vec*>(x + cb[i] * V);
       }
-      if (!plain) {
-        float a[NP][V], b[NP][V];
+    }
+  };
+  load(0);
+  __syncthreads();
+  if (p.rot) qn_fill_table<V>(p, tbl, spos, n_tok, np);
+  __syncthreads();
+#pragma unroll 1
+  for (int it = 0; it < total; ++it) {  // the same trip count for every lane: the shuffles name all of them
+    const int kind = it < first_k ? 0 : it < first_v ? 1 : 2;
+    const QnRows& R = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
+    const int row = grp + (it - (kind == 0 ? 0 : kind == 1 ? first_k : first_v)) * n_grp;
+    const bool live = row < n_tok * R.heads;
+    const int tl = live ? qn_token(R, row) : 0, h = row - tl * R.heads;
+    const float* w = sw + kind * 2 * QN_MAX_D;
+    const float* bias = w + QN_MAX_D;
+    Vec va[NP], vb[NP];
 #pragma unroll
-        for (int i = 0; i < NP; ++i)
+    for (int i = 0; i < NP; ++i) {
+      va[i] = na[i];
+      vb[i] = nb[i];
+    }
+    if (it + 1 < total) load(it + 1);
+    if (kind < 2 && (R.w || p.rot)) {  // else a copy, bit by bit
+      float a[NP][V], b[NP][V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            a[i][j] = live && ha[i] ? sb::to_f(va[i].e[j]) : 0.f;
-            b[i][j] = live && hb[i] ? sb::to_f(vb[i].e[j]) : 0.f;
-          }
-        if (R.w) {
-          float mu, r;
-          qn_stats<V, NP>(a, b, ha, hb, D, p.rms, p.eps, g, mu, r);
+      for (int i = 0; i < NP; ++i)
 #pragma unroll
-          for (int i = 0; i < NP; ++i) {
-            float wa[V], wb[V];
-            if (ha[i]) {
-              qn_read_weights<V>(w, ca[i], chunks, wa);
-#pragma unroll
-              for (int j = 0; j < V; ++j) a[i][j] = (a[i][j] - mu) * r * wa[j];
-            }
-            if (hb[i]) {
-              qn_read_weights<V>(w, cb[i], chunks, wb);
-#pragma unroll
-              for (int j = 0; j < V; ++j) b[i][j] = (b[i][j] - mu) * r * wb[j];
-            }
-            if (R.b) {
-              if (ha[i]) {
-                qn_read_weights<V>(bias, ca[i], chunks, wa);
-#pragma unroll
-                for (int j = 0; j < V; ++j) a[i][j] += wa[j];
-              }
-              if (hb[i]) {
-                qn_read_weights<V>(bias, cb[i], chunks, wb);
-#pragma unroll
-                for (int j = 0; j < V; ++j) b[i][j] += wb[j];
-              }
-            }
-          }
+        for (int j = 0; j < V; ++j) {
+          a[i][j] = live && ha[i] ? sb::to_f(va[i].e[j]) : 0.f;
+          b[i][j] = live && hb[i] ? sb::to_f(vb[i].e[j]) : 0.f;
         }
-        if (p.rot) {
-#pragma unroll
-          for (int i = 0; i < NP; ++i)
-            qn_rotate<V>(a[i], b[i], tbl + tl * np * V, lane + i * g, np, p.rot, p.interleaved, 1.f);
-        }
-#pragma unroll
-        for (int i = 0; i < NP; ++i)
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            va[i].e[j] = sb::from_f<T>(a[i][j]);
-            vb[i].e[j] = sb::from_f<T>(b[i][j]);
-          }
-      }
-      T* y = reinterpret_cast<T*>(R.y);
-      bool store = live;
-      if (PAGED && live) {
-        const int page = spage[tl];
-        if (kind == 0) {
-          y += (long)(t0 + tl) * R.y_tok + (long)h * R.y_head;
-          if (page == -2) {  // behind the last sequence: zeros
-#pragma unroll
-            for (int i = 0; i < NP; ++i)
-#pragma unroll
-              for (int j = 0; j < V; ++j) va[i].e[j] = vb[i].e[j] = sb::from_f<T>(0.f);
-          }
-        } else {
-          store = page >= 0;
-          y += (long)page * (kind == 1 ? p.k_page : p.v_page) + (long)sslot[tl] * (kind == 1 ? p.k_slot : p.v_slot) +
-               (long)h * R.y_head;
-        }
-      } else if (live) {
-        y += (long)(t0 + tl) * R.y_tok + (long)h * R.y_head;
-      }
-      if (store) {
+      if (R.w) {
+        float mu, r;
+        qn_stats<V, NP>(a, b, ha, hb, D, p.rms, p.eps, g, mu, r);
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          if (ha[i]) *reinterpret_cast<Vec*>(y + ca[i] * V) = va[i];
-          if (hb[i]) *reinterpret_cast<Vec*>(y + cb[i] * V) = vb[i];
+          float wa[V], wb[V];
+          if (ha[i]) {
+            qn_read_weights<V>(w, ca[i], chunks, wa);
+#pragma unroll
+            for (int j = 0; j < V; ++j) a[i][j] = (a[i][j] - mu) * r * wa[j];
+          }
+          if (hb[i]) {
+            qn_read_weights<V>(w, cb[i], chunks, wb);
+#pragma unroll
+            for (int j = 0; j < V; ++j) b[i][j] = (b[i][j] - mu) * r * wb[j];
+          }
+          if (R.b) {
+            if (ha[i]) {
+              qn_read_weights<V>(bias, ca[i], chunks, wa);
+#pragma unroll
+              for (int j = 0; j < V; ++j) a[i][j] += wa[j];
+            }
+            if (hb[i]) {
+              qn_read_weights<V>(bias, cb[i], chunks, wb);
+#pragma unroll
+              for (int j = 0; j < V; ++j) b[i][j] += wb[j];
+            }
+          }
         }
+      }
+      if (p.rot) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+          qn_rotate<V>(a[i], b[i], tbl + tl * np * V, lane + i * g, np, p.rot, p.interleaved, 1.f);
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          va[i].e[j] = sb::from_f<T>(a[i][j]);
+          vb[i].e[j] = sb::from_f<T>(b[i][j]);
+        }
+    }
+    T* y = reinterpret_cast<T*>(R.y);
+    bool store = live;
+    if (PAGED && live) {
+      const int page = spage[tl];
+      if (kind == 0) {
+        y += (long)(t0 + tl) * R.y_tok + (long)h * R.y_head;
+        if (page == -2) {  // behind the last sequence: zeros
+#pragma unroll
+          for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) va[i].e[j] = vb[i].e[j] = sb::from_f<T>(0.f);
+        }
+      } else {
+        store = page >= 0;
+        y += (long)page * (kind == 1 ? p.k_page : p.v_page) + (long)sslot[tl] * (kind == 1 ? p.k_slot : p.v_slot) +
+             (long)h * R.y_head;
+      }
+    } else if (live) {
+      y += (long)(t0 + tl) * R.y_tok + (long)h * R.y_head;
+    }
+    if (store) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        if (ha[i]) *reinterpret_cast<Vec*>(y + ca[i] * V) = va[i];
+        if (hb[i]) *reinterpret_cast<Vec*>(y + cb[i] * V) = vb[i];
       }
     }
   }
@@ -364,7 +383,8 @@ __global__ void __launch_bounds__(QN_THREADS, 4) qn_fwd_kernel(const __grid_cons
 // ============================================================================ backward
 // A block takes either q or k, walks over tiles of tokens and keeps its share of dw and db in registers (each lane owns
 // the same chunks in every row); the block's sums go to one row of `partial`, added up in a fixed order afterwards.
-template <typename T, int V, int NP>
+// RMS: no mean, and no biases whose gradients would have to be kept.
+template <typename T, int V, int NP, bool RMS>
 __global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_constant__ QnParams p) {
   extern __shared__ __align__(16) float smem[];
   using Vec = QnVec<T, V>;
@@ -390,10 +410,31 @@ __global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_cons
 #pragma unroll
     for (int j = 0; j < V; ++j) dwa[i][j] = dwb[i][j] = dba[i][j] = dbb[i][j] = 0.f;
   }
-  const int tiles = (p.T + p.tile - 1) / p.tile;
+  const int per_tile = is_q ? p.tile : p.tile_k, tiles = (p.T + per_tile - 1) / per_tile;
 #pragma unroll 1
   for (int tile = blk; tile < tiles; tile += n_blk) {
-    const int t0 = tile * p.tile, n_tok = min(p.tile, p.T - t0);
+    const int t0 = tile * per_tile, n_tok = min(per_tile, p.T - t0);
+    const int rows = n_tok * R.heads, iters = (rows + n_grp - 1) / n_grp;
+    Vec na[NP], nb[NP], ma[NP], mb[NP];  // x and dy of the next round
+    auto load = [&](int row) {
+      if (row < rows) {
+        const int tl = qn_token(R, row), h = row - tl * R.heads;
+        const T* x = reinterpret_cast<const T*>(R.x) + (long)(t0 + tl) * R.x_tok + (long)h * R.x_head;
+        const T* dy = reinterpret_cast<const T*>(R.dy) + (long)(t0 + tl) * R.dy_tok + (long)h * R.dy_head;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          if (ha[i]) {
+            na[i] = *reinterpret_cast<const Vec*>(x + ca[i] * V);
+            ma[i] = *reinterpret_cast<const Vec*>(dy + ca[i] * V);
+          }
+          if (hb[i]) {
+            nb[i] = *reinterpret_cast<const Vec*>(x + cb[i] * V);
+            mb[i] = *reinterpret_cast<const Vec*>(dy + cb[i] * V);
+          }
+        }
+      }
+    };
+    load(grp);
     __syncthreads();  // the table of the tile before is no longer read
     if (p.rot) {
       if (threadIdx.x < n_tok) spos[threadIdx.x] = p.pos[t0 + threadIdx.x];
@@ -401,26 +442,20 @@ __global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_cons
       qn_fill_table<V>(p, tbl, spos, n_tok, np);
     }
     __syncthreads();
-    const int rows = n_tok * R.heads, iters = (rows + n_grp - 1) / n_grp;
 #pragma unroll 1
     for (int it = 0; it < iters; ++it) {
       const int row = grp + it * n_grp;
       const bool live = row < rows;
-      const int tl = live ? row / R.heads : 0, h = row - tl * R.heads;
-      const T* x = reinterpret_cast<const T*>(R.x) + (long)(t0 + tl) * R.x_tok + (long)h * R.x_head;
-      const T* dy = reinterpret_cast<const T*>(R.dy) + (long)(t0 + tl) * R.dy_tok + (long)h * R.dy_head;
+      const int tl = live ? qn_token(R, row) : 0, h = row - tl * R.heads;
       Vec va[NP], vb[NP], ya[NP], yb[NP];
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        if (live && ha[i]) {
-          va[i] = *reinterpret_cast<const Vec*>(x + ca[i] * V);
-          ya[i] = *reinterpret_cast<const Vec*>(dy + ca[i] * V);
-        }
-        if (live && hb[i]) {
-          vb[i] = *reinterpret_cast<const Vec*>(x + cb[i] * V);
-          yb[i] = *reinterpret_cast<const Vec*>(dy + cb[i] * V);
-        }
+        va[i] = na[i];
+        vb[i] = nb[i];
+        ya[i] = ma[i];
+        yb[i] = mb[i];
       }
+      if (it + 1 < iters) load(row + n_grp);
       float a[NP][V], b[NP][V], da[NP][V], db[NP][V];
 #pragma unroll
       for (int i = 0; i < NP; ++i)
@@ -437,7 +472,7 @@ __global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_cons
           qn_rotate<V>(da[i], db[i], tbl + tl * np * V, lane + i * g, np, p.rot, p.interleaved, -1.f);
       }
       float mu, r;
-      qn_stats<V, NP>(a, b, ha, hb, D, p.rms, p.eps, g, mu, r);
+      qn_stats<V, NP>(a, b, ha, hb, D, RMS, p.eps, g, mu, r);
       float s1 = 0.f, s2 = 0.f;  // sums of g and of g * xhat
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
@@ -448,9 +483,9 @@ __global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_cons
           for (int j = 0; j < V; ++j) {
             a[i][j] = (a[i][j] - mu) * r;
             if (live) dwa[i][j] = fmaf(da[i][j], a[i][j], dwa[i][j]);
-            dba[i][j] += da[i][j];
+            if (!RMS) dba[i][j] += da[i][j];
             da[i][j] *= w[j];
-            s1 += da[i][j];
+            if (!RMS) s1 += da[i][j];
             s2 = fmaf(da[i][j], a[i][j], s2);
           }
         }
@@ -460,15 +495,15 @@ __global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_cons
           for (int j = 0; j < V; ++j) {
             b[i][j] = (b[i][j] - mu) * r;
             if (live) dwb[i][j] = fmaf(db[i][j], b[i][j], dwb[i][j]);
-            dbb[i][j] += db[i][j];
+            if (!RMS) dbb[i][j] += db[i][j];
             db[i][j] *= w[j];
-            s1 += db[i][j];
+            if (!RMS) s1 += db[i][j];
             s2 = fmaf(db[i][j], b[i][j], s2);
           }
         }
       }
       s2 = qn_group_sum(s2, g) / D;
-      s1 = p.rms ? 0.f : qn_group_sum(s1, g) / D;
+      s1 = RMS ? 0.f : qn_group_sum(s1, g) / D;
       T* y = reinterpret_cast<T*>(R.y) + (long)(t0 + tl) * R.y_tok + (long)h * R.y_head;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
@@ -494,8 +529,10 @@ __global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_cons
       for (int o = g; o < 32; o <<= 1) {
         dwa[i][j] += __shfl_xor_sync(0xffffffffu, dwa[i][j], o);
         dwb[i][j] += __shfl_xor_sync(0xffffffffu, dwb[i][j], o);
-        dba[i][j] += __shfl_xor_sync(0xffffffffu, dba[i][j], o);
-        dbb[i][j] += __shfl_xor_sync(0xffffffffu, dbb[i][j], o);
+        if (!RMS) {
+          dba[i][j] += __shfl_xor_sync(0xffffffffu, dba[i][j], o);
+          dbb[i][j] += __shfl_xor_sync(0xffffffffu, dbb[i][j], o);
+        }
       }
       if ((threadIdx.x & 31) < g) {
         float* dst = red + warp * 2 * QN_MAX_D;
@@ -538,25 +575,28 @@ int qn_log_lanes(int pairs, int cap) {
   while ((1 << l) < pairs && (1 << l) < cap) ++l;
   return l;
 }
-bool qn_vec_ok(const QnRows& r, int esize, bool with_dy) {
-  if (r.heads == 0) return true;
-  const long v = 16 / esize;
-  if ((reinterpret_cast<uintptr_t>(r.x) | reinterpret_cast<uintptr_t>(r.y)) & 15) return false;
-  if (r.x_tok % v || r.x_head % v || r.y_tok % v || r.y_head % v) return false;
-  return !with_dy || (!(reinterpret_cast<uintptr_t>(r.dy) & 15) && r.dy_tok % v == 0 && r.dy_head % v == 0);
+// Bytes (a power of two up to 16) that divide every address of the rows.
+long qn_align(const QnRows& r, int es) {
+  if (r.heads == 0) return 16;
+  const uintptr_t all = reinterpret_cast<uintptr_t>(r.x) | reinterpret_cast<uintptr_t>(r.y) | reinterpret_cast<uintptr_t>(r.dy) |
+                        (uintptr_t)((r.x_tok | r.x_head | r.y_tok | r.y_head | r.dy_tok | r.dy_head) * es) | 16;
+  return (long)(all & -all);
 }
 
-// Fills in what follows from the sizes; returns true when rows move as 16-byte chunks (V elements, one pair per lane):
-// aligned rows whose rotated part, for rotate-half, splits into whole chunks.  Everything else moves element by element.
-bool qn_plan(QnParams* p, int esize, bool vec_ok, double base) {
-  const int v = 16 / esize;
-  const bool fast = vec_ok && p->D % v == 0 && (p->rot == 0 || p->interleaved || (p->rot / 2) % v == 0) && p->D / v <= 64;
-  const int V = fast ? v : 1;
+// Fills in what follows from the sizes; returns the elements V that a lane moves at once: 16 bytes where all rows are so
+// aligned and, for rotate-half, the rotated half is whole chunks; else 2 elements; else 1 (3000 tokens x 41 heads of 80 in
+// fp32, 20 dimensions rotated: 1150 us with V = 1, see the measured table for V = 2).
+int qn_plan(QnParams* p, int es, long align, double base) {
+  auto fits = [&](int v) {
+    return align >= (long)v * es && p->D % v == 0 && (p->rot == 0 || (p->interleaved ? v % 2 == 0 : (p->rot / 2) % v == 0));
+  };
+  const int V = fits(16 / es) ? 16 / es : fits(2) ? 2 : 1;
   const int chunks = (p->D + V - 1) / V, pairs = (chunks + 1) / 2;
-  p->log_g = fast ? qn_log_lanes(pairs, 32) : 5;
+  p->log_g = qn_log_lanes(pairs, 32);
+  for (QnRows* r : {&p->q, &p->k, &p->v}) r->inv = r->heads ? (uint32_t)((1UL << 32) / r->heads + 1) : 0;
   for (int i = 0; i < p->rot / 2; ++i)
     p->turns[i] = pow(base, -2.0 * i / p->rot) / 6.283185307179586476925;
-  return fast;
+  return V;
 }
 int qn_table_bytes_per_token(const QnParams& p, int V) { return p.rot ? ((p.rot + 2 * V - 1) / (2 * V)) * V * 8 : 0; }
 
@@ -566,34 +606,33 @@ static int qn_check(const QnParams& p, int dtype) {
   if (dtype != SB_DT_F32 && dtype != SB_DT_BF16 && dtype != SB_DT_F16) return SB_ERR_BAD_ARG;
   if (p.w_dtype != SB_DT_F32 && p.w_dtype != SB_DT_BF16 && p.w_dtype != SB_DT_F16) return SB_ERR_BAD_ARG;
   if (p.D < 1 || p.T < 0 || p.q.heads < 0 || p.k.heads < 0) return SB_ERR_BAD_ARG;
-  if (p.D > QN_MAX_D) return SB_ERR_TOO_LARGE;
+  // the division by the head count is exact below 2^32 / heads rows, a tile has at most 64 heads of them
+  if (p.D > QN_MAX_D || p.q.heads > 8000 || p.k.heads > 8000) return SB_ERR_TOO_LARGE;
   if (p.rot < 0 || p.rot % 2 || p.rot > p.D) return SB_ERR_BAD_ARG;
   return SB_OK;
 }
 
 template <typename T>
-static int qn_launch_fwd(QnParams& p, bool paged, bool vec_ok, double base, int sms, cudaStream_t stream) {
-  const bool fast = qn_plan(&p, sizeof(T), vec_ok, base);
+static int qn_launch_fwd(QnParams& p, bool paged, long align, double base, int sms, cudaStream_t stream) {
+  const int V = qn_plan(&p, sizeof(T), align, base);
   constexpr int VF = 16 / sizeof(T);
-  const int per_tok = qn_table_bytes_per_token(p, fast ? VF : 1);
-  // Tokens per CTA: enough rows for four rounds of the CTA's row groups, so that the table and the weights are worth
-  // their barrier, but not so many that SMs go without a CTA.
-  const int heads = p.q.heads + p.k.heads + (paged ? p.v.heads : 0);
-  const int groups = QN_THREADS >> p.log_g;
-  int tile = (4 * groups + heads - 1) / heads;
+  const int per_tok = qn_table_bytes_per_token(p, V);
+  // Tokens per CTA: the launch is one wave where the table has room for that many, so that the weights, the table and
+  // their barriers are paid once per CTA.
+  int tile = (int)((p.T + (long)QN_FWD_BLOCKS * sms - 1) / ((long)QN_FWD_BLOCKS * sms));
   if (tile > QN_MAX_SLOTS) tile = QN_MAX_SLOTS;
   if (per_tok && tile > QN_TABLE_BYTES / per_tok) tile = QN_TABLE_BYTES / per_tok;
-  while (tile > 1 && (p.T + tile - 1) / tile < 2 * sms) tile = (tile + 1) / 2;
   p.tile = tile;
   const int smem = 4 * QN_MAX_D * 4 + tile * per_tok;
   const int grid = (p.T + tile - 1) / tile;
-  if (paged) {
-    if (fast) qn_fwd_kernel<T, VF, 1, true><<<grid, QN_THREADS, smem, stream>>>(p);
-    else qn_fwd_kernel<T, 1, 4, true><<<grid, QN_THREADS, smem, stream>>>(p);
-  } else {
-    if (fast) qn_fwd_kernel<T, VF, 1, false><<<grid, QN_THREADS, smem, stream>>>(p);
-    else qn_fwd_kernel<T, 1, 4, false><<<grid, QN_THREADS, smem, stream>>>(p);
-  }
+  auto launch = [&](auto paged_form) {
+    constexpr bool PAGED = decltype(paged_form)::value;
+    if (V == VF) qn_fwd_kernel<T, VF, 1, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
+    else if (V == 2) qn_fwd_kernel<T, 2, 2, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
+    else qn_fwd_kernel<T, 1, 4, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
+  };
+  if (paged) launch(std::true_type());
+  else launch(std::false_type());
   SB_CHECK_LAUNCH();
   return SB_OK;
 }
@@ -613,8 +652,8 @@ SB_API int sb200_qk_norm_rope_fwd(const void* q, const void* k, void* q_out, voi
   if (rot && (!pos || !(base > 0.0))) return SB_ERR_BAD_ARG;
   if (T == 0 || Hq + Hk == 0) return SB_OK;
   const int es = dtype == SB_DT_F32 ? 4 : 2;
-  const bool vec = qn_vec_ok(p.q, es, false) && qn_vec_ok(p.k, es, false);
-  SB_DISPATCH_DTYPE(dtype, E, { return qn_launch_fwd<E>(p, false, vec, base, sms, stream); });
+  const long align = std::min(qn_align(p.q, es), qn_align(p.k, es));
+  SB_DISPATCH_DTYPE(dtype, E, { return qn_launch_fwd<E>(p, false, align, base, sms, stream); });
   return SB_OK;
 }
 
@@ -645,10 +684,9 @@ SB_API int sb200_paged_append(const void* q, const void* k, const void* v, void*
   p.k_page = k_page; p.k_slot = k_slot; p.v_page = v_page; p.v_slot = v_slot;
   while ((1 << p.page_shift) < page_size) ++p.page_shift;
   const int es = dtype == SB_DT_F32 ? 4 : 2;
-  const long v16 = 16 / es;
-  const bool vec = qn_vec_ok(p.q, es, false) && qn_vec_ok(p.k, es, false) && qn_vec_ok(p.v, es, false) &&
-                   k_page % v16 == 0 && k_slot % v16 == 0 && v_page % v16 == 0 && v_slot % v16 == 0;
-  SB_DISPATCH_DTYPE(dtype, E, { return qn_launch_fwd<E>(p, true, vec, base, sms, stream); });
+  const uintptr_t slots = (uintptr_t)((k_page | k_slot | v_page | v_slot) * es) | 16;
+  const long align = std::min({qn_align(p.q, es), qn_align(p.k, es), qn_align(p.v, es), (long)(slots & -slots)});
+  SB_DISPATCH_DTYPE(dtype, E, { return qn_launch_fwd<E>(p, true, align, base, sms, stream); });
   return SB_OK;
 }
 
@@ -659,25 +697,34 @@ SB_API int sb200_qk_norm_rope_bwd_blocks(int T, int sms) {
 }
 
 template <typename T>
-static int qn_launch_bwd(QnParams& p, bool vec_ok, double base, int blocks, cudaStream_t stream) {
-  const bool fast = qn_plan(&p, sizeof(T), vec_ok, base);
+static int qn_launch_bwd(QnParams& p, long align, double base, int blocks, cudaStream_t stream) {
+  const int V = qn_plan(&p, sizeof(T), align, base);
   constexpr int VF = 16 / sizeof(T);
-  const int per_tok = qn_table_bytes_per_token(p, fast ? VF : 1);
-  const int heads = p.q.heads > p.k.heads ? p.q.heads : p.k.heads;
-  const int groups = QN_THREADS >> p.log_g;
+  const int per_tok = qn_table_bytes_per_token(p, V);
   // blocks shared out by rows, at least one each
   int qb = (int)(((long)blocks * p.q.heads + (p.q.heads + p.k.heads) / 2) / (p.q.heads + p.k.heads));
   p.q_blocks = qb < 1 ? 1 : qb > blocks - 1 ? blocks - 1 : qb;
-  int tile = (4 * groups + heads - 1) / heads;
-  if (tile > QN_MAX_SLOTS) tile = QN_MAX_SLOTS;
-  if (per_tok && tile > QN_TABLE_BYTES / per_tok) tile = QN_TABLE_BYTES / per_tok;
-  while (tile > 1 && (p.T + tile - 1) / tile < 4 * p.q_blocks) tile = (tile + 1) / 2;
-  p.tile = tile;
+  // Each block takes its tokens in as few and as even tiles as the table allows.
+  int cap = QN_MAX_SLOTS;
+  if (per_tok && cap > QN_TABLE_BYTES / per_tok) cap = QN_TABLE_BYTES / per_tok;
+  auto even = [&](int n_blocks) {
+    const int mine = (p.T + n_blocks - 1) / n_blocks, tiles = (mine + cap - 1) / cap;
+    return (mine + tiles - 1) / tiles;
+  };
+  p.tile = even(p.q_blocks);
+  p.tile_k = even(blocks - p.q_blocks);
+  const int tile = p.tile > p.tile_k ? p.tile : p.tile_k;
   int smem = QN_MAX_D * 4 + tile * per_tok;
   const int red = (QN_THREADS / 32) * 2 * QN_MAX_D * 4;
   if (smem < red) smem = red;
-  if (fast) qn_bwd_kernel<T, VF, 1><<<blocks, QN_THREADS, smem, stream>>>(p);
-  else qn_bwd_kernel<T, 1, 4><<<blocks, QN_THREADS, smem, stream>>>(p);
+  auto launch = [&](auto rms_form) {
+    constexpr bool RMS = decltype(rms_form)::value;
+    if (V == VF) qn_bwd_kernel<T, VF, 1, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
+    else if (V == 2) qn_bwd_kernel<T, 2, 2, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
+    else qn_bwd_kernel<T, 1, 4, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
+  };
+  if (p.rms) launch(std::true_type());
+  else launch(std::false_type());
   SB_CHECK_LAUNCH();
   return SB_OK;
 }
@@ -699,9 +746,9 @@ SB_API int sb200_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, const 
   if (int rc = qn_check(p, dtype)) return rc;
   if ((rot && (!pos || !(base > 0.0))) || !q_w || !k_w || T < 1 || Hq < 1 || Hk < 1 || blocks < 2) return SB_ERR_BAD_ARG;
   const int es = dtype == SB_DT_F32 ? 4 : 2;
-  const bool vec = qn_vec_ok(p.q, es, true) && qn_vec_ok(p.k, es, true);
+  const long align = std::min(qn_align(p.q, es), qn_align(p.k, es));
   int rc = SB_ERR_BAD_ARG;
-  SB_DISPATCH_DTYPE(dtype, E, { rc = qn_launch_bwd<E>(p, vec, base, blocks, stream); });
+  SB_DISPATCH_DTYPE(dtype, E, { rc = qn_launch_bwd<E>(p, align, base, blocks, stream); });
   if (rc || !partial) return rc;
   SB_DISPATCH_DTYPE(w_dtype, W, {
     qn_bwd_sum_kernel<W><<<dim3((2 * D + 31) / 32, 2), dim3(32, 32), 0, stream>>>(

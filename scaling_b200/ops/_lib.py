@@ -215,14 +215,23 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream() -> int:
+    """The current stream of the current device as an integer handle."""
+    if _raw_stream is not None:  # a tenth of the time that building a Stream object takes
+        return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+_NO_CONTEXT = contextlib.nullcontext()
 
 
 def on_device_of(t: torch.Tensor):
     """Context in which the device of ``t`` is current (launches, streams and workspaces follow the current device)."""
-    if t.device.index is None or t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if t.get_device() == torch.cuda.current_device():
+        return _NO_CONTEXT
     return torch.cuda.device(t.device)
 
 

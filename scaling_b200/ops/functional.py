@@ -600,6 +600,8 @@ def _common_dtype(*params: Optional[torch.Tensor]) -> tuple[Optional[torch.Tenso
     """Norm parameters of one kernel call in one type (fp32 where they differ or the kernels do not know the type)."""
     kinds = {p.dtype for p in params if p is not None}
     same = len(kinds) <= 1 and kinds <= set(_KERNEL_DTYPES)
+    if same and all(p is None or p.is_contiguous() for p in params):
+        return params
     return tuple(None if p is None else (p if same else p.float()).contiguous() for p in params)
 
 
@@ -607,19 +609,25 @@ def _unit_inner(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _qk_norm_rope_launch(q, k, wq, wk, bq, bk, pos, rot, base, interleaved, eps, rms):
+    T, Hq, D = q.shape
+    Hk = k.shape[1]
+    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+    ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+    q_tok, q_head, _ = q.stride()
+    k_tok, k_head, _ = k.stride()
+    with _lib.on_device_of(q):
+        check(lib().sb200_qk_norm_rope_fwd(
+            q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), wq.data_ptr(), wk.data_ptr(), ptr(bq), ptr(bk),
+            ptr(pos), T, Hq, Hk, D, q_tok, q_head, k_tok, k_head, eps, rms, rot, base, interleaved, dt(q.dtype),
+            dt(wq.dtype), sm_count(), stream()), "sb200_qk_norm_rope_fwd")
+    return qo, ko
+
+
 class _QKNormRopeFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, bq, bk, pos, rot, base, interleaved, eps, rms):  # type: ignore[override]
-        q, k = _unit_inner(q), _unit_inner(k)
-        T, Hq, D = q.shape
-        Hk = k.shape[1]
-        qo = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
-        ko = torch.empty((T, Hk, D), dtype=q.dtype, device=q.device)
-        with _lib.on_device_of(q):
-            check(lib().sb200_qk_norm_rope_fwd(
-                q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), wq.data_ptr(), wk.data_ptr(), ptr(bq), ptr(bk),
-                ptr(pos), T, Hq, Hk, D, q.stride(0), q.stride(1), k.stride(0), k.stride(1), eps, int(rms), rot, base,
-                int(interleaved), dt(q.dtype), dt(wq.dtype), sm_count(), stream()), "sb200_qk_norm_rope_fwd")
+        qo, ko = _qk_norm_rope_launch(q, k, wq, wk, bq, bk, pos, rot, base, interleaved, eps, rms)
         ctx.save_for_backward(q, k, wq, wk, pos)
         ctx.params = (wq, wk, bq, bk)  # the parameter objects themselves (for their persistent .grad buffers)
         ctx.cfg = (rot, base, interleaved, eps, rms)
@@ -633,8 +641,8 @@ class _QKNormRopeFn(torch.autograd.Function):
         dqo, dko = _unit_inner(dqo), _unit_inner(dko)
         T, Hq, D = q.shape
         Hk = k.shape[1]
-        dq = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
-        dk = torch.empty((T, Hk, D), dtype=q.dtype, device=q.device)
+        dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+        dk = torch.empty_like(k, memory_format=torch.contiguous_format)
         params = ctx.params
         wanted = [p is not None and ctx.needs_input_grad[2 + i] for i, p in enumerate(params)]
         with _lib.on_device_of(q):
@@ -683,9 +691,15 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     if q.dtype not in _KERNEL_DTYPES or q.shape[2] > 256:
         raise _lib.KernelError(f"qk_norm_rope: {q.dtype} with head size {q.shape[2]} is not supported (fp32, bf16, fp16 "
                                "up to 256)")
-    pos = positions.to(torch.int32).contiguous() if rot else None
+    pos = None
+    if rot:
+        pos = positions if positions.dtype == torch.int32 else positions.to(torch.int32)
+        pos = pos if pos.is_contiguous() else pos.contiguous()
     wq, wk, bq, bk = _common_dtype(q_weight, k_weight, q_bias, k_bias)
-    return _QKNormRopeFn.apply(q, k, wq, wk, bq, bk, pos, rot, base, interleaved, float(eps), bool(rms))
+    args = (_unit_inner(q), _unit_inner(k), wq, wk, bq, bk, pos, rot, base, interleaved, float(eps), bool(rms))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:6]):
+        return _QKNormRopeFn.apply(*args)
+    return _qk_norm_rope_launch(*args)
 
 
 # --------------------------------------------------------------------------- masked softmax

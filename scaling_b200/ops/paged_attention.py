@@ -127,7 +127,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     if d > 256:
         raise _lib.KernelError(f"paged_append: head size {d} is not supported (up to 256)")
     code = dt(k.dtype)
-    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = None if q is None else torch.empty_like(q, memory_format=torch.contiguous_format)
     if tokens == 0:
         return out
     k, v = _unit_inner(k), _unit_inner(v)
@@ -217,7 +217,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                "(bf16 / fp16, multiples of 8 up to 128, pages of 8 and more)")
     zero_tail = out is None
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if q.numel() == 0:
         return out
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("out", out)):
