@@ -75,6 +75,85 @@ __device__ __forceinline__ int qn_token(const QnRows& r, int row) { return r.hea
 // N consecutive elements as one access
 template <typename T, int N> struct alignas(sizeof(T) * N) QnVec { T e[N]; };
 
+// Arithmetic on a chunk, two fp32 operations per instruction: the kernels are close to bound by instructions.
+__device__ __forceinline__ void qn_fma2(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0, float c1) {
+  asm("{\n.reg .b64 x, y, z, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\n"
+      "fma.rn.f32x2 w, x, y, z;\nmov.b64 {%0, %1}, w;\n}\n"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void qn_mul2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+  asm("{\n.reg .b64 x, y, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 w, x, y;\nmov.b64 {%0, %1}, w;\n}\n"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+template <int V> __device__ __forceinline__ void qn_mul(float (&d)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V == 1) d[0] = a[0] * b[0];
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) qn_mul2(d[i], d[i + 1], a[i], a[i + 1], b[i], b[i + 1]);
+}
+template <int V> __device__ __forceinline__ void qn_scale(float (&d)[V], float b) {
+  if constexpr (V == 1) d[0] *= b;
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) qn_mul2(d[i], d[i + 1], d[i], d[i + 1], b, b);
+}
+// d = a * b + c
+template <int V>
+__device__ __forceinline__ void qn_fma(float (&d)[V], const float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+  if constexpr (V == 1) d[0] = fmaf(a[0], b[0], c[0]);
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) qn_fma2(d[i], d[i + 1], a[i], a[i + 1], b[i], b[i + 1], c[i], c[i + 1]);
+}
+// d = a * b + d with one factor for all
+template <int V> __device__ __forceinline__ void qn_axpy(float (&d)[V], const float (&a)[V], float b) {
+  if constexpr (V == 1) d[0] = fmaf(a[0], b, d[0]);
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) qn_fma2(d[i], d[i + 1], a[i], a[i + 1], b, b, d[i], d[i + 1]);
+}
+template <int V> __device__ __forceinline__ void qn_shift(float (&d)[V], float b) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) d[i] += b;
+}
+// sum of a * b over the chunk
+template <int V> __device__ __forceinline__ float qn_dot(const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V == 1) return a[0] * b[0];
+  else {
+    float s0, s1;
+    qn_mul2(s0, s1, a[0], a[1], b[0], b[1]);
+#pragma unroll
+    for (int i = 2; i < V; i += 2) qn_fma2(s0, s1, a[i], a[i + 1], b[i], b[i + 1], s0, s1);
+    return s0 + s1;
+  }
+}
+template <int V> __device__ __forceinline__ float qn_total(const float (&a)[V]) {
+  float s = a[0];
+#pragma unroll
+  for (int i = 1; i < V; ++i) s += a[i];
+  return s;
+}
+template <typename T, int V> __device__ __forceinline__ void qn_unpack(const QnVec<T, V>& v, float (&f)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) f[i] = sb::to_f(v.e[i]);
+}
+template <typename T, int V> __device__ __forceinline__ void qn_pack(const float (&f)[V], QnVec<T, V>& v) {
+  if constexpr (sizeof(T) == 2 && V > 1) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        *reinterpret_cast<__nv_bfloat162*>(&v.e[i]) = __floats2bfloat162_rn(f[i], f[i + 1]);
+      else
+        *reinterpret_cast<__half2*>(&v.e[i]) = __floats2half2_rn(f[i], f[i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v.e[i] = sb::from_f<T>(f[i]);
+  }
+}
+
 // What a lane holds of a row: NP pairs of chunks of V elements.  Pair p of lane l is number c = l + p G:
 //   rotate-half and c < rot / (2 V): A = c, B = c + rot / (2 V); otherwise A = 2 c, B = 2 c + 1.
 template <int V> struct QnChunks {
@@ -87,11 +166,13 @@ template <int V> struct QnChunks {
   }
 };
 
-// Place of element i (< V) of pair c in the sine table of one token, in float2 units.  Consecutive lanes touch
-// consecutive 16-byte words (no bank conflicts); np = pairs per row that the table covers.
+// Place of the cosine of element i (< V) of pair c in the table of one token, in floats.  A 16-byte word holds the cosines and
+// then the sines of two neighbours, consecutive lanes touch consecutive words (no bank conflicts); np = pairs per row that
+// the table covers.  The sine lies qn_sine<V>() behind.
 template <int V> __device__ __forceinline__ int qn_table_slot(int c, int i, int np) {
-  return V == 1 ? c : (((i >> 1) * np + c) << 1) + (i & 1);
+  return V == 1 ? 2 * c : (((i >> 1) * np + c) << 2) + (i & 1);
 }
+template <int V> __device__ __forceinline__ constexpr int qn_sine() { return V == 1 ? 1 : 2; }
 // Place of element e of a weight vector in shared memory: four consecutive elements stay together, chunks interleave.
 template <int V> __device__ __forceinline__ int qn_weight_slot(int e, int chunks) {
   if (V < 4) return e;
@@ -112,46 +193,47 @@ template <int V> __device__ __forceinline__ void qn_read_weights(const float* s,
   }
 }
 
-// Rotation of a chunk pair by the table's angles (sign +1: forward, -1: transposed).
-template <int V>
-__device__ __forceinline__ void qn_rotate(float (&a)[V], float (&b)[V], const float2* tbl, int c, int np, int rot,
-                                          int interleaved, float sign) {
+// Rotation of a chunk pair by the table's angles, BACK: the transposed one.
+template <int V, bool BACK>
+__device__ __forceinline__ void qn_rotate(float (&a)[V], float (&b)[V], const float* tbl, int c, int np, int rot,
+                                          int interleaved) {
   if constexpr (V == 1) {  // both conventions: the pair is (a, b)
-    const int angles = rot >> 1;
-    if (c < angles) {
-      const float2 t = tbl[c];
-      const float s = t.y * sign, x = a[0], y = b[0];
-      a[0] = x * t.x - y * s;
-      b[0] = y * t.x + x * s;
+    if (c < (rot >> 1)) {
+      const float cs = tbl[2 * c], sn = BACK ? -tbl[2 * c + 1] : tbl[2 * c + 1], x = a[0], y = b[0];
+      a[0] = x * cs - y * sn;
+      b[0] = y * cs + x * sn;
     }
   } else {
     if (c * 2 * V >= rot) return;  // neither chunk is rotated (rotate-half: c >= rot / (2 V) is the same test)
-    float2 t[V];
+    float cs[V], sn[V];
 #pragma unroll
     for (int i = 0; i < V; i += 2) {
-      const float4 u = *reinterpret_cast<const float4*>(tbl + ((i >> 1) * np + c) * 2);
-      t[i] = make_float2(u.x, u.y * sign);
-      t[i + 1] = make_float2(u.z, u.w * sign);
+      const float4 u = *reinterpret_cast<const float4*>(tbl + ((i >> 1) * np + c) * 4);
+      cs[i] = u.x;
+      cs[i + 1] = u.y;
+      sn[i] = BACK ? -u.z : u.z;
+      sn[i + 1] = BACK ? -u.w : u.w;
     }
     if (!interleaved) {
+      float x[V], ns[V];
+      qn_mul<V>(x, a, sn);  // the part of b that comes from a
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float x = a[i], y = b[i];
-        a[i] = x * t[i].x - y * t[i].y;
-        b[i] = y * t[i].x + x * t[i].y;
-      }
+      for (int i = 0; i < V; ++i) ns[i] = -sn[i];
+      qn_mul<V>(a, a, cs);
+      qn_fma<V>(a, b, ns, a);
+      qn_fma<V>(b, b, cs, x);
     } else {
 #pragma unroll
       for (int i = 0; i < V / 2; ++i) {
         if (2 * c * V + 2 * i < rot) {
           const float x = a[2 * i], y = a[2 * i + 1];
-          a[2 * i] = x * t[i].x - y * t[i].y;
-          a[2 * i + 1] = y * t[i].x + x * t[i].y;
+          a[2 * i] = x * cs[i] - y * sn[i];
+          a[2 * i + 1] = y * cs[i] + x * sn[i];
         }
         if ((2 * c + 1) * V + 2 * i < rot) {
           const float x = b[2 * i], y = b[2 * i + 1];
-          b[2 * i] = x * t[V / 2 + i].x - y * t[V / 2 + i].y;
-          b[2 * i + 1] = y * t[V / 2 + i].x + x * t[V / 2 + i].y;
+          b[2 * i] = x * cs[V / 2 + i] - y * sn[V / 2 + i];
+          b[2 * i + 1] = y * cs[V / 2 + i] + x * sn[V / 2 + i];
         }
       }
     }
@@ -165,7 +247,7 @@ __device__ __forceinline__ float qn_group_sum(float v, int g) {
 
 // Sines and cosines of a tile's tokens; positions come from `spos`.
 template <int V>
-__device__ __forceinline__ void qn_fill_table(const QnParams& p, float2* tbl, const int* spos, int n_tok, int np) {
+__device__ __forceinline__ void qn_fill_table(const QnParams& p, float* tbl, const int* spos, int n_tok, int np) {
   const int angles = p.rot >> 1;
   for (int i = threadIdx.x; i < n_tok * angles; i += QN_THREADS) {
     const int t = i / angles, a = i - t * angles;
@@ -173,7 +255,9 @@ __device__ __forceinline__ void qn_fill_table(const QnParams& p, float2* tbl, co
     const float rest = (float)(turns - rint(turns));
     float s, c;
     sincospif(2.f * rest, &s, &c);
-    tbl[t * np * V + qn_table_slot<V>(a / V, a % V, np)] = make_float2(c, s);
+    float* at = tbl + t * np * V * 2 + qn_table_slot<V>(a / V, a % V, np);
+    at[0] = c;
+    at[qn_sine<V>()] = s;
   }
 }
 
@@ -182,23 +266,24 @@ template <int V, int NP>
 __device__ __forceinline__ void qn_stats(const float (&a)[NP][V], const float (&b)[NP][V], const bool (&ha)[NP],
                                          const bool (&hb)[NP], int D, int rms, float eps, int g, float& mu, float& r) {
   mu = 0.f;
-  if (!rms) {
+  float ss = 0.f;
+  if (rms) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) ss += qn_dot<V>(a[p], a[p]) + qn_dot<V>(b[p], b[p]);
+  } else {
     float s = 0.f;
 #pragma unroll
-    for (int p = 0; p < NP; ++p)
-#pragma unroll
-      for (int i = 0; i < V; ++i) s += a[p][i] + b[p][i];
+    for (int p = 0; p < NP; ++p) s += qn_total<V>(a[p]) + qn_total<V>(b[p]);
     mu = qn_group_sum(s, g) / D;
+#pragma unroll
+    for (int p = 0; p < NP; ++p)  // around the mean, from registers: no cancellation
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float da = ha[p] ? a[p][i] - mu : 0.f, db = hb[p] ? b[p][i] - mu : 0.f;
+        ss = fmaf(da, da, ss);
+        ss = fmaf(db, db, ss);
+      }
   }
-  float ss = 0.f;  // around the mean, from registers: no cancellation
-#pragma unroll
-  for (int p = 0; p < NP; ++p)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float da = ha[p] ? a[p][i] - mu : 0.f, db = hb[p] ? b[p][i] - mu : 0.f;
-      ss = fmaf(da, da, ss);
-      ss = fmaf(db, db, ss);
-    }
   r = rsqrtf(qn_group_sum(ss, g) / D + eps);
 }
 
@@ -210,7 +295,7 @@ __global__ void __launch_bounds__(QN_THREADS, QN_FWD_BLOCKS) qn_fwd_kernel(const
   using Vec = QnVec<T, V>;
   const int D = p.D, chunks = (D + V - 1) / V, np = (p.rot + 2 * V - 1) / (2 * V);
   float* sw = smem;                                     // q weight, q bias, k weight, k bias
-  float2* tbl = reinterpret_cast<float2*>(smem + 4 * QN_MAX_D);
+  float* tbl = smem + 4 * QN_MAX_D;
   __shared__ int spos[QN_MAX_SLOTS];
   __shared__ int spage[QN_MAX_SLOTS], sslot[QN_MAX_SLOTS];  // spage -1: nothing to write, -2: behind the last sequence
   const int t0 = blockIdx.x * p.tile, n_tok = min(p.tile, p.T - t0);
@@ -263,7 +348,7 @@ __global__ void __launch_bounds__(QN_THREADS, QN_FWD_BLOCKS) qn_fwd_kernel(const
   const int rounds[3] = {(n_tok * p.q.heads + n_grp - 1) / n_grp, (n_tok * p.k.heads + n_grp - 1) / n_grp,
                          PAGED ? (n_tok * p.v.heads + n_grp - 1) / n_grp : 0};
   const int first_k = rounds[0], first_v = first_k + rounds[1], total = first_v + rounds[2];
-  Vec na[NP], nb[NP];
+  Vec na[NP] = {}, nb[NP] = {};  // chunks beyond the row stay zeros
   auto load = [&](int it) {
     const int kind = it < first_k ? 0 : it < first_v ? 1 : 2;
     const QnRows& R = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
@@ -301,38 +386,40 @@ __global__ void __launch_bounds__(QN_THREADS, QN_FWD_BLOCKS) qn_fwd_kernel(const
     if (kind < 2 && (R.w || p.rot)) {  // else a copy, bit by bit
       float a[NP][V], b[NP][V];
 #pragma unroll
-      for (int i = 0; i < NP; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          a[i][j] = live && ha[i] ? sb::to_f(va[i].e[j]) : 0.f;
-          b[i][j] = live && hb[i] ? sb::to_f(vb[i].e[j]) : 0.f;
-        }
+      for (int i = 0; i < NP; ++i) {
+        qn_unpack<T, V>(va[i], a[i]);
+        qn_unpack<T, V>(vb[i], b[i]);
+      }
       if (R.w) {
         float mu, r;
         qn_stats<V, NP>(a, b, ha, hb, D, p.rms, p.eps, g, mu, r);
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          float wa[V], wb[V];
+          float t[V];
+          if (!p.rms) {
+            qn_shift<V>(a[i], -mu);
+            qn_shift<V>(b[i], -mu);
+          }
+          qn_scale<V>(a[i], r);
+          qn_scale<V>(b[i], r);
           if (ha[i]) {
-            qn_read_weights<V>(w, ca[i], chunks, wa);
-#pragma unroll
-            for (int j = 0; j < V; ++j) a[i][j] = (a[i][j] - mu) * r * wa[j];
+            qn_read_weights<V>(w, ca[i], chunks, t);
+            qn_mul<V>(a[i], a[i], t);
           }
           if (hb[i]) {
-            qn_read_weights<V>(w, cb[i], chunks, wb);
-#pragma unroll
-            for (int j = 0; j < V; ++j) b[i][j] = (b[i][j] - mu) * r * wb[j];
+            qn_read_weights<V>(w, cb[i], chunks, t);
+            qn_mul<V>(b[i], b[i], t);
           }
           if (R.b) {
             if (ha[i]) {
-              qn_read_weights<V>(bias, ca[i], chunks, wa);
+              qn_read_weights<V>(bias, ca[i], chunks, t);
 #pragma unroll
-              for (int j = 0; j < V; ++j) a[i][j] += wa[j];
+              for (int j = 0; j < V; ++j) a[i][j] += t[j];
             }
             if (hb[i]) {
-              qn_read_weights<V>(bias, cb[i], chunks, wb);
+              qn_read_weights<V>(bias, cb[i], chunks, t);
 #pragma unroll
-              for (int j = 0; j < V; ++j) b[i][j] += wb[j];
+              for (int j = 0; j < V; ++j) b[i][j] += t[j];
             }
           }
         }
@@ -340,15 +427,13 @@ __global__ void __launch_bounds__(QN_THREADS, QN_FWD_BLOCKS) qn_fwd_kernel(const
       if (p.rot) {
 #pragma unroll
         for (int i = 0; i < NP; ++i)
-          qn_rotate<V>(a[i], b[i], tbl + tl * np * V, lane + i * g, np, p.rot, p.interleaved, 1.f);
+          qn_rotate<V, false>(a[i], b[i], tbl + tl * np * V * 2, lane + i * g, np, p.rot, p.interleaved);
       }
 #pragma unroll
-      for (int i = 0; i < NP; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          va[i].e[j] = sb::from_f<T>(a[i][j]);
-          vb[i].e[j] = sb::from_f<T>(b[i][j]);
-        }
+      for (int i = 0; i < NP; ++i) {
+        qn_pack<T, V>(a[i], va[i]);
+        qn_pack<T, V>(b[i], vb[i]);
+      }
     }
     T* y = reinterpret_cast<T*>(R.y);
     bool store = live;
@@ -394,7 +479,7 @@ __global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_cons
   const int blk = is_q ? blockIdx.x : blockIdx.x - p.q_blocks;
   const int n_blk = is_q ? p.q_blocks : (int)gridDim.x - p.q_blocks;
   float* sw = smem;
-  float2* tbl = reinterpret_cast<float2*>(smem + QN_MAX_D);
+  float* tbl = smem + QN_MAX_D;
   __shared__ int spos[QN_MAX_SLOTS];
   const int g = 1 << p.log_g, lane = threadIdx.x & (g - 1), grp = threadIdx.x >> p.log_g;
   const int n_grp = QN_THREADS >> p.log_g;
@@ -415,7 +500,7 @@ __global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_cons
   for (int tile = blk; tile < tiles; tile += n_blk) {
     const int t0 = tile * per_tile, n_tok = min(per_tile, p.T - t0);
     const int rows = n_tok * R.heads, iters = (rows + n_grp - 1) / n_grp;
-    Vec na[NP], nb[NP], ma[NP], mb[NP];  // x and dy of the next round
+    Vec na[NP] = {}, nb[NP] = {}, ma[NP] = {}, mb[NP] = {};  // x and dy of the next round; zeros beyond the row
     auto load = [&](int row) {
       if (row < rows) {
         const int tl = qn_token(R, row), h = row - tl * R.heads;
@@ -458,60 +543,57 @@ __global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_cons
       if (it + 1 < iters) load(row + n_grp);
       float a[NP][V], b[NP][V], da[NP][V], db[NP][V];
 #pragma unroll
-      for (int i = 0; i < NP; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          a[i][j] = live && ha[i] ? sb::to_f(va[i].e[j]) : 0.f;
-          b[i][j] = live && hb[i] ? sb::to_f(vb[i].e[j]) : 0.f;
-          da[i][j] = live && ha[i] ? sb::to_f(ya[i].e[j]) : 0.f;
-          db[i][j] = live && hb[i] ? sb::to_f(yb[i].e[j]) : 0.f;
-        }
+      for (int i = 0; i < NP; ++i) {
+        qn_unpack<T, V>(va[i], a[i]);
+        qn_unpack<T, V>(vb[i], b[i]);
+        qn_unpack<T, V>(ya[i], da[i]);
+        qn_unpack<T, V>(yb[i], db[i]);
+      }
       if (p.rot) {
 #pragma unroll
         for (int i = 0; i < NP; ++i)
-          qn_rotate<V>(da[i], db[i], tbl + tl * np * V, lane + i * g, np, p.rot, p.interleaved, -1.f);
+          qn_rotate<V, true>(da[i], db[i], tbl + tl * np * V * 2, lane + i * g, np, p.rot, p.interleaved);
       }
       float mu, r;
       qn_stats<V, NP>(a, b, ha, hb, D, RMS, p.eps, g, mu, r);
       float s1 = 0.f, s2 = 0.f;  // sums of g and of g * xhat
+      const bool keep = live;    // a group without a row repeats the row before: it counts once
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         float w[V];
-        if (ha[i]) {
-          qn_read_weights<V>(sw, ca[i], chunks, w);
+        auto chunk = [&](float (&x)[V], float (&dy)[V], float (&dw)[V], float (&dbias)[V], int c) {
+          if (!RMS) qn_shift<V>(x, -mu);
+          qn_scale<V>(x, r);
+          if (keep) {
+            qn_fma<V>(dw, dy, x, dw);
+            if (!RMS) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            a[i][j] = (a[i][j] - mu) * r;
-            if (live) dwa[i][j] = fmaf(da[i][j], a[i][j], dwa[i][j]);
-            if (!RMS) dba[i][j] += da[i][j];
-            da[i][j] *= w[j];
-            if (!RMS) s1 += da[i][j];
-            s2 = fmaf(da[i][j], a[i][j], s2);
+              for (int j = 0; j < V; ++j) dbias[j] += dy[j];
+            }
           }
-        }
-        if (hb[i]) {
-          qn_read_weights<V>(sw, cb[i], chunks, w);
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            b[i][j] = (b[i][j] - mu) * r;
-            if (live) dwb[i][j] = fmaf(db[i][j], b[i][j], dwb[i][j]);
-            if (!RMS) dbb[i][j] += db[i][j];
-            db[i][j] *= w[j];
-            if (!RMS) s1 += db[i][j];
-            s2 = fmaf(db[i][j], b[i][j], s2);
-          }
-        }
+          qn_read_weights<V>(sw, c, chunks, w);
+          qn_mul<V>(dy, dy, w);
+          if (!RMS) s1 += qn_total<V>(dy);
+          s2 += qn_dot<V>(dy, x);
+        };
+        if (ha[i]) chunk(a[i], da[i], dwa[i], dba[i], ca[i]);
+        if (hb[i]) chunk(b[i], db[i], dwb[i], dbb[i], cb[i]);
       }
       s2 = qn_group_sum(s2, g) / D;
       s1 = RMS ? 0.f : qn_group_sum(s1, g) / D;
       T* y = reinterpret_cast<T*>(R.y) + (long)(t0 + tl) * R.y_tok + (long)h * R.y_head;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          va[i].e[j] = sb::from_f<T>(r * (da[i][j] - s1 - a[i][j] * s2));
-          vb[i].e[j] = sb::from_f<T>(r * (db[i][j] - s1 - b[i][j] * s2));
+        if (!RMS) {
+          qn_shift<V>(da[i], -s1);
+          qn_shift<V>(db[i], -s1);
         }
+        qn_axpy<V>(da[i], a[i], -s2);
+        qn_axpy<V>(db[i], b[i], -s2);
+        qn_scale<V>(da[i], r);
+        qn_scale<V>(db[i], r);
+        qn_pack<T, V>(da[i], va[i]);
+        qn_pack<T, V>(db[i], vb[i]);
         if (live && ha[i]) *reinterpret_cast<Vec*>(y + ca[i] * V) = va[i];
         if (live && hb[i]) *reinterpret_cast<Vec*>(y + cb[i] * V) = vb[i];
       }
