@@ -223,14 +223,15 @@ __device__ __forceinline__ void qn_rotate(float (&a)[V], float (&b)[V], const fl
       qn_fma<V>(a, b, ns, a);
       qn_fma<V>(b, b, cs, x);
     } else {
+      const bool all = (c + 1) * 2 * V <= rot;
 #pragma unroll
       for (int i = 0; i < V / 2; ++i) {
-        if (2 * c * V + 2 * i < rot) {
+        if (all || 2 * c * V + 2 * i < rot) {
           const float x = a[2 * i], y = a[2 * i + 1];
           a[2 * i] = x * cs[i] - y * sn[i];
           a[2 * i + 1] = y * cs[i] + x * sn[i];
         }
-        if ((2 * c + 1) * V + 2 * i < rot) {
+        if (all || (2 * c + 1) * V + 2 * i < rot) {
           const float x = b[2 * i], y = b[2 * i + 1];
           b[2 * i] = x * cs[V / 2 + i] - y * sn[V / 2 + i];
           b[2 * i + 1] = y * cs[V / 2 + i] + x * sn[V / 2 + i];
@@ -240,8 +241,14 @@ __device__ __forceinline__ void qn_rotate(float (&a)[V], float (&b)[V], const fl
   }
 }
 
-__device__ __forceinline__ float qn_group_sum(float v, int g) {
-  for (int o = g >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+// Sum over the g = 2^LG lanes of a row (LG < 0: g known at run time only).
+template <int LG> __device__ __forceinline__ float qn_group_sum(float v, int g) {
+  if constexpr (LG >= 0) {
+#pragma unroll
+    for (int o = (1 << LG) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  } else {
+    for (int o = g >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  }
   return v;
 }
 
@@ -262,9 +269,9 @@ __device__ __forceinline__ void qn_fill_table(const QnParams& p, float* tbl, con
 }
 
 // Row statistics of x held as NP pairs; chunks beyond the row (ha / hb false) hold zeros.
-template <int V, int NP>
+template <int V, int NP, int LG>
 __device__ __forceinline__ void qn_stats(const float (&a)[NP][V], const float (&b)[NP][V], const bool (&ha)[NP],
-                                         const bool (&hb)[NP], int D, int rms, float eps, int g, float& mu, float& r) {
+                                         const bool (&hb)[NP], float inv_d, int rms, float eps, int g, float& mu, float& r) {
   mu = 0.f;
   float ss = 0.f;
   if (rms) {
@@ -274,7 +281,7 @@ __device__ __forceinline__ void qn_stats(const float (&a)[NP][V], const float (&
     float s = 0.f;
 #pragma unroll
     for (int p = 0; p < NP; ++p) s += qn_total<V>(a[p]) + qn_total<V>(b[p]);
-    mu = qn_group_sum(s, g) / D;
+    mu = qn_group_sum<LG>(s, g) * inv_d;
 #pragma unroll
     for (int p = 0; p < NP; ++p)  // around the mean, from registers: no cancellation
 #pragma unroll
@@ -284,12 +291,12 @@ __device__ __forceinline__ void qn_stats(const float (&a)[NP][V], const float (&
         ss = fmaf(db, db, ss);
       }
   }
-  r = rsqrtf(qn_group_sum(ss, g) / D + eps);
+  r = rsqrtf(fmaf(qn_group_sum<LG>(ss, g), inv_d, eps));
 }
 
 // ============================================================================ forward
 // One CTA per tile of tokens.  PAGED: k and v go to their slots of the cache, positions come from the sequence lengths.
-template <typename T, int V, int NP, bool PAGED>
+template <typename T, int V, int NP, int LG, bool PAGED>
 __global__ void __launch_bounds__(QN_THREADS, QN_FWD_BLOCKS) qn_fwd_kernel(const __grid_constant__ QnParams p) {
   extern __shared__ __align__(16) float smem[];
   using Vec = QnVec<T, V>;
@@ -299,8 +306,9 @@ __global__ void __launch_bounds__(QN_THREADS, QN_FWD_BLOCKS) qn_fwd_kernel(const
   __shared__ int spos[QN_MAX_SLOTS];
   __shared__ int spage[QN_MAX_SLOTS], sslot[QN_MAX_SLOTS];  // spage -1: nothing to write, -2: behind the last sequence
   const int t0 = blockIdx.x * p.tile, n_tok = min(p.tile, p.T - t0);
-  const int g = 1 << p.log_g, lane = threadIdx.x & (g - 1), grp = threadIdx.x >> p.log_g;
-  const int n_grp = QN_THREADS >> p.log_g;
+  const int log_g = LG >= 0 ? LG : p.log_g, g = 1 << log_g, lane = threadIdx.x & (g - 1), grp = threadIdx.x >> log_g;
+  const int n_grp = QN_THREADS >> log_g;
+  const float inv_d = 1.f / D;
 
   for (int i = threadIdx.x; i < D; i += QN_THREADS) {
     const int s = qn_weight_slot<V>(i, chunks);
@@ -344,145 +352,145 @@ __global__ void __launch_bounds__(QN_THREADS, QN_FWD_BLOCKS) qn_fwd_kernel(const
     ca[i] = c.a; cb[i] = c.b;
     ha[i] = c.a < chunks; hb[i] = c.b < chunks;
   }
-  // Rounds of the row groups over q, then k, then v; the loads of a round are issued a round ahead.
-  const int rounds[3] = {(n_tok * p.q.heads + n_grp - 1) / n_grp, (n_tok * p.k.heads + n_grp - 1) / n_grp,
-                         PAGED ? (n_tok * p.v.heads + n_grp - 1) / n_grp : 0};
-  const int first_k = rounds[0], first_v = first_k + rounds[1], total = first_v + rounds[2];
-  Vec na[NP] = {}, nb[NP] = {};  // chunks beyond the row stay zeros
-  auto load = [&](int it) {
-    const int kind = it < first_k ? 0 : it < first_v ? 1 : 2;
-    const QnRows& R = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
-    const int row = grp + (it - (kind == 0 ? 0 : kind == 1 ? first_k : first_v)) * n_grp;
-    if (row < n_tok * R.heads) {
-      const int tl = qn_token(R, row), h = row - tl * R.heads;
-      const T* x = reinterpret_cast<const T*>(R.x) + (long)(t0 + tl) * R.x_tok + (long)h * R.x_head;
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        if (ha[i]) na[i] = *reinterpret_cast<const Vec*>(x + ca[i] * V);
-        if (hb[i]) nb[i] = *reinterpret_cast<const Vec*>(x + cb[i] * V);
-      }
-    }
-  };
-  load(0);
   __syncthreads();
   if (p.rot) qn_fill_table<V>(p, tbl, spos, n_tok, np);
   __syncthreads();
-#pragma unroll 1
-  for (int it = 0; it < total; ++it) {  // the same trip count for every lane: the shuffles name all of them
-    const int kind = it < first_k ? 0 : it < first_v ? 1 : 2;
-    const QnRows& R = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
-    const int row = grp + (it - (kind == 0 ? 0 : kind == 1 ? first_k : first_v)) * n_grp;
-    const bool live = row < n_tok * R.heads;
-    const int tl = live ? qn_token(R, row) : 0, h = row - tl * R.heads;
-    const float* w = sw + kind * 2 * QN_MAX_D;
-    const float* bias = w + QN_MAX_D;
-    Vec va[NP], vb[NP];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      va[i] = na[i];
-      vb[i] = nb[i];
-    }
-    if (it + 1 < total) load(it + 1);
-    if (kind < 2 && (R.w || p.rot)) {  // else a copy, bit by bit
-      float a[NP][V], b[NP][V];
+  // The rows of q, then of k, then of v, each kind with its code (its addresses and strides are constants of the launch).
+  // The loads of a round of the row groups are issued a round ahead; weights stay in registers over the rounds.
+  auto all_rows = [&](auto kind_of, const QnRows& R) {
+    constexpr int kind = decltype(kind_of)::value;
+    const int rows = n_tok * R.heads;
+    const float* ws = sw + kind * 2 * QN_MAX_D;
+    const bool norm = kind < 2 && R.w;
+    float w1[NP][V], w2[NP][V];
+    if (norm) {
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        qn_unpack<T, V>(va[i], a[i]);
-        qn_unpack<T, V>(vb[i], b[i]);
+        if (ha[i]) qn_read_weights<V>(ws, ca[i], chunks, w1[i]);
+        if (hb[i]) qn_read_weights<V>(ws, cb[i], chunks, w2[i]);
       }
-      if (R.w) {
-        float mu, r;
-        qn_stats<V, NP>(a, b, ha, hb, D, p.rms, p.eps, g, mu, r);
+    }
+    Vec na[NP] = {}, nb[NP] = {};  // chunks beyond the row stay zeros
+    auto load = [&](int row) {
+      if (row < rows) {
+        const int tl = qn_token(R, row), h = row - tl * R.heads;
+        const T* x = reinterpret_cast<const T*>(R.x) + (long)(t0 + tl) * R.x_tok + (long)h * R.x_head;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          float t[V];
-          if (!p.rms) {
-            qn_shift<V>(a[i], -mu);
-            qn_shift<V>(b[i], -mu);
-          }
-          qn_scale<V>(a[i], r);
-          qn_scale<V>(b[i], r);
-          if (ha[i]) {
-            qn_read_weights<V>(w, ca[i], chunks, t);
-            qn_mul<V>(a[i], a[i], t);
-          }
-          if (hb[i]) {
-            qn_read_weights<V>(w, cb[i], chunks, t);
-            qn_mul<V>(b[i], b[i], t);
-          }
-          if (R.b) {
-            if (ha[i]) {
-              qn_read_weights<V>(bias, ca[i], chunks, t);
+          if (ha[i]) na[i] = *reinterpret_cast<const Vec*>(x + ca[i] * V);
+          if (hb[i]) nb[i] = *reinterpret_cast<const Vec*>(x + cb[i] * V);
+        }
+      }
+    };
+    load(grp);
+#pragma unroll 1
+    for (int base = 0; base < rows; base += n_grp) {  // the same trip count for every lane: the shuffles name all of them
+      const int row = base + grp;
+      const bool live = row < rows;
+      const int tl = live ? qn_token(R, row) : 0, h = row - tl * R.heads;
+      Vec va[NP], vb[NP];
 #pragma unroll
-              for (int j = 0; j < V; ++j) a[i][j] += t[j];
+      for (int i = 0; i < NP; ++i) {
+        va[i] = na[i];
+        vb[i] = nb[i];
+      }
+      load(row + n_grp);
+      if (norm || (kind < 2 && p.rot)) {  // else a copy, bit by bit
+        float a[NP][V], b[NP][V];
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          qn_unpack<T, V>(va[i], a[i]);
+          qn_unpack<T, V>(vb[i], b[i]);
+        }
+        if (norm) {
+          float mu, r;
+          qn_stats<V, NP, LG>(a, b, ha, hb, inv_d, p.rms, p.eps, g, mu, r);
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            if (!p.rms) {
+              qn_shift<V>(a[i], -mu);
+              qn_shift<V>(b[i], -mu);
             }
-            if (hb[i]) {
-              qn_read_weights<V>(bias, cb[i], chunks, t);
+            qn_scale<V>(a[i], r);
+            qn_scale<V>(b[i], r);
+            if (ha[i]) qn_mul<V>(a[i], a[i], w1[i]);
+            if (hb[i]) qn_mul<V>(b[i], b[i], w2[i]);
+            if (R.b) {
+              float t[V];
+              if (ha[i]) {
+                qn_read_weights<V>(ws + QN_MAX_D, ca[i], chunks, t);
 #pragma unroll
-              for (int j = 0; j < V; ++j) b[i][j] += t[j];
+                for (int j = 0; j < V; ++j) a[i][j] += t[j];
+              }
+              if (hb[i]) {
+                qn_read_weights<V>(ws + QN_MAX_D, cb[i], chunks, t);
+#pragma unroll
+                for (int j = 0; j < V; ++j) b[i][j] += t[j];
+              }
             }
           }
         }
-      }
-      if (p.rot) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i)
-          qn_rotate<V, false>(a[i], b[i], tbl + tl * np * V * 2, lane + i * g, np, p.rot, p.interleaved);
-      }
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        qn_pack<T, V>(a[i], va[i]);
-        qn_pack<T, V>(b[i], vb[i]);
-      }
-    }
-    T* y = reinterpret_cast<T*>(R.y);
-    bool store = live;
-    if (PAGED && live) {
-      const int page = spage[tl];
-      if (kind == 0) {
-        y += (long)(t0 + tl) * R.y_tok + (long)h * R.y_head;
-        if (page == -2) {  // behind the last sequence: zeros
+        if (p.rot) {
 #pragma unroll
           for (int i = 0; i < NP; ++i)
-#pragma unroll
-            for (int j = 0; j < V; ++j) va[i].e[j] = vb[i].e[j] = sb::from_f<T>(0.f);
+            qn_rotate<V, false>(a[i], b[i], tbl + tl * np * V * 2, lane + i * g, np, p.rot, p.interleaved);
         }
-      } else {
-        store = page >= 0;
-        y += (long)page * (kind == 1 ? p.k_page : p.v_page) + (long)sslot[tl] * (kind == 1 ? p.k_slot : p.v_slot) +
-             (long)h * R.y_head;
-      }
-    } else if (live) {
-      y += (long)(t0 + tl) * R.y_tok + (long)h * R.y_head;
-    }
-    if (store) {
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        if (ha[i]) *reinterpret_cast<Vec*>(y + ca[i] * V) = va[i];
-        if (hb[i]) *reinterpret_cast<Vec*>(y + cb[i] * V) = vb[i];
+        for (int i = 0; i < NP; ++i) {
+          qn_pack<T, V>(a[i], va[i]);
+          qn_pack<T, V>(b[i], vb[i]);
+        }
+      }
+      T* y = reinterpret_cast<T*>(R.y);
+      bool store = live;
+      if (PAGED && live) {
+        const int page = spage[tl];
+        if (kind == 0) {
+          y += (long)(t0 + tl) * R.y_tok + (long)h * R.y_head;
+          if (page == -2) {  // behind the last sequence: zeros
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+#pragma unroll
+              for (int j = 0; j < V; ++j) va[i].e[j] = vb[i].e[j] = sb::from_f<T>(0.f);
+          }
+        } else {
+          store = page >= 0;
+          y += (long)page * (kind == 1 ? p.k_page : p.v_page) + (long)sslot[tl] * (kind == 1 ? p.k_slot : p.v_slot) +
+               (long)h * R.y_head;
+        }
+      } else if (live) {
+        y += (long)(t0 + tl) * R.y_tok + (long)h * R.y_head;
+      }
+      if (store) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          if (ha[i]) *reinterpret_cast<Vec*>(y + ca[i] * V) = va[i];
+          if (hb[i]) *reinterpret_cast<Vec*>(y + cb[i] * V) = vb[i];
+        }
       }
     }
-  }
+  };
+  all_rows(std::integral_constant<int, 0>(), p.q);
+  all_rows(std::integral_constant<int, 1>(), p.k);
+  if constexpr (PAGED) all_rows(std::integral_constant<int, 2>(), p.v);
 }
 
 // ============================================================================ backward
 // A block takes either q or k, walks over tiles of tokens and keeps its share of dw and db in registers (each lane owns
 // the same chunks in every row); the block's sums go to one row of `partial`, added up in a fixed order afterwards.
 // RMS: no mean, and no biases whose gradients would have to be kept.
-template <typename T, int V, int NP, bool RMS>
-__global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_constant__ QnParams p) {
+template <typename T, int V, int NP, int LG, bool RMS>
+__device__ __forceinline__ void qn_bwd_rows(const QnParams& p, const QnRows& R, const int blk, const int n_blk,
+                                            const int per_tile) {
   extern __shared__ __align__(16) float smem[];
   using Vec = QnVec<T, V>;
   const int D = p.D, chunks = (D + V - 1) / V, np = (p.rot + 2 * V - 1) / (2 * V);
-  const bool is_q = (int)blockIdx.x < p.q_blocks;
-  const QnRows& R = is_q ? p.q : p.k;
-  const int blk = is_q ? blockIdx.x : blockIdx.x - p.q_blocks;
-  const int n_blk = is_q ? p.q_blocks : (int)gridDim.x - p.q_blocks;
   float* sw = smem;
   float* tbl = smem + QN_MAX_D;
   __shared__ int spos[QN_MAX_SLOTS];
-  const int g = 1 << p.log_g, lane = threadIdx.x & (g - 1), grp = threadIdx.x >> p.log_g;
-  const int n_grp = QN_THREADS >> p.log_g;
+  const int log_g = LG >= 0 ? LG : p.log_g, g = 1 << log_g, lane = threadIdx.x & (g - 1), grp = threadIdx.x >> log_g;
+  const int n_grp = QN_THREADS >> log_g;
+  const float inv_d = 1.f / D;
   for (int i = threadIdx.x; i < D; i += QN_THREADS) sw[qn_weight_slot<V>(i, chunks)] = qn_load_any(R.w, i, p.w_dtype);
   int ca[NP], cb[NP];
   bool ha[NP], hb[NP];
@@ -495,7 +503,7 @@ __global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_cons
 #pragma unroll
     for (int j = 0; j < V; ++j) dwa[i][j] = dwb[i][j] = dba[i][j] = dbb[i][j] = 0.f;
   }
-  const int per_tile = is_q ? p.tile : p.tile_k, tiles = (p.T + per_tile - 1) / per_tile;
+  const int tiles = (p.T + per_tile - 1) / per_tile;
 #pragma unroll 1
   for (int tile = blk; tile < tiles; tile += n_blk) {
     const int t0 = tile * per_tile, n_tok = min(per_tile, p.T - t0);
@@ -555,7 +563,7 @@ __global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_cons
           qn_rotate<V, true>(da[i], db[i], tbl + tl * np * V * 2, lane + i * g, np, p.rot, p.interleaved);
       }
       float mu, r;
-      qn_stats<V, NP>(a, b, ha, hb, D, RMS, p.eps, g, mu, r);
+      qn_stats<V, NP, LG>(a, b, ha, hb, inv_d, RMS, p.eps, g, mu, r);
       float s1 = 0.f, s2 = 0.f;  // sums of g and of g * xhat
       const bool keep = live;    // a group without a row repeats the row before: it counts once
 #pragma unroll
@@ -579,8 +587,8 @@ __global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_cons
         if (ha[i]) chunk(a[i], da[i], dwa[i], dba[i], ca[i]);
         if (hb[i]) chunk(b[i], db[i], dwb[i], dbb[i], cb[i]);
       }
-      s2 = qn_group_sum(s2, g) / D;
-      s1 = RMS ? 0.f : qn_group_sum(s1, g) / D;
+      s2 = qn_group_sum<LG>(s2, g) * inv_d;
+      s1 = RMS ? 0.f : qn_group_sum<LG>(s1, g) * inv_d;
       T* y = reinterpret_cast<T*>(R.y) + (long)(t0 + tl) * R.y_tok + (long)h * R.y_head;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
@@ -629,6 +637,13 @@ __global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_cons
     for (int wp = 0; wp < QN_THREADS / 32; ++wp) s += red[wp * 2 * QN_MAX_D + which * QN_MAX_D + e];
     p.partial[(size_t)blockIdx.x * 2 * D + i] = s;
   }
+}
+
+template <typename T, int V, int NP, int LG, bool RMS>
+__global__ void __launch_bounds__(QN_THREADS, 2) qn_bwd_kernel(const __grid_constant__ QnParams p) {
+  // code of its own for q and for k: addresses and strides are constants of the launch
+  if ((int)blockIdx.x < p.q_blocks) qn_bwd_rows<T, V, NP, LG, RMS>(p, p.q, blockIdx.x, p.q_blocks, p.tile);
+  else qn_bwd_rows<T, V, NP, LG, RMS>(p, p.k, blockIdx.x - p.q_blocks, gridDim.x - p.q_blocks, p.tile_k);
 }
 
 // Sums of the blocks' partial rows: blockIdx.y = 0 q, 1 k; 32 columns per block (of 2 D: dw then db), 32 row lanes.
@@ -709,9 +724,11 @@ static int qn_launch_fwd(QnParams& p, bool paged, long align, double base, int s
   const int grid = (p.T + tile - 1) / tile;
   auto launch = [&](auto paged_form) {
     constexpr bool PAGED = decltype(paged_form)::value;
-    if (V == VF) qn_fwd_kernel<T, VF, 1, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
-    else if (V == 2) qn_fwd_kernel<T, 2, 2, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
-    else qn_fwd_kernel<T, 1, 4, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
+    if (V == VF && p.log_g == 2) qn_fwd_kernel<T, VF, 1, 2, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
+    else if (V == VF && p.log_g == 3) qn_fwd_kernel<T, VF, 1, 3, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
+    else if (V == VF) qn_fwd_kernel<T, VF, 1, -1, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
+    else if (V == 2) qn_fwd_kernel<T, 2, 2, -1, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
+    else qn_fwd_kernel<T, 1, 4, -1, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
   };
   if (paged) launch(std::true_type());
   else launch(std::false_type());
@@ -801,9 +818,11 @@ static int qn_launch_bwd(QnParams& p, long align, double base, int blocks, cudaS
   if (smem < red) smem = red;
   auto launch = [&](auto rms_form) {
     constexpr bool RMS = decltype(rms_form)::value;
-    if (V == VF) qn_bwd_kernel<T, VF, 1, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
-    else if (V == 2) qn_bwd_kernel<T, 2, 2, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
-    else qn_bwd_kernel<T, 1, 4, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
+    if (V == VF && p.log_g == 2) qn_bwd_kernel<T, VF, 1, 2, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
+    else if (V == VF && p.log_g == 3) qn_bwd_kernel<T, VF, 1, 3, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
+    else if (V == VF) qn_bwd_kernel<T, VF, 1, -1, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
+    else if (V == 2) qn_bwd_kernel<T, 2, 2, -1, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
+    else qn_bwd_kernel<T, 1, 4, -1, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
   };
   if (p.rms) launch(std::true_type());
   else launch(std::false_type());
