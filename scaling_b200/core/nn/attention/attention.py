@@ -329,7 +329,11 @@ class ParallelSelfAttention(torch.nn.Module):
         npp = self.num_attention_heads_per_partition
         if self.qkv_in_one:
             qkv = self.query_key_value(x).view(T, npp, 3 * d)
-            q, k, v = qkv[..., :d], qkv[..., d:2 * d], qkv[..., 2 * d:]
+            if self.key_query_norm:
+                # the same views, but their gradients come back as one stack instead of three sums with padded zeros
+                q, k, v = qkv.view(T, npp, 3, d).unbind(2)
+            else:
+                q, k, v = qkv[..., :d], qkv[..., d:2 * d], qkv[..., 2 * d:]
         else:
             q = self.query(x).view(T, npp, d)
             x_kv = x
@@ -374,6 +378,24 @@ class ParallelSelfAttention(torch.nn.Module):
             return all_shard(norm(full).transpose(1, 2), self.topology).transpose(1, 2)
         return norm(t)
 
+    def _head_norm_fused(self, q: torch.Tensor) -> bool:
+        """Norms and rotation of queries and keys run as one kernel: on the GPU, with plain norm modules (no u-muP scales,
+        no hooks that want to see their outputs) and all heads on this rank."""
+        norms = (self.norm_query, self.norm_key)
+        return (q.is_cuda and self.model_parallel_size == 1 and q.dtype in (torch.bfloat16, torch.float16, torch.float32)
+                and q.shape[-1] <= 256 and q.numel() > 0
+                and (self.rotary_embedding is None or self.rotary_embedding.dimensions % 2 == 0)
+                and not any(n._use_umup or n._forward_hooks or n._forward_pre_hooks for n in norms))
+
+    def _head_norm_and_rotary(self, q: torch.Tensor, k: torch.Tensor,
+                              pos: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+        nq, nk, rot = self.norm_query, self.norm_key, self.rotary_embedding
+        rms = isinstance(nq, RMSNorm)
+        bias = (lambda n: None) if rms else (lambda n: getattr(n, n.bias_name))
+        rotary = None if rot is None else (rot.dimensions, rot.base, rot.interleaved)
+        return K.qk_norm_rope(q, k, nq.weight, nk.weight, q_bias=bias(nq), k_bias=bias(nk), positions=pos, rotary=rotary,
+                              eps=nq.config.layernorm_epsilon, rms=rms)
+
     # ------------------------------------------------------------------ forward
     def forward(self, x: torch.Tensor, cumulative_seq_lengths: Optional[torch.Tensor],
                 position_ids: Optional[torch.Tensor],
@@ -395,16 +417,23 @@ class ParallelSelfAttention(torch.nn.Module):
             return self._output_projection(hidden)
         q, k, v = self._project_qkv(x)
 
-        if self.key_query_norm:
-            assert self.norm_query is not None and self.norm_key is not None
-            q = self._qk_norm(q, self.norm_query)
-            k = self._qk_norm(k, self.norm_key)
-
+        pos = None
         if self.rotary_embedding is not None:
             if position_ids is not None:
                 pos = position_ids.reshape(-1)
             else:
                 pos = torch.arange(s, device=x.device, dtype=torch.int32).repeat(b)
+        fused = False
+        if self.key_query_norm:
+            assert self.norm_query is not None and self.norm_key is not None
+            fused = self._head_norm_fused(q)
+            if fused:
+                q, k = self._head_norm_and_rotary(q, k, pos)
+            else:
+                q = self._qk_norm(q, self.norm_query)
+                k = self._qk_norm(k, self.norm_key)
+
+        if self.rotary_embedding is not None and not fused:
             rot = self.rotary_embedding
             q = apply_rotary_tokens(q, pos, rot.dimensions, rot.base, rot.interleaved)
             k = apply_rotary_tokens(k, pos, rot.dimensions, rot.base, rot.interleaved)

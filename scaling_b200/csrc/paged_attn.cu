@@ -50,12 +50,9 @@ constexpr int PA_PANEL = 16384;   // 128 rows x 128 bytes
 constexpr int PA_ITEMS = 4;       // descriptors in flight
 constexpr int PA_COMBINE_THREADS = 256;
 constexpr unsigned long long PA_WAIT_NS = 4000000000ull;
-// What the start and the end of an item cost, in tiles: added to its length on the work line.
-constexpr int PA_WIDE_COST = 2, PA_NARROW_COST = 2;
 // ROWS (rows per item) tells the kernels apart in the functions that they share.
 template <int ROWS> struct PaKind {
   static constexpr bool NARROW = ROWS <= PA_NARROW_ROWS;
-  static constexpr int COST = NARROW ? PA_NARROW_COST : PA_WIDE_COST;
   static constexpr int SLOT_ROWS = NARROW ? ROWS : PA_TILE;  // rows per query slot
 };
 
@@ -75,6 +72,8 @@ struct PaParams {
   int boxes, k_page8, v_page8, k_outside, v_outside;
   int causal, window;  // window < 0: unlimited
   int narrow_max;      // sequences with at most this many rows belong to the narrow kernel
+  int cost;            // what the start and the end of an item cost, in tiles: added to its length on the work line
+  int whole;           // items count as one each and are not divided
   float sl2;
   float* part_o;       // [2 slots per CTA][part_rows][DP]
   float2* part_ml;     // [2 slots per CTA][part_rows]: reference (log2 domain) and sum
@@ -253,9 +252,10 @@ template <int ROWS> __device__ __forceinline__ void pa_item_keys(const PaParams&
 __device__ __forceinline__ int pa_tiles(int lo, int hi) { return max((hi + PA_TILE - 1) / PA_TILE - lo / PA_TILE, 1); }
 // length of item m on the line
 template <int ROWS> __device__ __forceinline__ int pa_item_cost(const PaParams& p, int n, int L, int m) {
+  if (p.whole) return 1;
   int lo, hi;
   pa_item_keys<ROWS>(p, n, L, m, lo, hi);
-  return pa_tiles(lo, hi) + PaKind<ROWS>::COST;
+  return pa_tiles(lo, hi) + p.cost;
 }
 // items of a sequence of n new tokens in this kernel, per KV head
 template <int ROWS> __device__ __forceinline__ int pa_items(const PaParams& p, int n) {
@@ -330,7 +330,7 @@ __device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int 
   PaCut& cut = c.cut;
   const int total = (int)all;
   // two tiles per CTA at least, one for each softmax group
-  cut.ctas = min((int)gridDim.x, (total + 1) / (2 + PaKind<ROWS>::COST));
+  cut.ctas = min((int)gridDim.x, p.whole ? total : (total + 1) / (2 + p.cost));
   if (total > 0) cut.ctas = max(cut.ctas, 1);
   if ((int)blockIdx.x >= cut.ctas) return;
   cut.per = total / cut.ctas;
@@ -388,7 +388,7 @@ template <int ROWS> __device__ __forceinline__ int pa_lead(int rows) { return Pa
 template <int ROWS, int PANELS>
 __device__ __forceinline__ void pa_schedule(const PaParams& p, PaCtrl<PaCfg<PANELS>::STAGES>& c, uint8_t* sQ, int chunks,
                                             int lane) {
-  constexpr int DP = PANELS * 64, COST = PaKind<ROWS>::COST;
+  constexpr int DP = PANELS * 64;
   constexpr int SLOT_ROWS = PaKind<ROWS>::SLOT_ROWS, SLOT_BYTES = PANELS * SLOT_ROWS * 128;
   volatile int* abort_flag = &c.abort;
   PaCursor cur;
@@ -406,7 +406,7 @@ __device__ __forceinline__ void pa_schedule(const PaParams& p, PaCtrl<PaCfg<PANE
       pa_item_keys<ROWS>(p, cur.s.n, cur.s.L, cur.m, lo, hi);
       tiles = pa_tiles(lo, hi);
       if (cur.tile < tiles) {
-        const int take = min(tiles - cur.tile, cur.left);
+        const int take = p.whole ? tiles : min(tiles - cur.tile, cur.left);
         const bool first = cur.tile == 0, last = cur.tile + take == tiles;
         const int tok0 = cur.m * ROWS / p.group;
         it = PaItem{cur.s.row0 + tok0, cur.s.L - cur.s.n + tok0, cur.s.L, cur.seq, cur.hk,
@@ -421,7 +421,7 @@ __device__ __forceinline__ void pa_schedule(const PaParams& p, PaCtrl<PaCfg<PANE
           }
         }
       }
-      const int used = min(tiles + COST - cur.tile, cur.left);
+      const int used = p.whole ? 1 : min(tiles + p.cost - cur.tile, cur.left);
       cur.left -= used;
       cur.place += used;
       cur.tile = 0;
@@ -946,6 +946,16 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     pa_load<R, PANELS, true, false>(p, c, sRing, &tmK, &tmV, lane);
   } else if (warp == 11) {
     pa_load<R, PANELS, false, true>(p, c, sRing, &tmK, &tmV, lane);
+    if (p.zero_tail) {  // rows behind the last sequence
+      const long first = p.batch > 0 ? min(max(p.cu[p.batch], 0), p.T) : 0, heads = (long)p.Hkv * p.group;
+      const int per_row = p.D / 8;
+      for (long row = first * heads + blockIdx.x; row < p.T * heads; row += gridDim.x) {
+        const long t = row / heads;
+        if (lane < per_row)
+          *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + t * p.o_tok + (row - t * heads) * p.o_head + lane * 8) =
+              make_uint4(0, 0, 0, 0);
+      }
+    }
   } else if (warp == 9) {
     if (lane == 0) {
       const uint64_t q_desc = sb::umma_smem_desc(sb::smem_u32(sQ), 16, 1024);
@@ -1261,15 +1271,6 @@ __global__ void __launch_bounds__(PA_COMBINE_THREADS, 4)
   __shared__ int swarp[WARPS];
   __shared__ int stask[3];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (pn.zero_tail) {  // rows behind the last sequence
-    const long first = pn.batch > 0 ? min(max(pn.cu[pn.batch], 0), pn.T) : 0, heads = (long)pn.Hkv * pn.group;
-    const long chunks = (pn.T - first) * heads * (pn.D / 8);
-    for (long c = (long)blockIdx.x * PA_COMBINE_THREADS + threadIdx.x; c < chunks; c += (long)gridDim.x * PA_COMBINE_THREADS) {
-      const long row = c / (pn.D / 8), t = row / heads;
-      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(pn.out) + (first + t) * pn.o_tok + (row - t * heads) * pn.o_head +
-                                (c - row * (pn.D / 8)) * 8) = make_uint4(0, 0, 0, 0);
-    }
-  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int quad = threadIdx.x % QUADS, pg = threadIdx.x / QUADS;
   int before = 0;  // tasks of the descriptors before `base`
@@ -1389,10 +1390,10 @@ int pa_tmap(CUtensorMap* m, const void* base, int D, int heads, int page_size, i
 }
 
 // CTAs of a launch: one per SM, fewer when not even the table's full length gives each of them two key tiles
-long pa_ctas(long T, int batch, int Hq, int Hkv, long cap, int item_rows, int sms) {
+long pa_ctas(long T, int batch, int Hq, int Hkv, long cap, int item_rows, bool whole, int sms) {
   const long items = (T * (Hq / Hkv) + item_rows - 1) / item_rows + batch;
   const long tiles = (cap + PA_TILE - 1) / PA_TILE + 1;
-  const long want = (items * Hkv * tiles + 1) / 2;
+  const long want = whole ? items * Hkv : (items * Hkv * tiles + 1) / 2;
   return want < 1 ? 1 : want < sms ? want : sms;
 }
 long pa_align(long v) { return (v + 255) & ~255L; }
@@ -1401,7 +1402,7 @@ long pa_align(long v) { return (v + 255) & ~255L; }
 // head) are narrow; with no more new tokens than sequences, as in a decoding step, all of them are, whatever their length:
 // the second launch then finds nothing (3 us), and a sequence that does have more rows is read once per 64 of them.
 struct PaPlan {
-  bool wide;
+  bool wide, whole;
   int narrow_max, narrow_rows, narrow_ctas, wide_ctas;
   long narrow_at, wide_at, bytes;
 };
@@ -1409,10 +1410,12 @@ PaPlan pa_plan(long T, int batch, int Hq, int Hkv, int D, long cap, int sms) {
   PaPlan w = {};
   const long rows = T * (Hq / Hkv), dp = D <= 64 ? 64 : 128;
   w.wide = rows > PA_NARROW_ROWS && T > batch;
+  // with up to eight tiles per item, dividing them costs more (a second launch, partial results) than it balances
+  w.whole = !w.wide && cap <= 8 * PA_TILE;
   w.narrow_max = w.wide ? PA_NARROW_ROWS : 0x7fffffff;
   w.narrow_rows = (int)(rows < PA_NARROW_ROWS ? rows : PA_NARROW_ROWS);
-  w.narrow_ctas = (int)pa_ctas(T, batch, Hq, Hkv, cap, PA_NARROW_ROWS, sms);
-  w.wide_ctas = w.wide ? (int)pa_ctas(T, batch, Hq, Hkv, cap, PA_WIDE_ROWS, sms) : 0;
+  w.narrow_ctas = (int)pa_ctas(T, batch, Hq, Hkv, cap, PA_NARROW_ROWS, w.whole, sms);
+  w.wide_ctas = w.wide ? (int)pa_ctas(T, batch, Hq, Hkv, cap, PA_WIDE_ROWS, false, sms) : 0;
   auto size = [&](long ctas, long r) { return pa_align(2 * ctas * r * dp * 4) + pa_align(2 * ctas * r * 8) + pa_align(ctas * 32); };
   w.narrow_at = 0;
   w.wide_at = size(w.narrow_ctas, w.narrow_rows);
@@ -1443,7 +1446,11 @@ int pa_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, PaParams p, const 
     if (dev < 64) set[dev] = true;
   }
   p.narrow_max = w.narrow_max;
+  p.whole = w.whole;
   PaParams pn = p, pw = p;
+  // measured 3 to 4 us per item, and 0.7 us per tile and 64 columns of the head; with 64 columns a mixed batch of 24
+  // sequences took 61 / 54 / 63 us at a cost of 2 / 4 / 8
+  pn.cost = pw.cost = PANELS == 1 ? 4 : 2;
   pa_place(&pn, ws + w.narrow_at, w.narrow_ctas, w.narrow_rows, PaCfg<PANELS>::DP);
   if (w.wide) {
     pa_place(&pw, ws + w.wide_at, w.wide_ctas, PA_WIDE_ROWS, PaCfg<PANELS>::DP);
@@ -1464,6 +1471,7 @@ int pa_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, PaParams p, const 
   cfg.numAttrs = w.wide ? 1 : 0;
   e = cudaLaunchKernelEx(&cfg, pa_narrow_kernel<PANELS, F16>, tmK, tmV, pn);
   if (e != cudaSuccess) return (int)e;
+  if (w.whole) return SB_OK;
   const int ctas = w.narrow_ctas + w.wide_ctas;
   cfg.gridDim = dim3(w.wide || ctas >= 128 ? 4 * 148 : 4 * ctas);
   cfg.blockDim = dim3(PA_COMBINE_THREADS);

@@ -1,0 +1,105 @@
+"""Self-attention with norms of queries and keys: norms and rotation in one kernel against the separate operations."""
+
+import pytest
+import torch
+
+from scaling_b200.core.nn.attention import ParallelSelfAttention
+from scaling_b200.core.nn.attention.attention import RelativePositionEmbeddingType
+from scaling_b200.core.nn.masked_softmax import MaskedSoftmaxConfig
+from scaling_b200.core.nn.norm import LayerNormConfig, NormType
+from scaling_b200.core.nn.rotary import RotaryConfig
+from scaling_b200.ops import functional as K
+
+
+def _attention(norm_type, device, dtype, heads=4, kv_heads=None, rotary="rotary", rot_dims=64, seed=0):
+    torch.manual_seed(seed)
+    kind = RelativePositionEmbeddingType(rotary)
+    m = ParallelSelfAttention(
+        hidden_size=64 * heads, num_attention_heads=heads, masked_softmax_config=MaskedSoftmaxConfig(kernel="flash_attention"),
+        rotary_config=RotaryConfig(dimensions=rot_dims), relative_position_embedding_type=kind, device=torch.device(device),
+        dtype=dtype, norm_type=norm_type, key_query_norm=True, layernorm_config=LayerNormConfig(),
+        qkv_in_one=kv_heads is None, num_kv_heads=kv_heads)
+    with torch.no_grad():
+        for n, p in m.named_parameters():
+            if n.startswith("norm_"):
+                p.add_(0.2 * torch.randn_like(p))
+    return m
+
+
+def _step(m, x, cu, pos):
+    for p in m.parameters():
+        p.grad = None
+    xi = x.detach().requires_grad_()
+    y = m(xi, cu, pos)
+    y.backward(torch.linspace(-1, 1, y.numel(), device=y.device).view_as(y).to(y.dtype))
+    return y.detach(), xi.grad, {n: p.grad for n, p in m.named_parameters()}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("norm_type", [NormType.RMS, NormType.LAYERNORM])
+@pytest.mark.parametrize("kv_heads,rotary,rot_dims", [(None, "rotary", 64), (2, "rotary_complex", 64), (None, "rotary", 16), (1, "none", 64)])
+def test_attention_with_head_norms_in_one_kernel(norm_type, kv_heads, rotary, rot_dims, monkeypatch):
+    dev = "cuda"
+    m = _attention(norm_type, dev, torch.bfloat16, kv_heads=kv_heads, rotary=rotary, rot_dims=rot_dims)
+    x = torch.randn(2, 40, 256, device=dev).bfloat16()
+    cu = torch.tensor([0, 25, 40, 80], dtype=torch.int32, device=dev)
+    pos = torch.arange(40, device=dev).repeat(2, 1)
+    calls = []
+    real = K.qk_norm_rope
+    monkeypatch.setattr(K, "qk_norm_rope", lambda *a, **k: (calls.append(1), real(*a, **k))[1])
+    fused = _step(m, x, cu, pos)
+    assert len(calls) == 1
+    monkeypatch.setattr(ParallelSelfAttention, "_head_norm_fused", lambda self, q: False)
+    separate = _step(m, x, cu, pos)
+    assert len(calls) == 1
+    # Both against the same module in fp32 on the CPU.  All roundings of the fused form are also made by the separate one
+    # (which makes two more per element and pass), so its distance is of the same size or smaller; a factor of two leaves
+    # room for the signs in which they happen to add up.  (The distance of the two from each other has no bound in terms of
+    # the result: the weights' gradients are sums in which large terms cancel.)
+    ref = _attention(norm_type, "cpu", torch.float32, kv_heads=kv_heads, rotary=rotary, rot_dims=rot_dims)
+    ref.load_state_dict({n: t.float().cpu() for n, t in m.state_dict().items()})
+    want = _step(ref, x.float().cpu(), cu.cpu(), pos.cpu())
+    triples = [(fused[0], separate[0], want[0]), (fused[1], separate[1], want[1])]
+    triples += [(fused[2][n], separate[2][n], want[2][n]) for n in fused[2]]
+    for a, b, w in triples:
+        assert (a is None) == (b is None) == (w is None)
+        if a is not None:
+            dist = lambda t: (t.float().cpu() - w).norm().item()  # noqa: E731
+            assert dist(a) <= 2.0 * dist(b) + 2.0 ** -8 * w.norm().item()
+
+
+@pytest.mark.gpu
+def test_hooks_on_the_norms_still_see_their_outputs():
+    m = _attention(NormType.RMS, "cuda", torch.bfloat16)
+    seen = []
+    handle = m.norm_query.register_forward_hook(lambda mod, args, out: seen.append(out.shape))
+    x = torch.randn(1, 16, 256, device="cuda").bfloat16()
+    cu = torch.tensor([0, 16], dtype=torch.int32, device="cuda")
+    a = m(x, cu, None)
+    handle.remove()
+    b = m(x, cu, None)
+    assert seen == [(16, 4, 64)]
+    assert (a.float() - b.float()).norm() <= 4 * 2.0 ** -8 * b.float().norm()
+
+
+def test_separate_operations_on_the_cpu():
+    m = _attention(NormType.LAYERNORM, "cpu", torch.float32)
+    x = torch.randn(2, 10, 256)
+    cu = torch.tensor([0, 10, 20], dtype=torch.int32)
+    y, dx, grads = _step(m, x, cu, None)
+    assert y.shape == x.shape and torch.isfinite(dx).all()
+    assert all(g is not None and torch.isfinite(g).all() for g in grads.values())
+
+
+@pytest.mark.gpu
+def test_cached_generation_step_uses_the_same_kernel():
+    """A prompt and then single tokens through the module's cache equal the whole sequence at once."""
+    m = _attention(NormType.RMS, "cuda", torch.bfloat16)
+    x = torch.randn(1, 21, 256, device="cuda").bfloat16()
+    cu = lambda n: torch.tensor([0, n], dtype=torch.int32, device="cuda")  # noqa: E731
+    with torch.no_grad():
+        whole = m(x, cu(21), None)
+        parts = [m(x[:, :20], cu(20), torch.arange(20, device="cuda")[None], use_cache=True, reset_cache=True),
+                 m(x[:, 20:], cu(1), torch.tensor([[20]], device="cuda"), use_cache=True)]
+    got = torch.cat(parts, 1)
+    assert (got.float() - whole.float()).norm() <= 4 * 2.0 ** -8 * whole.float().norm()
