@@ -223,25 +223,30 @@ __device__ __forceinline__ void qn_rotate(float (&a)[V], float (&b)[V], const fl
       qn_fma<V>(a, b, ns, a);
       qn_fma<V>(b, b, cs, x);
     } else {
-      const bool all = (c + 1) * 2 * V <= rot;
+      auto turn = [&](float (&z)[V], int i, int j) {
+        const float x = z[2 * i], y = z[2 * i + 1];
+        z[2 * i] = x * cs[j] - y * sn[j];
+        z[2 * i + 1] = y * cs[j] + x * sn[j];
+      };
+      if (rot % (2 * V) == 0) {  // whole chunks
 #pragma unroll
-      for (int i = 0; i < V / 2; ++i) {
-        if (all || 2 * c * V + 2 * i < rot) {
-          const float x = a[2 * i], y = a[2 * i + 1];
-          a[2 * i] = x * cs[i] - y * sn[i];
-          a[2 * i + 1] = y * cs[i] + x * sn[i];
+        for (int i = 0; i < V / 2; ++i) {
+          turn(a, i, i);
+          turn(b, i, V / 2 + i);
         }
-        if (all || (2 * c + 1) * V + 2 * i < rot) {
-          const float x = b[2 * i], y = b[2 * i + 1];
-          b[2 * i] = x * cs[V / 2 + i] - y * sn[V / 2 + i];
-          b[2 * i + 1] = y * cs[V / 2 + i] + x * sn[V / 2 + i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+          if (2 * c * V + 2 * i < rot) turn(a, i, i);
+          if ((2 * c + 1) * V + 2 * i < rot) turn(b, i, V / 2 + i);
         }
       }
     }
   }
 }
 
-// Sum over the g = 2^LG lanes of a row (LG < 0: g known at run time only).
+// LG >= 0: a row is exactly 2^LG lanes with both chunks, known when compiling (heads of 64 and 128); else anything.
+// Sum over the g lanes of a row.
 template <int LG> __device__ __forceinline__ float qn_group_sum(float v, int g) {
   if constexpr (LG >= 0) {
 #pragma unroll
@@ -350,7 +355,7 @@ __global__ void __launch_bounds__(QN_THREADS, QN_FWD_BLOCKS) qn_fwd_kernel(const
   for (int i = 0; i < NP; ++i) {
     const QnChunks<V> c(lane + i * g, p.rot, p.interleaved);
     ca[i] = c.a; cb[i] = c.b;
-    ha[i] = c.a < chunks; hb[i] = c.b < chunks;
+    ha[i] = LG >= 0 || c.a < chunks; hb[i] = LG >= 0 || c.b < chunks;
   }
   __syncthreads();
   if (p.rot) qn_fill_table<V>(p, tbl, spos, n_tok, np);
@@ -499,7 +504,7 @@ __device__ __forceinline__ void qn_bwd_rows(const QnParams& p, const QnRows& R, 
   for (int i = 0; i < NP; ++i) {
     const QnChunks<V> c(lane + i * g, p.rot, p.interleaved);
     ca[i] = c.a; cb[i] = c.b;
-    ha[i] = c.a < chunks; hb[i] = c.b < chunks;
+    ha[i] = LG >= 0 || c.a < chunks; hb[i] = LG >= 0 || c.b < chunks;
 #pragma unroll
     for (int j = 0; j < V; ++j) dwa[i][j] = dwb[i][j] = dba[i][j] = dbb[i][j] = 0.f;
   }
@@ -722,10 +727,11 @@ static int qn_launch_fwd(QnParams& p, bool paged, long align, double base, int s
   p.tile = tile;
   const int smem = 4 * QN_MAX_D * 4 + tile * per_tok;
   const int grid = (p.T + tile - 1) / tile;
+  const bool exact = V == VF && p.D == 2 * V << p.log_g;
   auto launch = [&](auto paged_form) {
     constexpr bool PAGED = decltype(paged_form)::value;
-    if (V == VF && p.log_g == 2) qn_fwd_kernel<T, VF, 1, 2, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
-    else if (V == VF && p.log_g == 3) qn_fwd_kernel<T, VF, 1, 3, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
+    if (exact && p.log_g == 2) qn_fwd_kernel<T, VF, 1, 2, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
+    else if (exact && p.log_g == 3) qn_fwd_kernel<T, VF, 1, 3, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
     else if (V == VF) qn_fwd_kernel<T, VF, 1, -1, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
     else if (V == 2) qn_fwd_kernel<T, 2, 2, -1, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
     else qn_fwd_kernel<T, 1, 4, -1, PAGED><<<grid, QN_THREADS, smem, stream>>>(p);
@@ -816,10 +822,11 @@ static int qn_launch_bwd(QnParams& p, long align, double base, int blocks, cudaS
   int smem = QN_MAX_D * 4 + tile * per_tok;
   const int red = (QN_THREADS / 32) * 2 * QN_MAX_D * 4;
   if (smem < red) smem = red;
+  const bool exact = V == VF && p.D == 2 * V << p.log_g;
   auto launch = [&](auto rms_form) {
     constexpr bool RMS = decltype(rms_form)::value;
-    if (V == VF && p.log_g == 2) qn_bwd_kernel<T, VF, 1, 2, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
-    else if (V == VF && p.log_g == 3) qn_bwd_kernel<T, VF, 1, 3, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
+    if (exact && p.log_g == 2) qn_bwd_kernel<T, VF, 1, 2, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
+    else if (exact && p.log_g == 3) qn_bwd_kernel<T, VF, 1, 3, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
     else if (V == VF) qn_bwd_kernel<T, VF, 1, -1, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
     else if (V == 2) qn_bwd_kernel<T, 2, 2, -1, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
     else qn_bwd_kernel<T, 1, 4, -1, RMS><<<blocks, QN_THREADS, smem, stream>>>(p);
