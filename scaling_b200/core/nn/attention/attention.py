@@ -385,7 +385,8 @@ class ParallelSelfAttention(torch.nn.Module):
         return (q.is_cuda and self.model_parallel_size == 1 and q.dtype in (torch.bfloat16, torch.float16, torch.float32)
                 and q.shape[-1] <= 256 and q.numel() > 0
                 and (self.rotary_embedding is None or self.rotary_embedding.dimensions % 2 == 0)
-                and not any(n._use_umup or n._forward_hooks or n._forward_pre_hooks for n in norms))
+                and not any(n._use_umup or n._forward_hooks or n._forward_pre_hooks or n._backward_hooks
+                            or n._backward_pre_hooks for n in norms))
 
     def _head_norm_and_rotary(self, q: torch.Tensor, k: torch.Tensor,
                               pos: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:

@@ -270,7 +270,12 @@ __device__ __forceinline__ int pa_scan(int v, int lane) {
   }
   return v;
 }
-__device__ __forceinline__ int pa_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
+// Lengths are kept in 32 bits: a sum that may not fit becomes the largest value, which pa_find refuses.
+__device__ __forceinline__ int pa_sum(unsigned v) {
+  const bool huge = __any_sync(0xffffffffu, v > 0x3ffffffu);
+  const unsigned sum = __reduce_add_sync(0xffffffffu, v & 0x3ffffffu);
+  return huge ? 0x7fffffff : (int)sum;
+}
 // Length of all items of one KV head of sequence 32 * chunk + lane (0 beyond the last sequence); the whole warp calls.
 template <int ROWS> __device__ __forceinline__ int pa_chunk_cost(const PaParams& p, int chunk, int lane, PaSeq& s) {
   const int b = chunk * 32 + lane;
@@ -284,9 +289,9 @@ template <int ROWS> __device__ __forceinline__ int pa_chunk_cost(const PaParams&
     many &= many - 1;
     const int n = __shfl_sync(0xffffffffu, s.n, src), L = __shfl_sync(0xffffffffu, s.L, src);
     const int cnt = pa_items<ROWS>(p, n);
-    int sum = 0;
-    for (int m = lane; m < cnt; m += 32) sum += pa_item_cost<ROWS>(p, n, L, m);
-    sum = pa_sum(sum);
+    long long mine = 0;
+    for (int m = lane; m < cnt; m += 32) mine += pa_item_cost<ROWS>(p, n, L, m);
+    const int sum = pa_sum((unsigned)min(mine, 0x7fffffffLL));
     if (lane == src) cost = sum;
   }
   return cost;
@@ -323,7 +328,7 @@ __device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int 
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   all *= p.Hkv;
-  if (all > 0x7fffffff) {  // months of work
+  if (all >= 0x7fffffff) {  // half a minute of work and more: reported, nothing done
     if (lane == 0) *p.status = SB_ERR_TOO_LARGE;
     return;
   }
@@ -548,7 +553,11 @@ template <int ROWS, int STAGES>
 __device__ __forceinline__ bool pa_begin(const PaParams& p, PaCtrl<STAGES>& c, uint8_t* smem, int warp, int lane) {
   constexpr int ISSUERS = PaKind<ROWS>::NARROW ? 1 : 2;  // warps that issue MMAs: each releases what the MMAs read
   if (sb::smem_u32(smem) & 1023) {
-    if (threadIdx.x == 0) *p.status = SB_ERR_BAD_ARG;
+    if (threadIdx.x == 0) {
+      *p.status = SB_ERR_BAD_ARG;
+      p.part_desc[8 * blockIdx.x] = 0;
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // as in pa_end
     return false;
   }
   if (threadIdx.x == 0) {
@@ -946,13 +955,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     pa_load<R, PANELS, true, false>(p, c, sRing, &tmK, &tmV, lane);
   } else if (warp == 11) {
     pa_load<R, PANELS, false, true>(p, c, sRing, &tmK, &tmV, lane);
-    if (p.zero_tail) {  // rows behind the last sequence
-      const long first = p.batch > 0 ? min(max(p.cu[p.batch], 0), p.T) : 0, heads = (long)p.Hkv * p.group;
-      const int per_row = p.D / 8;
-      for (long row = first * heads + blockIdx.x; row < p.T * heads; row += gridDim.x) {
-        const long t = row / heads;
+    if (p.zero_tail) {  // rows before the first and behind the last sequence
+      const int before = p.batch > 0 ? min(max(p.cu[0], 0), p.T) : 0, heads = p.Hkv * p.group;
+      const int gap = p.batch > 0 ? max(min(p.cu[p.batch], p.T), before) - before : 0, per_row = p.D / 8;
+      for (int at = blockIdx.x; at < (p.T - gap) * heads; at += gridDim.x) {
+        const int row = at < before * heads ? at : at + gap * heads, t = row / heads;
         if (lane < per_row)
-          *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + t * p.o_tok + (row - t * heads) * p.o_head + lane * 8) =
+          *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + (long)t * p.o_tok + (long)(row - t * heads) * p.o_head + lane * 8) =
               make_uint4(0, 0, 0, 0);
       }
     }
@@ -1214,7 +1223,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const float top = fminf(r0, r1);
         g0 = r0 == INFINITY ? 0.f : pa_exp2(top - r0);
         g1 = r1 == INFINITY ? 0.f : pa_exp2(top - r1);
-        const float sum = (g0 == 0.f ? 0.f : a0 * g0) + (g1 == 0.f ? 0.f : a1 * g1);
+        const float sum = a0 * g0 + a1 * g1;  // without a reference: 0, or NaN if every score was
         if (it.slot < 0) {
           const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // no visible key: zeros; NaN stays
           g0 *= inv;
@@ -1494,7 +1503,7 @@ SB_API long sb200_paged_attention_workspace(int T, int batch, int Hq, int Hkv, i
 // last new token at position lens[b] - 1; position j in row j % page_size of page table[b][j / page_size].  A query at
 // position i sees keys j <= i (causal), |i - j| <= window (window >= 0).  page_size is a power of two from 8, D a
 // multiple of 8 up to 128; pointers and strides are multiples of 16 bytes.  Rows behind the last sequence are left as
-// they are, or zeroed with zero_tail.  Visible pages outside the cache and lengths outside the table set *status.
+// they are, or zeroed with zero_tail (as rows before the first).  Visible pages outside the cache and lengths outside the table set *status.
 SB_API int sb200_paged_attention(const void* q, const void* k_cache, const void* v_cache, void* out, const int* table,
                                  const int* cu, const int* lens, void* workspace, long workspace_bytes, int T, int batch,
                                  int Hq, int Hkv, int D, int num_pages, int page_size, int cols, long table_ld, long q_tok,
@@ -1507,7 +1516,8 @@ SB_API int sb200_paged_attention(const void* q, const void* k_cache, const void*
   if (page_size < 8 || (page_size & (page_size - 1)) || !(scale > 0.f && scale < 1e30f)) return SB_ERR_BAD_ARG;
   if (dtype != SB_DT_BF16 && dtype != SB_DT_F16) return SB_ERR_BAD_ARG;
   const long cap = (long)cols * page_size;
-  if ((long)T * Hq > (1L << 30) || cap > (1L << 30) || batch > (1 << 17) || Hq / Hkv > (1 << 15)) return SB_ERR_TOO_LARGE;
+  // 2^26 positions: two items of one CTA then take less time than the bound of a wait (2.5 us per tile)
+  if ((long)T * Hq > (1L << 30) || cap > (1L << 26) || batch > (1 << 17) || Hq / Hkv > (1 << 15)) return SB_ERR_TOO_LARGE;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
        reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return SB_ERR_BAD_ARG;

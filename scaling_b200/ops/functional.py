@@ -688,6 +688,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     if not q.is_cuda or q.numel() == 0 or k.numel() == 0:
         return (head_norm_rope_reference(q, q_weight, q_bias, positions, rotary, eps, rms),
                 head_norm_rope_reference(k, k_weight, k_bias, positions, rotary, eps, rms))
+    if q.shape[0] >= 2 ** 31 - 2 ** 16:
+        raise _lib.KernelError(f"qk_norm_rope: {q.shape[0]} tokens pass 32 bits")
     if q.dtype not in _KERNEL_DTYPES or q.shape[2] > 256:
         raise _lib.KernelError(f"qk_norm_rope: {q.dtype} with head size {q.shape[2]} is not supported (fp32, bf16, fp16 "
                                "up to 256)")

@@ -49,6 +49,11 @@ def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch
             raise ValueError(f"{name} is on {t.device}, the cache on {k_cache.device}")
 
 
+def _check_sizes(what: str, *sizes: int) -> None:
+    if any(s >= 2 ** 31 - 2 ** 16 for s in sizes):
+        raise _lib.KernelError(f"{what}: sizes {sizes} pass 32 bits")
+
+
 def _check_rows(name: str, x: torch.Tensor, k_cache: torch.Tensor) -> None:
     if x.dim() != 3 or x.shape[2] != k_cache.shape[3] or x.dtype != k_cache.dtype or x.device != k_cache.device:
         raise ValueError(f"{name} {tuple(x.shape)} {x.dtype} {x.device} does not fit a cache "
@@ -126,6 +131,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
         return out
     if d > 256:
         raise _lib.KernelError(f"paged_append: head size {d} is not supported (up to 256)")
+    _check_sizes("paged_append", tokens, num_pages, page_table.shape[0], page_table.shape[1], page_size)
     code = dt(k.dtype)
     out = None if q is None else torch.empty_like(q, memory_format=torch.contiguous_format)
     if tokens == 0:
@@ -176,7 +182,7 @@ def paged_attention_reference(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
         v = v.masked_fill(~seen.any(0)[:, None, None], 0.0)
         qs = q[start:end].reshape(n, kv_heads, group, -1).to(acc)
         s = torch.einsum("nhgd,jhd->hgnj", qs, k).mul_(scale).masked_fill_(~seen, float("-inf"))
-        p = torch.nan_to_num(torch.softmax(s, -1), nan=0.0) if not seen.any(1).all() else torch.softmax(s, -1)
+        p = torch.softmax(s, -1).masked_fill(~seen.any(1)[:, None], 0.0)
         out[start:end] = torch.einsum("hgnj,jhd->nhgd", p, v).reshape(n, q.shape[1], -1).to(q.dtype)
     return out
 
@@ -191,12 +197,13 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Heads are a multiple of the cache's KV heads.  A query at position ``i`` of its sequence sees the cached positions
     ``j <= i`` (all of them without ``causal``) with ``|i - j| <= window``; keys of the new tokens are read from the
     cache, so they are written first (``paged_append``).  A query that sees nothing gives zeros.  Pages that no query of
-    the call sees may be missing from the table.  Rows behind the last sequence are left as they were in ``out`` and are
-    zero without it.  Whatever the cache holds behind a sequence's last token has no effect; keys and values of its
-    tokens are finite.  On GPUs: bf16 and fp16, head sizes that are multiples of 8 up to 128, pages of 8 tokens and more.
-    In inference only: no backward pass."""
+    the call sees may be missing from the table.  Rows of no sequence are left as they were in ``out`` and are zero
+    without it; ``out`` may be ``q`` itself and overlaps no other tensor.  Whatever the cache holds behind a sequence's
+    last token has no effect; keys and values of its tokens are finite.  On GPUs: bf16 and fp16, head sizes that are
+    multiples of 8 up to 128, pages of 8 tokens and more, page tables of up to 2^26 positions, up to 2^30 query rows and
+    2^30 products of 256 rows (64 in decoding) with 128 keys.  In inference only: no backward pass."""
     _check_cache(k_cache, v_cache, page_table, cu_seqlens, seq_lens)
-    _no_grad_inputs("paged_attention", q, k_cache, v_cache)
+    _no_grad_inputs("paged_attention", q, k_cache, v_cache, out)
     _check_rows("q", q, k_cache)
     tokens, heads, d = q.shape
     num_pages, page_size, kv_heads = k_cache.shape[:3]
@@ -209,6 +216,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError(f"window must not be negative, got {window}")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device):
         raise ValueError(f"out {tuple(out.shape)} {out.dtype} {out.device} does not match q {tuple(q.shape)} {q.dtype}")
+    if out is not None and any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
+        raise ValueError(f"rows of out share memory (strides {out.stride()})")
     if not q.is_cuda:
         return paged_attention_reference(q, k_cache, v_cache, page_table, cu_seqlens, seq_lens, causal, scale, window,
                                          torch.zeros_like(q) if out is None else out)
@@ -230,8 +239,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                    f"got {t.stride()}")
     if num_pages == 0:
         raise ValueError("the cache has no pages")
+    _check_sizes("paged_attention", tokens * heads, num_pages, page_table.shape[0], page_table.shape[1], page_size)
     if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
+        q = q.clone(memory_format=torch.contiguous_format)  # also where only the start is off
     with _lib.on_device_of(q):
         batch, cols, sms = seq_lens.shape[0], page_table.shape[1], sm_count()
         size = lib().sb200_paged_attention_workspace(tokens, batch, heads, kv_heads, d, cols * page_size, sms)

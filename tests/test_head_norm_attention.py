@@ -82,6 +82,16 @@ def test_hooks_on_the_norms_still_see_their_outputs():
     assert (a.float() - b.float()).norm() <= 4 * 2.0 ** -8 * b.float().norm()
 
 
+@pytest.mark.gpu
+def test_backward_hooks_on_the_norms_still_run():
+    m = _attention(NormType.RMS, "cuda", torch.bfloat16)
+    seen = []
+    m.norm_key.register_full_backward_hook(lambda mod, gi, go: seen.append(go[0].shape))
+    x = torch.randn(1, 16, 256, device="cuda").bfloat16().requires_grad_()
+    m(x, torch.tensor([0, 16], dtype=torch.int32, device="cuda"), None).float().sum().backward()
+    assert seen == [(16, 4, 64)]
+
+
 def test_separate_operations_on_the_cpu():
     m = _attention(NormType.LAYERNORM, "cpu", torch.float32)
     x = torch.randn(2, 10, 256)

@@ -533,3 +533,107 @@ def test_prompt_in_chunks_then_tokens_equals_one_pass(dim, heads, kv_heads, wind
     qn, _ = K.qk_norm_rope(torch.cat([x[0][0], x[1][0]]), torch.cat([x[0][1], x[1][1]]), wq, wk, positions=pos, rotary=rotary)
     whole.q = qn
     _check_attention(whole, torch.cat(outs[0] + outs[1]), True, window)
+
+
+def _rows_that_are_not_numbers(device, dtype):
+    """A query of NaN beside one that sees nothing, in a short sequence, a long one that is cut into parts, and a chunk."""
+    b = _attend_batch([20, 3000, 2], [1, 1, 5], 16, 4, 2, 64, dtype, device)
+    b.q[0] = float("nan")
+    b.q[1, 3] = float("nan")
+    return b
+
+
+def _check_rows_that_are_not_numbers(b):
+    out = paged_attention(b.q, *b.args())
+    assert torch.isnan(out[0]).all() and torch.isnan(out[1, 3]).all()
+    assert torch.count_nonzero(out[2:5]) == 0  # three more new tokens than the sequence has
+    clean = b.q.nan_to_num(0.0)
+    want, bound = attention_in_64_bits(b, True, 0.125, None, q=clean)
+    keep = torch.ones(out.shape[:2], dtype=torch.bool, device=out.device)
+    keep[0], keep[1, 3] = False, False
+    assert ((out.double() - want).abs() <= bound)[keep].all()
+
+
+def test_bad_queries_stay_alone_in_the_torch_expression():
+    _check_rows_that_are_not_numbers(_rows_that_are_not_numbers("cpu", torch.bfloat16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("more", [False, True])
+def test_bad_queries_stay_alone(more):
+    b = _rows_that_are_not_numbers(DEV, torch.bfloat16)
+    _check_rows_that_are_not_numbers(b)
+    if more:  # in a chunk's rows
+        b = _attend_batch([700], [300], 16, 4, 2, 64, torch.bfloat16, DEV)
+        want = paged_attention(b.q, *b.args())
+        b.q[100] = float("nan")
+        out = paged_attention(b.q, *b.args())
+        assert torch.isnan(out[100]).all()
+        keep = torch.arange(300, device=DEV) != 100
+        assert torch.equal(out[keep], want[keep])
+
+
+def test_outputs_whose_rows_share_memory_are_refused():
+    b = _attend_batch([20], [4], 16, 4, 2, 64, torch.bfloat16, "cpu")
+    shared = torch.zeros(1, 4, 64, dtype=torch.bfloat16).expand(4, 4, 64)
+    with pytest.raises(ValueError, match="share memory"):
+        paged_attention(b.q, *b.args(), out=shared)
+    with pytest.raises(KernelError, match="no backward"):
+        paged_attention(b.q, *b.args(), out=torch.zeros_like(b.q).requires_grad_())
+
+
+@pytest.mark.gpu
+def test_rows_before_the_first_sequence():
+    b = _attend_batch([50, 300], [3, 140], 16, 4, 2, 64, torch.bfloat16, DEV, spare_rows=9)
+    want = paged_attention(b.q, *b.args())
+    cu = b.cu + 7
+    moved = torch.cat((b.q[-7:], b.q[:-7]))
+    for _ in range(3):  # memory of earlier results is reused
+        garbage = torch.full_like(moved, float("nan"))
+        del garbage
+        out = paged_attention(moved, b.k_cache, b.v_cache, b.table, cu, b.seq_lens)
+        assert torch.count_nonzero(out[:7]) == 0 and torch.count_nonzero(out[7 + b.tokens:]) == 0
+        assert torch.equal(out[7:7 + b.tokens], want[:b.tokens])
+        del out
+    K.check_status()
+
+
+@pytest.mark.gpu
+def test_queries_off_the_16_byte_boundary_and_in_the_place_of_the_output():
+    b = _attend_batch([50, 300, 4000], [3, 140, 1], 16, 4, 2, 64, torch.bfloat16, DEV)
+    want = paged_attention(b.q, *b.args())
+    flat = torch.zeros(b.q.numel() + 4, dtype=torch.bfloat16, device=DEV)
+    off = flat[4:].view(b.q.shape)
+    off.copy_(b.q)
+    assert off.is_contiguous() and off.data_ptr() % 16
+    assert torch.equal(paged_attention(off, *b.args()), want)
+    q = b.q.clone()
+    assert paged_attention(q, *b.args(), out=q) is q
+    assert torch.equal(q, want)
+
+
+@pytest.mark.gpu
+def test_more_work_than_32_bits_of_tiles_is_refused():
+    """Prompts of a million tokens with 64 heads over one KV head: the lengths on the work line add up to more than 2^31."""
+    cache = torch.zeros(1, 128, 1, 8, dtype=torch.bfloat16, device=DEV)
+    table = torch.zeros(1, 2 ** 14, dtype=torch.int32, device=DEV)
+    q = torch.zeros(2 ** 20, 64, 8, dtype=torch.bfloat16, device=DEV)
+    cu = torch.tensor([0, 2 ** 20], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([2 ** 21], dtype=torch.int32, device=DEV)
+    K.check_status()
+    paged_attention(q, cache, cache, table, cu, lens)
+    with pytest.raises(KernelError, match="size"):
+        K.check_status()
+    K.check_status()
+
+
+@pytest.mark.gpu
+def test_page_tables_of_too_many_positions_are_refused():
+    cache = torch.zeros(1, 128, 1, 8, dtype=torch.bfloat16, device=DEV)
+    q = torch.zeros(1, 1, 8, dtype=torch.bfloat16, device=DEV)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([5], dtype=torch.int32, device=DEV)
+    paged_attention(q, cache, cache, torch.zeros(1, 2 ** 19, dtype=torch.int32, device=DEV), cu, lens)
+    with pytest.raises(KernelError):
+        paged_attention(q, cache, cache, torch.zeros(1, 2 ** 19 + 1, dtype=torch.int32, device=DEV), cu, lens)
+    K.check_status()
