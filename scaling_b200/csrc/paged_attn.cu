@@ -31,6 +31,16 @@
 // of V (a page of 16 tokens is a copy of its own, and one warp alone issues them no faster than the memory delivers), 9 MMA
 // issuer.  Wide: 8 loader of both, 9 and 11 MMA issuers of the two groups.
 //
+// What bounds it, measured on one B200 (6.57 TB/s copy, 1634 TFLOP/s):
+//   decoding, 64 requests of up to 8000 tokens, 32 heads over 8 of 128, pages of 16: 148 to 156 us (5.7 to 6.0 TB/s, 0.87 to
+//     0.92 of the copy): the stream of K and V.
+//   decoding, two long contexts, 40 heads over one of 128: 42 us (3.1 TB/s): about 3 us per item end, the softmax of 40 rows
+//     per key and the joining of some 70 parts per row, against 20 us for the bytes.
+//   chunks of 2048 tokens on long contexts, heads of 128: 420 to 435 us, 980 to 1015 TFLOP/s (0.60 to 0.62): per half tile the
+//     chain S product -> wait -> 64 exponentials per row -> wait -> P V product; two groups and two S each hide most of it.
+//   one request: 10.6 us: launch, work line, queries, tile, epilogue in a chain; nothing to overlap.
+//   24 ragged sequences of 1 to 300 new tokens: 56 to 60 us, two kernels one after the other on most SMs and 3 to 4 us per item.
+//
 // Rounding: scores, sums and outputs are fp32; P is rounded to the 16-bit element type for the second product (half a
 // step per probability, averaged over the row), the output once.
 #include <cuda.h>
@@ -929,7 +939,7 @@ template <typename F> __device__ __forceinline__ float pa_transpose_reduce(float
 }
 
 // All loops over the rows go by blocks of 16 and are not unrolled further: code that does not fit the instruction caches
-// costs more than the work here (unrolled over 64 rows the kernel took 48 us where it now takes less than half).  So what a
+// costs more than the work here (unrolled over 64 rows the long decode above took 59 us, now 42).  So what a
 // thread keeps of the rows between tiles has to be little: row r is kept by lane r % 32 of every warp.
 template <int PANELS, bool F16>
 __global__ void __launch_bounds__(PA_THREADS, 1)
@@ -1409,7 +1419,7 @@ long pa_align(long v) { return (v + 255) & ~255L; }
 
 // Which kernels a call takes, and their places in its workspace.  Sequences with at most 64 rows (new tokens x heads per KV
 // head) are narrow; with no more new tokens than sequences, as in a decoding step, all of them are, whatever their length:
-// the second launch then finds nothing (3 us), and a sequence that does have more rows is read once per 64 of them.
+// the wide launch would find nothing and cost its 3 us, and a sequence that does have more rows is read once per 64 of them.
 struct PaPlan {
   bool wide, whole;
   int narrow_max, narrow_rows, narrow_ctas, wide_ctas;
@@ -1499,9 +1509,9 @@ SB_API long sb200_paged_attention_workspace(int T, int batch, int Hq, int Hkv, i
 }
 
 // out[t, h] for the new tokens of `batch` sequences, q / out [T, Hq, D] (token and head strides in elements), caches
-// [num_pages, page_size, Hkv, D] (page, row and head strides; a page stride is a multiple of 8 row strides), bf16 or fp16.  Sequence b: rows cu[b] .. cu[b + 1] of q, its
-// last new token at position lens[b] - 1; position j in row j % page_size of page table[b][j / page_size].  A query at
-// position i sees keys j <= i (causal), |i - j| <= window (window >= 0).  page_size is a power of two from 8, D a
+// [num_pages, page_size, Hkv, D] (page, row and head strides; a page stride is a multiple of 8 row strides), bf16 or fp16.
+// Sequence b: rows cu[b] .. cu[b + 1] of q, its last new token at position lens[b] - 1; position j in row j % page_size of
+// page table[b][j / page_size].  A query at position i sees keys j <= i (causal), |i - j| <= window (window >= 0).  page_size is a power of two from 8, D a
 // multiple of 8 up to 128; pointers and strides are multiples of 16 bytes.  Rows behind the last sequence are left as
 // they are, or zeroed with zero_tail (as rows before the first).  Visible pages outside the cache and lengths outside the table set *status.
 SB_API int sb200_paged_attention(const void* q, const void* k_cache, const void* v_cache, void* out, const int* table,

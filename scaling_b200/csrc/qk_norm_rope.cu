@@ -15,6 +15,13 @@
 // rotation needs no exchange; only the row sums go through shuffles.  Statistics, weights, sines and products stay in
 // fp32 and are rounded once, at the store.
 //
+// Measured on one B200 (copy 6.57 TB/s), forward and backward together: 8192 tokens, 32 + 8 heads of 128, RMS, interleaved
+// rotation, bf16: 124 us = 3.4 TB/s (0.52 of the copy); 16384 tokens, 12 + 12 heads of 64, layer norm with biases, packed
+// projection: 92 us (0.42); a decoding step's append 6.5 us; an append of 8000 prompt tokens, 41 heads: 43 us (0.47).
+// Bound by instructions, not by memory: 55 to 61 % of the issue slots, 30 % of the DRAM cycles: conversions, the norm's
+// shuffles, and three passes of fp32 arithmetic per element.  Hence the packed fp32 forms, weights in registers, code of its
+// own per kind of row and per common head size.
+//
 // Angles: a position of 10^5 times a frequency near 1 in fp32 is off by 10^-2 rad.  The host computes turns per position
 // base^(-2 i / rot) / (2 pi) in fp64; a thread multiplies by the position, drops the whole turns in fp64 and takes
 // sincospi of what is left in fp32.  One thread per (token, pair) fills a table in shared memory that all heads of the
@@ -28,7 +35,7 @@
 namespace {
 
 constexpr int QN_THREADS = 256;
-constexpr int QN_FWD_BLOCKS = 3;          // per SM
+constexpr int QN_FWD_BLOCKS = 3;          // per SM (4 of them, with fewer registers: 150 us where the 7B step took 134)
 constexpr int QN_MAX_D = 256;
 constexpr int QN_MAX_SLOTS = 64;          // tokens per tile
 constexpr int QN_TABLE_BYTES = 24 * 1024; // sine table of a tile
@@ -87,6 +94,11 @@ __device__ __forceinline__ void qn_mul2(float& d0, float& d1, float a0, float a1
       : "=f"(d0), "=f"(d1)
       : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
 }
+__device__ __forceinline__ void qn_add2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+  asm("{\n.reg .b64 x, y, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 w, x, y;\nmov.b64 {%0, %1}, w;\n}\n"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
 template <int V> __device__ __forceinline__ void qn_mul(float (&d)[V], const float (&a)[V], const float (&b)[V]) {
   if constexpr (V == 1) d[0] = a[0] * b[0];
   else
@@ -115,8 +127,16 @@ template <int V> __device__ __forceinline__ void qn_axpy(float (&d)[V], const fl
     for (int i = 0; i < V; i += 2) qn_fma2(d[i], d[i + 1], a[i], a[i + 1], b, b, d[i], d[i + 1]);
 }
 template <int V> __device__ __forceinline__ void qn_shift(float (&d)[V], float b) {
+  if constexpr (V == 1) d[0] += b;
+  else
 #pragma unroll
-  for (int i = 0; i < V; ++i) d[i] += b;
+    for (int i = 0; i < V; i += 2) qn_add2(d[i], d[i + 1], d[i], d[i + 1], b, b);
+}
+template <int V> __device__ __forceinline__ void qn_add(float (&d)[V], const float (&a)[V]) {
+  if constexpr (V == 1) d[0] += a[0];
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) qn_add2(d[i], d[i + 1], d[i], d[i + 1], a[i], a[i + 1]);
 }
 // sum of a * b over the chunk
 template <int V> __device__ __forceinline__ float qn_dot(const float (&a)[V], const float (&b)[V]) {
@@ -130,10 +150,13 @@ template <int V> __device__ __forceinline__ float qn_dot(const float (&a)[V], co
   }
 }
 template <int V> __device__ __forceinline__ float qn_total(const float (&a)[V]) {
-  float s = a[0];
+  if constexpr (V == 1) return a[0];
+  else {
+    float s0 = a[0], s1 = a[1];
 #pragma unroll
-  for (int i = 1; i < V; ++i) s += a[i];
-  return s;
+    for (int i = 2; i < V; i += 2) qn_add2(s0, s1, s0, s1, a[i], a[i + 1]);
+    return s0 + s1;
+  }
 }
 template <typename T, int V> __device__ __forceinline__ void qn_unpack(const QnVec<T, V>& v, float (&f)[V]) {
 #pragma unroll
@@ -273,30 +296,26 @@ __device__ __forceinline__ void qn_fill_table(const QnParams& p, float* tbl, con
   }
 }
 
-// Row statistics of x held as NP pairs; chunks beyond the row (ha / hb false) hold zeros.
+// Takes the mean off x (not for RMS) and returns the reciprocal deviation r.  x is held as NP pairs; chunks beyond the row
+// (ha / hb false) hold zeros and keep them.
 template <int V, int NP, int LG>
-__device__ __forceinline__ void qn_stats(const float (&a)[NP][V], const float (&b)[NP][V], const bool (&ha)[NP],
-                                         const bool (&hb)[NP], float inv_d, int rms, float eps, int g, float& mu, float& r) {
-  mu = 0.f;
-  float ss = 0.f;
-  if (rms) {
-#pragma unroll
-    for (int p = 0; p < NP; ++p) ss += qn_dot<V>(a[p], a[p]) + qn_dot<V>(b[p], b[p]);
-  } else {
+__device__ __forceinline__ float qn_stats(float (&a)[NP][V], float (&b)[NP][V], const bool (&ha)[NP], const bool (&hb)[NP],
+                                          float inv_d, int rms, float eps, int g) {
+  if (!rms) {
     float s = 0.f;
 #pragma unroll
     for (int p = 0; p < NP; ++p) s += qn_total<V>(a[p]) + qn_total<V>(b[p]);
-    mu = qn_group_sum<LG>(s, g) * inv_d;
+    const float mu = qn_group_sum<LG>(s, g) * inv_d;
 #pragma unroll
-    for (int p = 0; p < NP; ++p)  // around the mean, from registers: no cancellation
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float da = ha[p] ? a[p][i] - mu : 0.f, db = hb[p] ? b[p][i] - mu : 0.f;
-        ss = fmaf(da, da, ss);
-        ss = fmaf(db, db, ss);
-      }
+    for (int p = 0; p < NP; ++p) {
+      if (ha[p]) qn_shift<V>(a[p], -mu);
+      if (hb[p]) qn_shift<V>(b[p], -mu);
+    }
   }
-  r = rsqrtf(fmaf(qn_group_sum<LG>(ss, g), inv_d, eps));
+  float ss = 0.f;  // around the mean, from registers: no cancellation
+#pragma unroll
+  for (int p = 0; p < NP; ++p) ss += qn_dot<V>(a[p], a[p]) + qn_dot<V>(b[p], b[p]);
+  return rsqrtf(fmaf(qn_group_sum<LG>(ss, g), inv_d, eps));
 }
 
 // ============================================================================ forward
@@ -408,30 +427,24 @@ __global__ void __launch_bounds__(QN_THREADS, QN_FWD_BLOCKS) qn_fwd_kernel(const
           qn_unpack<T, V>(vb[i], b[i]);
         }
         if (norm) {
-          float mu, r;
-          qn_stats<V, NP, LG>(a, b, ha, hb, inv_d, p.rms, p.eps, g, mu, r);
+          const float r = qn_stats<V, NP, LG>(a, b, ha, hb, inv_d, p.rms, p.eps, g);
 #pragma unroll
           for (int i = 0; i < NP; ++i) {
-            if (!p.rms) {
-              qn_shift<V>(a[i], -mu);
-              qn_shift<V>(b[i], -mu);
-            }
             qn_scale<V>(a[i], r);
             qn_scale<V>(b[i], r);
-            if (ha[i]) qn_mul<V>(a[i], a[i], w1[i]);
-            if (hb[i]) qn_mul<V>(b[i], b[i], w2[i]);
             if (R.b) {
               float t[V];
               if (ha[i]) {
                 qn_read_weights<V>(ws + QN_MAX_D, ca[i], chunks, t);
-#pragma unroll
-                for (int j = 0; j < V; ++j) a[i][j] += t[j];
+                qn_fma<V>(a[i], a[i], w1[i], t);
               }
               if (hb[i]) {
                 qn_read_weights<V>(ws + QN_MAX_D, cb[i], chunks, t);
-#pragma unroll
-                for (int j = 0; j < V; ++j) b[i][j] += t[j];
+                qn_fma<V>(b[i], b[i], w2[i], t);
               }
+            } else {
+              if (ha[i]) qn_mul<V>(a[i], a[i], w1[i]);
+              if (hb[i]) qn_mul<V>(b[i], b[i], w2[i]);
             }
           }
         }
@@ -567,22 +580,17 @@ __device__ __forceinline__ void qn_bwd_rows(const QnParams& p, const QnRows& R, 
         for (int i = 0; i < NP; ++i)
           qn_rotate<V, true>(da[i], db[i], tbl + tl * np * V * 2, lane + i * g, np, p.rot, p.interleaved);
       }
-      float mu, r;
-      qn_stats<V, NP, LG>(a, b, ha, hb, inv_d, RMS, p.eps, g, mu, r);
+      const float r = qn_stats<V, NP, LG>(a, b, ha, hb, inv_d, RMS, p.eps, g);
       float s1 = 0.f, s2 = 0.f;  // sums of g and of g * xhat
       const bool keep = live;    // a group without a row repeats the row before: it counts once
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         float w[V];
         auto chunk = [&](float (&x)[V], float (&dy)[V], float (&dw)[V], float (&dbias)[V], int c) {
-          if (!RMS) qn_shift<V>(x, -mu);
           qn_scale<V>(x, r);
           if (keep) {
             qn_fma<V>(dw, dy, x, dw);
-            if (!RMS) {
-#pragma unroll
-              for (int j = 0; j < V; ++j) dbias[j] += dy[j];
-            }
+            if (!RMS) qn_add<V>(dbias, dy);
           }
           qn_read_weights<V>(sw, c, chunks, w);
           qn_mul<V>(dy, dy, w);
@@ -686,8 +694,8 @@ long qn_align(const QnRows& r, int es) {
 }
 
 // Fills in what follows from the sizes; returns the elements V that a lane moves at once: 16 bytes where all rows are so
-// aligned and, for rotate-half, the rotated half is whole chunks; else 2 elements; else 1 (3000 tokens x 41 heads of 80 in
-// fp32, 20 dimensions rotated: 1150 us with V = 1, see the measured table for V = 2).
+// aligned and, for rotate-half, the rotated half is whole chunks; else 2 elements; else 1 (2999 tokens x 41 heads of 80 in
+// fp32, 20 dimensions rotated, forward and backward: 1152 us with V = 1, 143 us with V = 2).
 int qn_plan(QnParams* p, int es, long align, double base) {
   auto fits = [&](int v) {
     return align >= (long)v * es && p->D % v == 0 && (p->rot == 0 || (p->interleaved ? v % 2 == 0 : (p->rot / 2) % v == 0));
@@ -696,8 +704,10 @@ int qn_plan(QnParams* p, int es, long align, double base) {
   const int chunks = (p->D + V - 1) / V, pairs = (chunks + 1) / 2;
   p->log_g = qn_log_lanes(pairs, 32);
   for (QnRows* r : {&p->q, &p->k, &p->v}) r->inv = r->heads ? (uint32_t)((1UL << 32) / r->heads + 1) : 0;
+  // every eighth by pow, the others as products of at most seven factors: off by a few 2^-53, and a call takes 2 us less
+  const double step = p->rot ? pow(base, -2.0 / p->rot) : 1.0;
   for (int i = 0; i < p->rot / 2; ++i)
-    p->turns[i] = pow(base, -2.0 * i / p->rot) / 6.283185307179586476925;
+    p->turns[i] = i % 8 ? p->turns[i - 1] * step : pow(base, -2.0 * i / p->rot) / 6.283185307179586476925;
   return V;
 }
 int qn_table_bytes_per_token(const QnParams& p, int V) { return p.rot ? ((p.rot + 2 * V - 1) / (2 * V)) * V * 8 : 0; }
