@@ -16,11 +16,11 @@
 // fp32 and are rounded once, at the store.
 //
 // Measured on one B200 (copy 6.57 TB/s), forward and backward together: 8192 tokens, 32 + 8 heads of 128, RMS, interleaved
-// rotation, bf16: 124 us = 3.4 TB/s (0.52 of the copy); 16384 tokens, 12 + 12 heads of 64, layer norm with biases, packed
-// projection: 92 us (0.42); a decoding step's append 6.5 us; an append of 8000 prompt tokens, 41 heads: 43 us (0.47).
-// Bound by instructions, not by memory: 55 to 61 % of the issue slots, 30 % of the DRAM cycles: conversions, the norm's
-// shuffles, and three passes of fp32 arithmetic per element.  Hence the packed fp32 forms, weights in registers, code of its
-// own per kind of row and per common head size.
+// rotation, bf16: 116 us = 3.6 TB/s (0.55 of the copy); 16384 tokens, 12 + 12 heads of 64, layer norm with biases, packed
+// projection: 84 us (0.46); a decoding step's append 6.4 us; an append of some 6000 prompt tokens, 40 + 1 heads: 39 us (0.52).
+// Bound by instructions and by the latency that 24 warps per SM can cover, not by the memory's rate: 55 to 61 % of the issue
+// slots, 30 % of the DRAM cycles.  Per element there are conversions, the norm's shuffles and three passes of fp32
+// arithmetic; hence the packed fp32 forms, weights in registers, code of its own per kind of row and per common head size.
 //
 // Angles: a position of 10^5 times a frequency near 1 in fp32 is off by 10^-2 rad.  The host computes turns per position
 // base^(-2 i / rot) / (2 pi) in fp64; a thread multiplies by the position, drops the whole turns in fp64 and takes
@@ -78,6 +78,24 @@ __device__ __forceinline__ float qn_load_any(const void* p, int i, int dtype) {
 }
 
 __device__ __forceinline__ int qn_token(const QnRows& r, int row) { return r.heads == 1 ? row : (int)__umulhi(row, r.inv); }
+
+// Asks L2 for row `row` of a tile that starts at token t0: the lanes' 32-byte pieces of x (and of dy).  Registers hold the
+// rows of one round ahead and no more; two further rounds under way take the 7B training step from 122 to 116 us (four:
+// 118, eight: 125).  Only where a lane's piece is 16-byte chunks: with two-element accesses the addresses cost more.
+constexpr int QN_AHEAD = 2;
+template <typename T, int V>
+__device__ __forceinline__ void qn_ask(const QnRows& r, int t0, int row, int rows, int D, int lane, bool grad) {
+  if constexpr (V * sizeof(T) == 16) {
+    if (row >= rows || lane * (2 * V) >= D) return;
+    const int tl = qn_token(r, row), h = row - tl * r.heads;
+    const T* x = reinterpret_cast<const T*>(r.x) + (long)(t0 + tl) * r.x_tok + (long)h * r.x_head + lane * (2 * V);
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(x));
+    if (grad) {
+      const T* dy = reinterpret_cast<const T*>(r.dy) + (long)(t0 + tl) * r.dy_tok + (long)h * r.dy_head + lane * (2 * V);
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(dy));
+    }
+  }
+}
 
 // N consecutive elements as one access
 template <typename T, int N> struct alignas(sizeof(T) * N) QnVec { T e[N]; };
@@ -158,22 +176,26 @@ template <int V> __device__ __forceinline__ float qn_total(const float (&a)[V]) 
     return s0 + s1;
   }
 }
+// A chunk of eight 16-bit elements lies in registers as its four even elements and then its four odd ones: the halves of a
+// 32-bit word are taken apart anyway, and the rotation of interleaved pairs becomes packed arithmetic.
+template <int V> __device__ __forceinline__ constexpr int qn_reg(int e) { return V == 8 ? (e >> 1) + (e & 1) * 4 : e; }
+template <int V> __device__ __forceinline__ constexpr int qn_elem(int r) { return V == 8 ? (r & 3) * 2 + (r >> 2) : r; }
 template <typename T, int V> __device__ __forceinline__ void qn_unpack(const QnVec<T, V>& v, float (&f)[V]) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) f[i] = sb::to_f(v.e[i]);
+  for (int i = 0; i < V; ++i) f[i] = sb::to_f(v.e[qn_elem<V>(i)]);
 }
 template <typename T, int V> __device__ __forceinline__ void qn_pack(const float (&f)[V], QnVec<T, V>& v) {
   if constexpr (sizeof(T) == 2 && V > 1) {
 #pragma unroll
     for (int i = 0; i < V; i += 2) {
       if constexpr (std::is_same<T, __nv_bfloat16>::value)
-        *reinterpret_cast<__nv_bfloat162*>(&v.e[i]) = __floats2bfloat162_rn(f[i], f[i + 1]);
+        *reinterpret_cast<__nv_bfloat162*>(&v.e[i]) = __floats2bfloat162_rn(f[qn_reg<V>(i)], f[qn_reg<V>(i + 1)]);
       else
-        *reinterpret_cast<__half2*>(&v.e[i]) = __floats2half2_rn(f[i], f[i + 1]);
+        *reinterpret_cast<__half2*>(&v.e[i]) = __floats2half2_rn(f[qn_reg<V>(i)], f[qn_reg<V>(i + 1)]);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v.e[i] = sb::from_f<T>(f[i]);
+    for (int i = 0; i < V; ++i) v.e[i] = sb::from_f<T>(f[qn_reg<V>(i)]);
   }
 }
 
@@ -189,17 +211,17 @@ template <int V> struct QnChunks {
   }
 };
 
-// Place of the cosine of element i (< V) of pair c in the table of one token, in floats.  A 16-byte word holds the cosines and
+// Place of the cosine of angle i (< V; of the register for rotate-half) of pair c in the table of one token, in floats.  A 16-byte word holds the cosines and
 // then the sines of two neighbours, consecutive lanes touch consecutive words (no bank conflicts); np = pairs per row that
 // the table covers.  The sine lies qn_sine<V>() behind.
 template <int V> __device__ __forceinline__ int qn_table_slot(int c, int i, int np) {
   return V == 1 ? 2 * c : (((i >> 1) * np + c) << 2) + (i & 1);
 }
 template <int V> __device__ __forceinline__ constexpr int qn_sine() { return V == 1 ? 1 : 2; }
-// Place of element e of a weight vector in shared memory: four consecutive elements stay together, chunks interleave.
+// Place of element e of a weight vector in shared memory: four consecutive registers stay together, chunks interleave.
 template <int V> __device__ __forceinline__ int qn_weight_slot(int e, int chunks) {
   if (V < 4) return e;
-  const int c = e / V, j = e % V;
+  const int c = e / V, j = qn_reg<V>(e % V);
   return ((j >> 2) * chunks + c) * 4 + (j & 3);
 }
 
@@ -246,12 +268,27 @@ __device__ __forceinline__ void qn_rotate(float (&a)[V], float (&b)[V], const fl
       qn_fma<V>(a, b, ns, a);
       qn_fma<V>(b, b, cs, x);
     } else {
+      constexpr int E = V / 2;
       auto turn = [&](float (&z)[V], int i, int j) {
-        const float x = z[2 * i], y = z[2 * i + 1];
-        z[2 * i] = x * cs[j] - y * sn[j];
-        z[2 * i + 1] = y * cs[j] + x * sn[j];
+        const int at = qn_reg<V>(2 * i), to = qn_reg<V>(2 * i + 1);
+        const float x = z[at], y = z[to];
+        z[at] = x * cs[j] - y * sn[j];
+        z[to] = y * cs[j] + x * sn[j];
       };
-      if (rot % (2 * V) == 0) {  // whole chunks
+      if (V == 8 && rot % (2 * V) == 0) {  // whole chunks, even and odd elements side by side
+        auto turn2 = [&](float (&z)[V], int i, int j) {
+          float t0, t1;
+          qn_mul2(t0, t1, z[i], z[i + 1], sn[j], sn[j + 1]);
+          qn_mul2(z[i], z[i + 1], z[i], z[i + 1], cs[j], cs[j + 1]);
+          qn_fma2(z[i], z[i + 1], z[E + i], z[E + i + 1], -sn[j], -sn[j + 1], z[i], z[i + 1]);
+          qn_fma2(z[E + i], z[E + i + 1], z[E + i], z[E + i + 1], cs[j], cs[j + 1], t0, t1);
+        };
+#pragma unroll
+        for (int i = 0; i < E; i += 2) {
+          turn2(a, i, i);
+          turn2(b, i, E + i);
+        }
+      } else if (rot % (2 * V) == 0) {
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
           turn(a, i, i);
@@ -290,7 +327,7 @@ __device__ __forceinline__ void qn_fill_table(const QnParams& p, float* tbl, con
     const float rest = (float)(turns - rint(turns));
     float s, c;
     sincospif(2.f * rest, &s, &c);
-    float* at = tbl + t * np * V * 2 + qn_table_slot<V>(a / V, a % V, np);
+    float* at = tbl + t * np * V * 2 + qn_table_slot<V>(a / V, p.interleaved ? a % V : qn_reg<V>(a % V), np);
     at[0] = c;
     at[qn_sine<V>()] = s;
   }
@@ -419,6 +456,7 @@ __global__ void __launch_bounds__(QN_THREADS, QN_FWD_BLOCKS) qn_fwd_kernel(const
         vb[i] = nb[i];
       }
       load(row + n_grp);
+      qn_ask<T, V>(R, t0, row + QN_AHEAD * n_grp, rows, D, lane, false);
       if (norm || (kind < 2 && p.rot)) {  // else a copy, bit by bit
         float a[NP][V], b[NP][V];
 #pragma unroll
@@ -567,6 +605,7 @@ __device__ __forceinline__ void qn_bwd_rows(const QnParams& p, const QnRows& R, 
         yb[i] = mb[i];
       }
       if (it + 1 < iters) load(row + n_grp);
+      qn_ask<T, V>(R, t0, row + QN_AHEAD * n_grp, rows, D, lane, true);
       float a[NP][V], b[NP][V], da[NP][V], db[NP][V];
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
@@ -639,8 +678,9 @@ __device__ __forceinline__ void qn_bwd_rows(const QnParams& p, const QnRows& R, 
       }
       if ((threadIdx.x & 31) < g) {
         float* dst = red + warp * 2 * QN_MAX_D;
-        if (ha[i]) { dst[ca[i] * V + j] = dwa[i][j]; dst[QN_MAX_D + ca[i] * V + j] = dba[i][j]; }
-        if (hb[i]) { dst[cb[i] * V + j] = dwb[i][j]; dst[QN_MAX_D + cb[i] * V + j] = dbb[i][j]; }
+        const int ea = ca[i] * V + qn_elem<V>(j), eb = cb[i] * V + qn_elem<V>(j);
+        if (ha[i]) { dst[ea] = dwa[i][j]; dst[QN_MAX_D + ea] = dba[i][j]; }
+        if (hb[i]) { dst[eb] = dwb[i][j]; dst[QN_MAX_D + eb] = dbb[i][j]; }
       }
     }
   __syncthreads();
