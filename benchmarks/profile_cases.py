@@ -214,10 +214,56 @@ def case_adamw(iters: int) -> dict:
     return {"kernel": "adamw_kernel", "ms": ms, "gbs": nbytes / ms / 1e6, "bytes": nbytes}
 
 
+def case_head_norm(iters: int) -> dict:
+    """Per-head RMS norm + interleaved rotation, forward + backward: 8192 tokens, 32 and 8 heads of 128."""
+    mk = lambda h: torch.randn(8192, h, 128, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    q, k, dq, dk = mk(32).requires_grad_(), mk(8).requires_grad_(), mk(32), mk(8)
+    w = [torch.ones(128, device="cuda", dtype=torch.bfloat16, requires_grad=True) for _ in range(2)]
+    pos = torch.arange(8192, device="cuda", dtype=torch.int32)
+
+    def step():
+        out = K.qk_norm_rope(q, k, w[0], w[1], positions=pos, rotary=(128, 10000.0, True))
+        torch.autograd.grad(out, [q, k, *w], [dq, dk])
+
+    ms = _time(step, iters, _flush_buffer())
+    return {"kernel": "qk_norm_rope forward + backward", "ms": ms, "bytes": 5 * (q.numel() + k.numel()) * 2,
+            "gbs": 5 * (q.numel() + k.numel()) * 2 / ms / 1e6}
+
+
+def _paged(batch: int, new: int, length: int, heads: int, kv_heads: int, dim: int, page: int):
+    pages = -(-length // page)
+    mk = lambda *shape: torch.randn(*shape, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    table = torch.randperm(batch * pages, device="cuda").to(torch.int32).view(batch, pages)
+    cu = torch.arange(0, (batch + 1) * new, new, device="cuda", dtype=torch.int32)
+    lens = torch.full((batch,), length, device="cuda", dtype=torch.int32)
+    return (mk(batch * new, heads, dim), mk(batch * pages, page, kv_heads, dim), mk(batch * pages, page, kv_heads, dim),
+            table, cu, lens)
+
+
+def case_paged_decode(iters: int) -> dict:
+    """One new token of 64 sequences of 4000 tokens, 32 heads over 8 of 128, pages of 16."""
+    from scaling_b200.ops.paged_attention import paged_attention
+
+    args = _paged(64, 1, 4000, 32, 8, 128, 16)
+    ms = _time(lambda: paged_attention(*args), iters, _flush_buffer())
+    moved = 2 * 64 * 4000 * 8 * 128 * 2
+    return {"kernel": "paged_attn (narrow)", "ms": ms, "bytes": moved, "gbs": moved / ms / 1e6}
+
+
+def case_paged_chunk(iters: int) -> dict:
+    """Chunks of 2048 new tokens at the end of two sequences of 6000, 32 heads over 8 of 128, pages of 64."""
+    from scaling_b200.ops.paged_attention import paged_attention
+
+    args = _paged(2, 2048, 6000, 32, 8, 128, 64)
+    ms = _time(lambda: paged_attention(*args), iters, _flush_buffer())
+    pairs = 2 * 32 * (2048 * (6000 - 2048) + 2048 * 2049 / 2)
+    return {"kernel": "paged_attn (wide)", "ms": ms, "tflops": 4 * 128 * pairs / ms / 1e9}
+
+
 CASES = {"gemm_fp8": case_gemm_fp8, "gemm_fp8_large": case_gemm_fp8_large, "gemm_fwd": case_gemm_fwd, "gemm_plain": case_gemm_plain, "gemm_wgrad": case_gemm_wgrad,
          "attention_fwd": case_attention_fwd, "attention_bwd": case_attention_bwd,
          "attention_fwd_d64": case_attention_fwd_d64, "attention_fwd_d128": case_attention_fwd_d128, "attention_bwd_d128": case_attention_bwd_d128, "norm": case_norm,
-         "adamw": case_adamw}
+         "adamw": case_adamw, "head_norm": case_head_norm, "paged_decode": case_paged_decode, "paged_chunk": case_paged_chunk}
 
 
 def main() -> None:

@@ -18,8 +18,8 @@
 // Measured on one B200 (copy 6.57 TB/s), forward and backward together: 8192 tokens, 32 + 8 heads of 128, RMS, interleaved
 // rotation, bf16: 116 us = 3.6 TB/s (0.55 of the copy); 16384 tokens, 12 + 12 heads of 64, layer norm with biases, packed
 // projection: 84 us (0.46); a decoding step's append 6.4 us; an append of some 6000 prompt tokens, 40 + 1 heads: 39 us (0.52).
-// Bound by instructions and by the latency that 24 warps per SM can cover, not by the memory's rate: 55 to 61 % of the issue
-// slots, 30 % of the DRAM cycles.  Per element there are conversions, the norm's shuffles and three passes of fp32
+// Bound by latency at the occupancy that the registers leave (three blocks per SM forward, two backward; 51 and 39 % of the
+// issue slots, 35 % of the DRAM cycles).  Per element there are conversions, the norm's shuffles and three passes of fp32
 // arithmetic; hence the packed fp32 forms, weights in registers, code of its own per kind of row and per common head size.
 //
 // Angles: a position of 10^5 times a frequency near 1 in fp32 is off by 10^-2 rad.  The host computes turns per position

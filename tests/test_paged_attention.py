@@ -637,3 +637,23 @@ def test_page_tables_of_too_many_positions_are_refused():
     with pytest.raises(KernelError):
         paged_attention(q, cache, cache, torch.zeros(1, 2 ** 19 + 1, dtype=torch.int32, device=DEV), cu, lens)
     K.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [1, 255, 256, 257, 513, 1000])
+def test_append_of_many_sequences(batch):
+    """Sequences with none to three new tokens, some of them empty: each token finds its own sequence."""
+    rng = random.Random(batch)
+    new = [rng.choice([0, 0, 1, 1, 2, 3]) for _ in range(batch)]
+    lens = [n + rng.choice([0, 1, 15, 16, 40]) for n in new]
+    if sum(new) == 0:
+        new[0], lens[0] = 2, 20
+    b = Batch(lens, new, 16, 1, 16, torch.float32, DEV, heads=2, spare_rows=4, fill=0.0)
+    q = paged_append(b.k, b.v, *b.args(), q=b.q)
+    want_k, want_v = torch.zeros_like(b.k_cache), torch.zeros_like(b.v_cache)
+    for t, (s, pos) in enumerate(b.positions()):
+        page, slot = b.place(s, pos)
+        want_k[page, slot], want_v[page, slot] = b.k[t], b.v[t]
+    assert torch.equal(b.k_cache, want_k) and torch.equal(b.v_cache, want_v)
+    assert torch.equal(q[:b.tokens], b.q[:b.tokens]) and torch.count_nonzero(q[b.tokens:]) == 0
+    K.check_status()
