@@ -24,30 +24,44 @@ def on_gpu(*ts: Optional[torch.Tensor]) -> bool:
     return any(t is not None and t.is_cuda for t in ts)
 
 
-# --------------------------------------------------------------------------- status word
-_STATUS: dict[int, torch.Tensor] = {}
+# --------------------------------------------------------------------------- status words
+_STATUS: dict[int, tuple[torch.Tensor, torch.Tensor]] = {}
 
 
-def status_word() -> torch.Tensor:
-    """Per-device int32 that kernels with bounded waits set when a wait expires."""
+def _status_words() -> tuple[torch.Tensor, torch.Tensor]:
     d = torch.cuda.current_device()
     if d not in _STATUS:
-        _STATUS[d] = torch.zeros(1, dtype=torch.int32, device=f"cuda:{d}")
+        both = torch.zeros(2, dtype=torch.int32, device=f"cuda:{d}")
+        _STATUS[d] = (both[:1], both[1:])
     return _STATUS[d]
 
 
+def status_word() -> torch.Tensor:
+    """Per-device int32 that kernels with bounded waits set when a wait expires.  Optimizer steps read it: results that
+    such a kernel left incomplete must not reach the parameters."""
+    return _status_words()[0]
+
+
+def argument_word() -> torch.Tensor:
+    """Per-device int32 for errors that spoil the call's own outputs and nothing else: tables and lengths of a paged cache
+    that are wrong on the device.  ``check_status`` reads it, optimizer steps do not."""
+    return _status_words()[1]
+
+
 def check_status() -> None:
-    """Synchronising read of the status word; raises CommTimeout if a device-side wait gave up."""
+    """Synchronising read of the status words; raises CommTimeout if a device-side wait gave up, KernelError if a call
+    found a bad argument on the device.  An error is raised once."""
     if not torch.cuda.is_available():
         return
     d = torch.cuda.current_device()
     if d in _STATUS:
-        v = int(_STATUS[d].item())
-        if v != 0:
-            _STATUS[d].zero_()
-            if d in _GEMM_WS:
-                _GEMM_WS[d][:4096].zero_()  # an aborted split-K launch may have left tile counters behind
-            check(v, "device status word")
+        for word in _STATUS[d]:
+            v = int(word.item())
+            if v != 0:
+                word.zero_()
+                if word is _STATUS[d][0] and d in _GEMM_WS:
+                    _GEMM_WS[d][:4096].zero_()  # an aborted split-K launch may have left tile counters behind
+                check(v, "device status word")
 
 
 # --------------------------------------------------------------------------- GEMM

@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from ._lib import check, dt, lib, ptr, sm_count, stream
-from .functional import _common_dtype, _unit_inner, check_head_norm, head_norm_rope_reference, rotary_args, status_word
+from .functional import _common_dtype, _unit_inner, argument_word, check_head_norm, head_norm_rope_reference, rotary_args
 
 
 def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -148,7 +148,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
             0 if q is None else q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), k_cache.stride(0),
             k_cache.stride(1), k_cache.stride(2), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2),
             page_table.stride(0), page_table.shape[1], num_pages, page_size, float(eps), int(rms), rot, base,
-            int(interleaved), code, w_code, sm_count(), status_word().data_ptr(), stream()), "sb200_paged_append")
+            int(interleaved), code, w_code, sm_count(), argument_word().data_ptr(), stream()), "sb200_paged_append")
     return out
 
 
@@ -252,5 +252,5 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             num_pages, page_size, cols, page_table.stride(0), q.stride(0), q.stride(1), out.stride(0), out.stride(1),
             k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), v_cache.stride(0), v_cache.stride(1),
             v_cache.stride(2), int(causal), -1 if window is None else min(int(window), 2 ** 30), scale, int(zero_tail),
-            dt(q.dtype), sms, status_word().data_ptr(), stream()), "sb200_paged_attention")
+            dt(q.dtype), sms, argument_word().data_ptr(), stream()), "sb200_paged_attention")
     return out

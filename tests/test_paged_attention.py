@@ -657,3 +657,45 @@ def test_append_of_many_sequences(batch):
     assert torch.equal(b.k_cache, want_k) and torch.equal(b.v_cache, want_v)
     assert torch.equal(q[:b.tokens], b.q[:b.tokens]) and torch.count_nonzero(q[b.tokens:]) == 0
     K.check_status()
+
+
+def _optimizer():
+    from scaling_b200.core.nn.parameter_meta import CoreParameterMeta
+    from scaling_b200.core.optimizer import (LearningRateSchedulerConfig, Optimizer, OptimizerConfig, OptimizerParamGroup,
+                                             OptimizerParamGroupConfig)
+    from scaling_b200.parallel import Topology, TopologyConfig
+
+    topology = Topology(TopologyConfig.from_dict({
+        "world_size": 1, "model_parallel_size": 1, "pipe_parallel_size": 1, "global_rank": 0, "local_slot": 0,
+        "micro_batch_size": 1, "gradient_accumulation_steps": 1}))
+    p = torch.nn.Parameter(torch.ones(64, device=DEV))
+    CoreParameterMeta.register_on_parameter(p, is_model_parallel=False, layer_index=0, parameter_name="w")
+    group = OptimizerParamGroup([("w", p, p.core_parameter_meta)], OptimizerParamGroupConfig(
+        name="g", weight_decay=0.0, learning_rate_scheduler=LearningRateSchedulerConfig(
+            learning_rate=0.1, learning_rate_decay_style="constant")))
+    return p, Optimizer(OptimizerConfig(zero=False), [group], topology)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["append", "page", "length"])
+def test_bad_places_do_not_reach_the_optimizer(what):
+    """An error in a table or a length belongs to its call: the next optimizer step is taken, the error is still raised."""
+    K.check_status()
+    b = _attend_batch([200, 150], [6, 3], 16, 4, 2, 64, torch.bfloat16, DEV)
+    kc, vc, table, cu, sl = b.args()
+    p, opt = _optimizer()
+    if what == "append":
+        paged_append(b.k, b.v, kc, vc, table, cu, torch.full_like(sl, -3))
+    elif what == "page":
+        table[0, 3] = kc.shape[0]
+        paged_attention(b.q, kc, vc, table, cu, sl)
+    else:
+        sl[0] = 10 ** 6
+        paged_attention(b.q, kc, vc, table, cu, sl)
+    before = p.detach().clone()
+    p.grad.fill_(1.0)
+    out = opt.step()
+    assert not out.overflow and not torch.equal(p.detach(), before)
+    with pytest.raises(KernelError):
+        K.check_status()
+    K.check_status()
