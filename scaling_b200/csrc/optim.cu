@@ -267,3 +267,8 @@ SB_API int sb200_bind_device(int device) {
   e = cudaFree(nullptr);  // forces the primary context to be current on this thread
   return (int)e;
 }
+// Sets the calling thread's stream capture mode (a cudaStreamCaptureMode) and returns the one before, or -1.
+SB_API int sb200_exchange_capture_mode(int mode) {
+  cudaStreamCaptureMode m = (cudaStreamCaptureMode)mode;
+  return cudaThreadExchangeStreamCaptureMode(&m) == cudaSuccess ? (int)m : -1;
+}

@@ -71,6 +71,7 @@ _SIGS = {
     "sb200_qk_norm_rope_bwd": [c_void_p] * 14 + [c_int] * 5 + [c_long] * 8 + [c_float, c_int, c_int, c_double, c_int, c_int, c_int, c_int, c_void_p],
     "sb200_paged_append": [c_void_p] * 14 + [c_int] * 5 + [c_long] * 13 + [c_int] * 3 + [c_float, c_int, c_int, c_double, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "sb200_paged_attention_workspace": [c_int] * 5 + [c_long, c_int],
+    "sb200_exchange_capture_mode": [c_int],
     "sb200_paged_attention": [c_void_p] * 8 + [c_long] + [c_int] * 8 + [c_long] * 11 + [c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p],
     "sb200_masked_softmax_fwd": [c_void_p, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_float, c_int, c_void_p],
     "sb200_masked_softmax_bwd": [c_void_p, c_void_p, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_float, c_int, c_void_p],
@@ -141,7 +142,8 @@ class _Counting:
 
 
 _NO_LAUNCH = {"sb200_p2p_max_ranks", "sb200_colsum_splits", "sb200_norm_bwd_partial_rows", "sb200_norm_bwd_partial_rows_h", "sb200_sumsq_max_partials",
-              "sb200_bind_device", "sb200_fa_last_driver_error", "sb200_qk_norm_rope_bwd_blocks", "sb200_paged_attention_workspace"}
+              "sb200_bind_device", "sb200_fa_last_driver_error", "sb200_qk_norm_rope_bwd_blocks", "sb200_paged_attention_workspace",
+              "sb200_exchange_capture_mode"}
 
 
 def kernel_calls() -> int:
@@ -233,6 +235,28 @@ def on_device_of(t: torch.Tensor):
     if t.get_device() == torch.cuda.current_device():
         return _NO_CONTEXT
     return torch.cuda.device(t.device)
+
+
+_CAPTURE_RELAXED = 2  # cudaStreamCaptureModeRelaxed
+
+
+@contextlib.contextmanager
+def outside_captures():
+    """Context with a current stream that takes part in no graph capture, and whose work is complete at its end: what is
+    allocated and written inside belongs to no graph, even where the caller's stream is being captured."""
+    before = lib().sb200_exchange_capture_mode(_CAPTURE_RELAXED)  # else a capture forbids allocating and waiting
+    try:
+        for _ in range(64):  # streams come from a pool: one of them may be the captured one
+            side = torch.cuda.Stream()
+            with torch.cuda.stream(side):
+                if not torch.cuda.is_current_stream_capturing():
+                    yield
+                    side.synchronize()
+                    return
+        raise KernelError("every stream is being captured")
+    finally:
+        if before >= 0:
+            lib().sb200_exchange_capture_mode(before)
 
 
 _SM_COUNT: dict[int, int] = {}

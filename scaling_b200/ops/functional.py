@@ -31,7 +31,8 @@ _STATUS: dict[int, tuple[torch.Tensor, torch.Tensor]] = {}
 def _status_words() -> tuple[torch.Tensor, torch.Tensor]:
     d = torch.cuda.current_device()
     if d not in _STATUS:
-        both = torch.zeros(2, dtype=torch.int32, device=f"cuda:{d}")
+        with _lib.outside_captures():  # a captured call must not clear the words at every replay
+            both = torch.zeros(2, dtype=torch.int32, device=f"cuda:{d}")
         _STATUS[d] = (both[:1], both[1:])
     return _STATUS[d]
 

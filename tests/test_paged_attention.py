@@ -699,3 +699,25 @@ def test_bad_places_do_not_reach_the_optimizer(what):
     with pytest.raises(KernelError):
         K.check_status()
     K.check_status()
+
+
+@pytest.mark.gpu
+def test_errors_outlast_replays_where_the_first_call_was_captured(monkeypatch):
+    """The status words are made by the first call: inside a capture, too, they belong to no graph."""
+    b = Batch([20, 5], [6, 1], 16, 2, 64, torch.bfloat16, DEV)
+    paged_append(b.k, b.v, *b.args())
+    K.check_status()
+    monkeypatch.setattr(K, "_STATUS", {})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged_append(b.k, b.v, *b.args())
+    K.check_status()
+    good = b.table.clone()
+    b.table[0, 1] = -1
+    graph.replay()
+    b.table.copy_(good)
+    graph.replay()  # a good call does not take the error back
+    with pytest.raises(KernelError):
+        K.check_status()
+    graph.replay()
+    K.check_status()
