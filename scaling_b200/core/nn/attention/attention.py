@@ -17,6 +17,7 @@ from enum import Enum
 from typing import Any, Callable, Dict, List, Optional, Tuple, Union
 
 import torch
+from torch.nn.modules.module import _has_any_global_hook
 
 from ....ops import functional as K
 from ....ops.attention import attention_mask_from_cu_seqlens, flash_attention
@@ -380,9 +381,9 @@ class ParallelSelfAttention(torch.nn.Module):
 
     def _head_norm_fused(self, q: torch.Tensor) -> bool:
         """Norms and rotation of queries and keys run as one kernel: on the GPU, with plain norm modules (no u-muP scales,
-        no hooks that want to see their outputs) and all heads on this rank."""
+        no hooks that want to see their outputs, registered for a module or for all of them) and all heads on this rank."""
         norms = (self.norm_query, self.norm_key)
-        return (q.is_cuda and self.model_parallel_size == 1 and q.dtype in (torch.bfloat16, torch.float16, torch.float32)
+        return (q.is_cuda and not _has_any_global_hook() and self.model_parallel_size == 1 and q.dtype in (torch.bfloat16, torch.float16, torch.float32)
                 and q.shape[-1] <= 256 and q.numel() > 0
                 and (self.rotary_embedding is None or self.rotary_embedding.dimensions % 2 == 0)
                 and not any(n._use_umup or n._forward_hooks or n._forward_pre_hooks or n._backward_hooks

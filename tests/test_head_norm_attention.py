@@ -113,3 +113,38 @@ def test_cached_generation_step_uses_the_same_kernel():
                  m(x[:, 20:], cu(1), torch.tensor([[20]], device="cuda"), use_cache=True)]
     got = torch.cat(parts, 1)
     assert (got.float() - whole.float()).norm() <= 4 * 2.0 ** -8 * whole.float().norm()
+
+
+class _Metrics:
+    """Takes the place of the logger and of the training context."""
+
+    iterations = 0
+
+    def __init__(self):
+        self.names = set()
+
+    def log_metrics(self, metrics, **_):
+        self.names.update(metrics)
+
+    def warning(self, *_):
+        pass
+
+
+@pytest.mark.gpu
+def test_traced_steps_record_the_norms():
+    from scaling_b200.core.logging.tensor_statistics_recorder import (TensorStatistics, TensorStatisticsRecorder,
+                                                                      TensorStatisticsRecorderConfig)
+
+    m = _attention(NormType.RMS, "cuda", torch.bfloat16)
+    model = torch.nn.Module()
+    model._layers = torch.nn.ModuleList([m])
+    log = _Metrics()
+    config = TensorStatisticsRecorderConfig(statistics=[("*", [TensorStatistics.MEAN])])
+    recorder = TensorStatisticsRecorder(config, log, model, logger=log)
+    x = torch.randn(1, 16, 256, device="cuda").bfloat16().requires_grad_()
+    cu = torch.tensor([0, 16], dtype=torch.int32, device="cuda")
+    with recorder.trace():
+        m(x, cu, None).float().sum().backward()
+    for norm in ("norm_query", "norm_key"):
+        for mode in ("forward", "backward"):
+            assert f"activation_statistics/layers.0.{norm}_{mode}_mean" in log.names
