@@ -380,14 +380,16 @@ class ParallelSelfAttention(torch.nn.Module):
         return norm(t)
 
     def _head_norm_fused(self, q: torch.Tensor) -> bool:
-        """Norms and rotation of queries and keys run as one kernel: on the GPU, with plain norm modules (no u-muP scales,
-        no hooks that want to see their outputs, registered for a module or for all of them) and all heads on this rank."""
+        """Norms and rotation of queries and keys run as one kernel: on the GPU, with plain norm modules (of this package's
+        classes, no u-muP scales, no hooks that want to see their outputs, registered for a module or for all of them) and
+        all heads on this rank."""
         norms = (self.norm_query, self.norm_key)
-        return (q.is_cuda and not _has_any_global_hook() and self.model_parallel_size == 1 and q.dtype in (torch.bfloat16, torch.float16, torch.float32)
-                and q.shape[-1] <= 256 and q.numel() > 0
+        return (q.is_cuda and not _has_any_global_hook() and self.model_parallel_size == 1
+                and q.dtype in (torch.bfloat16, torch.float16, torch.float32) and q.shape[-1] <= 256 and q.numel() > 0
                 and (self.rotary_embedding is None or self.rotary_embedding.dimensions % 2 == 0)
+                and type(norms[0]) is type(norms[1]) and type(norms[0]) in (LayerNorm, RMSNorm)
                 and not any(n._use_umup or n._forward_hooks or n._forward_pre_hooks or n._backward_hooks
-                            or n._backward_pre_hooks for n in norms))
+                            or n._backward_pre_hooks or "forward" in vars(n) for n in norms))
 
     def _head_norm_and_rotary(self, q: torch.Tensor, k: torch.Tensor,
                               pos: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:

@@ -148,3 +148,32 @@ def test_traced_steps_record_the_norms():
     for norm in ("norm_query", "norm_key"):
         for mode in ("forward", "backward"):
             assert f"activation_statistics/layers.0.{norm}_{mode}_mean" in log.names
+
+
+class _Half(torch.nn.Module):
+    def forward(self, x):
+        return 0.5 * x
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["module", "one module", "forward"])
+def test_norm_modules_that_were_exchanged_are_called(how):
+    """Modules put in place of the norms, and a forward of an instance's own, run instead of the kernel."""
+    m = _attention(NormType.RMS, "cuda", torch.float32, rotary="none")
+    x = torch.randn(1, 16, 256, device="cuda")
+    cu = torch.tensor([0, 16], dtype=torch.int32, device="cuda")
+    seen = {}
+    core = m.scaled_dot_product_attention
+    real = core.forward
+    core.forward = lambda q, k, v, *a, **kw: (seen.update(q=q, k=k), real(q, k, v, *a, **kw))[1]
+    with torch.no_grad():
+        q, k, _ = m._project_qkv(x)
+        want_k = K.rms_norm(k, m.norm_key.weight, m.norm_key.eps)
+        if how == "forward":
+            m.norm_query.forward = lambda t: 0.5 * t
+        else:
+            m.norm_query = _Half()
+        if how == "module":
+            m.norm_key, want_k = _Half(), 0.5 * k
+        m(x, cu, None)
+    assert torch.equal(seen["q"], 0.5 * q) and torch.equal(seen["k"], want_k)
