@@ -172,6 +172,11 @@ class FlashAttention(_AttentionCore):
         return self._post(out)
 
 
+def _norm_epsilon(norm: Union[LayerNorm, RMSNorm]) -> float:
+    """What the module's own forward adds to the denominator."""
+    return norm.eps if isinstance(norm, RMSNorm) else norm.config.layernorm_epsilon
+
+
 class ParallelSelfAttention(torch.nn.Module):
     def __init__(self, hidden_size: int, num_attention_heads: int, masked_softmax_config: MaskedSoftmaxConfig,
                  causal: bool = True, num_local_attention_heads: int = 0,
@@ -388,6 +393,7 @@ class ParallelSelfAttention(torch.nn.Module):
                 and q.dtype in (torch.bfloat16, torch.float16, torch.float32) and q.shape[-1] <= 256 and q.numel() > 0
                 and (self.rotary_embedding is None or self.rotary_embedding.dimensions % 2 == 0)
                 and type(norms[0]) is type(norms[1]) and type(norms[0]) in (LayerNorm, RMSNorm)
+                and _norm_epsilon(norms[0]) == _norm_epsilon(norms[1])
                 and not any(n._use_umup or n._forward_hooks or n._forward_pre_hooks or n._backward_hooks
                             or n._backward_pre_hooks or "forward" in vars(n) for n in norms))
 
@@ -398,7 +404,7 @@ class ParallelSelfAttention(torch.nn.Module):
         bias = (lambda n: None) if rms else (lambda n: getattr(n, n.bias_name))
         rotary = None if rot is None else (rot.dimensions, rot.base, rot.interleaved)
         return K.qk_norm_rope(q, k, nq.weight, nk.weight, q_bias=bias(nq), k_bias=bias(nk), positions=pos, rotary=rotary,
-                              eps=nq.config.layernorm_epsilon, rms=rms)
+                              eps=_norm_epsilon(nq), rms=rms)
 
     # ------------------------------------------------------------------ forward
     def forward(self, x: torch.Tensor, cumulative_seq_lengths: Optional[torch.Tensor],

@@ -177,3 +177,23 @@ def test_norm_modules_that_were_exchanged_are_called(how):
             m.norm_key, want_k = _Half(), 0.5 * k
         m(x, cu, None)
     assert torch.equal(seen["q"], 0.5 * q) and torch.equal(seen["k"], want_k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eps", [(0.5, 0.5), (0.5, 1e-5)])
+def test_the_modules_own_epsilon_is_used(eps):
+    m = _attention(NormType.RMS, "cuda", torch.float32, rotary="none")
+    m.norm_query.eps, m.norm_key.eps = eps
+    x = 0.1 * torch.randn(1, 16, 256, device="cuda")
+    cu = torch.tensor([0, 16], dtype=torch.int32, device="cuda")
+    seen = {}
+    core = m.scaled_dot_product_attention
+    real = core.forward
+    core.forward = lambda q, k, v, *a, **kw: (seen.update(q=q, k=k), real(q, k, v, *a, **kw))[1]
+    with torch.no_grad():
+        q, k, _ = m._project_qkv(x)
+        m(x, cu, None)
+    for got, t, norm in ((seen["q"], q, m.norm_query), (seen["k"], k, m.norm_key)):
+        want = t.double() * torch.rsqrt(t.double().pow(2).mean(-1, keepdim=True) + norm.eps) * norm.weight.double()
+        # a sum of 64 squares, the division, the root and two products: below 32 half steps of fp32
+        assert ((got - want).abs() <= 32 * 2.0 ** -24 * want.abs() + 2.0 ** -120).all()
