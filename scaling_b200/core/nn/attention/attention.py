@@ -438,6 +438,8 @@ class ParallelSelfAttention(torch.nn.Module):
             assert self.norm_query is not None and self.norm_key is not None
             fused = self._head_norm_fused(q)
             if fused:
+                if pos is not None and pos.dtype.is_floating_point:  # accepted, as by the separate rotation
+                    pos = pos.to(torch.int32)
                 q, k = self._head_norm_and_rotary(q, k, pos)
             else:
                 q = self._qk_norm(q, self.norm_query)

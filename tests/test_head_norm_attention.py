@@ -197,3 +197,15 @@ def test_the_modules_own_epsilon_is_used(eps):
         want = t.double() * torch.rsqrt(t.double().pow(2).mean(-1, keepdim=True) + norm.eps) * norm.weight.double()
         # a sum of 64 squares, the division, the root and two products: below 32 half steps of fp32
         assert ((got - want).abs() <= 32 * 2.0 ** -24 * want.abs() + 2.0 ** -120).all()
+
+
+@pytest.mark.gpu
+def test_floating_point_position_ids():
+    m = _attention(NormType.RMS, "cuda", torch.bfloat16)
+    x = torch.randn(2, 16, 256, device="cuda").bfloat16()
+    cu = torch.tensor([0, 16, 32], dtype=torch.int32, device="cuda")
+    pos = torch.arange(16, device="cuda").repeat(2, 1)
+    with torch.no_grad():
+        want = m(x, cu, pos)
+        for kind in (torch.float32, torch.float64, torch.int32, torch.int16):
+            assert torch.equal(m(x, cu, pos.to(kind)), want)
