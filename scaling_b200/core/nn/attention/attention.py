@@ -447,8 +447,11 @@ class ParallelSelfAttention(torch.nn.Module):
 
         if self.rotary_embedding is not None and not fused:
             rot = self.rotary_embedding
-            q = apply_rotary_tokens(q, pos, rot.dimensions, rot.base, rot.interleaved)
-            k = apply_rotary_tokens(k, pos, rot.dimensions, rot.base, rot.interleaved)
+            rotary = (rot.dimensions, rot.base, rot.interleaved)
+            if self.key_query_norm:  # the angles of the fused form: what a layer computes does not depend on the way it runs
+                q, k = K.head_rotation(q, pos, rotary), K.head_rotation(k, pos, rotary)
+            else:
+                q, k = apply_rotary_tokens(q, pos, *rotary), apply_rotary_tokens(k, pos, *rotary)
 
         if use_cache:
             if not self.causal:

@@ -719,6 +719,41 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     return _qk_norm_rope_launch(*args)
 
 
+def _head_rotation_launch(x, pos, rot, base, interleaved):
+    T, H, D = x.shape
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    with _lib.on_device_of(x):
+        check(lib().sb200_qk_norm_rope_fwd(
+            x.data_ptr(), None, y.data_ptr(), None, None, None, None, None, pos.data_ptr(), T, H, 0, D, x.stride(0),
+            x.stride(1), 0, 0, 0.0, 1, rot, base, interleaved, dt(x.dtype), 0, sm_count(), stream()),
+            "sb200_qk_norm_rope_fwd")
+    return y
+
+
+class _HeadRotationFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, pos, rot, base, interleaved):  # type: ignore[override]
+        ctx.save_for_backward(pos)
+        ctx.cfg = (rot, base, interleaved)
+        return _head_rotation_launch(_unit_inner(x), pos, rot, base, interleaved)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):  # type: ignore[override]
+        (pos,) = ctx.saved_tensors  # the transposed rotation is the one by the opposite angle
+        return _head_rotation_launch(_unit_inner(dy), -pos, *ctx.cfg), None, None, None, None
+
+
+def head_rotation(x: torch.Tensor, positions: torch.Tensor, rotary: tuple[int, float, bool]) -> torch.Tensor:
+    """The rotation of ``qk_norm_rope`` on its own, with the same angles: ``x [tokens, heads, d]`` after a norm that ran as
+    a module.  (``rope`` forms its angles in fp32: 1e-2 rad off at position 10^5.)"""
+    rot, base, interleaved = rotary_args(rotary, x.shape[2])
+    if x.is_cuda and x.dtype in _KERNEL_DTYPES and x.shape[2] <= 256 and 0 < x.numel() and x.shape[0] < 2 ** 31 - 2 ** 16:
+        return _HeadRotationFn.apply(x, positions.to(torch.int32).contiguous(), rot, base, interleaved)
+    y = x if x.dtype == torch.float64 else x.float()
+    return rotate_reference(y, positions, (rot, base, interleaved)).to(x.dtype)
+
+
 # --------------------------------------------------------------------------- masked softmax
 class _MaskedSoftmaxFn(torch.autograd.Function):
     @staticmethod

@@ -209,3 +209,25 @@ def test_floating_point_position_ids():
         want = m(x, cu, pos)
         for kind in (torch.float32, torch.float64, torch.int32, torch.int16):
             assert torch.equal(m(x, cu, pos.to(kind)), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rotary", ["rotary", "rotary_complex"])
+def test_far_positions_have_the_same_angles_in_every_form(rotary):
+    """One kernel, or separate operations because of a hook: the same queries and keys at positions of some millions."""
+    m = _attention(NormType.RMS, "cuda", torch.float32, rotary=rotary)
+    x = torch.randn(1, 64, 256, device="cuda")
+    cu = torch.tensor([0, 64], dtype=torch.int32, device="cuda")
+    pos = torch.arange(64, device="cuda")[None] * 79190 + 10 ** 6
+    seen = []
+    core = m.scaled_dot_product_attention
+    real = core.forward
+    core.forward = lambda q, k, v, *a, **kw: (seen.append((q, k)), real(q, k, v, *a, **kw))[1]
+    with torch.no_grad():
+        m(x, cu, pos)
+        handle = m.norm_query.register_forward_hook(lambda *a: None)
+        m(x, cu, pos)
+        handle.remove()
+    for a, b in zip(*seen):
+        # 64 half steps for the norm and the rotation in one kernel, 32 + 32 for the separate ones, of max|y|
+        assert ((a - b).abs() <= 128 * 2.0 ** -24 * a.abs().amax(-1, keepdim=True) * 2.0 ** 0.5).all()

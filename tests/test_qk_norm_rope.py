@@ -342,3 +342,39 @@ def test_more_rows_than_32_bits_of_elements():
         want, size = definition(x[t:t + 1], w, None, pos[t:t + 1], (64, 10000.0, False), 1e-5, True)
         _close(a[t:t + 1], want, size, FWD_STEPS, f"token {t}")
         _close(b[t:t + 1], want[:, :1], size[:, :1], FWD_STEPS, f"token {t}")
+
+
+# Rotation alone: the angle and its sine and cosine 8 steps (see above), two products and a sum of the pair 3, each of at
+# most sqrt(2) max|x|: below 32 in all.
+TURN_STEPS = 32
+
+
+def _check_head_rotation(x, pos, rotary, g):
+    leaf = x.detach().requires_grad_()
+    y = K.head_rotation(leaf, pos, rotary)
+    (dx,) = torch.autograd.grad(y, leaf, g)
+    _close(y, _turn(x.double(), pos, rotary, 1.0), x.double().abs().amax(-1, keepdim=True), TURN_STEPS, "y")
+    _close(dx, _turn(g.double(), pos, rotary, -1.0), g.double().abs().amax(-1, keepdim=True), TURN_STEPS, "dx")
+    with torch.no_grad():
+        assert torch.equal(K.head_rotation(x, pos, rotary), y)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rotary", [(16, 10000.0, False), (16, 500000.0, True), (6, 10000.0, True)])
+def test_rotation_alone_torch_expression(rotary, dtype):
+    q, _, _, _, pos, g, _ = _inputs(9, 3, 1, 16, dtype, dtype, True, "cpu")
+    _check_head_rotation(q, pos, rotary, g)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,H,D,rotary", [(1, 1, 64, (64, 10000.0, False)), (130, 12, 128, (128, 10000.0, True)),
+                                          (67, 5, 80, (20, 10000.0, False)), (33, 3, 50, (6, 500000.0, True)),
+                                          (9, 2, 256, (256, 10000.0, False)), (700, 71, 64, (32, 10000.0, False)),
+                                          (9, 2, 320, (64, 10000.0, False))])
+def test_rotation_alone_kernel(T, H, D, rotary, dtype):
+    q, _, _, _, pos, g, _ = _inputs(T, H, 1, D, dtype, dtype, True, DEV)
+    pos[0] = 10 ** 9
+    _check_head_rotation(q, pos, rotary, g)
+    turned = q.permute(1, 2, 0).contiguous().permute(2, 0, 1)  # as heads that were gathered over ranks come
+    assert torch.equal(K.head_rotation(turned, pos, rotary), K.head_rotation(q, pos, rotary))
