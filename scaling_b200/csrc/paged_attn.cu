@@ -280,11 +280,12 @@ __device__ __forceinline__ int pa_scan(int v, int lane) {
   }
   return v;
 }
-// Lengths are kept in 32 bits: a sum that may not fit becomes the largest value, which pa_find refuses.
-__device__ __forceinline__ int pa_sum(unsigned v) {
-  const bool huge = __any_sync(0xffffffffu, v > 0x3ffffffu);
-  const unsigned sum = __reduce_add_sync(0xffffffffu, v & 0x3ffffffu);
-  return huge ? 0x7fffffff : (int)sum;
+// Sum over the lanes.  Lengths are kept in 32 bits: one that does not fit becomes the largest value, which pa_find refuses
+// (a part of the whole that large makes the whole too large, however the sequences are grouped).
+__device__ __forceinline__ int pa_sum(long long v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return (int)min(v, 0x7fffffffLL);
 }
 // Length of all items of one KV head of sequence 32 * chunk + lane (0 beyond the last sequence); the whole warp calls.
 template <int ROWS> __device__ __forceinline__ int pa_chunk_cost(const PaParams& p, int chunk, int lane, PaSeq& s) {
@@ -301,7 +302,7 @@ template <int ROWS> __device__ __forceinline__ int pa_chunk_cost(const PaParams&
     const int cnt = pa_items<ROWS>(p, n);
     long long mine = 0;
     for (int m = lane; m < cnt; m += 32) mine += pa_item_cost<ROWS>(p, n, L, m);
-    const int sum = pa_sum((unsigned)min(mine, 0x7fffffffLL));
+    const int sum = pa_sum(mine);
     if (lane == src) cost = sum;
   }
   return cost;

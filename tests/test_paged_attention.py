@@ -721,3 +721,33 @@ def test_errors_outlast_replays_where_the_first_call_was_captured(monkeypatch):
         K.check_status()
     graph.replay()
     K.check_status()
+
+
+@pytest.mark.gpu
+def test_long_prompts_are_taken_beside_many_sequences_as_alone():
+    """2^19 tokens with 16 heads per KV head: some 2^26 products of 256 rows with 128 keys, far below 2^31.  Sequences
+    without new tokens do not change where the work is cut, so the outputs are equal bit by bit."""
+    n, heads = 2 ** 19, 16
+    g = torch.Generator(device=DEV).manual_seed(3)
+    kc, vc = (torch.randn(1, 128, 1, 8, generator=g, device=DEV).bfloat16() for _ in range(2))
+    q = torch.randn(n, heads, 8, generator=g, device=DEV).bfloat16()
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    K.check_status()
+    outs = []
+    for others in (0, 32):
+        table = torch.zeros(1 + others, n // 128, dtype=torch.int32, device=DEV)
+        outs.append(paged_attention(q, kc, vc, table, ints([0] + [n] * (1 + others)), ints([n] + [5] * others)))
+        K.check_status()
+    assert torch.equal(outs[0], outs[1])
+    for i in (0, 1, 127, 128, 300, n - 1):  # every page is the same one: position j has key j % 128
+        seen = torch.arange(i + 1, device=DEV)
+        count = torch.bincount(seen % 128, minlength=128).double()
+        k, v = kc[0, :, 0].double(), vc[0, :, 0].double()
+        z = q[i].double() @ k.t() / 8 ** 0.5
+        p = torch.exp(z - z.amax(-1, keepdim=True)) * count
+        want = p @ v / p.sum(-1, keepdim=True)
+        # as in attention_in_64_bits; the chain of additions has at most (i + 1) links of 2^-24 on average, full steps here
+        size = (q[i].double().abs() @ k.abs().t()).amax(-1, keepdim=True) / 8 ** 0.5
+        rel = 2.0 ** -8 + 2 * (size * 16 * 2.0 ** -23 + 2.0 ** -21) + (i + 1) * 2.0 ** -23
+        w = p @ v.abs() / p.sum(-1, keepdim=True)
+        assert ((outs[0][i].double() - want).abs() <= rel * w + 2.0 ** -8 * (want.abs() + rel * w)).all(), i
