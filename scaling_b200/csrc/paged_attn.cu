@@ -317,9 +317,10 @@ struct PaCut {
     return place < longer ? place / (per + 1) : rest + (place - longer) / per;
   }
 };
-struct PaCursor {  // where a CTA's piece of the line starts, and how long it is
+struct PaCursor {  // where a CTA's piece of the line starts, and how long it is; refused: the line is too long for any
   PaSeq s;
   int seq, hk, m, tile, left, place;
+  bool refused;
   PaCut cut;
 };
 
@@ -339,8 +340,9 @@ __device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int 
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   all *= p.Hkv;
-  if (all >= 0x7fffffff) {  // half a minute of work and more: reported, nothing done
+  if (all >= 0x7fffffff) {  // half a minute of work and more: reported, pa_schedule writes zeros
     if (lane == 0) *p.status = SB_ERR_TOO_LARGE;
+    c.refused = true;
     return;
   }
   PaCut& cut = c.cut;
@@ -399,6 +401,21 @@ __device__ __forceinline__ uint32_t pa_k_place(int t, int lead) { return t < lea
 __device__ __forceinline__ uint32_t pa_v_place(int t, int lead, int count) { return t + min(t + lead, count); }
 template <int ROWS> __device__ __forceinline__ int pa_lead(int rows) { return PaKind<ROWS>::NARROW ? 4 : rows > PA_TILE ? 1 : 2; }
 
+// Zeros for this kernel's sequences, shared out over the CTAs: a call that does nothing else leaves no older memory there.
+template <int ROWS> __device__ __forceinline__ void pa_zero_refused(const PaParams& p, int lane) {
+  const int per_head = p.D / 8, per_token = p.Hkv * p.group * per_head;
+  for (int b = 0; b < p.batch; ++b) {
+    const PaSeq s = pa_seq(p, b);
+    if (pa_items<ROWS>(p, s.n) == 0) continue;
+    for (int t = blockIdx.x; t < s.n; t += gridDim.x)
+      for (int i = lane; i < per_token; i += 32) {
+        const int h = i / per_head;
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + (long)(s.row0 + t) * p.o_tok + (long)h * p.o_head +
+                                  (i - h * per_head) * 8) = make_uint4(0, 0, 0, 0);
+      }
+  }
+}
+
 // ============================================================================ roles that both kernels share
 // Warp 10: cuts the piece into items, publishes their descriptors and copies their queries.
 template <int ROWS, int PANELS>
@@ -410,6 +427,7 @@ __device__ __forceinline__ void pa_schedule(const PaParams& p, PaCtrl<PaCfg<PANE
   PaCursor cur;
   pa_find<ROWS>(p, reinterpret_cast<const int*>(sQ), chunks, lane, cur);
   __syncwarp();
+  if (cur.refused) pa_zero_refused<ROWS>(p, lane);
   int* desc = p.part_desc + 8 * blockIdx.x;
   bool starts = false, ok = true;
   int q_cnt = 0;

@@ -751,3 +751,24 @@ def test_long_prompts_are_taken_beside_many_sequences_as_alone():
         rel = 2.0 ** -8 + 2 * (size * 16 * 2.0 ** -23 + 2.0 ** -21) + (i + 1) * 2.0 ** -23
         w = p @ v.abs() / p.sum(-1, keepdim=True)
         assert ((outs[0][i].double() - want).abs() <= rel * w + 2.0 ** -8 * (want.abs() + rel * w)).all(), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("given", [False, True])
+def test_a_refused_call_leaves_zeros(given):
+    """Lengths that add up to more than 2^31: nothing of what the memory held before is in the output."""
+    n, heads, spare = 2 ** 20, 64, 3
+    cache = torch.ones(1, 128, 1, 8, dtype=torch.bfloat16, device=DEV)
+    q = torch.zeros(n + spare, heads, 8, dtype=torch.bfloat16, device=DEV)
+    table = torch.zeros(1, 2 ** 14, dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([2 ** 21], dtype=torch.int32, device=DEV)
+    K.check_status()
+    out = torch.full_like(q, 7.0)
+    if not given:
+        del out  # its memory is given to the call's result
+    out = paged_attention(q, cache, cache, table, cu, lens, out=out if given else None)
+    with pytest.raises(KernelError, match="size"):
+        K.check_status()
+    assert torch.count_nonzero(out[:n]) == 0
+    assert (out[n:] == (7 if given else 0)).all()
