@@ -87,7 +87,7 @@ struct PaParams {
   float sl2;
   float* part_o;       // [2 slots per CTA][part_rows][DP]
   float2* part_ml;     // [2 slots per CTA][part_rows]: reference (log2 domain) and sum
-  int* part_desc;      // [CTAs][8]: item that starts in this CTA and ends in a later one
+  int* part_desc;      // [CTAs][8]: item that starts in this CTA and ends in a later one (first word: there is one; -1: refused)
   int part_rows, zero_tail;
   int* status;
 };
@@ -340,7 +340,7 @@ __device__ __forceinline__ void pa_find(const PaParams& p, const int* sums, int 
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   all *= p.Hkv;
-  if (all >= 0x7fffffff) {  // half a minute of work and more: reported, pa_schedule writes zeros
+  if (all >= 0x7fffffff) {  // half a minute of work and more: reported, the last kernel writes zeros
     if (lane == 0) *p.status = SB_ERR_TOO_LARGE;
     c.refused = true;
     return;
@@ -401,21 +401,6 @@ __device__ __forceinline__ uint32_t pa_k_place(int t, int lead) { return t < lea
 __device__ __forceinline__ uint32_t pa_v_place(int t, int lead, int count) { return t + min(t + lead, count); }
 template <int ROWS> __device__ __forceinline__ int pa_lead(int rows) { return PaKind<ROWS>::NARROW ? 4 : rows > PA_TILE ? 1 : 2; }
 
-// Zeros for this kernel's sequences, shared out over the CTAs: a call that does nothing else leaves no older memory there.
-template <int ROWS> __device__ __forceinline__ void pa_zero_refused(const PaParams& p, int lane) {
-  const int per_head = p.D / 8, per_token = p.Hkv * p.group * per_head;
-  for (int b = 0; b < p.batch; ++b) {
-    const PaSeq s = pa_seq(p, b);
-    if (pa_items<ROWS>(p, s.n) == 0) continue;
-    for (int t = blockIdx.x; t < s.n; t += gridDim.x)
-      for (int i = lane; i < per_token; i += 32) {
-        const int h = i / per_head;
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + (long)(s.row0 + t) * p.o_tok + (long)h * p.o_head +
-                                  (i - h * per_head) * 8) = make_uint4(0, 0, 0, 0);
-      }
-  }
-}
-
 // ============================================================================ roles that both kernels share
 // Warp 10: cuts the piece into items, publishes their descriptors and copies their queries.
 template <int ROWS, int PANELS>
@@ -427,7 +412,6 @@ __device__ __forceinline__ void pa_schedule(const PaParams& p, PaCtrl<PaCfg<PANE
   PaCursor cur;
   pa_find<ROWS>(p, reinterpret_cast<const int*>(sQ), chunks, lane, cur);
   __syncwarp();
-  if (cur.refused) pa_zero_refused<ROWS>(p, lane);
   int* desc = p.part_desc + 8 * blockIdx.x;
   bool starts = false, ok = true;
   int q_cnt = 0;
@@ -507,7 +491,7 @@ __device__ __forceinline__ void pa_schedule(const PaParams& p, PaCtrl<PaCfg<PANE
     }
     q_cnt += slots;
   }
-  if (lane == 0) desc[0] = starts && ok;
+  if (lane == 0) desc[0] = cur.refused ? -1 : starts && ok;
 }
 
 // K tiles, V tiles, or both in the order of the ring.
@@ -1300,6 +1284,23 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 // A task is a block of rows of an item that several CTAs worked on: eight rows with a thread per four columns, or, with many
 // parts, one row whose parts are dealt to eight groups of threads that are joined in order.  Every block lists the tasks
 // (one descriptor per CTA) and takes every gridDim-th, so the launch is one wave whatever the items are.
+
+// Zeros for the sequences of a kernel that refused the call's work: nothing else writes there, and the memory may hold
+// older tensors.  Called from the last kernel, as a function: inside the kernels that refuse, the code took 5 % of a decoding
+// step's time although it does not run (147 -> 154 us), inlined in the last one 1 us.
+template <int ROWS> __device__ __noinline__ void pa_zero_refused(const PaParams& p) {
+  const int per_head = p.D / 8, per_token = p.Hkv * p.group * per_head;
+  for (int b = 0; b < p.batch; ++b) {
+    const PaSeq s = pa_seq(p, b);
+    if (pa_items<ROWS>(p, s.n) == 0) continue;
+    for (int t = blockIdx.x; t < s.n; t += gridDim.x)
+      for (int i = threadIdx.x; i < per_token; i += PA_COMBINE_THREADS) {
+        const int h = i / per_head;
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + (long)(s.row0 + t) * p.o_tok + (long)h * p.o_head +
+                                  (i - h * per_head) * 8) = make_uint4(0, 0, 0, 0);
+      }
+  }
+}
 template <int PANELS, bool F16>
 __global__ void __launch_bounds__(PA_COMBINE_THREADS, 4)
     pa_combine_kernel(const __grid_constant__ PaParams pn, const __grid_constant__ PaParams pw, int narrow_ctas, int ctas) {
@@ -1307,7 +1308,7 @@ __global__ void __launch_bounds__(PA_COMBINE_THREADS, 4)
   __shared__ float4 so[PG][QUADS];
   __shared__ float2 sml[PG];
   __shared__ int swarp[WARPS];
-  __shared__ int stask[3];
+  __shared__ int stask[3], srefused[2];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int quad = threadIdx.x % QUADS, pg = threadIdx.x / QUADS;
@@ -1318,7 +1319,10 @@ __global__ void __launch_bounds__(PA_COMBINE_THREADS, 4)
     if (mine < ctas) {
       const int local = mine < narrow_ctas ? mine : mine - narrow_ctas;
       const int* desc = (mine < narrow_ctas ? pn : pw).part_desc + 8 * local;
-      if (desc[0]) tasks = desc[5] - local < PG ? (desc[4] + PG - 1) / PG : desc[4];
+      const int head = desc[0];
+      if (mine == 0) srefused[0] = head < 0;
+      if (mine == narrow_ctas) srefused[1] = head < 0;
+      if (head > 0) tasks = desc[5] - local < PG ? (desc[4] + PG - 1) / PG : desc[4];
     }
     const int inc = pa_scan(tasks, lane);
     __syncthreads();
@@ -1391,6 +1395,8 @@ __global__ void __launch_bounds__(PA_COMBINE_THREADS, 4)
     }
     before += all;
   }
+  if (srefused[0]) pa_zero_refused<PA_NARROW_ROWS>(pn);
+  if (ctas > narrow_ctas && srefused[1]) pa_zero_refused<PA_WIDE_ROWS>(pw);
 }
 
 typedef CUresult (*PaEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
