@@ -970,6 +970,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     pa_load<R, PANELS, true, false>(p, c, sRing, &tmK, &tmV, lane);
   } else if (warp == 11) {
     pa_load<R, PANELS, false, true>(p, c, sRing, &tmK, &tmV, lane);
+    if (blockIdx.x == 0) {  // sequences that do not follow one another inside the rows: reported (pa_seq cuts them)
+      for (int b = lane; b < p.batch; b += 32)
+        if (p.cu[b] < 0 || p.cu[b + 1] < p.cu[b] || p.cu[b + 1] > p.T) *p.status = SB_ERR_BAD_ARG;
+    }
     if (p.zero_tail) {  // rows before the first and behind the last sequence
       const int before = p.batch > 0 ? min(max(p.cu[0], 0), p.T) : 0, heads = p.Hkv * p.group;
       const int gap = p.batch > 0 ? max(min(p.cu[p.batch], p.T), before) - before : 0, per_row = p.D / 8;
@@ -1540,7 +1544,8 @@ SB_API long sb200_paged_attention_workspace(int T, int batch, int Hq, int Hkv, i
 // Sequence b: rows cu[b] .. cu[b + 1] of q, its last new token at position lens[b] - 1; position j in row j % page_size of
 // page table[b][j / page_size].  A query at position i sees keys j <= i (causal), |i - j| <= window (window >= 0).  page_size is a power of two from 8, D a
 // multiple of 8 up to 128; pointers and strides are multiples of 16 bytes.  Rows behind the last sequence are left as
-// they are, or zeroed with zero_tail (as rows before the first).  Visible pages outside the cache and lengths outside the table set *status.
+// they are, or zeroed with zero_tail (as rows before the first).  Visible pages outside the
+// cache, lengths outside the table and sequences that do not follow one another inside the T rows set *status.
 SB_API int sb200_paged_attention(const void* q, const void* k_cache, const void* v_cache, void* out, const int* table,
                                  const int* cu, const int* lens, void* workspace, long workspace_bytes, int T, int batch,
                                  int Hq, int Hkv, int D, int num_pages, int page_size, int cols, long table_ld, long q_tok,

@@ -404,6 +404,9 @@ __global__ void __launch_bounds__(QN_THREADS, QN_FWD_BLOCKS) qn_fwd_kernel(const
     } else {
       spos[threadIdx.x] = p.pos ? p.pos[t] : 0;
     }
+  } else if (PAGED && blockIdx.x == 0 && threadIdx.x >= QN_MAX_SLOTS) {  // threads without a token
+    for (int b = threadIdx.x - QN_MAX_SLOTS; b < p.batch; b += QN_THREADS - QN_MAX_SLOTS)
+      if (p.cu[b] < 0 || p.cu[b + 1] < p.cu[b] || p.cu[b + 1] > p.T) *p.status = SB_ERR_BAD_ARG;
   }
   int ca[NP], cb[NP];
   bool ha[NP], hb[NP];
@@ -815,7 +818,8 @@ SB_API int sb200_qk_norm_rope_fwd(const void* q, const void* k, void* q_out, voi
 // The paged form.  Row t belongs to the sequence b with cu[b] <= t < cu[b + 1]; its position is
 // lens[b] - cu[b + 1] + t, and k / v go to row pos % page_size of page table[b][pos / page_size] of the caches
 // [num_pages, page_size, Hk, D] (page, row and head strides in elements, page_size a power of two).  A position outside
-// the table or a page outside the cache writes nothing and sets *status.  Rows behind the last sequence give zeros in
+// the table or a page outside the cache writes nothing and sets *status, as do sequences that do not follow one another
+// inside the T rows.  Rows behind the last sequence give zeros in
 // q_out and touch no page.  pos may override the rotation angles; q may be null (Hq = 0).
 SB_API int sb200_paged_append(const void* q, const void* k, const void* v, void* q_out, void* k_cache, void* v_cache,
                               const void* q_w, const void* k_w, const void* q_b, const void* k_b, const int* pos,

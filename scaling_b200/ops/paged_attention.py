@@ -65,13 +65,20 @@ def _no_grad_inputs(what: str, *ts: Optional[torch.Tensor]) -> None:
         raise _lib.KernelError(f"{what} has no backward pass: call it under torch.no_grad()")
 
 
+def _row_ends(cu_seqlens: torch.Tensor, tokens: int) -> list[int]:
+    cu = cu_seqlens.tolist()
+    if any(not 0 <= a <= b <= tokens for a, b in zip(cu, cu[1:])):
+        raise ValueError(f"cu_seqlens {cu} do not follow one another inside {tokens} rows")
+    return cu
+
+
 def _token_places(page_table: torch.Tensor, cu_seqlens: torch.Tensor, seq_lens: torch.Tensor, tokens: int,
                   page_size: int, num_pages: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(row, position, page, slot) of the new tokens that belong to a sequence; raises on a token without a place."""
     rows, places = [], []
-    cu, lens = cu_seqlens.tolist(), seq_lens.tolist()
+    cu, lens = _row_ends(cu_seqlens, tokens), seq_lens.tolist()
     for b, length in enumerate(lens):
-        start, end = max(cu[b], 0), min(cu[b + 1], tokens)
+        start, end = cu[b], cu[b + 1]
         rows.extend(range(start, end))
         places.extend((b, length - cu[b + 1] + t) for t in range(start, end))
     row = torch.tensor(rows, dtype=torch.int64)
@@ -159,11 +166,11 @@ def paged_attention_reference(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     size, kv_heads = k_cache.shape[1], k_cache.shape[2]
     acc = torch.float64 if q.dtype == torch.float64 else torch.float32
     group = q.shape[1] // kv_heads
-    cu = cu_seqlens.tolist()
+    cu = _row_ends(cu_seqlens, q.shape[0])
     for b, length in enumerate(seq_lens.tolist()):
-        start, end = min(max(cu[b], 0), q.shape[0]), min(cu[b + 1], q.shape[0])
+        start, end = cu[b], cu[b + 1]
         n = end - start
-        if n <= 0:
+        if n == 0:
             continue
         if not 0 <= length <= page_table.shape[1] * size:
             raise ValueError(f"sequence {b} has length {length}, its page table {page_table.shape[1] * size} places")

@@ -772,3 +772,33 @@ def test_a_refused_call_leaves_zeros(given):
         K.check_status()
     assert torch.count_nonzero(out[:n]) == 0
     assert (out[n:] == (7 if given else 0)).all()
+
+
+WRONG_ROWS = [[0, 4, 9], [0, 8, 6], [-2, 3, 7], [3, 1, 7]]  # of two sequences in seven rows
+
+
+@pytest.mark.parametrize("cu", WRONG_ROWS)
+def test_rows_that_do_not_follow_one_another_on_the_cpu(cu):
+    b = _attend_batch([20, 30], [4, 3], 16, 2, 2, 64, torch.float32, "cpu")
+    kc, vc, table, _, sl = b.args()
+    wrong = torch.tensor(cu, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        paged_append(b.k, b.v, kc, vc, table, wrong, sl)
+    with pytest.raises(ValueError):
+        paged_attention(b.q, kc, vc, table, wrong, sl)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("others", [0, 300])
+@pytest.mark.parametrize("cu", WRONG_ROWS)
+def test_rows_that_do_not_follow_one_another_are_reported(cu, others):
+    b = _attend_batch([20, 30] + [9] * others, [4, 3] + [0] * others, 16, 2, 2, 64, torch.bfloat16, DEV)
+    kc, vc, table, good, sl = b.args()
+    last = max(cu[2], 0)
+    wrong = torch.tensor(cu + [last] * others, dtype=torch.int32, device=DEV)
+    for call in (lambda c: paged_append(b.k, b.v, kc, vc, table, c, sl), lambda c: paged_attention(b.q, kc, vc, table, c, sl)):
+        call(wrong)
+        with pytest.raises(KernelError):
+            K.check_status()
+        call(good)
+        K.check_status()
