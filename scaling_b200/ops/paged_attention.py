@@ -54,6 +54,17 @@ def _check_sizes(what: str, *sizes: int) -> None:
         raise _lib.KernelError(f"{what}: sizes {sizes} pass 32 bits")
 
 
+def _refuse_shared_memory(name: str, t: torch.Tensor) -> None:
+    """Written tensors need memory of their own for every element (sufficient: each stride spans the smaller ones)."""
+    if t.is_contiguous():
+        return
+    span = 1
+    for stride, size in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
+        if stride < span:
+            raise ValueError(f"elements of {name} share memory: rows {tuple(t.shape)} with strides {t.stride()}")
+        span += stride * (size - 1)
+
+
 def _check_rows(name: str, x: torch.Tensor, k_cache: torch.Tensor) -> None:
     if x.dim() != 3 or x.shape[2] != k_cache.shape[3] or x.dtype != k_cache.dtype or x.device != k_cache.device:
         raise ValueError(f"{name} {tuple(x.shape)} {x.dtype} {x.device} does not fit a cache "
@@ -120,6 +131,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
             raise ValueError(f"q has {q.shape[0]} tokens, k {k.shape[0]}")
     elif q_weight is not None or q_bias is not None:
         raise ValueError("norm parameters for queries without queries")
+    _refuse_shared_memory("k_cache", k_cache)
+    _refuse_shared_memory("v_cache", v_cache)
     rot, base, interleaved = rotary_args(rotary, k.shape[2])
     if positions is not None and (positions.shape != (k.shape[0],) or positions.dtype != torch.int32
                                   or positions.device != k.device or not positions.is_contiguous()):
@@ -223,8 +236,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError(f"window must not be negative, got {window}")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device):
         raise ValueError(f"out {tuple(out.shape)} {out.dtype} {out.device} does not match q {tuple(q.shape)} {q.dtype}")
-    if out is not None and any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
-        raise ValueError(f"rows of out share memory (strides {out.stride()})")
+    if out is not None:
+        _refuse_shared_memory("out", out)
     if not q.is_cuda:
         return paged_attention_reference(q, k_cache, v_cache, page_table, cu_seqlens, seq_lens, causal, scale, window,
                                          torch.zeros_like(q) if out is None else out)

@@ -802,3 +802,23 @@ def test_rows_that_do_not_follow_one_another_are_reported(cu, others):
             K.check_status()
         call(good)
         K.check_status()
+
+
+def test_written_tensors_whose_elements_share_memory_are_refused():
+    b = _attend_batch([20], [4], 16, 4, 2, 64, torch.bfloat16, "cpu")
+    kc, vc, table, cu, sl = b.args()
+    flat = torch.zeros(kc.numel(), dtype=torch.bfloat16)
+    for shared in (kc[:, :, :1].expand(kc.shape), kc[:1].expand(kc.shape), flat.as_strided(kc.shape, (64, 64, 64, 1)),
+                   flat.as_strided(kc.shape, (16 * 128 - 64, 128, 64, 1))):
+        for caches in ((shared, vc), (kc, shared)):
+            with pytest.raises(ValueError, match="share memory"):
+                paged_append(b.k, b.v, *caches, table, cu, sl)
+        paged_attention(b.q, shared, vc, table, cu, sl)  # caches that are read only may be any view
+    with pytest.raises(ValueError, match="share memory"):
+        paged_attention(b.q, *b.args(), out=flat.as_strided((4, 4, 64), (128, 64, 1)))
+    # layouts in use: pages of keys and values side by side, heads before tokens, more columns than the head has
+    for view in (torch.zeros(kc.shape[0], 2, *kc.shape[1:], dtype=torch.bfloat16)[:, 0],
+                 torch.zeros(kc.shape[0], 2, 16, 64, dtype=torch.bfloat16).transpose(1, 2),
+                 torch.zeros(*kc.shape[:3], 72, dtype=torch.bfloat16)[..., :64],
+                 torch.zeros(kc.shape[0], 16, 2, 2, 64, dtype=torch.bfloat16)[:, :, :, 1]):
+        paged_append(b.k, b.v, view, view.clone(), table, cu, sl)
