@@ -822,3 +822,58 @@ def test_written_tensors_whose_elements_share_memory_are_refused():
                  torch.zeros(*kc.shape[:3], 72, dtype=torch.bfloat16)[..., :64],
                  torch.zeros(kc.shape[0], 16, 2, 2, 64, dtype=torch.bfloat16)[:, :, :, 1]):
         paged_append(b.k, b.v, view, view.clone(), table, cu, sl)
+
+
+def _many(batch, kind, seed):
+    """(lens, new) of more sequences than a warp has lanes: the work is found by groups of 32 of them."""
+    rng = random.Random(seed)
+    long = lambda: rng.choice([0, 1, 15, 127, 128, 129, 640, 1500, rng.randrange(3500)])  # noqa: E731
+    if kind == "tokens":  # one new token each
+        new = [1] * batch
+    elif kind == "mixed":  # single tokens, a few tokens, chunks of more than 64 rows
+        new = [rng.choice([1, 1, 1, 2, 5, 17, 40, 90]) if b % 3 else 1 for b in range(batch)]
+    else:  # runs of sequences without new tokens, longer than a group, between the others
+        new = [rng.choice([1, 3, 30]) if b in (2, batch // 2, batch - 1) else 0 for b in range(batch)]
+    lens = [n + long() for n in new]
+    lens[rng.randrange(batch)] = 3600  # the table is wider than the plan for short ones takes
+    return lens, new
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,dim,window", [(4, 1, 64, None), (4, 2, 128, None), (6, 2, 64, 700)])
+@pytest.mark.parametrize("kind", ["tokens", "mixed", "runs"])
+@pytest.mark.parametrize("batch", [33, 64, 100])
+def test_more_sequences_than_lanes_with_divided_items(batch, kind, heads, kv_heads, dim, window):
+    lens, new = _many(batch, kind, batch)
+    b = _attend_batch(lens, new, 16, heads, kv_heads, dim, torch.bfloat16, DEV)
+    out = paged_attention(b.q, *b.args(), window=window)
+    K.check_status()
+    _check_attention(b, out, True, window)
+    assert torch.equal(out, paged_attention(b.q, *b.args(), window=window))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_captured_chunks_and_tokens_follow_new_lengths(dim):
+    """Both kernels and the joining of parts in one graph, replayed with other lengths, offsets and tables."""
+    lens, new = _many(40, "mixed", 5)
+    b = _attend_batch(lens, new, 16, 4, 1, dim, torch.bfloat16, DEV)
+    paged_attention(b.q, *b.args())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = paged_attention(b.q, *b.args())
+    full = b.seq_lens.clone()
+    half = torch.tensor([max(n, length // 2) for n, length in zip(new, lens)], dtype=torch.int32, device=DEV)
+    turned = torch.tensor([0] + new[::-1], device=DEV).cumsum(0).to(torch.int32)
+    for lengths, cu, table in ((full, b.cu, b.table), (half, b.cu, b.table), (full.flip(0), turned, b.table.flip(0))):
+        args = (b.k_cache, b.v_cache, table.clone(), cu.clone(), lengths.clone())
+        want = paged_attention(b.q, *args)
+        keep = [t.clone() for t in (b.table, b.cu, b.seq_lens)]
+        b.table.copy_(args[2]), b.cu.copy_(args[3]), b.seq_lens.copy_(args[4])
+        out.fill_(float("nan"))
+        graph.replay()
+        assert torch.equal(out, want)
+        b.table.copy_(keep[0]), b.cu.copy_(keep[1]), b.seq_lens.copy_(keep[2])
+    K.check_status()
+    _check_attention(b, paged_attention(b.q, *b.args()), True, None)
