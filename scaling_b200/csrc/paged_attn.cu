@@ -45,6 +45,8 @@
 // step per probability, averaged over the row), the output once.
 #include <cuda.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace {
@@ -679,7 +681,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         if (count == 0) break;
         // step u: with two_q tile u / 2 and its halves in turn, else tile u and half x.  Both groups take every tile in
         // the ring's order: the parity of a barrier that a warp has not followed phase by phase says nothing.
-        const int lead = two_q ? 1 : 2, n = two_q ? 2 * count : count, shift = two_q;
+        const int lead = two_q ? 1 : 2, n = two_q ? 2 * count : count;
         const int qu = q_cnt + (two_q ? x : 0), qs = qu & 1;
         ok = pa_wait_lane(&c.q_full[qs], (qu >> 1) & 1, abort_flag);
         // ring places of the next K and V tile, as stage and parity
@@ -1287,10 +1289,6 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 }
 
 // ============================================================================ joining the partial results
-// A task is a block of rows of an item that several CTAs worked on: eight rows with a thread per four columns, or, with many
-// parts, one row whose parts are dealt to eight groups of threads that are joined in order.  Every block lists the tasks
-// (one descriptor per CTA) and takes every gridDim-th, so the launch is one wave whatever the items are.
-
 // Zeros for the sequences of a kernel that refused the call's work: nothing else writes there, and the memory may hold
 // older tensors.  Called from the last kernel, as a function: inside the kernels that refuse, the code took 5 % of a decoding
 // step's time although it does not run (147 -> 154 us), inlined in the last one 1 us.
@@ -1307,6 +1305,11 @@ template <int ROWS> __device__ __noinline__ void pa_zero_refused(const PaParams&
       }
   }
 }
+
+// A task is a block of rows of an item that several CTAs worked on: PG rows (8, or 16 where a head has up to 64 columns) with a
+// thread per four columns, or, with PG parts and more, one row whose parts are dealt to PG groups of threads that are joined in
+// order.  Every block lists the tasks (one descriptor per CTA) and takes every gridDim-th, so the launch is one wave whatever the
+// items are.
 template <int PANELS, bool F16>
 __global__ void __launch_bounds__(PA_COMBINE_THREADS, 4)
     pa_combine_kernel(const __grid_constant__ PaParams pn, const __grid_constant__ PaParams pw, int narrow_ctas, int ctas) {
@@ -1453,11 +1456,12 @@ long pa_align(long v) { return (v + 255) & ~255L; }
 // the wide launch would find nothing and cost its 3 us, and a sequence that does have more rows is read once per 64 of them.
 struct PaPlan {
   bool wide, whole;
-  int narrow_max, narrow_rows, narrow_ctas, wide_ctas;
+  int narrow_max, narrow_rows, narrow_ctas, wide_ctas, sms;
   long narrow_at, wide_at, bytes;
 };
 PaPlan pa_plan(long T, int batch, int Hq, int Hkv, int D, long cap, int sms) {
   PaPlan w = {};
+  w.sms = sms;
   const long rows = T * (Hq / Hkv), dp = D <= 64 ? 64 : 128;
   w.wide = rows > PA_NARROW_ROWS && T > batch;
   // with up to eight tiles per item, dividing them costs more (a second launch, partial results) than it balances
@@ -1523,7 +1527,8 @@ int pa_launch(const CUtensorMap& tmK, const CUtensorMap& tmV, PaParams p, const 
   if (e != cudaSuccess) return (int)e;
   if (w.whole) return SB_OK;
   const int ctas = w.narrow_ctas + w.wide_ctas;
-  cfg.gridDim = dim3(w.wide || ctas >= 128 ? 4 * 148 : 4 * ctas);
+  // one wave of the four blocks per SM that fit; fewer for few descriptors (an item of the wide kernel has up to 32 tasks)
+  cfg.gridDim = dim3(std::min(4 * w.sms, (w.wide ? 32 : 4) * ctas));
   cfg.blockDim = dim3(PA_COMBINE_THREADS);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;

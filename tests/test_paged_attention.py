@@ -877,3 +877,15 @@ def test_captured_chunks_and_tokens_follow_new_lengths(dim):
         b.table.copy_(keep[0]), b.cu.copy_(keep[1]), b.seq_lens.copy_(keep[2])
     K.check_status()
     _check_attention(b, paged_attention(b.q, *b.args()), True, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sms", [1, 7, 40])
+def test_work_shared_out_over_fewer_multiprocessors(sms, monkeypatch):
+    from scaling_b200.ops import paged_attention as module
+
+    monkeypatch.setattr(module, "sm_count", lambda: sms)
+    for lens, new in (([3000, 900], [1, 1]), ([3000, 900, 5], [200, 1, 5])):
+        b = _attend_batch(lens, new, 16, 8, 2, 128, torch.bfloat16, DEV)
+        _check_attention(b, paged_attention(b.q, *b.args()), True, None)
+    K.check_status()
