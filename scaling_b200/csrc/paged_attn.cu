@@ -60,6 +60,10 @@ constexpr int PA_THREADS = PA_WARPS * 32;
 constexpr int PA_REGS_FEW = 80, PA_REGS_MANY = 208;
 constexpr int PA_PANEL = 16384;   // 128 rows x 128 bytes
 constexpr int PA_ITEMS = 4;       // descriptors in flight
+// The tensor core truncates when it adds to TMEM: with equal weights an output of one was 0.997 after 2^20 keys and 0.987 after
+// 2^22.  So a group's sums (O and the row sums) go to a second place after that many tiles of 128 keys (2^14 keys) and
+// start from zero; what is added there is rounded to nearest.
+constexpr int PA_FOLD = 128;
 constexpr int PA_COMBINE_THREADS = 256;
 // A wait can last as long as one item: 2^19 tiles at the longest.  Measured per tile: 2 to 3 us, 5.5 us where all CTAs read
 // the same page; so 1 to 3 s, and some room for other work on the GPU.
@@ -643,6 +647,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   using Cfg = PaCfg<PANELS>;
   constexpr int DP = Cfg::DP, TILE_BYTES = Cfg::TILE_BYTES, STAGES = Cfg::STAGES;
   constexpr uint32_t S_COL = 0, O_COL = 256;  // two S of 64 columns per group, two O of DP
+  constexpr int FOLD = 2 * PA_FOLD;           // in half tiles
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;  // two slots of 128 rows
   uint8_t* sRing = smem + Cfg::FRONT;
@@ -718,7 +723,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             const uint64_t vd = v_desc + vs * (TILE_BYTES >> 4) + half * half_step;
 #pragma unroll
             for (int kk = 0; kk < PA_HALF / 16; ++kk)
-              pa_umma_ts(o_col, s_col + b * PA_HALF + kk * 8, vd + kk * v_step, idesc_o, u > 0 || kk != 0);
+              pa_umma_ts(o_col, s_col + b * PA_HALF + kk * 8, vd + kk * v_step, idesc_o, u % FOLD != 0 || kk != 0);
           }
           if (next) {
             const uint64_t qd = q_desc + qs * (TILE_BYTES >> 4), kd = k_desc + ks * (TILE_BYTES >> 4) + half * half_step;
@@ -758,6 +763,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const uint32_t o_addr = t_lane + O_COL + x * DP;
     const float sl2 = p.sl2;
     uint32_t ring = 0, s_cnt0 = 0, s_cnt1 = 0, merges = 0;  // s_cnt: steps taken on each buffer
+    // second place of this thread's row: the second partial slot, which no item but the CTA's last one writes, at its end
+    float* const far = p.part_o + ((2L * blockIdx.x + 1) * p.part_rows + x * PA_TILE + r) * DP;
     bool ok = true;
     for (int i = 0; ok; ++i) {
       const int islot = i % PA_ITEMS;
@@ -781,6 +788,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         hi = p.causal ? min(pos + 1, it.L) : (p.window >= 0 ? (int)min((long)it.L, (long)pos + p.window + 1) : it.L);
       }
       float ref = -INFINITY, l = 0.f;
+      float far_ref = -INFINITY, far_l = 0.f;  // what the sums of the second place refer to, and its row sum
       const int n = two_q ? 2 * it.count : it.count;  // half tiles of this group
       for (int u = 0; u < n; ++u) {
         const int t = two_q ? u >> 1 : u, b = u & 1, half = two_q ? b : x;
@@ -805,7 +813,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             m4[(j >> 1) & 3] = pa_max3(m4[(j >> 1) & 3], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
           const float mx = pa_max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
           const bool move = (mx - ref) * sl2 > 8.f || (ref == -INFINITY && mx > -INFINITY);
-          if (__any_sync(0xffffffffu, move)) {
+          const bool fold = u > 0 && u % FOLD == 0;
+          if (fold || __any_sync(0xffffffffu, move)) {
             const float next = move ? mx : ref;
             const float alpha = move ? (ref == -INFINITY ? 0.f : pa_exp2((ref - next) * sl2)) : 1.f;
             ref = next;
@@ -816,14 +825,30 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
               if (u + 1 < n ? !pa_wait(&c.s_full[x * 2 + (b ^ 1)], (b ? s_cnt0 : s_cnt1) & 1, abort_flag)
                             : !pa_wait(&c.p_empty[x * 2], i & 1, abort_flag)) { ok = false; break; }
               sb::tc_fence_after();
-#pragma unroll
+              const float beta = far_ref == -INFINITY ? 0.f : pa_exp2((far_ref - ref) * sl2);
+#pragma unroll 1
               for (int ch = 0; ch < DP / 32; ++ch) {
                 uint32_t o[32];
                 sb::tmem_ld32(o_addr + ch * 32, o);
                 sb::tmem_ld_wait();
 #pragma unroll
                 for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-                pa_tmem_st32(o_addr + ch * 32, o);
+                if (!fold) {
+                  pa_tmem_st32(o_addr + ch * 32, o);
+                } else {
+#pragma unroll
+                  for (int j = 0; j < 32; j += 4) {
+                    float4* at = reinterpret_cast<float4*>(far + ch * 32 + j);
+                    const float4 v = u > FOLD ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+                    *at = make_float4(fmaf(v.x, beta, __uint_as_float(o[j])), fmaf(v.y, beta, __uint_as_float(o[j + 1])),
+                                      fmaf(v.z, beta, __uint_as_float(o[j + 2])), fmaf(v.w, beta, __uint_as_float(o[j + 3])));
+                  }
+                }
+              }
+              if (fold) {
+                far_l = fmaf(far_l, beta, l);
+                far_ref = ref;
+                l = 0.f;
               }
             }
           }
@@ -856,6 +881,26 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       if (!ok) break;
       if (!pa_wait(&c.p_empty[x * 2 + 1], i & 1, abort_flag)) break;  // the last product
       sb::tc_fence_after();
+      if (n > FOLD && warp_rows > 0) {  // back from the second place
+        const float beta = far_ref == -INFINITY ? 0.f : pa_exp2((far_ref - ref) * sl2);
+        l = fmaf(far_l, beta, l);
+#pragma unroll 1
+        for (int ch = 0; ch < DP / 32; ++ch) {
+          uint32_t o[32];
+          sb::tmem_ld32(o_addr + ch * 32, o);
+          sb::tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(far + ch * 32 + j);
+            o[j] = __float_as_uint(fmaf(v.x, beta, __uint_as_float(o[j])));
+            o[j + 1] = __float_as_uint(fmaf(v.y, beta, __uint_as_float(o[j + 1])));
+            o[j + 2] = __float_as_uint(fmaf(v.z, beta, __uint_as_float(o[j + 2])));
+            o[j + 3] = __float_as_uint(fmaf(v.w, beta, __uint_as_float(o[j + 3])));
+          }
+          pa_tmem_st32(o_addr + ch * 32, o);
+        }
+        sb::tmem_st_wait();
+      }
       // the two states of a row: fa, fb scale the groups' outputs to a common reference
       float fa = x == 0 ? 1.f : 0.f, fb = 1.f - fa;
       int c0 = 0, c1 = DP / 32;
@@ -954,7 +999,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   using Cfg = PaCfg<PANELS>;
   constexpr int DP = Cfg::DP, TILE_BYTES = Cfg::TILE_BYTES, STAGES = Cfg::STAGES;
   constexpr int R = PA_NARROW_ROWS, Q_SLOT = PANELS * R * 128, P_BYTES = PA_TILE * 128;
-  constexpr uint32_t S_COL = 0, O_COL = 256;  // four S^T and two O^T of 64 columns
+  constexpr uint32_t S_COL = 0, O_COL = 256, FAR_COL = 384;  // four S^T, two O^T and their second places, of 64 columns
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;                    // two slots of 64 rows
   uint8_t* sP = smem + 2 * 16384;        // [group][key][64 rows], 128-byte swizzle
@@ -1036,7 +1081,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             const uint64_t vd = v_desc + st * (TILE_BYTES >> 4), pd = p_desc + x * (P_BYTES >> 4);
 #pragma unroll
             for (int kk = 0; kk < PA_TILE / 16; ++kk)
-              sb::umma_f16_ss(tmem_base + O_COL + x * R, vd + kk * v_step, pd + kk * (2048 >> 4), idesc_o, t > 1 || kk != 0);
+              sb::umma_f16_ss(tmem_base + O_COL + x * R, vd + kk * v_step, pd + kk * (2048 >> 4), idesc_o,
+                              (t >> 1) % PA_FOLD != 0 || kk != 0);
             sb::umma_commit(&c.empty[st]);
             sb::umma_commit(&c.p_empty[x]);
           }
@@ -1075,8 +1121,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                                   : (p.window >= 0 ? (int)min((long)it.L, (long)it.pos0 + p.window + 1) : it.L);
       int cur = 0;
       float* ref = sRef + x * 2 * R;
-      // row sums: of the first 16 rows per key in every thread, of the others over the warp's keys in lane row % 32
-      float l[16], l0 = 0.f, l1 = 0.f;
+      // row sums: of the first 16 rows per key in every thread, of the others over the warp's keys in lane row % 32; far0 and
+      // far1 take all of them from time to time
+      float l[16], l0 = 0.f, l1 = 0.f, far0 = 0.f, far1 = 0.f;
 #pragma unroll
       for (int u = 0; u < 16; ++u) l[u] = 0.f;
       for (int t = x; t < n; t += 2) {
@@ -1147,7 +1194,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           }
           return top;
         };
-        bool need = t < 2;  // no reference yet
+        const bool fold = t >= 2 && (t >> 1) % PA_FOLD == 0;
+        bool need = t < 2 || fold;  // no reference yet, or another place for the sums
         if (!need) {
           const int mine = __any_sync(0xffffffffu, probabilities() > 8.f);
           int* flags = c.need[x][votes & 1];
@@ -1180,22 +1228,39 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           cur ^= 1;
           l0 *= alpha[0];
           l1 *= alpha[1];
+          far0 *= alpha[0];
+          far1 *= alpha[1];
 #pragma unroll
           for (int u = 0; u < 16; ++u) l[u] *= __shfl_sync(0xffffffffu, alpha[0], u);
           if (t >= 2) {
+            const int folds = (t >> 1) / PA_FOLD;  // with this one
 #pragma unroll 1
             for (int b = 0; b < nb; ++b) {
-              uint32_t o[16];
-              sb::tmem_ld16(t_lane + O_COL + x * R + b * 16, o);
+              float o[16], f[16], a[16];
+              sb::tmem_ld16(t_lane + O_COL + x * R + b * 16, reinterpret_cast<uint32_t(&)[16]>(o));
+              sb::tmem_ld16(t_lane + FAR_COL + x * R + b * 16, reinterpret_cast<uint32_t(&)[16]>(f));
               sb::tmem_ld_wait();
 #pragma unroll
               for (int u = 0; u < 16; ++u) {
-                const float a = __shfl_sync(0xffffffffu, b < 2 ? alpha[0] : alpha[1], (b & 1) * 16 + u);
-                o[u] = __float_as_uint(__uint_as_float(o[u]) * a);
+                a[u] = __shfl_sync(0xffffffffu, b < 2 ? alpha[0] : alpha[1], (b & 1) * 16 + u);
+                o[u] *= a[u];
               }
-              pa_tmem_st16(t_lane + O_COL + x * R + b * 16, o);
+              if (!fold) pa_tmem_st16(t_lane + O_COL + x * R + b * 16, reinterpret_cast<uint32_t*>(o));
+              if (folds > 0) {
+#pragma unroll
+                for (int u = 0; u < 16; ++u) f[u] = (folds > fold ? f[u] * a[u] : 0.f) + (fold ? o[u] : 0.f);
+                pa_tmem_st16(t_lane + FAR_COL + x * R + b * 16, reinterpret_cast<uint32_t*>(f));
+              }
             }
             sb::tmem_st_wait();
+            if (fold) {
+              const float sum16 = pa_transpose_reduce(l, lane, [](float a, float b) { return a + b; });
+              far0 += lane < 16 ? sum16 : l0;
+              far1 += l1;
+              l0 = l1 = 0.f;
+#pragma unroll
+              for (int u = 0; u < 16; ++u) l[u] = 0.f;
+            }
           }
           if (!meet()) { ok = false; break; }  // every warp has read the maxima: P goes to the same place
           probabilities();
@@ -1223,6 +1288,23 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       }
       const float sum16 = pa_transpose_reduce(l, lane, [](float a, float b) { return a + b; });
       if (lane < 16) l0 = sum16;
+      if (n - x > 2 * PA_FOLD) {  // back from the second place
+        l0 += far0;
+        l1 += far1;
+        sb::tc_fence_after();
+#pragma unroll 1
+        for (int b = 0; b < nb; ++b) {
+          float o[16], f[16];
+          sb::tmem_ld16(t_lane + O_COL + x * R + b * 16, reinterpret_cast<uint32_t(&)[16]>(o));
+          sb::tmem_ld16(t_lane + FAR_COL + x * R + b * 16, reinterpret_cast<uint32_t(&)[16]>(f));
+          sb::tmem_ld_wait();
+#pragma unroll
+          for (int u = 0; u < 16; ++u) o[u] += f[u];
+          pa_tmem_st16(t_lane + O_COL + x * R + b * 16, reinterpret_cast<uint32_t*>(o));
+        }
+        sb::tmem_st_wait();
+        sb::tc_fence_before();
+      }
       wmax[quad * R + lane] = l0;  // P of this group is not in use: its place takes the warps' sums
       wmax[quad * R + 32 + lane] = l1;
       if (quad == 0 && lane == 0) c.need[x][0][0] = cur;  // no vote is under way

@@ -889,3 +889,47 @@ def test_work_shared_out_over_fewer_multiprocessors(sms, monkeypatch):
         b = _attend_batch(lens, new, 16, 8, 2, 128, torch.bfloat16, DEV)
         _check_attention(b, paged_attention(b.q, *b.args()), True, None)
     K.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length,new,heads,dim", [(2 ** 22, 1, 1, 64), (2 ** 22 + 77, 2, 20, 128),   # narrow, 1 and 40 rows
+                                                  (2 ** 26, 1, 1, 64),                                # the longest table
+                                                  (2 ** 20 - 3, 20, 4, 128),                          # wide, 80 rows
+                                                  (2 ** 20 + 130, 40, 4, 64), (2 ** 20, 65, 4, 128)])  # 160 and 260 rows
+def test_long_contexts_in_one_piece(length, new, heads, dim, monkeypatch):
+    """One CTA adds up millions of keys: the sums are as exact as those of 2^14 keys.  Positions share pages, so that a key's
+    weight is multiplied by how often it is seen; later keys have larger scores, so that the references move."""
+    from scaling_b200.ops import paged_attention as module
+
+    monkeypatch.setattr(module, "sm_count", lambda: 1)
+    dtype, page, pages = torch.float16, 128, 48
+    g = torch.Generator().manual_seed(length)
+    kc = torch.randn(pages, page, 1, dim, generator=g)
+    vc = 1.0 + 0.5 * torch.randn(pages, page, 1, dim, generator=g)
+    kc[pages // 2:] *= 2.0
+    kc, vc = (t.to(dtype).to(DEV) for t in (kc, vc))
+    cols = -(-length // page)
+    table = torch.arange(cols) % (pages // 2)
+    table[cols // 2:] += pages // 2
+    table = table.int().to(DEV)
+    q = (1.5 * torch.randn(new, heads, dim, generator=g)).to(dtype).to(DEV)
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    out = paged_attention(q, kc, vc, table[None], ints(0, new), ints(length))
+    K.check_status()
+    position = torch.arange(length, device=DEV)
+    key = table[position // page].long() * page + position % page
+    k, v = kc.reshape(-1, dim).double(), vc.reshape(-1, dim).double()
+    half, scale = torch.finfo(dtype).eps / 2, dim ** -0.5
+    for i in range(new):
+        count = torch.bincount(key[:length - new + i + 1], minlength=pages * page).double()
+        z = q[i].double() @ k.t() * scale
+        w = torch.exp(z - z.amax(-1, keepdim=True)) * count
+        w /= w.sum(-1, keepdim=True)
+        want = w @ v
+        # as in attention_in_64_bits, with chains of 2^14 additions, and of one rounded addition for each of these
+        size = (q[i].double().abs() @ k.abs().t()).amax(-1, keepdim=True) * scale
+        rel = half + 2 * (size * (dim + 8) * 2.0 ** -23 + 2.0 ** -21) + 2 ** 14 * 2.0 ** -23 + length / 2 ** 14 * 2.0 ** -24
+        bound = rel * (w @ v.abs())
+        bound += half * (want.abs() + bound)
+        err = (out[i].double() - want).abs()
+        assert (err <= bound).all(), f"{(err / bound).max().item():.3g} of the bound"
