@@ -264,7 +264,11 @@ SB_API int sb200_embedding_bwd(const long* sorted_ids, const long* order, const 
 SB_API int sb200_bind_device(int device) {
   cudaError_t e = cudaSetDevice(device);
   if (e != cudaSuccess) return (int)e;
-  e = cudaFree(nullptr);  // forces the primary context to be current on this thread
+  // forces the primary context to be current on this thread; nothing is freed, so a capture under way need not forbid it
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  const bool relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+  e = cudaFree(nullptr);
+  if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
   return (int)e;
 }
 // Sets the calling thread's stream capture mode (a cudaStreamCaptureMode) and returns the one before, or -1.

@@ -933,3 +933,47 @@ def test_long_contexts_in_one_piece(length, new, heads, dim, monkeypatch):
         bound += half * (want.abs() + bound)
         err = (out[i].double() - want).abs()
         assert (err <= bound).all(), f"{(err / bound).max().item():.3g} of the bound"
+
+
+FIRST_CALL = '''
+import torch
+from scaling_b200.ops import functional as K
+from scaling_b200.ops.paged_attention import paged_append, paged_attention
+
+make = lambda *shape: torch.randn(*shape, device="cuda").bfloat16()
+ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+q, k, v, w, kc, vc = make(3, 4, 64), make(3, 2, 64), make(3, 2, 64), make(64), make(4, 16, 2, 64), make(4, 16, 2, 64)
+cache = (kc, vc, ints(0, 1, 2)[None], ints(0, 3), ints(20))
+rotary = dict(positions=ints(17, 18, 19), rotary=(64, 10000.0, False))
+leaves = [t.clone().requires_grad_() for t in (q, k, w)]
+
+
+def step():
+    outs = K.qk_norm_rope(*leaves, leaves[2], **rotary)
+    return outs[0].detach(), *torch.autograd.grad(outs, leaves, (q, k))
+
+
+calls = {"append": lambda: (paged_append(k, v, *cache, q=q), kc.clone()), "attend": lambda: (paged_attention(q, *cache),),
+         "norm": lambda: K.qk_norm_rope(q, k, w, w, **rotary), "step": step}
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = calls["WHICH"]()
+graph.replay()
+K.check_status()
+assert all(torch.equal(a, b) for a, b in zip(got, calls["WHICH"]()))
+print("FIRST-CALL-OK")
+'''
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["append", "attend", "norm", "step"])
+def test_the_first_call_of_a_process_inside_a_capture(which):
+    """Loading the library, binding the thread and making the status words are no part of the graph and do not break it."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    res = subprocess.run([sys.executable, "-c", FIRST_CALL.replace("WHICH", which)], capture_output=True, text=True,
+                         cwd=Path(__file__).resolve().parent.parent, timeout=300)
+    assert res.returncode == 0 and "FIRST-CALL-OK" in res.stdout, res.stderr[-3000:]
