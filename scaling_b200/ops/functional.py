@@ -33,7 +33,7 @@ def _status_words() -> tuple[torch.Tensor, torch.Tensor]:
     if d not in _STATUS:
         with _lib.outside_captures():  # a captured call must not clear the words at every replay
             both = torch.zeros(2, dtype=torch.int32, device=f"cuda:{d}")
-        _STATUS[d] = (both[:1], both[1:])
+        _STATUS.setdefault(d, (both[:1], both[1:]))  # threads whose first calls meet share one pair
     return _STATUS[d]
 
 
