@@ -244,13 +244,15 @@ struct PaSeq { int row0, n, L; };
 
 __device__ __forceinline__ PaSeq pa_seq(const PaParams& p, int b) {
   PaSeq s;
-  s.row0 = min(max(p.cu[b], 0), p.T);
-  s.n = min(max(p.cu[b + 1], s.row0), p.T) - s.row0;
+  const int start = p.cu[b], end = p.cu[b + 1];
+  s.row0 = min(max(start, 0), p.T);
+  s.n = min(max(end, s.row0), p.T) - s.row0;
   const long cap = (long)p.cols << p.page_shift;
   int L = p.lens[b];
-  if (L < 0 || L > cap) {  // a length that the table does not cover: reported, cut to what it covers
+  if (L < 0 || L > cap || start != s.row0 || end != s.row0 + s.n) {
+    // a length that the table does not cover, rows that do not follow one another inside the T: reported, cut to what there is
     *p.status = SB_ERR_BAD_ARG;
-    L = L < 0 ? 0 : (int)cap;
+    L = (int)min((long)max(L, 0), cap);
   }
   s.L = L;
   return s;
@@ -1017,10 +1019,6 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     pa_load<R, PANELS, true, false>(p, c, sRing, &tmK, &tmV, lane);
   } else if (warp == 11) {
     pa_load<R, PANELS, false, true>(p, c, sRing, &tmK, &tmV, lane);
-    if (blockIdx.x == 0) {  // sequences that do not follow one another inside the rows: reported (pa_seq cuts them)
-      for (int b = lane; b < p.batch; b += 32)
-        if (p.cu[b] < 0 || p.cu[b + 1] < p.cu[b] || p.cu[b + 1] > p.T) *p.status = SB_ERR_BAD_ARG;
-    }
     if (p.zero_tail) {  // rows before the first and behind the last sequence
       const int before = p.batch > 0 ? min(max(p.cu[0], 0), p.T) : 0, heads = p.Hkv * p.group;
       const int gap = p.batch > 0 ? max(min(p.cu[p.batch], p.T), before) - before : 0, per_row = p.D / 8;
