@@ -31,18 +31,20 @@
 // of V (a page of 16 tokens is a copy of its own, and one warp alone issues them no faster than the memory delivers), 9 MMA
 // issuer.  Wide: 8 loader of both, 9 and 11 MMA issuers of the two groups.
 //
-// What bounds it, measured on one B200 (6.57 TB/s copy, 1634 TFLOP/s):
-//   decoding, 64 requests of up to 8000 tokens, 32 heads over 8 of 128, pages of 16: 148 to 156 us (5.7 to 6.0 TB/s, 0.87 to
+// What bounds it, measured on one B200 (6.57 TB/s copy, 1634 TFLOP/s), device time in a captured graph:
+//   decoding, 64 requests of up to 8000 tokens, 32 heads over 8 of 128, pages of 16: 147 to 150 us (5.9 to 6.0 TB/s, 0.90 to
 //     0.92 of the copy): the stream of K and V.
-//   decoding, two long contexts, 40 heads over one of 128: 42 us (3.1 TB/s): about 3 us per item end, the softmax of 40 rows
-//     per key and the joining of some 70 parts per row, against 20 us for the bytes.
-//   chunks of 2048 tokens on long contexts, heads of 128: 420 to 435 us, 980 to 1015 TFLOP/s (0.60 to 0.62): per half tile the
+//   decoding, two long contexts, 40 heads over one of 128: 43 to 45 us (2.9 TB/s): about 3 us per item end, the softmax of 40
+//     rows per key and the joining of some 70 parts per row, against 20 us for the bytes.
+//   chunks of 2048 tokens on long contexts, heads of 128: 420 to 440 us, 970 to 1015 TFLOP/s (0.59 to 0.62): per half tile the
 //     chain S product -> wait -> 64 exponentials per row -> wait -> P V product; two groups and two S each hide most of it.
-//   one request: 10.6 us: launch, work line, queries, tile, epilogue in a chain; nothing to overlap.
-//   24 ragged sequences of 1 to 300 new tokens: 56 to 60 us, two kernels one after the other on most SMs and 3 to 4 us per item.
+//     Calls back to back without pause take 474 us, because the power cap lowers the clock.
+//   one request: 10.8 us (an eager call 30: the enqueue): launch, work line, queries, tile, epilogue in a chain.
+//   24 ragged sequences of 1 to 300 new tokens: 55 to 60 us, two kernels one after the other on most SMs and 3 to 4 us per item.
 //
-// Rounding: scores, sums and outputs are fp32; P is rounded to the 16-bit element type for the second product (half a
-// step per probability, averaged over the row), the output once.
+// Rounding: scores, sums and outputs are fp32; P is rounded to the 16-bit element type for the second product, the output once.
+// The rounding of P is the larger part of what a result is off: relative to the 64-bit value 0.0023 in bf16 and 0.00025 in
+// fp16, where the output's rounding alone gives 0.0017 and 0.00021.
 #include <cuda.h>
 
 #include <algorithm>

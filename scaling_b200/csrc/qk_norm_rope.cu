@@ -15,9 +15,10 @@
 // rotation needs no exchange; only the row sums go through shuffles.  Statistics, weights, sines and products stay in
 // fp32 and are rounded once, at the store.
 //
-// Measured on one B200 (copy 6.57 TB/s), forward and backward together: 8192 tokens, 32 + 8 heads of 128, RMS, interleaved
-// rotation, bf16: 116 us = 3.6 TB/s (0.55 of the copy); 16384 tokens, 12 + 12 heads of 64, layer norm with biases, packed
-// projection: 84 us (0.46); a decoding step's append 6.4 us; an append of some 6000 prompt tokens, 40 + 1 heads: 39 us (0.52).
+// Measured on one B200 (copy 6.57 TB/s), device time in a captured graph, forward and backward together: 8192 tokens, 32 + 8
+// heads of 128, RMS, interleaved rotation, bf16: 115 us = 3.6 TB/s (0.55 of the copy); 16384 tokens, 12 + 12 heads of 64, layer
+// norm with biases, packed projection: 83 us (0.46); a decoding step's append 6.5 us; an append of some 6000 prompt tokens,
+// 40 + 1 heads: 39 us (0.51).  Eager calls take 165, 183, 32 and 41 us: the first three are bound by the enqueue.
 // Bound by latency at the occupancy that the registers leave (three blocks per SM forward, two backward; 51 and 39 % of the
 // issue slots, 35 % of the DRAM cycles).  Per element there are conversions, the norm's shuffles and three passes of fp32
 // arithmetic; hence the packed fp32 forms, weights in registers, code of its own per kind of row and per common head size.
@@ -624,7 +625,7 @@ __device__ __forceinline__ void qn_bwd_rows(const QnParams& p, const QnRows& R, 
       }
       const float r = qn_stats<V, NP, LG>(a, b, ha, hb, inv_d, RMS, p.eps, g);
       float s1 = 0.f, s2 = 0.f;  // sums of g and of g * xhat
-      const bool keep = live;    // a group without a row repeats the row before: it counts once
+      const bool keep = live;    // a group without a row works on what it loaded last (or zeros): it must not count
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         float w[V];

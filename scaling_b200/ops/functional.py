@@ -687,7 +687,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     ``k [tokens, kv_heads, d]`` (any strides) give new contiguous tensors; differentiable in q, k, weights and biases.
 
     Every head of every token is normalised over its ``d`` elements (``rms``: RMSNorm, else LayerNorm with optional
-    biases), scaled by the weight ``[d]``, and its first ``rotary[0]`` elements are rotated by ``positions[token]``;
+    biases), scaled by the weight ``[d]``, and its first ``rotary[0]`` elements are rotated by ``positions[token]`` (32 bits);
     ``rotary = (rotary dimensions, base, interleaved)`` or None.  Equals ``rope(rms_norm(q, ...), ...)`` up to
     rounding: the result is rounded once, angles are exact at far positions.  Head sizes up to 256."""
     for name, x, w, b in (("q", q, q_weight, q_bias), ("k", k, k_weight, k_bias)):

@@ -219,9 +219,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     cache, so they are written first (``paged_append``).  A query that sees nothing gives zeros.  Pages that no query of
     the call sees may be missing from the table.  Rows of no sequence are left as they were in ``out`` and are zero
     without it; ``out`` may be ``q`` itself and overlaps no other tensor.  Whatever the cache holds behind a sequence's
-    last token has no effect; keys and values of its tokens are finite.  On GPUs: bf16 and fp16, head sizes that are
-    multiples of 8 up to 128, pages of 8 tokens and more, page tables of up to 2^26 positions, up to 2^30 query rows and
-    2^30 products of 256 rows (64 in decoding) with 128 keys.  In inference only: no backward pass."""
+    last token has no effect; keys and values of its tokens are finite.  On GPUs: bf16 and fp16 (probabilities are rounded
+    to that type, sums are not), head sizes that are multiples of 8 up to 128, pages of 8 tokens and more, page tables of up
+    to 2^26 positions, 2^17 sequences, 2^30 query rows and 2^15 heads per KV head; products of 256 rows (64 in decoding)
+    with 128 keys, and four more for each block of rows, add up to less than 2^31 (else zeros and an error that
+    ``check_status`` raises).  In inference only: no backward pass."""
     _check_cache(k_cache, v_cache, page_table, cu_seqlens, seq_lens)
     _no_grad_inputs("paged_attention", q, k_cache, v_cache, out)
     _check_rows("q", q, k_cache)
