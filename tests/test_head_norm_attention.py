@@ -231,3 +231,41 @@ def test_far_positions_have_the_same_angles_in_every_form(rotary):
     for a, b in zip(*seen):
         # 64 half steps for the norm and the rotation in one kernel, 32 + 32 for the separate ones, of max|y|
         assert ((a - b).abs() <= 128 * 2.0 ** -24 * a.abs().amax(-1, keepdim=True) * 2.0 ** 0.5).all()
+
+
+def _tensor_parallel_worker(rank, world_size, port, device, kv_heads):
+    from tests.test_core_distributed import _topology
+
+    t = _topology(rank, world_size, port, mp=world_size)
+    m = ParallelSelfAttention(
+        hidden_size=128, num_attention_heads=8, masked_softmax_config=MaskedSoftmaxConfig(), topology=t,
+        rotary_config=RotaryConfig(dimensions=16), relative_position_embedding_type=RelativePositionEmbeddingType.ROTARY,
+        norm_type=NormType.RMS, key_query_norm=True, layernorm_config=LayerNormConfig(), qkv_in_one=False,
+        num_kv_heads=kv_heads)
+    g = torch.Generator().manual_seed(11)
+    draw = lambda *shape: torch.randn(*shape, generator=g)  # noqa: E731
+    full = {"query": draw(128, 128) / 8, "key": draw(kv_heads * 16, 128) / 8, "value": draw(kv_heads * 16, 128) / 8}
+    with torch.no_grad():
+        for name, w in full.items():
+            getattr(m, name).weight.copy_(w.chunk(world_size)[rank])
+            getattr(m, name).bias.zero_()
+        m.dense.weight.copy_((draw(128, 128) / 8).chunk(world_size, 1)[rank])
+        m.dense.bias.zero_()
+        m.norm_query.weight.copy_(1 + 0.2 * draw(16))
+        m.norm_key.weight.copy_(1 + 0.2 * draw(16))
+    x = draw(2, 12, 128).requires_grad_()
+    y = m(x, torch.tensor([0, 12, 24], dtype=torch.int32), torch.arange(12).repeat(2, 1) * 7919 + 10 ** 6)
+    y.square().sum().backward()
+    return y.detach(), x.grad, m.norm_query.weight.grad, m.norm_key.weight.grad
+
+
+@pytest.mark.dist
+@pytest.mark.parametrize("kv_heads", [4])
+def test_head_norms_and_far_positions_under_tensor_parallelism(kv_heads):
+    """The same outputs and gradients as on one rank; fp32 sums of at most 128 terms in another order."""
+    from tests.utils import dist_launcher
+
+    (want,) = dist_launcher(_tensor_parallel_worker, 1, kv_heads=kv_heads)
+    for got in dist_launcher(_tensor_parallel_worker, 2, kv_heads=kv_heads):
+        for a, b in zip(got, want):
+            assert (a - b).norm() <= 512 * 2.0 ** -24 * b.norm()

@@ -977,3 +977,13 @@ def test_the_first_call_of_a_process_inside_a_capture(which):
     res = subprocess.run([sys.executable, "-c", FIRST_CALL.replace("WHICH", which)], capture_output=True, text=True,
                          cwd=Path(__file__).resolve().parent.parent, timeout=300)
     assert res.returncode == 0 and "FIRST-CALL-OK" in res.stdout, res.stderr[-3000:]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 128), (12, 12, 64)])
+def test_chunks_with_many_items_per_multiprocessor(heads, kv_heads, dim):
+    """Long chunks of many heads behind long contexts: every CTA takes several items of many tiles, most of them divided."""
+    b = _attend_batch([6000, 4100], [1000, 700], 64, heads, kv_heads, dim, torch.bfloat16, DEV)
+    out = paged_attention(b.q, *b.args())
+    K.check_status()
+    _check_attention(b, out, True, None)
