@@ -747,6 +747,9 @@ class _HeadRotationFn(torch.autograd.Function):
 def head_rotation(x: torch.Tensor, positions: torch.Tensor, rotary: tuple[int, float, bool]) -> torch.Tensor:
     """The rotation of ``qk_norm_rope`` on its own, with the same angles: ``x [tokens, heads, d]`` after a norm that ran as
     a module.  (``rope`` forms its angles in fp32: 1e-2 rad off at position 10^5.)"""
+    if x.dim() != 3 or positions.dim() != 1 or positions.shape[0] != x.shape[0] or positions.device != x.device:
+        raise ValueError(f"the rotation of {tuple(x.shape)} on {x.device} needs one position per token there, got "
+                         f"{tuple(positions.shape)} on {positions.device}")
     rot, base, interleaved = rotary_args(rotary, x.shape[2])
     if x.is_cuda and x.dtype in _KERNEL_DTYPES and x.shape[2] <= 256 and 0 < x.numel() and x.shape[0] < 2 ** 31 - 2 ** 16:
         return _HeadRotationFn.apply(x, positions.to(torch.int32).contiguous(), rot, base, interleaved)

@@ -61,7 +61,7 @@ def _refuse_shared_memory(name: str, t: torch.Tensor) -> None:
     span = 1
     for stride, size in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
         if stride < span:
-            raise ValueError(f"elements of {name} share memory: rows {tuple(t.shape)} with strides {t.stride()}")
+            raise ValueError(f"elements of {name} share memory: shape {tuple(t.shape)} with strides {t.stride()}")
         span += stride * (size - 1)
 
 

@@ -378,3 +378,26 @@ def test_rotation_alone_kernel(T, H, D, rotary, dtype):
     _check_head_rotation(q, pos, rotary, g)
     turned = q.permute(1, 2, 0).contiguous().permute(2, 0, 1)  # as heads that were gathered over ranks come
     assert torch.equal(K.head_rotation(turned, pos, rotary), K.head_rotation(q, pos, rotary))
+
+
+def _rotation_refused(device):
+    q, _, _, _, pos, _, _ = _inputs(9, 3, 1, 16, torch.float32, torch.float32, True, device)
+    rotary = (16, 10000.0, False)
+    K.head_rotation(q, pos, rotary)
+    K.head_rotation(q, pos.float(), rotary)
+    for x, p, r in ((q, pos[:8], rotary), (q, pos[:1], rotary), (q, pos[None], rotary), (q, torch.cat((pos, pos)), rotary),
+                    (q[0], pos, rotary), (q, pos, (18, 10000.0, False)), (q, pos, (7, 10000.0, False))):
+        with pytest.raises(ValueError):
+            K.head_rotation(x, p, r)
+
+
+def test_rotation_alone_refusals():
+    _rotation_refused("cpu")
+
+
+@pytest.mark.gpu
+def test_rotation_alone_gpu_refusals():
+    _rotation_refused(DEV)
+    q, _, _, _, pos, _, _ = _inputs(9, 3, 1, 16, torch.float32, torch.float32, True, DEV)
+    with pytest.raises(ValueError):
+        K.head_rotation(q, pos.cpu(), (16, 10000.0, False))
