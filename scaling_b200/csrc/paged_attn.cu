@@ -38,7 +38,7 @@
 //     rows per key and the joining of some 70 parts per row, against 20 us for the bytes.
 //   chunks of 2048 tokens on long contexts, heads of 128: 420 to 440 us, 970 to 1015 TFLOP/s (0.59 to 0.62): per half tile the
 //     chain S product -> wait -> 64 exponentials per row -> wait -> P V product; two groups and two S each hide most of it.
-//     Calls back to back without pause take 474 us, because the power cap lowers the clock.
+//     Calls back to back without pause take 474 to 482 us, because the power cap lowers the clock.
 //   one request: 10.8 us (an eager call 30: the enqueue): launch, work line, queries, tile, epilogue in a chain.
 //   24 ragged sequences of 1 to 300 new tokens: 55 to 60 us, two kernels one after the other on most SMs and 3 to 4 us per item.
 //
